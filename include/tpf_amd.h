@@ -508,6 +508,43 @@ int tpf_attn_pair_rows_forward_bf16(const void* qkv, const void* rest, int64_t r
                                     int64_t workspace_bytes, int64_t B, int64_t O, int64_t N,
                                     int64_t H, int64_t D, double scale, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Cross attention to states of another length: out = softmax(scale q k^T +
+ * mask) v, forward and backward.
+ *
+ * q [B, H, Nq, D], k and v [B, Hk, Nk, D] with H a multiple of Hk (query head
+ * h reads kv head h / (H / Hk)), each through its element strides of the first
+ * three axes (multiples of 8, 0 for a broadcast axis; channels contiguous);
+ * out [B, Nq, H, D] contiguous.  D is a multiple of 8 up to 128.  mask, one
+ * entry per state [B, Nk] with batch stride mask_stride (0: shared): bytes
+ * (0 drops the state) or f32 added to the scores (-inf drops it).  K and V of a
+ * dropped state are never used, whatever they hold.  A row without a state
+ * gives 0, and gradients of 0.  Every tensor starts on 16 bytes.
+ * lse: f32 [B, H, Nq], or [2, B, H, Nq] with an f32 mask: the rows' softmax
+ * statistics for the backward; null when none follows.
+ * The forward serves BF16 and FP16, the backward BF16.
+ * ---------------------------------------------------------------------- */
+enum { TPF_BF16 = 0, TPF_F16 = 1, TPF_F32 = 2 };
+enum { TPF_MASK_NONE = 0, TPF_MASK_BYTES = 1, TPF_MASK_F32 = 2 };
+typedef struct tpf_xattn_shape {
+  int64_t B, H, Hk, Nq, Nk, D;
+  int64_t dtype, mask_kind, mask_stride;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, head, position */
+} tpf_xattn_shape;
+int64_t tpf_xattn_forward_workspace_bytes(const tpf_xattn_shape* shape);
+int tpf_xattn_forward(const void* q, const void* k, const void* v, const void* mask, void* out,
+                      float* lse, void* workspace, int64_t workspace_bytes,
+                      const tpf_xattn_shape* shape, double scale, void* stream);
+/* Gradients of q, k and v from the forward's out and lse and the upstream
+ * gradient dout [B, Nq, H, D] (contiguous).  grad_strides: the element strides
+ * (batch, head, position) of dq, dk and dv, nine values. */
+int64_t tpf_xattn_backward_workspace_bytes(const tpf_xattn_shape* shape);
+int tpf_xattn_backward_bf16(const void* q, const void* k, const void* v, const void* mask,
+                            const void* out, const void* dout, const float* lse, void* dq, void* dk,
+                            void* dv, void* workspace, int64_t workspace_bytes,
+                            const tpf_xattn_shape* shape, const int64_t* grad_strides,
+                            double scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -64,3 +64,7 @@ __all__ += ["set_tpf_bf16_cast_for_fp32_training", "set_turbopairformer_strict",
 from .layernorm import layer_norm_bf16  # noqa: E402
 
 __all__ += ["layer_norm_bf16"]
+
+from .cross_attention import cross_attention  # noqa: E402
+
+__all__ += ["cross_attention"]

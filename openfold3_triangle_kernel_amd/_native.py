@@ -145,6 +145,10 @@ SIGNATURES: dict[str, tuple] = {
         _I32,
         [_P] * 21 + [_I32, _I64, _I64, _I64] + [_P] * 10 + [_I64, _P],
     ),
+    "tpf_xattn_forward_workspace_bytes": (_I64, [_P]),
+    "tpf_xattn_forward": (_I32, [_P] * 7 + [_I64, _P, _F64, _P]),
+    "tpf_xattn_backward_workspace_bytes": (_I64, [_P]),
+    "tpf_xattn_backward_bf16": (_I32, [_P] * 11 + [_I64, _P, _P, _F64, _P]),
 }
 
 _LOCK = threading.Lock()

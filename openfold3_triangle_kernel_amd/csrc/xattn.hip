@@ -1,0 +1,550 @@
+// Cross attention to states of another length: forward.
+//
+//   s_ij = scale q_i . k_j + mask_j,  p = softmax_j(s),  o_i = sum_j p_ij v_j
+//
+// over R = G * Nq rows of a kv head and its Nk states (xattn.hpp), in one pass
+// over the states with a running maximum and sum.  A wave owns 32 QB rows and
+// forms S^T = K Q^T, so a lane holds one row's scores: maxima and sums are
+// lane-local up to one exchange with lane ^ 32, and the S^T tile goes back into
+// the matrix cores as it stands for O^T += V^T P^T.  A row without a live state
+// gives 0.
+#include "gemm_core.hpp"  // xcd_order
+#include "tpf_status.hpp"
+#include "xattn.hpp"
+
+namespace tpf {
+
+constexpr float kXaLow = -3.402823466e38f;
+
+// Running softmax state of a wave's rows; scores and maxima m are in raw units
+// (before the scale).  The maximum is raised only once a row's scores pass it by
+// 8 powers of two: p then stays below 256, which 32-bit sums and either operand
+// type hold, and the outputs are rescaled a few times per call instead of every
+// tile.  p is one fused multiply-add and an exponential, 2^(c s - c m); where a
+// tile has additive values, which may be of any size, the maximum is taken off
+// first, 2^(c (s - m)).
+template <int DP, int QB, bool F16>
+struct XRows {
+  static constexpr int DS = DP / 16, DB = DP / 32;
+  bf16x8 q[QB][DS];
+  f32x16 o[QB][DB];
+  float m[QB], l[QB];
+
+  __device__ __forceinline__ void init(const XAttnArgs& a, int b, int hk, int r0) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const int r = r0 + 32 * qb + (lane & 31);
+      int g, i;
+      xa_row(a, r < a.R ? r : a.R - 1, g, i);
+      const u16* p = a.q + b * a.q_sb + (int64_t)(hk * a.G + g) * a.q_sh + (int64_t)i * a.q_sn;
+#pragma unroll
+      for (int s = 0; s < DS; ++s) {
+        const int d = 16 * s + 8 * (lane >> 5);
+        q[qb][s] = d < a.D ? *reinterpret_cast<const bf16x8*>(p + d) : zero8();
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[qb][db] = zero16();
+      m[qb] = kXaLow;
+      l[qb] = 0.f;
+    }
+  }
+
+  // KB blocks of 32 states from k0 on, in the tiles K and V.
+  template <int KB>
+  __device__ __forceinline__ void step(const XAttnArgs& a, const u16* K, const u16* V, uint64_t live,
+                                       const float* fmask, int k0) {
+    f32x16 s[QB][KB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) s[qb][kb] = zero16();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int d = 0; d < DS; ++d) {
+        const bf16x8 kf = xa_frag<DP>(K, 32 * kb, d);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) s[qb][kb] = xa_mfma<F16>(kf, q[qb][d], s[qb][kb]);
+      }
+    const uint64_t whole = KB == 2 ? ~0ull : 0xffffffffull;
+    if (live != whole || fmask) {
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+          xa_mask32(s[qb][kb], (uint32_t)(live >> (32 * kb)), fmask, k0 + 32 * kb, a.Nk, a.inv_scale,
+                    a.mask_floor);
+    }
+    bf16x8 p[QB][2 * KB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      float t = s[qb][0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t = fmaxf(t, s[qb][kb][r]);
+      t = xor32_max(t);
+      if (__ballot((t - m[qb]) * a.c > 8.f)) {
+        const float mn = fmaxf(m[qb], t), al = fast_exp2((m[qb] - mn) * a.c);
+        m[qb] = mn;
+        l[qb] *= al;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[qb][db][r] *= al;
+      }
+      float off = -m[qb] * a.c, sum = 0.f;
+      if (fmask) {
+        off = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[qb][kb][r] -= m[qb];
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[qb][kb][r] = fast_exp2(fmaf(s[qb][kb][r], a.c, off));
+          sum += s[qb][kb][r];
+        }
+        p[qb][2 * kb] = xa_pack8<F16>(s[qb][kb], 0);
+        p[qb][2 * kb + 1] = xa_pack8<F16>(s[qb][kb], 8);
+      }
+      l[qb] += sum;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const bf16x8 vf = xa_frag_t<DP>(V, 32 * kb, t, db);
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) o[qb][db] = xa_mfma<F16>(vf, p[qb][2 * kb + t], o[qb][db]);
+        }
+  }
+};
+
+// 1 / sum, and 0 for a row without a live state (compared by bits: a sum that
+// is NaN stays NaN).
+__device__ __forceinline__ float xa_inverse(float l) {
+  return __float_as_uint(l) == 0u ? 0.f : 1.f / l;
+}
+
+// A row's statistics for the backward: log2 of the sum and the raw maximum, or
+// without additive masks the two as one log-sum-exp.
+__device__ __forceinline__ void xa_store_stats(const XAttnArgs& a, int64_t row, float m, float l) {
+  const float ll = __log2f(l);
+  if (a.mask_kind == kMaskF32) {
+    a.lse[row] = ll;
+    a.lse[(int64_t)a.B * a.Hk * a.R + row] = m;
+  } else {
+    a.lse[row] = fmaf(m, a.c, ll);
+  }
+}
+
+// Writes a row's outputs that this lane holds (channels 32 db + 8 g4 + 4 h + e).
+template <int DB, bool F16>
+__device__ __forceinline__ void xa_store_row(const XAttnArgs& a, int b, int hk, int r,
+                                             const f32x16 (&o)[DB], float inv) {
+  const int h = (threadIdx.x >> 5) & 1;
+  int g, i;
+  xa_row(a, r, g, i);
+  u16* p = a.out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const int d = 32 * db + 8 * g4 + 4 * h;
+      if (d < a.D) {
+        uint2 v;
+        v.x = xa_pair<F16>(o[db][4 * g4] * inv, o[db][4 * g4 + 1] * inv);
+        v.y = xa_pair<F16>(o[db][4 * g4 + 2] * inv, o[db][4 * g4 + 3] * inv);
+        *reinterpret_cast<uint2*>(p + d) = v;
+      }
+    }
+}
+
+// Four waves of 32 QB rows share K and V tiles of 64 states, two stages deep.
+// Tiles without a live state are passed over.
+template <int DP, int QB, bool F16>
+__global__ __launch_bounds__(256, QB == 2 && DP > 64 ? 1 : 2) void xattn_fwd_kernel(XAttnArgs a) {
+  constexpr int KT = 64, TILE = KT * DP;
+  __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t total = (int64_t)a.B * a.Hk * a.splits * a.tiles;
+  const int64_t T = xcd_order(total);
+  if (T < 0) return;
+  const int tile = (int)(T % a.tiles);
+  const int64_t u = T / a.tiles;
+  const int split = (int)(u % a.splits);
+  const int64_t bh = u / a.splits;
+  const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
+  const int r0 = tile * 128 * QB + w * 32 * QB;
+  const int kbeg = split * a.chunk, kend = min(a.Nk, kbeg + a.chunk);
+  const u16* kp = a.k + b * a.k_sb + hk * a.k_sh;
+  const u16* vp = a.v + b * a.v_sb + hk * a.v_sh;
+
+  XMask mask;
+  mask.init(a, b);
+  XTileLoader<DP, KT, 4> lk, lv;
+  lk.init(w, a.k_sn, a.D);
+  lv.init(w, a.v_sn, a.D);
+  XRows<DP, QB, F16> rows;
+  rows.init(a, b, hk, r0);
+
+  // (k0, live): the tile in flight or in use; raw: the masks of the one after.
+  int k0 = kbeg - KT;
+  uint64_t live = 0;
+  bool values = false;
+  uint32_t raw = mask.load(kbeg, kend);
+  auto advance = [&]() {  // to the next tile with a live state; false past the end
+    for (;;) {
+      k0 += KT;
+      if (k0 >= kend) return false;
+      live = mask.live(raw);
+      values = mask.values(raw);
+      raw = mask.load(k0 + KT, kend);
+      if (live) return true;
+    }
+  };
+  bool more = advance();
+  if (more) {
+    lk.issue(kp + (int64_t)k0 * a.k_sn, live, w, smem[0][0]);
+    lv.issue(vp + (int64_t)k0 * a.v_sn, live, w, smem[0][1]);
+  }
+  int st = 0;
+  while (more) {
+    const int kc = k0;
+    const uint64_t lc = live;
+    const bool vc = values;
+    wait_vmcnt<0>();
+    lds_barrier();
+    more = advance();
+    if (more) {
+      lk.issue(kp + (int64_t)k0 * a.k_sn, live, w, smem[st ^ 1][0]);
+      lv.issue(vp + (int64_t)k0 * a.v_sn, live, w, smem[st ^ 1][1]);
+    }
+    rows.template step<2>(a, smem[st][0], smem[st][1], lc, vc ? mask.f : nullptr, kc);
+    st ^= 1;
+  }
+
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const int r = r0 + 32 * qb + (lane & 31);
+    const float l = xor32_sum(rows.l[qb]);
+    if (r >= a.R) continue;
+    if (a.splits == 1) {
+      xa_store_row<DP / 32, F16>(a, b, hk, r, rows.o[qb], xa_inverse(l));
+      if (a.lse && lane < 32) xa_store_stats(a, bh * a.R + r, rows.m[qb], l);
+    } else {
+      const int64_t pr = (bh * a.splits + split) * a.R + r;
+      if (lane < 32) {
+        a.part_ml[2 * pr] = rows.m[qb];
+        a.part_ml[2 * pr + 1] = l;
+      }
+      float* p = a.part_o + pr * a.D;
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const int d = 32 * db + 8 * g4 + 4 * (lane >> 5);
+          if (d < a.D) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = rows.o[qb][db][4 * g4 + e];
+            *reinterpret_cast<f32x4*>(p + d) = v;
+          }
+        }
+    }
+  }
+}
+
+// Few rows (at most 32 QB, one decoded token above all): the states' bytes are
+// the bound.  Every wave streams tiles of 32 states of its own, two stages deep
+// without a barrier, and the four waves' results meet in LDS at the end.
+template <int DP, int QB, bool F16>
+__global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
+  constexpr int KT = 32, TILE = KT * DP, NI = KT * DP / 512;
+  constexpr int OP = DP + 4;  // pitch of the joined rows (f32)
+  __shared__ __attribute__((aligned(1024))) u16 smem[4][2][2][TILE];
+  static_assert(sizeof(smem) >= 4 * 32 * (OP + 2) * 4, "the join fits");
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t T = xcd_order((int64_t)a.B * a.Hk * a.splits);
+  if (T < 0) return;
+  const int64_t bh = T / a.splits;
+  const int split = (int)(T - bh * a.splits);
+  const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
+  const int kbeg = split * a.chunk, kend = min(a.Nk, kbeg + a.chunk);
+  const u16* kp = a.k + b * a.k_sb + hk * a.k_sh;
+  const u16* vp = a.v + b * a.v_sb + hk * a.v_sh;
+
+  XMask mask;
+  mask.init(a, b);
+  XTileLoader<DP, KT, 1> lk, lv;
+  lk.init(0, a.k_sn, a.D);
+  lv.init(0, a.v_sn, a.D);
+  XRows<DP, QB, F16> rows;
+  rows.init(a, b, hk, 0);
+
+  int k0 = kbeg + KT * (w - 4);
+  uint64_t live = 0;
+  bool values = false;
+  auto load = [&](int k) { return mask.load(k, min(kend, k + KT)); };
+  uint32_t raw = load(k0 + 4 * KT);
+  auto advance = [&]() {
+    for (;;) {
+      k0 += 4 * KT;
+      if (k0 >= kend) return false;
+      live = mask.live(raw);
+      values = mask.values(raw);
+      raw = load(k0 + 4 * KT);
+      if (live) return true;
+    }
+  };
+  auto issue = [&](int st) {
+    lk.issue(kp + (int64_t)k0 * a.k_sn, live, 0, smem[w][st][0]);
+    lv.issue(vp + (int64_t)k0 * a.v_sn, live, 0, smem[w][st][1]);
+  };
+  bool more = advance();
+  if (more) issue(0);
+  int st = 0;
+  while (more) {
+    const int kc = k0;
+    const uint64_t lc = live;
+    const bool vc = values;
+    more = advance();
+    if (more) {
+      issue(st ^ 1);
+      wait_vmcnt<2 * NI>();  // this tile's loads are older than the next one's
+    } else {
+      wait_vmcnt<0>();
+    }
+    rows.template step<1>(a, smem[w][st][0], smem[w][st][1], lc, vc ? mask.f : nullptr, kc);
+    st ^= 1;
+  }
+
+  float* O = reinterpret_cast<float*>(&smem[0][0][0][0]);
+  float* ML = O + 4 * 32 * OP;
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    __syncthreads();
+    const float lw = xor32_sum(rows.l[qb]);
+    float* ow = O + (w * 32 + (lane & 31)) * OP;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = rows.o[qb][db][4 * g4 + e];
+        *reinterpret_cast<f32x4*>(ow + 32 * db + 8 * g4 + 4 * (lane >> 5)) = v;
+      }
+    if (lane < 32) {
+      ML[2 * (w * 32 + lane)] = rows.m[qb];
+      ML[2 * (w * 32 + lane) + 1] = lw;
+    }
+    __syncthreads();
+    const int rl = threadIdx.x >> 3, r = 32 * qb + rl;
+    if (r >= a.R) continue;
+    float m = kXaLow, l = 0.f, f[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) m = fmaxf(m, ML[2 * (x * 32 + rl)]);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      f[x] = fast_exp2((ML[2 * (x * 32 + rl)] - m) * a.c);
+      l += f[x] * ML[2 * (x * 32 + rl) + 1];
+    }
+    const int64_t pr = (bh * a.splits + split) * a.R + r;
+    const float inv = xa_inverse(l);
+    int g, i;
+    xa_row(a, r, g, i);
+    for (int d = 4 * (threadIdx.x & 7); d < a.D; d += 32) {
+      f32x4 o = (f32x4)0.f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(O + (x * 32 + rl) * OP + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += f[x] * v[e];
+      }
+      if (a.splits == 1) {
+        uint2 v;
+        v.x = xa_pair<F16>(o[0] * inv, o[1] * inv);
+        v.y = xa_pair<F16>(o[2] * inv, o[3] * inv);
+        *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d) =
+            v;
+      } else {
+        *reinterpret_cast<f32x4*>(a.part_o + pr * a.D + d) = o;
+      }
+    }
+    if ((threadIdx.x & 7) == 0) {
+      if (a.splits == 1) {
+        if (a.lse) xa_store_stats(a, bh * a.R + r, m, l);
+      } else {
+        a.part_ml[2 * pr] = m;
+        a.part_ml[2 * pr + 1] = l;
+      }
+    }
+  }
+}
+
+// Joins the key splits: o = sum_s 2^(c (m_s - m)) o_s / sum_s 2^(c (m_s - m)) l_s
+// in ascending order.  A thread forms four channels of one row.
+template <bool F16>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
+  const int dv = a.D / 4;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = t / dv;
+  if (row >= (int64_t)a.B * a.Hk * a.R) return;
+  const int d = 4 * (int)(t - row * dv);
+  const int64_t bh = row / a.R;
+  const int r = (int)(row - bh * a.R);
+  const float* ml = a.part_ml + 2 * (bh * a.splits * a.R + r);
+  const float* po = a.part_o + (bh * a.splits * a.R + r) * a.D + d;
+  float m = kXaLow;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[2 * (int64_t)s * a.R]);
+  float l = 0.f;
+  f32x4 o = (f32x4)0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float w = fast_exp2((ml[2 * (int64_t)s * a.R] - m) * a.c);
+    l += w * ml[2 * (int64_t)s * a.R + 1];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(po + (int64_t)s * a.R * a.D);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += w * v[e];
+  }
+  const float inv = xa_inverse(l);
+  int g, i;
+  xa_row(a, r, g, i);
+  const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
+  uint2 v;
+  v.x = xa_pair<F16>(o[0] * inv, o[1] * inv);
+  v.y = xa_pair<F16>(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d) = v;
+  if (a.lse && d == 0) xa_store_stats(a, row, m, l);
+}
+
+// Workgroups that the forward wants before it splits the states no further:
+// two rounds of the chip's 256 CUs for the streaming kernel (one workgroup a
+// CU), one round of two a CU for the tile kernel.
+static void xattn_plan(XAttnArgs& a) {
+  const bool few = a.R <= 64;
+  const int64_t rows = few ? 64 : (a.D > 64 ? 128 : 256);
+  a.tiles = (int)((a.R + rows - 1) / rows);
+  const int64_t groups = (int64_t)a.B * a.Hk * a.tiles;
+  const int64_t step = few ? 512 : 256;  // keys that a split is worth
+  int64_t s = 512 / groups;
+  const int64_t most = (a.Nk + step - 1) / step;
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  if (s < 1) s = 1;
+  const int64_t tiles = (a.Nk + 63) / 64;
+  a.chunk = (int)((tiles + s - 1) / s) * 64;
+  a.splits = (int)((a.Nk + a.chunk - 1) / a.chunk);
+  if (a.splits < 1) a.splits = 1;
+}
+
+static int64_t xattn_part_floats(const XAttnArgs& a) {
+  return a.splits > 1 ? (int64_t)a.B * a.Hk * a.splits * a.R * (a.D + 2) : 0;
+}
+
+// Sizes and strides as the kernels need them; 0 or an error code.
+int xattn_check(XAttnArgs& a, const tpf_xattn_shape* s, double scale, const char* fn) {
+  if (!s) return set_error(TPF_ERR_ARG, "%s: null shape", fn);
+  if (s->B < 1 || s->H < 1 || s->Hk < 1 || s->Nq < 1 || s->Nk < 1 || s->D < 8 || s->D > 128 ||
+      s->D % 8 || s->H % s->Hk)
+    return set_error(TPF_ERR_SHAPE, "%s: bad shape B=%lld H=%lld Hk=%lld Nq=%lld Nk=%lld D=%lld", fn,
+                     (long long)s->B, (long long)s->H, (long long)s->Hk, (long long)s->Nq,
+                     (long long)s->Nk, (long long)s->D);
+  const int64_t G = s->H / s->Hk, lim = (int64_t)1 << 30;
+  if (s->Nk > lim || s->Nq > lim || s->B > lim || s->H > lim || G * s->Nq > lim ||
+      (double)s->B * s->Hk * ((double)(G * s->Nq) / 64 + 1) * 64 > 2e9 ||
+      (double)s->B * s->Hk * ((double)s->Nk / 64 + 1) > 2e9)
+    return set_error(TPF_ERR_SHAPE, "%s: too many rows or states", fn);
+  for (int i = 0; i < 3; ++i) {
+    const int64_t* st = i == 0 ? s->q_stride : i == 1 ? s->k_stride : s->v_stride;
+    for (int j = 0; j < 3; ++j)
+      if (st[j] < 0 || st[j] % 8)
+        return set_error(TPF_ERR_SHAPE, "%s: strides must be multiples of 8 elements", fn);
+    if (i && st[2] >= ((int64_t)1 << 23))
+      return set_error(TPF_ERR_SHAPE, "%s: state stride too large", fn);
+  }
+  if (s->dtype != TPF_BF16 && s->dtype != TPF_F16)
+    return set_error(TPF_ERR_ARG, "%s: dtype must be TPF_BF16 or TPF_F16", fn);
+  if (s->mask_kind < 0 || s->mask_kind > 2 || s->mask_stride < 0)
+    return set_error(TPF_ERR_ARG, "%s: bad mask", fn);
+  if (!(scale > 0.0) || !(scale < 1e30))
+    return set_error(TPF_ERR_ARG, "%s: the scale must be positive", fn);
+  a.q_sb = s->q_stride[0]; a.q_sh = s->q_stride[1]; a.q_sn = s->q_stride[2];
+  a.k_sb = s->k_stride[0]; a.k_sh = s->k_stride[1]; a.k_sn = s->k_stride[2];
+  a.v_sb = s->v_stride[0]; a.v_sh = s->v_stride[1]; a.v_sn = s->v_stride[2];
+  a.mask_sb = s->mask_stride;
+  a.mask_kind = s->mask_kind;
+  a.B = (int)s->B; a.H = (int)s->H; a.Hk = (int)s->Hk; a.G = (int)G; a.Nq = (int)s->Nq;
+  a.Nk = (int)s->Nk; a.D = (int)s->D; a.R = (int)(G * s->Nq);
+  a.div_nq = make_fastdiv((uint32_t)s->Nq);
+  a.c = (float)(scale * 1.4426950408889634);
+  a.inv_scale = (float)(1.0 / scale);
+  a.mask_floor = -1.5e38f;  // finite masks stay finite in raw units
+  return TPF_OK;
+}
+
+template <int DP, bool F16>
+static void xattn_launch(const XAttnArgs& a, hipStream_t s) {
+  const int64_t groups = (int64_t)a.B * a.Hk * a.splits;
+  if (a.R <= 64) {
+    const dim3 grid((unsigned)((groups + 7) / 8 * 8));
+    if (a.R <= 32) hipLaunchKernelGGL((xattn_few_kernel<DP, 1, F16>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((xattn_few_kernel<DP, 2, F16>), grid, dim3(256), 0, s, a);
+  } else {
+    constexpr int QB = DP > 64 ? 1 : 2;
+    const dim3 grid((unsigned)((groups * a.tiles + 7) / 8 * 8));
+    hipLaunchKernelGGL((xattn_fwd_kernel<DP, QB, F16>), grid, dim3(256), 0, s, a);
+  }
+}
+
+template <bool F16>
+static void xattn_forward(const XAttnArgs& a, hipStream_t s) {
+  if (a.D <= 32) xattn_launch<32, F16>(a, s);
+  else if (a.D <= 64) xattn_launch<64, F16>(a, s);
+  else if (a.D <= 96) xattn_launch<96, F16>(a, s);
+  else xattn_launch<128, F16>(a, s);
+  if (a.splits > 1) {
+    const int64_t n = (int64_t)a.B * a.Hk * a.R * (a.D / 4);
+    hipLaunchKernelGGL(xattn_join_kernel<F16>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+  }
+}
+
+}  // namespace tpf
+
+extern "C" int64_t tpf_xattn_forward_workspace_bytes(const tpf_xattn_shape* shape) {
+  tpf::XAttnArgs a{};
+  if (tpf::xattn_check(a, shape, 1.0, "tpf_xattn_forward_workspace_bytes")) return -1;
+  tpf::xattn_plan(a);
+  return tpf::xattn_part_floats(a) * 4;
+}
+
+extern "C" int tpf_xattn_forward(const void* q, const void* k, const void* v, const void* mask,
+                                 void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                 const tpf_xattn_shape* shape, double scale, void* stream) {
+  const char* fn = "tpf_xattn_forward";
+  if (!q || !k || !v || !out) return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
+  tpf::XAttnArgs a{};
+  if (int rc = tpf::xattn_check(a, shape, scale, fn)) return rc;
+  if ((a.mask_kind != 0) != (mask != nullptr))
+    return tpf::set_error(TPF_ERR_ARG, "%s: mask pointer and mask kind disagree", fn);
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)workspace) % 16)
+    return tpf::set_error(TPF_ERR_ARG, "%s: tensors must start on 16 bytes", fn);
+  tpf::xattn_plan(a);
+  const int64_t floats = tpf::xattn_part_floats(a);
+  if (floats && (!workspace || workspace_bytes < floats * 4))
+    return tpf::set_error(TPF_ERR_ARG, "%s: workspace too small", fn);
+  a.q = (const tpf::u16*)q; a.k = (const tpf::u16*)k; a.v = (const tpf::u16*)v;
+  a.mask = mask; a.out = (tpf::u16*)out; a.lse = lse;
+  a.part_o = (float*)workspace;
+  a.part_ml = floats ? a.part_o + (int64_t)a.B * a.Hk * a.splits * a.R * a.D : nullptr;
+  if (shape->dtype == TPF_F16) tpf::xattn_forward<true>(a, (hipStream_t)stream);
+  else tpf::xattn_forward<false>(a, (hipStream_t)stream);
+  return tpf::check_launch(fn);
+}

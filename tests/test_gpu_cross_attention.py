@@ -1,0 +1,390 @@
+"""Cross attention against the formulas in 64 bits.
+
+Tolerances count roundings.  With u = finfo(type).eps / 2: the probabilities enter
+the second product rounded (u each), outputs are rounded once (u), and the scores
+carry D + 4 roundings of 32 bits, ds = (D + 4) 2^-24 scale sum |q||k|, which a
+softmax turns into a relative error of at most 2 ds (numerator and sum); the
+exponential and the sums add 2^-20 and (Nk / 32 + 64) 2^-24.  FP16 probabilities
+below 2^-14 are subnormal: 2^-25 each, the largest being at least 1.
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _make(dev, B, H, Hk, Nq, Nk, D, dtype=torch.bfloat16, layout="head", seed=0, qscale=1.5):
+    g = torch.Generator().manual_seed(seed)
+
+    def heads(h, n, scale=1.0):
+        if layout == "seq":
+            t = torch.randn(B, n, h, D, generator=g).mul(scale).to(dtype).to(dev)
+            return t.transpose(1, 2)
+        if layout == "fused":  # a slice of a wider projection
+            t = torch.randn(B, n, h, 2 * D, generator=g).mul(scale).to(dtype).to(dev)
+            return t[..., D:].transpose(1, 2)
+        return torch.randn(B, h, n, D, generator=g).mul(scale).to(dtype).to(dev)
+
+    return heads(H, Nq, qscale), heads(Hk, Nk), heads(Hk, Nk)
+
+
+def _mask(dev, kind, B, Nk, seed=0):
+    g = torch.Generator().manual_seed(100 + seed)
+    if kind == "none":
+        return None
+    if kind == "tail":
+        live = Nk - torch.randint(0, Nk // 2 + 1, (B, 1), generator=g)
+        return (torch.arange(Nk) < live).to(dev)
+    if kind == "random":
+        return (torch.rand(B, Nk, generator=g) < 0.4).to(dev)
+    if kind == "empty":
+        m = torch.rand(B, Nk, generator=g) < 0.7
+        m[0] = False
+        return m.to(dev)
+    if kind == "add":
+        m = torch.randn(B, Nk, generator=g)
+        m[torch.rand(B, Nk, generator=g) < 0.3] = float("-inf")
+        return m.to(dev)
+    if kind == "add_empty":
+        m = torch.randn(B, Nk, generator=g)
+        m[0] = float("-inf")
+        return m.to(dev)
+    raise AssertionError(kind)
+
+
+def _reference(q, k, v, mask, scale, dout=None):
+    """Outputs, their error bounds, and the same of the gradients, in 64 bits."""
+    dtype = q.dtype
+    u = torch.finfo(dtype).eps / 2
+    sub = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    B, H, Nq, D = q.shape
+    Hk, Nk = k.shape[1:3]
+    G = H // Hk
+    q, k, v = (t.detach().double().cpu() for t in (q, k, v))
+    live = torch.ones(B, Nk, dtype=torch.bool)
+    add = torch.zeros(B, Nk, dtype=torch.float64)
+    if mask is not None:
+        mask = mask.cpu()
+        if mask.dtype == torch.bool:
+            live = mask.expand(B, Nk)
+        else:
+            add = mask.double().expand(B, Nk)
+            live = ~torch.isneginf(add)
+    k = torch.where(live[:, None, :, None], k, 0.0)
+    v = torch.where(live[:, None, :, None], v, 0.0)
+    ke, ve = (t.repeat_interleave(G, 1) for t in (k, v))
+    s = scale * q @ ke.transpose(-1, -2) + torch.where(live, add, 0.0)[:, None, None, :]
+    s = s.masked_fill(~live[:, None, None, :], float("-inf"))
+    top = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(torch.isinf(top), 0.0, top))
+    total = p.sum(-1, keepdim=True)
+    p = p / torch.where(total == 0, 1.0, total)
+    o = p @ ve
+    ds_ = (D + 4) * 2.0 ** -24 * (scale * (q.abs() @ ke.abs().transpose(-1, -2))).amax(-1, keepdim=True)
+    ds_ = ds_ + 2.0 ** -22 * torch.where(live, add, 0.0).abs().amax(-1)[:, None, None, None]
+    rel = 2 * ds_ + 2.0 ** -20 + (Nk / 32 + 64) * 2.0 ** -24
+    eo = u * o.abs() + (u + rel) * (p @ ve.abs()) * (1 + u) + sub * ve.abs().sum(-2, keepdim=True) + 2 * sub
+    outs, errs = [o.transpose(1, 2)], [eo.transpose(1, 2)]
+    if dout is None:
+        return outs, errs
+    do = dout.detach().double().cpu().transpose(1, 2)
+    dp = do @ ve.transpose(-1, -2)
+    delta = (do * o).sum(-1, keepdim=True)
+    edelta = (do.abs() * eo).sum(-1, keepdim=True) + D * 2.0 ** -24 * (do.abs() * o.abs()).sum(-1, keepdim=True)
+    edp = (D + 4) * 2.0 ** -24 * (do.abs() @ ve.abs().transpose(-1, -2))
+    ds = p * (dp - delta)
+    eds = (u + rel) * ds.abs() * (1 + u) + p * (edelta + edp) * (1 + u + rel)
+    sums = (G * Nq / 16 + Nk / 16 + 64) * 2.0 ** -24
+
+    def group(t):  # sums over the query heads of a kv head
+        return t.reshape(B, Hk, G, Nk, D).sum(2)
+
+    dq, dk = scale * ds @ ke, group(scale * ds.transpose(-1, -2) @ q)
+    dv = group(p.transpose(-1, -2) @ do)
+    edq = u * dq.abs() + scale * ((eds + sums * ds.abs()) @ ke.abs()) * (1 + u)
+    edk = u * dk.abs() + group(scale * (eds + sums * ds.abs()).transpose(-1, -2) @ q.abs()) * (1 + u)
+    edv = u * dv.abs() + group(((u + rel + sums) * p).transpose(-1, -2) @ do.abs()) * (1 + u)
+    return outs + [dq, dk, dv], errs + [edq, edk, edv]
+
+
+def _check(got, want, tol, names=("out", "dq", "dk", "dv")):
+    for g, w, t, name in zip(got, want, tol, names):
+        g = g.detach().double().cpu()
+        assert g.shape == w.shape, name
+        over = ((g - w).abs() - t - 1e-30).max().item()
+        assert over <= 0, f"{name}: {over:.3e} over the bound"
+
+
+FORWARD = [
+    # B, H, Hk, Nq, Nk, D, type, layout, mask
+    (1, 1, 1, 1, 1, 8, "bf16", "head", "none"),
+    (2, 8, 8, 1, 77, 64, "bf16", "head", "none"),
+    (3, 8, 2, 1, 1000, 128, "bf16", "seq", "tail"),
+    (2, 8, 1, 1, 4099, 128, "fp16", "fused", "random"),
+    (2, 32, 1, 2, 513, 96, "bf16", "head", "empty"),
+    (1, 4, 4, 65, 33, 32, "bf16", "head", "none"),
+    (2, 4, 2, 100, 200, 64, "fp16", "seq", "add"),
+    (2, 2, 1, 129, 64, 40, "bf16", "fused", "random"),
+    (1, 3, 3, 300, 129, 80, "bf16", "seq", "none"),
+    (2, 6, 2, 257, 500, 128, "bf16", "head", "add_empty"),
+    (2, 2, 2, 70, 63, 20, "bf16", "head", "tail"),
+    (1, 1, 1, 64, 2500, 72, "fp16", "head", "none"),
+    (1, 2, 1, 130, 6000, 128, "bf16", "head", "tail"),
+]
+_T = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+@pytest.mark.parametrize("case", FORWARD, ids=str)
+def test_forward(gpu, case):
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    B, H, Hk, Nq, Nk, D, t, layout, mk = case
+    q, k, v = _make(gpu, B, H, Hk, Nq, Nk, D, _T[t], layout)
+    mask = _mask(gpu, mk, B, Nk)
+    want, tol = _reference(q, k, v, mask, 1 / math.sqrt(D))
+    with torch.no_grad():
+        out = cross_attention(q, k, v, mask)
+    assert out.shape == (B, Nq, H, D) and out.is_contiguous()
+    _check([out], want, tol)
+    if mk in ("empty", "add_empty"):
+        assert torch.equal(out[0], torch.zeros_like(out[0]))
+
+
+BACKWARD = [
+    # B, H, Hk, Nq, Nk, D, layout, mask
+    (1, 1, 1, 1, 1, 8, "head", "none"),
+    (2, 4, 2, 1, 65, 64, "seq", "tail"),
+    (2, 4, 4, 33, 100, 32, "head", "random"),
+    (2, 8, 2, 129, 257, 64, "fused", "empty"),
+    (3, 4, 1, 67, 190, 80, "seq", "add_empty"),
+    (1, 2, 2, 130, 64, 96, "head", "none"),
+    (2, 4, 2, 200, 333, 128, "seq", "tail"),
+    (1, 8, 1, 300, 1500, 128, "head", "add"),
+    (1, 2, 1, 16, 3001, 40, "head", "random"),
+    (1, 1, 1, 1500, 65, 20, "seq", "none"),
+]
+
+
+@pytest.mark.parametrize("case", BACKWARD, ids=str)
+def test_backward(gpu, case):
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    B, H, Hk, Nq, Nk, D, layout, mk = case
+    q, k, v = (t.requires_grad_(True) for t in _make(gpu, B, H, Hk, Nq, Nk, D, layout=layout, seed=3))
+    mask = _mask(gpu, mk, B, Nk, 3)
+    dout = torch.randn(B, Nq, H, D, generator=torch.Generator().manual_seed(9)).bfloat16().to(gpu)
+    want, tol = _reference(q, k, v, mask, 1 / math.sqrt(D), dout)
+    out = cross_attention(q, k, v, mask)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    _check([out, *grads], want, tol)
+    again = torch.autograd.grad(cross_attention(q, k, v, mask), (q, k, v), dout)
+    for a, b in zip(grads, again):
+        assert torch.equal(a, b)
+
+
+def test_gradients_against_differences(gpu):
+    """Directional differences of the 64-bit formula at the BF16 operands: the
+    gradient's own roundings (2^-9 relative, a few of them) bound the deviation."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = (t.requires_grad_(True) for t in _make(gpu, 1, 2, 1, 40, 50, 64, seed=5))
+    mask = _mask(gpu, "tail", 1, 50, 5)
+    dout = torch.randn(1, 40, 2, 64, generator=torch.Generator().manual_seed(2)).bfloat16().to(gpu)
+    grads = torch.autograd.grad(cross_attention(q, k, v, mask), (q, k, v), dout)
+    base = [t.detach().double().cpu() for t in (q, k, v)]
+
+    def loss(ops):
+        return (_reference(*ops, mask, 1 / 8.0)[0][0] * dout.double().cpu()).sum().item()
+
+    for n in range(3):
+        g = grads[n].double().cpu()
+        step = g / g.norm()
+        h = 1e-5
+        ops = [list(base), list(base)]
+        ops[0][n], ops[1][n] = base[n] + h * step, base[n] - h * step
+        slope = (loss(ops[0]) - loss(ops[1])) / (2 * h)
+        assert abs(slope - g.norm().item()) <= 2.0 ** -7 * g.norm().item()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("Nq,D", [(1, 128), (70, 64), (200, 128)])
+def test_dropped_states_are_never_used(gpu, bad, Nq, D):
+    """Whatever K and V hold at dropped states, results are those of zeros there."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 2, 4, 2, Nq, 150, D, seed=7)
+    for mask in (_mask(gpu, "random", 2, 150, 7), _mask(gpu, "add_empty", 2, 150, 7)):
+        dead = (~mask if mask.dtype == torch.bool else torch.isneginf(mask))[:, None, :, None]
+        runs = []
+        for fill in (0.0, bad):
+            ops = [t.detach().clone().requires_grad_(True)
+                   for t in (q, k.masked_fill(dead, fill), v.masked_fill(dead, fill))]
+            out = cross_attention(*ops, mask)
+            runs.append([out, *torch.autograd.grad(out, ops, torch.ones_like(out))])
+        for a, b in zip(*runs):
+            assert torch.isfinite(b).all() and torch.equal(a, b)
+        assert not runs[1][2][dead.expand_as(k)].any() and not runs[1][3][dead.expand_as(v)].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Nq", [1, 100])
+def test_lowest_finite_mask(gpu, dtype, Nq):
+    """A row whose states all carry the type's lowest value has live states: the
+    scores vanish beside it, the row is their mean (as in 32-bit arithmetic) for
+    the 32-bit range, and it drops out beside states without it."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 2, 2, 2, Nq, 130, 64, seed=8)
+    low = torch.finfo(dtype).min
+    mask = torch.zeros(2, 130, dtype=dtype, device=gpu)
+    mask[0, 40:] = low
+    mask[1] = low
+    with torch.no_grad():
+        out = cross_attention(q, k, v, mask)
+        part = cross_attention(q[:1], k[:1, :, :40], v[:1, :, :40])
+    assert torch.equal(out[:1], part) or (out[:1].float() - part.float()).abs().max() <= 2.0 ** -7
+    if dtype != torch.float16:
+        mean = v[1].double().mean(-2)  # [H, D]
+        u = 2.0 ** -8
+        bound = 2 * u * v[1].double().abs().mean(-2) + 1e-6
+        assert ((out[1].double() - mean).abs() <= bound).all()
+    assert torch.isfinite(out).all()
+
+
+def test_masks_that_broadcast(gpu):
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 6, 2, 1, 70, 90, 32, seed=4)
+    q, k, v = (t.reshape(2, 3, *t.shape[1:]) for t in (q, k, v))
+    with torch.no_grad():
+        for m in (_mask(gpu, "random", 1, 90)[0], _mask(gpu, "random", 3, 90),
+                  _mask(gpu, "random", 2, 90)[:, None], _mask(gpu, "add", 1, 90)[0].bfloat16(),
+                  _mask(gpu, "random", 90, 6).t()[:3]):
+            full = m.expand(2, 3, 90).contiguous()
+            assert torch.equal(cross_attention(q, k, v, m), cross_attention(q, k, v, full))
+
+
+def test_broadcast_and_offset_operands(gpu):
+    """Expanded operands sum their gradients, storage off the 16 bytes is copied."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 1, 4, 2, 33, 70, 64, seed=6)
+    dout = torch.randn(3, 33, 4, 64, generator=torch.Generator().manual_seed(1)).bfloat16().to(gpu)
+    ks, vs = k.clone().requires_grad_(True), v.clone().requires_grad_(True)
+    q3 = q.repeat(3, 1, 1, 1)
+    out = cross_attention(q3, ks.expand(3, -1, -1, -1), vs.expand(3, -1, -1, -1))
+    got = torch.autograd.grad(out, (ks, vs), dout)
+    k3, v3 = (t.repeat(3, 1, 1, 1).requires_grad_(True) for t in (k, v))
+    out3 = cross_attention(q3, k3, v3)
+    want = torch.autograd.grad(out3, (k3, v3), dout)
+    assert torch.equal(out, out3)
+    for g, w in zip(got, want):
+        full = w.double().sum(0, keepdim=True)
+        # The three terms are added in BF16: two roundings of partial sums.
+        assert ((g.double() - full).abs() <= 2 * 2.0 ** -8 * w.double().abs().sum(0)).all()
+    flat = torch.zeros(k.numel() + 8, device=gpu, dtype=k.dtype)
+    for off in (1, 3, 4):
+        shifted = flat[off:off + k.numel()].view(k.shape)
+        shifted.copy_(k)
+        with torch.no_grad():
+            assert torch.equal(cross_attention(q, shifted, v), cross_attention(q, k, v))
+    wide = torch.zeros(1, 2, 70, 67, device=gpu, dtype=k.dtype)  # odd state stride
+    wide[..., :64] = k
+    with torch.no_grad():
+        assert torch.equal(cross_attention(q, wide[..., :64], v), cross_attention(q, k, v))
+
+
+@pytest.mark.parametrize("Nq,Nk", [(0, 5), (5, 0), (0, 0)])
+def test_empty_axes(gpu, Nq, Nk):
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q = torch.full((2, 4, Nq, 64), float("nan"), device=gpu, dtype=torch.bfloat16, requires_grad=True)
+    k = torch.ones(2, 2, Nk, 64, device=gpu, dtype=torch.bfloat16, requires_grad=True)
+    out = cross_attention(q, k, k)
+    assert out.shape == (2, Nq, 4, 64) and not out.any()
+    out.sum().backward()
+    assert not q.grad.any() and not k.grad.any()
+
+
+def test_long_cache_offsets(gpu):
+    """A cache whose byte offsets pass 32 bits: sequence-major states 2^21 apart."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    Nk, stride = 1500, 1 << 21  # 6.3 GB
+    base = torch.zeros(Nk * stride, device=gpu, dtype=torch.bfloat16)
+    k = base.as_strided((1, 1, Nk, 64), (8, 8, stride, 1), 0)
+    v = base.as_strided((1, 1, Nk, 64), (8, 8, stride, 1), 128)
+    g = torch.Generator().manual_seed(0)
+    k.copy_(torch.randn(1, 1, Nk, 64, generator=g).bfloat16())
+    v.copy_(torch.randn(1, 1, Nk, 64, generator=g).bfloat16())
+    for Nq in (1, 100):
+        q = torch.randn(1, 1, Nq, 64, generator=g).bfloat16().to(gpu)
+        with torch.no_grad():
+            assert torch.equal(cross_attention(q, k, v), cross_attention(q, k.contiguous(),
+                                                                         v.contiguous()))
+
+
+def test_another_stream_and_graph(gpu):
+    """Forward and backward on a side stream, and captured and replayed."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 2, 8, 2, 100, 700, 64, seed=11)
+    mask = _mask(gpu, "tail", 2, 700, 11)
+    dout = torch.randn(2, 100, 8, 64, generator=torch.Generator().manual_seed(1)).bfloat16().to(gpu)
+
+    def step(ops):
+        leaves = [t.detach().requires_grad_(True) for t in ops]
+        out = cross_attention(*leaves, mask)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    want = step((q, k, v))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step((q, k, v))
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    ops = [t.clone() for t in (q, k, v)]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = step(ops)
+    for seed in range(4):
+        new = _make(gpu, 2, 8, 2, 100, 700, 64, seed=20 + seed)
+        for t, n in zip(ops, new):
+            t.copy_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step(new)):
+            assert torch.equal(a, b)
+
+
+def test_refusals(gpu):
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    def ops(B=1, H=2, Hk=2, Nq=4, Nk=8, D=64, dtype=torch.bfloat16):
+        return [torch.zeros(B, h, n, D, device=gpu, dtype=dtype) for h, n in ((H, Nq), (Hk, Nk), (Hk, Nk))]
+
+    for args, match in (
+            ((*ops(dtype=torch.float32), None), "BF16 or FP16"),
+            ((*ops(D=136), None), "D<=128"),
+            ((*ops(H=3), None), "multiple"),
+            ((ops()[0], ops()[1], ops(Nk=9)[2], None), "one shape"),
+            ((ops(B=2)[0], *ops()[1:], None), "batch prefix"),
+            ((*ops(), torch.zeros(7, device=gpu)), "broadcast"),
+            ((*ops(), torch.zeros(8, device=gpu, dtype=torch.int32)), "boolean"),
+            ((*ops(), torch.zeros(8)), "one device"),
+            ((*ops(), torch.zeros(8, device=gpu, requires_grad=True)), "must not require"),
+            ((*ops(), None, 0.0), "scale"),
+            ((*ops(), None, float("inf")), "scale")):
+        with pytest.raises(ValueError, match=match):
+            cross_attention(*args)
+    half = [t.requires_grad_(True) for t in ops(dtype=torch.float16)]
+    with pytest.raises(ValueError, match="gradients need BF16"):
+        cross_attention(*half)
+    with torch.no_grad():
+        cross_attention(*half)
