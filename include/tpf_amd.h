@@ -508,6 +508,51 @@ int tpf_attn_pair_rows_forward_bf16(const void* qkv, const void* rest, int64_t r
                                     int64_t workspace_bytes, int64_t B, int64_t O, int64_t N,
                                     int64_t H, int64_t D, double scale, void* stream);
 
+/* Element types of the entry points that take more than one. */
+enum { TPF_BF16 = 0, TPF_F16 = 1, TPF_F32 = 2 };
+
+/* ------------------------------------------------------------------------
+ * Layer norm over rows [R, C] of any channel count, with 32-bit statistics.
+ *
+ * x has x_ld elements between rows, channels contiguous, aligned to the element;
+ * y, dy [R, C] contiguous; dx at dx_ld.  weight, bias [C] of type param_dtype, null
+ * for 1 and 0.  mean, rstd: f32 [R], null when not wanted.  codes [R, P] and
+ * scales [R, P / 32] (P: C rounded up to a multiple of 32; codes on 8 bytes): the
+ * normalised rows in 8 bits, written by the forward and read by the backward in
+ * the place of x and mean; null when not wanted.  dweight, dbias [C] in
+ * param_dtype, null when not wanted (with both null no workspace is needed).
+ * ---------------------------------------------------------------------- */
+int tpf_norm_forward(const void* x, int64_t x_ld, int64_t R, int64_t C, int64_t dtype,
+                     const void* weight, const void* bias, int64_t param_dtype, double eps,
+                     void* y, float* mean, float* rstd, void* codes, void* scales, void* stream);
+int64_t tpf_norm_backward_workspace_bytes(int64_t R, int64_t C);
+int tpf_norm_backward(const void* dy, const void* x, int64_t x_ld, const void* codes,
+                      const void* scales, const float* mean, const float* rstd, int64_t R,
+                      int64_t C, int64_t dtype, const void* weight, int64_t param_dtype, void* dx,
+                      int64_t dx_ld, void* dweight, void* dbias, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Activations in 8 bits.  32 channels of a row share 2^k, k the smallest whole
+ * number >= -120 with round(max / 2^k) <= 127, at most 121 (9 for FP16 rows),
+ * where larger quotients are held as 127: codes uint8 [R, P] (128 +
+ * round(x / 2^k), ties to even; 128 past C), scales uint8 [R, P / 32] (k + 127; 255
+ * for a block with an infinity or NaN, which decodes to NaN), P being C rounded
+ * up to a multiple of 32.  The plain side has ld elements between rows.
+ *
+ * tpf_wgrad_act8: dw [N, K] = dy^T x of BF16 rows dy [R, N] (ld_dy between rows)
+ * and x [R, K] in 8 bits, BF16 products summed in f32, in BF16 or FP32; N and K
+ * multiples of 8, tensors on 16 bytes.
+ * ---------------------------------------------------------------------- */
+int tpf_act8_pack(const void* x, int64_t ld, int64_t R, int64_t C, int64_t dtype, void* codes,
+                  void* scales, void* stream);
+int tpf_act8_unpack(const void* codes, const void* scales, int64_t R, int64_t C, void* x,
+                    int64_t ld, int64_t dtype, void* stream);
+int64_t tpf_wgrad_act8_workspace_bytes(int64_t R, int64_t N, int64_t K, int64_t ld_dy);
+int tpf_wgrad_act8(const void* dy, int64_t ld_dy, const void* codes, const void* scales,
+                   int64_t R, int64_t N, int64_t K, void* dw, int64_t dw_dtype, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Cross attention to states of another length: out = softmax(scale q k^T +
  * mask) v, forward and backward.
@@ -524,7 +569,6 @@ int tpf_attn_pair_rows_forward_bf16(const void* qkv, const void* rest, int64_t r
  * statistics for the backward; null when none follows.
  * The forward serves BF16 and FP16, the backward BF16.
  * ---------------------------------------------------------------------- */
-enum { TPF_BF16 = 0, TPF_F16 = 1, TPF_F32 = 2 };
 enum { TPF_MASK_NONE = 0, TPF_MASK_BYTES = 1, TPF_MASK_F32 = 2 };
 typedef struct tpf_xattn_shape {
   int64_t B, H, Hk, Nq, Nk, D;

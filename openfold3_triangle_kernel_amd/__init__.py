@@ -61,9 +61,18 @@ from .routing import (  # noqa: E402
 __all__ += ["set_tpf_bf16_cast_for_fp32_training", "set_turbopairformer_strict",
             "stock_invocation_count", "turbopairformer_strict_enabled"]
 
-from .layernorm import layer_norm_bf16  # noqa: E402
+from .layernorm import layer_norm, layer_norm_bf16  # noqa: E402
 
-__all__ += ["layer_norm_bf16"]
+__all__ += ["layer_norm", "layer_norm_bf16"]
+
+from .activations import (  # noqa: E402
+    CompressedActivation,
+    compress_activation,
+    decompress_activation,
+    linear,
+)
+
+__all__ += ["CompressedActivation", "compress_activation", "decompress_activation", "linear"]
 
 from .cross_attention import cross_attention  # noqa: E402
 

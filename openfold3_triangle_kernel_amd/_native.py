@@ -145,6 +145,16 @@ SIGNATURES: dict[str, tuple] = {
         _I32,
         [_P] * 21 + [_I32, _I64, _I64, _I64] + [_P] * 10 + [_I64, _P],
     ),
+    "tpf_norm_forward": (
+        _I32, [_P] + [_I64] * 4 + [_P, _P, _I64, _F64] + [_P] * 6),
+    "tpf_norm_backward_workspace_bytes": (_I64, [_I64, _I64]),
+    "tpf_norm_backward": (
+        _I32, [_P, _P, _I64] + [_P] * 4 + [_I64] * 3 + [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P]),
+    "tpf_act8_pack": (_I32, [_P] + [_I64] * 4 + [_P] * 3),
+    "tpf_act8_unpack": (_I32, [_P, _P, _I64, _I64, _P, _I64, _I64, _P]),
+    "tpf_wgrad_act8_workspace_bytes": (_I64, [_I64] * 4),
+    "tpf_wgrad_act8": (
+        _I32, [_P, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
     "tpf_xattn_forward_workspace_bytes": (_I64, [_P]),
     "tpf_xattn_forward": (_I32, [_P] * 7 + [_I64, _P, _F64, _P]),
     "tpf_xattn_backward_workspace_bytes": (_I64, [_P]),

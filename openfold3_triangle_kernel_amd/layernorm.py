@@ -1,4 +1,11 @@
-"""BF16 LayerNorm with FP32 statistics over pair rows (``csrc/layernorm.hip``).
+"""LayerNorm with FP32 statistics.
+
+``layer_norm`` (``csrc/norm.hip``): BF16, FP16 or FP32 rows of any channel count,
+parameters of any of these types, its backward from the rows or from their
+normalised values in 8 bits.
+
+``layer_norm_bf16`` (``csrc/layernorm.hip``): BF16 pair rows read through the strides
+of a pair grid.
 
 Replaces the torch LayerNorm that OpenFold3's pair-stack modules apply to
 their input (``openfold3/core/model/primitives/normalization.py:54-78``:
@@ -12,8 +19,10 @@ dgamma / dbeta from fixed-order partial sums (deterministic).
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
+from .activations import _DTYPES, as_rows, check_rows, code_buffers
 from .attention import _device_ctx
 
 
@@ -114,4 +123,102 @@ def layer_norm_bf16(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Te
     return _LayerNormBf16.apply(x, weight, bias, eps)
 
 
-__all__ = ["layer_norm_bf16"]
+def _norm_forward(x2, w, b, eps, save):
+    """(y, mean, rstd, codes, scales) of rows x2; what ``save`` does not ask for is None."""
+    R, C = x2.shape
+    dev = x2.device
+    y = torch.empty((R, C), device=dev, dtype=x2.dtype)
+    mean = torch.empty(R, device=dev, dtype=torch.float32) if save == "full" else None
+    rstd = torch.empty(R, device=dev, dtype=torch.float32) if save else None
+    codes, scales = code_buffers(R, C, dev) if save == "int8" else (None, None)
+    p = w if w is not None else b
+    ptr = _native.ptr
+    with _device_ctx(dev):
+        _native.call("tpf_norm_forward", x2.data_ptr(), x2.stride(0) if R > 1 else C, R, C,
+                     _DTYPES[x2.dtype], ptr(w), ptr(b), 0 if p is None else _DTYPES[p.dtype], eps,
+                     y.data_ptr(), ptr(mean), ptr(rstd), ptr(codes), ptr(scales),
+                     _native.stream_of(x2))
+    return y, mean, rstd, codes, scales
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2, weight, bias, w, b, eps, save):
+        y, mean, rstd, codes, scales = _norm_forward(x2, w, b, eps, save)
+        ctx.save_for_backward(x2 if save == "full" else None, mean, rstd, codes, scales, w)
+        ctx.args = (x2.dtype, x2.shape, None if weight is None else weight.dtype,
+                    None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x2, mean, rstd, codes, scales, w = ctx.saved_tensors
+        dtype, (R, C), wtype, btype = ctx.args
+        dev = dy.device
+        dy = dy.to(dtype).contiguous()
+        dx = torch.empty((R, C), device=dev, dtype=dtype)
+        # The fold writes the gradients in the parameters' type where both share one.
+        types = {t for t, n in ((wtype, 1), (btype, 2)) if t is not None and ctx.needs_input_grad[n]}
+        ptype = types.pop() if len(types) == 1 else torch.float32
+        dw = torch.empty(C, device=dev, dtype=ptype) if ctx.needs_input_grad[1] else None
+        db = torch.empty(C, device=dev, dtype=ptype) if ctx.needs_input_grad[2] else None
+        ws, ws_bytes = None, 0
+        if w is not None and w.dtype != ptype:
+            w = w.to(ptype)
+        if dw is not None or db is not None:
+            ws_bytes = int(_native.query("tpf_norm_backward_workspace_bytes", R, C))
+            ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        ptr = _native.ptr
+        with _device_ctx(dev):
+            _native.call("tpf_norm_backward", dy.data_ptr(), ptr(x2),
+                         0 if x2 is None else x2.stride(0) if R > 1 else C, ptr(codes), ptr(scales),
+                         ptr(mean), rstd.data_ptr(), R, C, _DTYPES[dtype], ptr(w), _DTYPES[ptype],
+                         dx.data_ptr(), C, ptr(dw), ptr(db), ptr(ws), ws_bytes,
+                         _native.stream_of(dy))
+        return (dx, None if dw is None else dw.to(wtype), None if db is None else db.to(btype), None,
+                None, None, None)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-5,
+               save: str = "full") -> torch.Tensor:
+    """LayerNorm over the last dimension of ``x`` [*, C] (BF16, FP16 or FP32, any C),
+    with statistics and affine parameters in 32 bits; contiguous, of ``x``'s type.
+
+    ``weight`` and ``bias`` [C] are BF16, FP16 or FP32 and may be None.  The backward
+    reads ``x`` (``save="full"``) or, with ``save="int8"``, the normalised rows kept in 8
+    bits a value (``compress_activation``'s form): its results are then the
+    gradient's formula at the decoded values, and ``x`` is not kept.
+    """
+    if save not in ("full", "int8"):
+        raise ValueError('save must be "full" or "int8"')
+    check_rows("layer_norm", x)
+    C = x.shape[-1]
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if not isinstance(p, torch.Tensor) or tuple(p.shape) != (C,):
+            raise ValueError(f"{name} must have shape ({C},)")
+        if p.dtype not in _DTYPES or p.device != x.device:
+            raise ValueError(f"{name} must be BF16, FP16 or FP32 on the input's device")
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    if x.numel() == 0:
+        out = x
+        for p, op in ((weight, torch.mul), (bias, torch.add)):
+            out = out if p is None else op(out, p.to(x.dtype))
+        return out.clone() if out is x else out
+    w, b = (None if p is None else p.detach().contiguous() for p in (weight, bias))
+    if w is not None and b is not None and w.dtype != b.dtype:
+        w, b = w.float(), b.float()
+    grad = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, weight, bias))
+    if grad:
+        y = _LayerNormFn.apply(as_rows(x), weight, bias, w, b, float(eps), save)
+    else:
+        y = _norm_forward(as_rows(x.detach()), w, b, float(eps), None)[0]
+    return y.view(x.shape)
+
+
+__all__ = ["layer_norm", "layer_norm_bf16"]
