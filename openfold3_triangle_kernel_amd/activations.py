@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .attention import _device_supported
+from .attention import _device_supported, _is_gfx950
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # TPF_BF16, TPF_F16, TPF_F32
 _BLOCK = 32
@@ -39,6 +39,12 @@ class CompressedActivation:
     @property
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
+
+
+def host_path(*tensors) -> bool:
+    """Whether a call on these tensors may be tried on the C++ host path."""
+    return (_native.host_eligible(*tensors) and tensors[0].is_cuda
+            and _is_gfx950(tensors[0].device) and _native.host() is not None)
 
 
 def check_rows(what: str, x) -> None:
@@ -182,6 +188,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, save: str = "int8") -> torch.T
     """
     if save not in ("int8", "full"):
         raise ValueError('save must be "int8" or "full"')
+    if save == "int8" and host_path(x, weight):
+        # The common form entirely in C++; None (nothing launched) for any other.
+        out = _native.host().linear(x, weight)
+        if out is not None:
+            return out
     check_rows("linear", x)
     if x.dtype != torch.bfloat16:
         raise ValueError("linear needs a BF16 input")

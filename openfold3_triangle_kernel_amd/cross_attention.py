@@ -20,6 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
+from .activations import host_path
 from .attention import _device_supported
 
 _MAX_HEAD_DIM = 128
@@ -180,6 +181,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     FP16 is for inference.  ``1 <= D <= 128`` (copied to a multiple of 8 where it is
     none).  Other cases raise ``ValueError`` before any launch.
     """
+    if host_path(q, k, v) and (key_mask is None or _native.host_eligible(key_mask)):
+        # The common form entirely in C++; None (nothing launched) for any other.
+        out = _native.host().cross_attention(q, k, v, key_mask, scale)
+        if out is not None:
+            return out
     _check(q, k, v, key_mask, scale)
     head_dim = q.shape[-1]
     if scale is None:

@@ -1,4 +1,4 @@
-// Host path of the two operators for plain eager GPU tensors, in C++.
+// Host path of the operators for plain eager GPU tensors, in C++.
 //
 // The Python facades stay the definition of the operators: they validate,
 // report and handle every form.  A small call is bound by what the host does
@@ -15,6 +15,8 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <atomic>
 #include <cctype>
@@ -355,6 +357,293 @@ std::optional<Tensor> trimul(const Tensor& z, const std::optional<Tensor>& mask_
   return z.dim() == 4 ? out : out.view(z.sizes());
 }
 
+// --------------------------------------------------------- shared by the below
+
+// Gradients asked for with create_graph: as Python's once_differentiable,
+// differentiating them again raises.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list marked;
+  for (const Tensor& g : grads) {
+    Tensor t = g.defined() ? g.detach() : g;
+    if (t.defined()) t.set_requires_grad(true);
+    marked.push_back(t);
+  }
+  auto err = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked with @once_differentiable",
+      (int64_t)marked.size());
+  return (*err)(std::move(marked));
+}
+
+const void* cptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* mptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor bytes(const Tensor& like_, int64_t n) {
+  return n > 0 ? at::empty({n}, like(like_, at::kByte)) : Tensor();
+}
+int64_t type_code(at::ScalarType t) {
+  return t == at::kBFloat16 ? TPF_BF16 : t == at::kHalf ? TPF_F16 : t == at::kFloat ? TPF_F32 : -1;
+}
+
+// ----------------------------------------------------------- cross attention
+
+void strides3(const Tensor& t, int64_t* out) {
+  for (int i = 0; i < 3; ++i) out[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+// q [B, H, Nq, D], k and v [B, Hk, Nk, D] as the kernels read them.
+tpf_xattn_shape xattn_shape(const Tensor& q, const Tensor& k, const Tensor& v, int64_t kind,
+                            int64_t mask_stride) {
+  tpf_xattn_shape s{q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), q.size(3),
+                    type_code(q.scalar_type()), kind, mask_stride, {}, {}, {}};
+  strides3(q, s.q_stride);
+  strides3(k, s.k_stride);
+  strides3(v, s.v_stride);
+  return s;
+}
+
+Tensor xattn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask,
+                     int64_t kind, int64_t mask_stride, double scale, Tensor* lse) {
+  const tpf_xattn_shape s = xattn_shape(q, k, v, kind, mask_stride);
+  Tensor out = at::empty({s.B, s.Nq, s.H, s.D}, q.options());
+  if (lse) *lse = at::empty({kind == TPF_MASK_F32 ? 2 : 1, s.B, s.H, s.Nq}, like(q, at::kFloat));
+  const int64_t n = tpf_xattn_forward_workspace_bytes(&s);
+  const Tensor ws = bytes(q, n);
+  check(tpf_xattn_forward(cptr(q), cptr(k), cptr(v), cptr(mask), out.data_ptr(),
+                          lse ? (float*)lse->data_ptr() : nullptr, mptr(ws), n < 0 ? 0 : n, &s, scale,
+                          stream()),
+        "tpf_xattn_forward");
+  return out;
+}
+
+struct XattnFn : torch::autograd::Function<XattnFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const std::optional<Tensor>& mask_in, int64_t kind, int64_t mask_stride,
+                        double scale) {
+    const Tensor mask = mask_in.value_or(Tensor());
+    Tensor lse;
+    Tensor out = xattn_forward(q, k, v, mask, kind, mask_stride, scale, &lse);
+    ctx->save_for_backward({q, k, v, mask, out, lse});
+    ctx->saved_data["kind"] = kind;
+    ctx->saved_data["stride"] = mask_stride;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &mask = sv[3], &out = sv[4], &lse = sv[5];
+    const tpf_xattn_shape s = xattn_shape(q, k, v, ctx->saved_data["kind"].toInt(),
+                                          ctx->saved_data["stride"].toInt());
+    const Tensor dout = kernel_grad(grads[0]);
+    Tensor d[3] = {at::empty_like(q), at::empty_like(k), at::empty_like(v)};
+    int64_t gs[9];
+    for (int i = 0; i < 3; ++i) strides3(d[i], gs + 3 * i);
+    const int64_t n = tpf_xattn_backward_workspace_bytes(&s);
+    const Tensor ws = bytes(q, n < 16 ? 16 : n);
+    check(tpf_xattn_backward_bf16(cptr(q), cptr(k), cptr(v), cptr(mask), cptr(out), cptr(dout),
+                                  (const float*)cptr(lse), mptr(d[0]), mptr(d[1]), mptr(d[2]),
+                                  mptr(ws), n, &s, gs, ctx->saved_data["scale"].toDouble(), stream()),
+          "tpf_xattn_backward_bf16");
+    return once({d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+bool xattn_operand(const Tensor& t) {
+  if (t.stride(3) != 1 || !aligned16(t)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && (t.stride(i) % 8 || t.stride(i) >= (int64_t(1) << 23))) return false;
+  return true;
+}
+
+std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                                      const std::optional<Tensor>& mask_in,
+                                      std::optional<double> scale_in) {
+  if (transforms_active() || !q.is_cuda()) return std::nullopt;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  for (const Tensor* t : {&q, &k, &v})
+    if (!plain(*t, dev) || t->dim() != 4 || t->numel() == 0 || t->scalar_type() != q.scalar_type())
+      return std::nullopt;
+  const auto type = q.scalar_type();
+  const bool grad = at::GradMode::is_enabled() &&
+                    (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  if (type != at::kBFloat16 && (type != at::kHalf || grad)) return std::nullopt;
+  const int64_t B = q.size(0), D = q.size(3), Nk = k.size(2);
+  if (k.sizes() != v.sizes() || k.size(0) != B || k.size(3) != D || D % 8 || D > 128 ||
+      q.size(1) % k.size(1))
+    return std::nullopt;
+  for (const Tensor* t : {&q, &k, &v})
+    if (!xattn_operand(*t)) return std::nullopt;
+  const double scale = scale_in ? *scale_in : 1.0 / std::sqrt((double)D);
+  if (!(scale > 0.0 && scale < 1e30)) return std::nullopt;
+  Tensor mask;
+  int64_t kind = TPF_MASK_NONE, mask_stride = 0;
+  if (mask_in) {
+    mask = *mask_in;
+    const auto mt = mask.scalar_type();
+    if (!plain(mask, dev) || mask.requires_grad() || (mt != at::kBool && mt != at::kFloat) ||
+        !mask.is_contiguous() || mask.dim() < 1 || mask.dim() > 2 || mask.size(-1) != Nk ||
+        (mask.dim() == 2 && mask.size(0) != B && mask.size(0) != 1))
+      return std::nullopt;
+    kind = mt == at::kBool ? TPF_MASK_BYTES : TPF_MASK_F32;
+    mask_stride = mask.dim() == 2 && mask.size(0) > 1 ? Nk : 0;
+  }
+  if (grad) return XattnFn::apply(q, k, v, mask_in, kind, mask_stride, scale);
+  return xattn_forward(q, k, v, mask, kind, mask_stride, scale, nullptr);
+}
+
+// ---------------------------------------------------------------- layer norm
+
+// Rows x2 [R, C]; what a backward needs of `keep` (0 nothing, 1 the rows, 2 the
+// 8-bit form): mean, rstd, codes, scales.
+Tensor norm_forward(const Tensor& x2, const Tensor& w, const Tensor& b, double eps, int keep,
+                    Tensor* st) {
+  const int64_t R = x2.size(0), C = x2.size(1), blocks = (C + 31) / 32;
+  Tensor y = at::empty({R, C}, x2.options());
+  if (keep == 1) st[0] = at::empty({R}, like(x2, at::kFloat));
+  if (keep) st[1] = at::empty({R}, like(x2, at::kFloat));
+  if (keep == 2) {
+    st[2] = at::empty({R, blocks * 32}, like(x2, at::kByte));
+    st[3] = at::empty({R, blocks}, like(x2, at::kByte));
+  }
+  const Tensor& p = w.defined() ? w : b;
+  check(tpf_norm_forward(cptr(x2), R > 1 ? x2.stride(0) : C, R, C, type_code(x2.scalar_type()),
+                         cptr(w), cptr(b), p.defined() ? type_code(p.scalar_type()) : 0, eps,
+                         y.data_ptr(), (float*)mptr(st[0]), (float*)mptr(st[1]), mptr(st[2]),
+                         mptr(st[3]), stream()),
+        "tpf_norm_forward");
+  return y;
+}
+
+struct NormFn : torch::autograd::Function<NormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x2, const std::optional<Tensor>& weight,
+                        const std::optional<Tensor>& bias, double eps, bool int8) {
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    Tensor st[4];
+    Tensor y = norm_forward(x2, w, b, eps, int8 ? 2 : 1, st);
+    ctx->save_for_backward({int8 ? Tensor() : x2, st[0], st[1], st[2], st[3], w});
+    ctx->saved_data["type"] = (int64_t)x2.scalar_type();
+    ctx->saved_data["ptype"] =
+        (int64_t)(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat);
+    ctx->saved_data["want"] = (int64_t)((w.defined() && w.requires_grad() ? 1 : 0) |
+                                        (b.defined() && b.requires_grad() ? 2 : 0));
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x2 = s[0], &w = s[5];
+    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    const auto ptype = (at::ScalarType)ctx->saved_data["ptype"].toInt();
+    const int64_t want = ctx->saved_data["want"].toInt();
+    const Tensor dy = grads[0].to(type).contiguous();
+    const int64_t R = dy.size(0), C = dy.size(1);
+    Tensor dx = at::empty({R, C}, dy.options()), dw, db, ws;
+    if (want & 1) dw = at::empty({C}, like(dy, ptype));
+    if (want & 2) db = at::empty({C}, like(dy, ptype));
+    const int64_t n = want ? tpf_norm_backward_workspace_bytes(R, C) : 0;
+    if (want) ws = bytes(dy, n);
+    check(tpf_norm_backward(cptr(dy), cptr(x2), x2.defined() && R > 1 ? x2.stride(0) : C, cptr(s[3]),
+                            cptr(s[4]), (const float*)cptr(s[1]), (const float*)cptr(s[2]), R, C,
+                            type_code(type), cptr(w), type_code(ptype), dx.data_ptr(), C, mptr(dw),
+                            mptr(db), mptr(ws), n, stream()),
+          "tpf_norm_backward");
+    return once({dx, dw, db, Tensor(), Tensor()});
+  }
+};
+
+std::optional<Tensor> layer_norm(const Tensor& x, const std::optional<Tensor>& weight,
+                                 const std::optional<Tensor>& bias, double eps, bool int8) {
+  if (transforms_active() || !x.is_cuda()) return std::nullopt;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  if (!plain(x, dev) || x.dim() < 1 || x.numel() == 0 || type_code(x.scalar_type()) < 0 ||
+      x.size(-1) > (1 << 24) || !(eps >= 0.0))
+    return std::nullopt;
+  const bool strided = x.dim() == 2 && x.stride(1) == 1;
+  if (!strided && !x.is_contiguous()) return std::nullopt;
+  const int64_t C = x.size(-1);
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  for (const Tensor* p : {&w, &b})
+    if (p->defined() && (!plain(*p, dev) || p->dim() != 1 || p->size(0) != C || !p->is_contiguous() ||
+                         type_code(p->scalar_type()) < 0))
+      return std::nullopt;
+  if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type()) return std::nullopt;
+  const Tensor x2 = x.dim() == 2 ? x : x.view({-1, C});
+  const bool grad = at::GradMode::is_enabled() &&
+                    (x.requires_grad() || (w.defined() && w.requires_grad()) ||
+                     (b.defined() && b.requires_grad()));
+  Tensor st[4];
+  const Tensor y = grad ? NormFn::apply(x2, weight, bias, eps, int8) : norm_forward(x2, w, b, eps, 0, st);
+  return x.dim() == 2 ? y : y.view(x.sizes());
+}
+
+// -------------------------------------------------------------------- linear
+
+// a [R, K] times b^T (b_kc: b [N, K]) or b [K, N], contiguous BF16.
+Tensor row_gemm(const Tensor& a, const Tensor& b, bool b_kc) {
+  const int64_t R = a.size(0), K = a.size(1), N = b_kc ? b.size(0) : b.size(1);
+  Tensor out = at::empty({R, N}, a.options());
+  check(tpf_gemm_bf16(cptr(a), 1, K, 0, cptr(b), b_kc ? 1 : 0, b.size(1), 0, out.data_ptr(), 0, N, 0,
+                      R, N, K, 1, 1.0, stream()),
+        "tpf_gemm_bf16");
+  return out;
+}
+
+struct LinearFn : torch::autograd::Function<LinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
+    const int64_t R = x.size(0), K = x.size(1), blocks = (K + 31) / 32;
+    Tensor codes, scales;
+    if (w.requires_grad()) {
+      codes = at::empty({R, blocks * 32}, like(x, at::kByte));
+      scales = at::empty({R, blocks}, like(x, at::kByte));
+      check(tpf_act8_pack(cptr(x), K, R, K, TPF_BF16, mptr(codes), mptr(scales), stream()),
+            "tpf_act8_pack");
+    }
+    ctx->save_for_backward({w, codes, scales});
+    ctx->saved_data["dx"] = x.requires_grad();
+    return row_gemm(x, w, true);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor& w = s[0];
+    const Tensor dy = kernel_grad(grads[0]);
+    const int64_t R = dy.size(0), N = w.size(0), K = w.size(1);
+    Tensor dx, dw;
+    if (ctx->saved_data["dx"].toBool()) dx = row_gemm(dy, w, false);
+    if (s[1].defined()) {
+      dw = at::empty({N, K}, w.options());
+      const int64_t n = tpf_wgrad_act8_workspace_bytes(R, N, K, N);
+      const Tensor ws = bytes(dy, n);
+      check(tpf_wgrad_act8(cptr(dy), N, cptr(s[1]), cptr(s[2]), R, N, K, dw.data_ptr(), TPF_BF16,
+                           mptr(ws), n < 0 ? 0 : n, stream()),
+            "tpf_wgrad_act8");
+    }
+    return once({dx, dw});
+  }
+};
+
+// BF16 input and weight, the input kept in 8 bits.
+std::optional<Tensor> linear(const Tensor& x, const Tensor& w) {
+  if (transforms_active() || !x.is_cuda()) return std::nullopt;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  for (const Tensor* t : {&x, &w})
+    if (!plain(*t, dev) || t->scalar_type() != at::kBFloat16 || t->numel() == 0 ||
+        !t->is_contiguous() || !aligned16(*t))
+      return std::nullopt;
+  if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1)) return std::nullopt;
+  const int64_t N = w.size(0), K = w.size(1), R = x.numel() / K, most = (int64_t(1) << 30) - 1;
+  if (N % 8 || K % 8 || R > most / (N > K ? N : K) || N > most / (N > K ? N : K) ||
+      K > most / (N > K ? N : K))
+    return std::nullopt;
+  const Tensor x2 = x.dim() == 2 ? x : x.view({R, K});
+  const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
+  const Tensor y = grad ? LinearFn::apply(x2, w) : row_gemm(x2, w, true);
+  if (x.dim() == 2) return y;
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = N;
+  return y.view(shape);
+}
+
 }  // namespace
 
 // Refuses the import beside another torch or C-ABI library than it was built
@@ -380,5 +669,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return attention(q, k, v, res_mask, pair_bias, backward, shadow);
   });
   m.def("trimul", &trimul, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("cross_attention", &cross_attention, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("layer_norm", &layer_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("linear", &linear, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("set_workspace_budget", [](int64_t bytes) { g_budget.store(bytes); });
 }

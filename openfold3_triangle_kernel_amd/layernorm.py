@@ -22,7 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .activations import _DTYPES, as_rows, check_rows, code_buffers
+from .activations import _DTYPES, as_rows, check_rows, code_buffers, host_path
 from .attention import _device_ctx
 
 
@@ -193,6 +193,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     """
     if save not in ("full", "int8"):
         raise ValueError('save must be "full" or "int8"')
+    if host_path(*(t for t in (x, weight, bias) if t is not None)):
+        # The common form entirely in C++; None (nothing launched) for any other.
+        out = _native.host().layer_norm(x, weight, bias, eps, save == "int8")
+        if out is not None:
+            return out
     check_rows("layer_norm", x)
     C = x.shape[-1]
     for name, p in (("weight", weight), ("bias", bias)):
