@@ -185,13 +185,20 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XAttnGrad ga) {
 
 // dK and dV: four waves of 32 states each pass over tiles of RT rows of Q and
 // dO.  A state's column of the tiles depends on that state alone, so dead
-// states are left to run and their gradients written as 0.
+// states are left to run and their gradients written as 0.  Above 64 channels
+// V stays in LDS (and at 128 the tiles have 32 rows), so that a wave fits 256
+// registers and two run on a SIMD.  A tile inside one query head (all of them when Nq is a
+// multiple of RT) is loaded at fixed lane offsets from its first row; others
+// find each row's address.
 template <int DP, bool ADD>
-__global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void xattn_dkdv_kernel(XAttnGrad ga) {
-  constexpr int RT = 64, TILE = RT * DP, DS = DP / 16, DB = DP / 32, CPR = DP / 8;
+__global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
+  constexpr bool VLDS = DP > 64;
+  constexpr int RT = DP == 128 ? 32 : 64, TILE = RT * DP, DS = DP / 16, DB = DP / 32, CPR = DP / 8;
   constexpr int NI = RT * CPR / 256;
+  static_assert(RT * CPR % 256 == 0, "whole instructions");
   __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
-  __shared__ __attribute__((aligned(1024))) float stats[2][ADD ? 3 : 2][RT];
+  __shared__ __attribute__((aligned(1024))) float stats[2][ADD ? 3 : 2][64];
+  __shared__ __attribute__((aligned(1024))) u16 vs[VLDS ? 128 * DP : 8];
   const XAttnArgs& a = ga.f;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
   const int64_t BH = (int64_t)a.B * a.Hk;
@@ -214,16 +221,21 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void xattn_dkdv_kernel(XAttnG
     live = live && !xa_dead(m);
     add = live ? fmaxf(m * a.inv_scale, a.mask_floor) : 0.f;
   }
-  bf16x8 kf[DS], vf[DS];
+  bf16x8 kf[DS], vf[VLDS ? 1 : DS];
   {
     const u16* kp = a.k + b * a.k_sb + hk * a.k_sh + (int64_t)kc * a.k_sn;
     const u16* vp = a.v + b * a.v_sb + hk * a.v_sh + (int64_t)kc * a.v_sn;
+    const int row = w * 32 + (lane & 31);
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
       const int d = 16 * s + 8 * h;
       const bool in = live && d < a.D;
       kf[s] = in ? *reinterpret_cast<const bf16x8*>(kp + d) : zero8();
-      vf[s] = in ? *reinterpret_cast<const bf16x8*>(vp + d) : zero8();
+      const bf16x8 x = in ? *reinterpret_cast<const bf16x8*>(vp + d) : zero8();
+      if constexpr (VLDS)
+        *reinterpret_cast<bf16x8*>(vs + row * DP + ((2 * s + h) ^ xa_swz<DP>(row)) * 8) = x;
+      else
+        vf[s] = x;
     }
   }
   f32x16 dk[DB], dv[DB];
@@ -233,26 +245,51 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void xattn_dkdv_kernel(XAttnG
     dv[db] = zero16();
   }
 
-  auto issue = [&](int r0, int st) {
+  // Fixed offsets of this lane's rows and chunks in a tile inside one head.
+  const int64_t o_sn = (int64_t)a.H * a.D;
+  uint32_t qo[NI], oo[NI];
 #pragma unroll
-    for (int t = 0; t < NI; ++t) {
-      const int p = 64 * (NI * w + t) + lane, row = p / CPR;
-      const int chunk = (p - row * CPR) ^ xa_swz<DP>(row);
-      const int r = r0 + row;
-      const u16 *qs = (const u16*)kXaNone, *os = (const u16*)kXaNone;
-      if (r < rend && 8 * chunk < a.D) {
-        int g, i;
-        xa_row(a, r, g, i);
-        qs = a.q + b * a.q_sb + (int64_t)(hk * a.G + g) * a.q_sh + (int64_t)i * a.q_sn + 8 * chunk;
-        os = ga.dout + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + 8 * chunk;
+  for (int t = 0; t < NI; ++t) {
+    const int p = 64 * (NI * w + t) + lane, row = p / CPR;
+    const int chunk = (p - row * CPR) ^ xa_swz<DP>(row);
+    qo[t] = 8 * chunk < a.D ? (uint32_t)(row * a.q_sn + 8 * chunk) * 2u : kBufOOB;
+    oo[t] = 8 * chunk < a.D ? (uint32_t)(row * o_sn + 8 * chunk) * 2u : kBufOOB;
+  }
+  const bool near = a.q_sn < (1 << 23) && o_sn < (1 << 23);  // 64 rows within 2 GiB
+  auto issue = [&](int r0, int st) {
+    char* dst = reinterpret_cast<char*>(smem[st][0]) + NI * w * 1024;
+    int g0, i0;
+    xa_row(a, r0, g0, i0);
+    if (near && i0 + RT <= a.Nq && r0 + RT <= rend) {
+      const i32x4 qr = buffer_rsrc(a.q + b * a.q_sb + (int64_t)(hk * a.G + g0) * a.q_sh +
+                                   (int64_t)i0 * a.q_sn);
+      const i32x4 dr = buffer_rsrc(ga.dout + (((int64_t)b * a.Nq + i0) * a.H + hk * a.G + g0) * a.D);
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        buf2lds16(qr, qo[t], dst + t * 1024);
+        buf2lds16(dr, oo[t], dst + t * 1024 + TILE * 2);
       }
-      char* dst = reinterpret_cast<char*>(smem[st][0]) + (NI * w + t) * 1024;
-      g2lds16(qs, dst);
-      g2lds16(os, dst + TILE * 2);
+    } else {
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        const int p = 64 * (NI * w + t) + lane, row = p / CPR;
+        const int chunk = (p - row * CPR) ^ xa_swz<DP>(row);
+        const int r = r0 + row;
+        const u16 *qs = (const u16*)kXaNone, *os = (const u16*)kXaNone;
+        if (r < rend && 8 * chunk < a.D) {
+          int g, i;
+          xa_row(a, r, g, i);
+          qs = a.q + b * a.q_sb + (int64_t)(hk * a.G + g) * a.q_sh + (int64_t)i * a.q_sn + 8 * chunk;
+          os = ga.dout + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + 8 * chunk;
+        }
+        g2lds16(qs, dst + t * 1024);
+        g2lds16(os, dst + t * 1024 + TILE * 2);
+      }
     }
-    if (w < (ADD ? 3 : 2)) {  // wave 0: lse, 1: delta, 2: maxima of the 64 rows
+    if (w < (ADD ? 3 : 2)) {  // wave 0: lse, 1: delta, 2: maxima of the tile's rows
       const float* src = w == 0 ? ga.lse : w == 1 ? ga.delta : ga.top;
-      g2lds4(r0 + lane < rend ? src + bh * a.R + r0 + lane : kXaNone + (w ? 0 : 4), stats[st][w]);
+      g2lds4(lane < RT && r0 + lane < rend ? src + bh * a.R + r0 + lane : kXaNone + (w ? 0 : 4),
+             stats[st][w]);
     }
   };
 
@@ -271,7 +308,9 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void xattn_dkdv_kernel(XAttnG
 #pragma unroll
         for (int d = 0; d < DS; ++d) s = mfma32(xa_frag<DP>(Q, 32 * rb, d), kf[d], s);
 #pragma unroll
-        for (int d = 0; d < DS; ++d) dp = mfma32(xa_frag<DP>(dO, 32 * rb, d), vf[d], dp);
+        for (int d = 0; d < DS; ++d)
+          dp = mfma32(xa_frag<DP>(dO, 32 * rb, d),
+                      VLDS ? xa_frag<DP>(vs, 32 * w, d) : vf[VLDS ? 0 : d], dp);
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
           const f32x4 ls = *reinterpret_cast<const f32x4*>(&stats[st][0][32 * rb + 8 * g4 + 4 * h]);
