@@ -59,6 +59,7 @@ struct XRows {
     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) s[qb][kb] = zero16();
+    if constexpr (DP > 96) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -67,6 +68,7 @@ struct XRows {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) s[qb][kb] = xa_mfma<F16>(kf, q[qb][d], s[qb][kb]);
       }
+    if constexpr (DP > 96) __builtin_amdgcn_s_setprio(0);
     const uint64_t whole = KB == 2 ? ~0ull : 0xffffffffull;
     if (live != whole || fmask) {
 #pragma unroll
@@ -114,6 +116,7 @@ struct XRows {
       }
       l[qb] += sum;
     }
+    if constexpr (DP > 96) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -124,6 +127,7 @@ struct XRows {
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) o[qb][db] = xa_mfma<F16>(vf, p[qb][2 * kb + t], o[qb][db]);
         }
+    if constexpr (DP > 96) __builtin_amdgcn_s_setprio(0);
   }
 };
 
@@ -425,24 +429,27 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
   if (a.lse && d == 0) xa_store_stats(a, row, m, l);
 }
 
-// Workgroups that the forward wants before it splits the states no further:
-// two rounds of the chip's 256 CUs for the streaming kernel (one workgroup a
-// CU), one round of two a CU for the tile kernel.
+// Up to 64 rows run on the streaming kernel, 32 or 64 at once; more on the tile
+// kernel, 128 rows a workgroup, or 256 up to 64 channels where those fill the
+// chip twice (512): each K and V fragment then feeds two products (64 channels,
+// 4096 x 4096, 32 heads: 172 us against 186), while smaller grids do better with
+// twice the workgroups (512 x 1500, 128 heads: 40 us against 45).  Either kernel
+// splits the states only while it has less than one workgroup a CU: further
+// splits cost more in prologues and partials than they level (16 tokens of 32
+// heads, 8191 ragged states: 86 us at 256 workgroups, 90 at 512, 117 at 2048).
 static void xattn_plan(XAttnArgs& a) {
   const bool few = a.R <= 64;
-  const int64_t rows = few ? 64 : (a.D > 64 ? 128 : 256);
-  a.tiles = (int)((a.R + rows - 1) / rows);
-  const int64_t groups = (int64_t)a.B * a.Hk * a.tiles;
-  const int64_t step = few ? 512 : 256;  // keys that a split is worth
-  int64_t s = 512 / groups;
-  const int64_t most = (a.Nk + step - 1) / step;
+  const int64_t BH = (int64_t)a.B * a.Hk;
+  a.qb = few ? (a.R > 32 ? 2 : 1) : a.D <= 64 && BH * ((a.R + 255) / 256) >= 512 ? 2 : 1;
+  a.tiles = few ? 1 : (int)((a.R + 128 * a.qb - 1) / (128 * a.qb));
+  int64_t s = 256 / (BH * a.tiles);
+  const int64_t most = (a.Nk + 511) / 512;  // a split is worth 512 states
   if (s > most) s = most;
   if (s > 64) s = 64;
   if (s < 1) s = 1;
   const int64_t tiles = (a.Nk + 63) / 64;
   a.chunk = (int)((tiles + s - 1) / s) * 64;
   a.splits = (int)((a.Nk + a.chunk - 1) / a.chunk);
-  if (a.splits < 1) a.splits = 1;
 }
 
 static int64_t xattn_part_floats(const XAttnArgs& a) {
@@ -493,15 +500,19 @@ int xattn_check(XAttnArgs& a, const tpf_xattn_shape* s, double scale, const char
 template <int DP, bool F16>
 static void xattn_launch(const XAttnArgs& a, hipStream_t s) {
   const int64_t groups = (int64_t)a.B * a.Hk * a.splits;
+  const dim3 grid((unsigned)((groups * a.tiles + 7) / 8 * 8));
   if (a.R <= 64) {
-    const dim3 grid((unsigned)((groups + 7) / 8 * 8));
-    if (a.R <= 32) hipLaunchKernelGGL((xattn_few_kernel<DP, 1, F16>), grid, dim3(256), 0, s, a);
+    if (a.qb == 1) hipLaunchKernelGGL((xattn_few_kernel<DP, 1, F16>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((xattn_few_kernel<DP, 2, F16>), grid, dim3(256), 0, s, a);
-  } else {
-    constexpr int QB = DP > 64 ? 1 : 2;
-    const dim3 grid((unsigned)((groups * a.tiles + 7) / 8 * 8));
-    hipLaunchKernelGGL((xattn_fwd_kernel<DP, QB, F16>), grid, dim3(256), 0, s, a);
+    return;
   }
+  if constexpr (DP <= 64) {
+    if (a.qb == 2) {
+      hipLaunchKernelGGL((xattn_fwd_kernel<DP, 2, F16>), grid, dim3(256), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((xattn_fwd_kernel<DP, 1, F16>), grid, dim3(256), 0, s, a);
 }
 
 template <bool F16>

@@ -33,7 +33,8 @@ struct XAttnArgs {
   float c;          // scale * log2(e)
   float inv_scale;  // additive masks enter the raw scores divided by the scale
   float mask_floor; // lowest finite raw mask value
-  int splits, chunk, tiles;  // key splits, keys per split (a multiple of 64), row tiles
+  int splits, chunk, tiles;  // state splits, states per split (a multiple of 64), row tiles
+  int qb;           // blocks of 32 rows a wave
   float* part_o;    // [B*Hk, splits, R, D] unnormalised outputs of the splits
   float* part_ml;   // [B*Hk, splits, R, 2] their raw maxima and sums
 };

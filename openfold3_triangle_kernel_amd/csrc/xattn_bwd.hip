@@ -345,15 +345,20 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
                ga.part_v ? ga.part_v + po : nullptr, 1.f, !live);
 }
 
-// Sums the partials [splits, BH, n, D] of dQ (ROWS: n = R) or dK / dV (n = Nk)
-// in ascending order; a thread forms four channels.
-template <bool ROWS>
-__global__ __launch_bounds__(256) void xattn_fold_kernel(const float* part, int splits, int n,
-                                                         XAttnGrad ga, u16* dst, int64_t s0,
-                                                         int64_t s1, int64_t s2, float scale) {
+// Sums the partials [splits, BH, n, D] of the split launches in ascending order,
+// four channels a thread: workgroups [0, first_k) dQ, [first_k, first_v) dK, the rest
+// dV.
+__global__ __launch_bounds__(256) void xattn_fold_kernel(XAttnGrad ga, unsigned first_k,
+                                                         unsigned first_v) {
   const XAttnArgs& a = ga.f;
-  const int dv = a.D / 4;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, row = t / dv;
+  const int which = blockIdx.x < first_k ? 0 : blockIdx.x < first_v ? 1 : 2;
+  const int64_t block = blockIdx.x - (which == 0 ? 0 : which == 1 ? first_k : first_v);
+  const float* part = which == 0 ? ga.part_q : which == 1 ? ga.part_k : ga.part_v;
+  u16* dst = which == 0 ? ga.dq : which == 1 ? ga.dk : ga.dv;
+  const int64_t* st = which == 0 ? ga.dq_s : which == 1 ? ga.dk_s : ga.dv_s;
+  const float scale = which == 2 ? 1.f : ga.scale;
+  const int n = which ? a.Nk : a.R, splits = which ? ga.rsplits : a.splits, dv = a.D / 4;
+  const int64_t t = block * 256 + threadIdx.x, row = t / dv;
   const int64_t BH = (int64_t)a.B * a.Hk;
   if (row >= BH * n) return;
   const int d = 4 * (int)(t - row * dv);
@@ -367,7 +372,7 @@ __global__ __launch_bounds__(256) void xattn_fold_kernel(const float* part, int 
   const int r = (int)(row - bh * n);
   const int b = (int)(bh / a.Hk);
   int head = (int)(bh - (int64_t)b * a.Hk), pos = r;
-  if (ROWS) {
+  if (which == 0) {
     int g, i;
     xa_row(a, r, g, i);
     head = head * a.G + g;
@@ -376,7 +381,7 @@ __global__ __launch_bounds__(256) void xattn_fold_kernel(const float* part, int 
   uint2 x;
   x.x = xa_pair<false>(o[0] * scale, o[1] * scale);
   x.y = xa_pair<false>(o[2] * scale, o[3] * scale);
-  *reinterpret_cast<uint2*>(dst + b * s0 + head * s1 + (int64_t)pos * s2 + d) = x;
+  *reinterpret_cast<uint2*>(dst + b * st[0] + head * st[1] + (int64_t)pos * st[2] + d) = x;
 }
 
 // Each launch is split once its tiles leave CUs idle: up to 512 workgroups (two
@@ -485,15 +490,10 @@ extern "C" int tpf_xattn_backward_bf16(const void* q, const void* k, const void*
   if (a.mask_kind == tpf::kMaskF32) tpf::grad_pick<true>(g, s);
   else tpf::grad_pick<false>(g, s);
   const int64_t BH = (int64_t)a.B * a.Hk;
-  auto blocks = [&](int64_t n) { return dim3((unsigned)((BH * n * (a.D / 4) + 255) / 256)); };
-  if (g.part_q)
-    hipLaunchKernelGGL(tpf::xattn_fold_kernel<true>, blocks(a.R), dim3(256), 0, s, g.part_q, a.splits,
-                       a.R, g, g.dq, g.dq_s[0], g.dq_s[1], g.dq_s[2], g.scale);
-  if (g.part_k) {
-    hipLaunchKernelGGL(tpf::xattn_fold_kernel<false>, blocks(a.Nk), dim3(256), 0, s, g.part_k,
-                       g.rsplits, a.Nk, g, g.dk, g.dk_s[0], g.dk_s[1], g.dk_s[2], g.scale);
-    hipLaunchKernelGGL(tpf::xattn_fold_kernel<false>, blocks(a.Nk), dim3(256), 0, s, g.part_v,
-                       g.rsplits, a.Nk, g, g.dv, g.dv_s[0], g.dv_s[1], g.dv_s[2], 1.f);
-  }
+  auto blocks = [&](bool some, int64_t n) { return some ? (BH * n * (a.D / 4) + 255) / 256 : 0; };
+  const int64_t nq = blocks(g.part_q, a.R), nk = blocks(g.part_k, a.Nk);
+  if (nq + nk)
+    hipLaunchKernelGGL(tpf::xattn_fold_kernel, dim3((unsigned)(nq + 2 * nk)), dim3(256), 0, s, g,
+                       (unsigned)nq, (unsigned)(nq + nk));
   return tpf::check_launch(fn);
 }
