@@ -544,6 +544,12 @@ int tpf_norm_backward(const void* dy, const void* x, int64_t x_ld, const void* c
  * and x [R, K] in 8 bits, BF16 products summed in f32, in BF16 or FP32; N and K
  * multiples of 8, tensors on 16 bytes.
  * ---------------------------------------------------------------------- */
+/* y [M, N] = a b^T (b [N, K], b_kc = 1) or a b (b [K, N], b_kc = 0) of BF16 rows a
+ * [M, K] (a_ld elements between rows), b and y contiguous, f32 sums rounded once to
+ * BF16; K and N multiples of 8, a and b on 16 bytes and below 2 GiB.  A row's result
+ * does not depend on M. */
+int tpf_row_gemm_bf16(const void* a, int64_t a_ld, const void* b, int b_kc, void* y, int64_t M,
+                      int64_t N, int64_t K, void* stream);
 int tpf_act8_pack(const void* x, int64_t ld, int64_t R, int64_t C, int64_t dtype, void* codes,
                   void* scales, void* stream);
 int tpf_act8_unpack(const void* codes, const void* scales, int64_t R, int64_t C, void* x,

@@ -150,6 +150,7 @@ SIGNATURES: dict[str, tuple] = {
     "tpf_norm_backward_workspace_bytes": (_I64, [_I64, _I64]),
     "tpf_norm_backward": (
         _I32, [_P, _P, _I64] + [_P] * 4 + [_I64] * 3 + [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P]),
+    "tpf_row_gemm_bf16": (_I32, [_P, _I64, _P, _I32, _P, _I64, _I64, _I64, _P]),
     "tpf_act8_pack": (_I32, [_P] + [_I64] * 4 + [_P] * 3),
     "tpf_act8_unpack": (_I32, [_P, _P, _I64, _I64, _P, _I64, _I64, _P]),
     "tpf_wgrad_act8_workspace_bytes": (_I64, [_I64] * 4),

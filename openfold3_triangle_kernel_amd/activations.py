@@ -118,9 +118,8 @@ def _row_gemm(a: torch.Tensor, b: torch.Tensor, b_kc: bool) -> torch.Tensor:
     with _native.device_ctx(a.device):
         for r in range(0, R, step):
             n = min(step, R - r)
-            _native.call("tpf_gemm_bf16", a.data_ptr() + 2 * r * ld, 1, ld, 0, b.data_ptr(),
-                         int(b_kc), b.stride(0), 0, out.data_ptr() + 2 * r * N, 0, N, 0, n, N, K, 1,
-                         1.0, _native.stream_of(a))
+            _native.call("tpf_row_gemm_bf16", a.data_ptr() + 2 * r * ld, ld, b.data_ptr(), int(b_kc),
+                         out.data_ptr() + 2 * r * N, n, N, K, _native.stream_of(a))
     return out
 
 

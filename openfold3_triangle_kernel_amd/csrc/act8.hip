@@ -98,7 +98,10 @@ static int act8_check(ActArgs& a, const void* plain, int64_t ld, int64_t R, int6
 // layouts of gemm_core.hpp, both operands read transposed from LDS).  dy goes
 // into LDS directly; the codes come through registers, one step ahead, and are
 // decoded once per tile on their way: a thread decodes one block of 32 (one
-// scale), and every decoded value is exact in BF16.
+// scale), and every decoded value is exact in BF16.  8192 x 1024 -> 4096: 103 us (670
+// TFLOP/s), as long as torch's product of the same BF16 operands takes; 256-wide
+// tiles of eight waves, 128 x 64 a wave, and decoding between the products measured
+// 102 to 114 us and were not kept.
 struct Wgrad8Args {
   const __bf16* dy;
   int64_t ld;
@@ -214,21 +217,38 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
     }
 }
 
-// Sums the splits in ascending order, four values a thread.
+// Sums the splits, four values a thread: RANGES threads share them, each a range in
+// ascending order, and the ranges join in order.  Eight ranges where there are many
+// splits, which have few values (128 of 512 x 128: 7.8 us with one range).
+template <int RANGES>
 __global__ __launch_bounds__(256) void wgrad8_fold_kernel(const float* part, int64_t n, int splits,
                                                           void* dw, int out_f32) {
-  const int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
-  if (i >= n) return;  // n is a multiple of 64
+  constexpr int G = 256 / RANGES;
+  __shared__ f32x4 red[RANGES][G];
+  const int g = threadIdx.x % G, q = threadIdx.x / G;
+  const int64_t i = 4 * ((int64_t)blockIdx.x * G + g);
+  const bool in = i < n;  // n is a multiple of 64
+  const int per = (splits + RANGES - 1) / RANGES, p1 = min(splits, (q + 1) * per);
   f32x4 s = (f32x4)0.f;
-  int p = 0;
-  for (; p + 8 <= splits; p += 8) {
-    f32x4 v[8];
+  int p = q * per;
+  if (in) {
+    for (; p + 8 <= p1; p += 8) {
+      f32x4 v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = ld4f_nt(part + (int64_t)(p + e) * n + i);
+      for (int e = 0; e < 8; ++e) v[e] = ld4f_nt(part + (int64_t)(p + e) * n + i);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += v[e];
+      for (int e = 0; e < 8; ++e) s += v[e];
+    }
+    for (; p < p1; ++p) s += ld4f_nt(part + (int64_t)p * n + i);
   }
-  for (; p < splits; ++p) s += ld4f_nt(part + (int64_t)p * n + i);
+  if constexpr (RANGES > 1) {
+    red[q][g] = s;
+    __syncthreads();
+    if (q) return;
+#pragma unroll
+    for (int e = 1; e < RANGES; ++e) s += red[e][g];
+  }
+  if (!in) return;
   if (out_f32) {
     *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(dw) + i) = s;
   } else {
@@ -313,8 +333,14 @@ extern "C" int tpf_wgrad_act8(const void* dy, int64_t ld_dy, const void* codes, 
   const int64_t tiles = ((N + 127) / 128) * ((K + 127) / 128) * a.splits;
   if ((tiles + 7) / 8 * 8 > INT32_MAX) return tpf::set_error(TPF_ERR_SHAPE, "%s: too large", fn);
   hipLaunchKernelGGL(tpf::wgrad8_kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0, s, a);
-  if (a.part)
-    hipLaunchKernelGGL(tpf::wgrad8_fold_kernel, dim3((unsigned)((N * K / 4 + 255) / 256)), dim3(256),
-                       0, s, a.part, N * K, a.splits, dw, a.out_f32);
+  if (a.part) {
+    const int64_t n = N * K;
+    if (a.splits >= 32)
+      hipLaunchKernelGGL(tpf::wgrad8_fold_kernel<8>, dim3((unsigned)((n / 4 + 31) / 32)), dim3(256), 0,
+                         s, a.part, n, a.splits, dw, a.out_f32);
+    else
+      hipLaunchKernelGGL(tpf::wgrad8_fold_kernel<1>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256),
+                         0, s, a.part, n, a.splits, dw, a.out_f32);
+  }
   return tpf::check_launch(fn);
 }

@@ -2,7 +2,8 @@
 // folded in fixed order): the TriMul dW5 and the pair-stack
 // projection weight gradients.  Own translation unit for its stage shape:
 // 64-deep k-steps, two stages (measured best for these long-K, few-tile
-// products; the contraction shape in gemm.hip is 32 deep, three stages).
+// products; the contraction shape in gemm.hip is 32 deep, three stages).  The
+// linear layer's products (tpf_row_gemm_bf16) run on this shape too.
 #define TPF_GEMM_IMPL gk64
 #include "gemm_impl.hpp"
 
@@ -64,4 +65,36 @@ extern "C" int tpf_wgrad_bf16(const void* dy, int64_t ld_dy, const void* x, int6
   int rc = tpf::gemm_launch_wgrad(g, s, fn);
   if (rc) return rc;
   return tpf::fold_launch((const float*)workspace, dw, M * N, M * N, splits, s, fn);
+}
+
+// y [M, N] = a [M, K] b^T (b [N, K], b_kc = 1) or a b (b [K, N]) of contiguous BF16
+// rows, f32 sums rounded once.  More than one tile of columns runs on 64-deep k-steps:
+// 84 us against the 32-deep 101 at 8192 x 1024 -> 4096, 76 against 83 the other way
+// (818 and 900 TFLOP/s).  One tile of columns is a stream of a, which the 32-deep
+// shape keeps more stages of in flight: 49 us against 55 at 147456 x 512 -> 128.  The
+// weight-stationary row kernel takes the shapes that it has, as in tpf_gemm_bf16.
+// No choice depends on M, and all sum in the same order.
+extern "C" int tpf_row_gemm_bf16(const void* a, int64_t a_ld, const void* b, int b_kc, void* y,
+                                 int64_t M, int64_t N, int64_t K, void* stream) {
+  const char* fn = "tpf_row_gemm_bf16";
+  if (!a || !b || !y) return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
+  if (M < 1 || N < 1 || K < 1 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
+    return tpf::set_error(TPF_ERR_SHAPE, "%s: bad shape", fn);
+  const int64_t b_ld = b_kc ? K : N;
+  hipStream_t s = (hipStream_t)stream;
+  int rc = TPF_OK;
+  if (tpf::rowgemm_try((const __bf16*)a, a_ld, (const __bf16*)b, b_kc, b_ld, (__bf16*)y, N, M, N, K, s,
+                       &rc, fn))
+    return rc;
+  tpf::GemmArgs g{};
+  g.A = (const __bf16*)a; g.a_ld = a_ld;
+  g.B = (const __bf16*)b; g.b_ld = b_ld;
+  g.C = y; g.c_ld = N;
+  g.M = (int)M; g.N = (int)N; g.K = (int)K; g.ksplit = 1; g.k_chunk = (int)K; g.alpha = 1.f;
+  if (N <= tpf::kGN) return tpf::gemm_launch(g, 1, b_kc ? 1 : 0, 0, 1, s, fn);
+  if ((rc = tpf::gemm_prepare(g, 1, b_kc ? 1 : 0, 0, 1, fn))) return rc;
+  const dim3 grid((unsigned)((tpf::gemm_tiles(g) + 7) / 8 * 8));
+  if (b_kc) hipLaunchKernelGGL((tpf::gemm_bf16_kernel<true, true, false>), grid, dim3(256), 0, s, g);
+  else hipLaunchKernelGGL((tpf::gemm_bf16_kernel<true, false, false>), grid, dim3(256), 0, s, g);
+  return tpf::check_launch(fn);
 }

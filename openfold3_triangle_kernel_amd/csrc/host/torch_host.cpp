@@ -582,9 +582,8 @@ std::optional<Tensor> layer_norm(const Tensor& x, const std::optional<Tensor>& w
 Tensor row_gemm(const Tensor& a, const Tensor& b, bool b_kc) {
   const int64_t R = a.size(0), K = a.size(1), N = b_kc ? b.size(0) : b.size(1);
   Tensor out = at::empty({R, N}, a.options());
-  check(tpf_gemm_bf16(cptr(a), 1, K, 0, cptr(b), b_kc ? 1 : 0, b.size(1), 0, out.data_ptr(), 0, N, 0,
-                      R, N, K, 1, 1.0, stream()),
-        "tpf_gemm_bf16");
+  check(tpf_row_gemm_bf16(cptr(a), K, cptr(b), b_kc ? 1 : 0, out.data_ptr(), R, N, K, stream()),
+        "tpf_row_gemm_bf16");
   return out;
 }
 
