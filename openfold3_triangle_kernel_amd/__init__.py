@@ -77,3 +77,7 @@ __all__ += ["CompressedActivation", "compress_activation", "decompress_activatio
 from .cross_attention import cross_attention  # noqa: E402
 
 __all__ += ["cross_attention"]
+
+from .cross_block import CrossAttention  # noqa: E402
+
+__all__ += ["CrossAttention"]

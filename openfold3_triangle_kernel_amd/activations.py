@@ -14,8 +14,9 @@ infinity or NaN decodes to NaN.
 
 from __future__ import annotations
 
+import functools
+
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
 from .attention import _device_supported, _is_gfx950
@@ -39,6 +40,25 @@ class CompressedActivation:
     @property
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
+
+
+def differentiable_once(backward):
+    """The ``backward`` of a Function whose kernels have no second derivative: with
+    ``create_graph`` its gradients raise when they are differentiated, instead of
+    passing for constants."""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        err = torch._C._functions.DelayedError(
+            b"trying to differentiate twice a function that was marked with @once_differentiable",
+            len(out))
+        return err(*(t if t is None else t.detach().requires_grad_(True) for t in out))
+
+    return wrapper
 
 
 def host_path(*tensors) -> bool:
@@ -84,6 +104,11 @@ def _pack(x2: torch.Tensor):
 
 def compress_activation(x: torch.Tensor) -> CompressedActivation:
     """``x`` [*, C] (BF16, FP16 or FP32) in 8 bits; no gradient passes through."""
+    if host_path(x):
+        # The common form entirely in C++; None (nothing launched) for any other.
+        packed = _native.host().act8_pack(x)
+        if packed is not None:
+            return CompressedActivation(*packed, x.shape, x.dtype)
     check_rows("compress_activation", x)
     return CompressedActivation(*_pack(as_rows(x.detach())), x.shape, x.dtype)
 
@@ -96,8 +121,24 @@ def decompress_activation(saved: CompressedActivation,
     dtype = saved.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise ValueError("decompress_activation gives BF16, FP16 or FP32")
-    out = torch.empty(saved.shape, device=saved.codes.device, dtype=dtype)
+    if host_path(saved.codes, saved.scales):
+        out = _native.host().act8_unpack(saved.codes, saved.scales, saved.shape, dtype)
+        if out is not None:
+            return out
+    if not saved.shape or saved.shape[-1] < 1:
+        raise ValueError("decompress_activation: the shape has no channels")
     C = saved.shape[-1]
+    rows = saved.shape.numel() // C
+    blocks = -(-C // _BLOCK)
+    for t, width in ((saved.codes, blocks * _BLOCK), (saved.scales, blocks)):
+        if t.dtype != torch.uint8 or tuple(t.shape) != (rows, width) or not t.is_contiguous():
+            raise ValueError("decompress_activation: codes or scales do not fit the shape")
+    if saved.codes.device != saved.scales.device:
+        raise ValueError("decompress_activation: codes and scales on different devices")
+    ok, reason = _device_supported(saved.codes)
+    if not ok:
+        raise ValueError(f"decompress_activation: {reason}")
+    out = torch.empty(saved.shape, device=saved.codes.device, dtype=dtype)
     if out.numel():
         with _native.device_ctx(out.device):
             _native.call("tpf_act8_unpack", saved.codes.data_ptr(), saved.scales.data_ptr(),
@@ -162,7 +203,7 @@ class _LinearFn(torch.autograd.Function):
         return _row_gemm(x, w, True)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, dy):
         w, *kept = ctx.saved_tensors
         dy = _gemm_rows(dy.to(torch.bfloat16))

@@ -17,10 +17,9 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from .activations import host_path
+from .activations import differentiable_once, host_path
 from .attention import _device_supported
 
 _MAX_HEAD_DIM = 128
@@ -148,7 +147,7 @@ class _CrossAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, d_out):
         q, k, v, mask, out, lse = ctx.saved_tensors
         kind, mask_stride, scale = ctx.args

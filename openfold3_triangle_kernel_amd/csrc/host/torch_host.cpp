@@ -576,6 +576,41 @@ std::optional<Tensor> layer_norm(const Tensor& x, const std::optional<Tensor>& w
   return x.dim() == 2 ? y : y.view(x.sizes());
 }
 
+// ------------------------------------------------------- activations in 8 bits
+
+std::optional<std::tuple<Tensor, Tensor>> act8_pack(const Tensor& x) {
+  if (transforms_active() || !x.is_cuda()) return std::nullopt;
+  if (!plain(x, c10::hip::current_device()) || x.dim() < 1 || x.numel() == 0 ||
+      type_code(x.scalar_type()) < 0 || x.size(-1) > (1 << 24) ||
+      !(x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1)))
+    return std::nullopt;
+  const int64_t C = x.size(-1), R = x.numel() / C, blocks = (C + 31) / 32;
+  Tensor codes = at::empty({R, blocks * 32}, like(x, at::kByte));
+  Tensor scales = at::empty({R, blocks}, like(x, at::kByte));
+  check(tpf_act8_pack(cptr(x), x.dim() == 2 && R > 1 ? x.stride(0) : C, R, C,
+                      type_code(x.scalar_type()), mptr(codes), mptr(scales), stream()),
+        "tpf_act8_pack");
+  return std::make_tuple(codes, scales);
+}
+
+std::optional<Tensor> act8_unpack(const Tensor& codes, const Tensor& scales,
+                                  const std::vector<int64_t>& shape, at::ScalarType dtype) {
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  if (transforms_active() || !plain(codes, dev) || !plain(scales, dev) || shape.empty() ||
+      codes.numel() == 0 || type_code(dtype) < 0)
+    return std::nullopt;
+  const int64_t C = shape.back(), R = codes.size(0), blocks = (C + 31) / 32;
+  if (C < 1 || c10::multiply_integers(shape) != R * C || codes.dim() != 2 || scales.dim() != 2 ||
+      codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte ||
+      codes.size(1) != 32 * blocks || scales.size(0) != R || scales.size(1) != blocks ||
+      !codes.is_contiguous() || !scales.is_contiguous())
+    return std::nullopt;
+  Tensor out = at::empty(shape, like(codes, dtype));
+  check(tpf_act8_unpack(cptr(codes), cptr(scales), R, C, out.data_ptr(), C, type_code(dtype), stream()),
+        "tpf_act8_unpack");
+  return out;
+}
+
 // -------------------------------------------------------------------- linear
 
 // a [R, K] times b^T (b_kc: b [N, K]) or b [K, N], contiguous BF16.
@@ -670,6 +705,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("trimul", &trimul, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("cross_attention", &cross_attention, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("layer_norm", &layer_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("act8_pack", &act8_pack, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("act8_unpack", &act8_unpack, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("linear", &linear, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("set_workspace_budget", [](int64_t bytes) { g_budget.store(bytes); });
 }

@@ -19,10 +19,9 @@ dgamma / dbeta from fixed-order partial sums (deterministic).
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from .activations import _DTYPES, as_rows, check_rows, code_buffers, host_path
+from .activations import _DTYPES, as_rows, check_rows, code_buffers, differentiable_once, host_path
 from .attention import _device_ctx
 
 
@@ -151,7 +150,7 @@ class _LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, dy):
         x2, mean, rstd, codes, scales, w = ctx.saved_tensors
         dtype, (R, C), wtype, btype = ctx.args
@@ -193,7 +192,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     """
     if save not in ("full", "int8"):
         raise ValueError('save must be "full" or "int8"')
-    if host_path(*(t for t in (x, weight, bias) if t is not None)):
+    if host_path(x, *(t for t in (weight, bias) if t is not None)):
         # The common form entirely in C++; None (nothing launched) for any other.
         out = _native.host().layer_norm(x, weight, bias, eps, save == "int8")
         if out is not None:

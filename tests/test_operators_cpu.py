@@ -1,0 +1,175 @@
+"""Refusals of the cross-attention, layer-norm and 8-bit activation operators without a
+GPU: host tensors and bad arguments raise before any native call, the C ABI answers
+bad shapes with a status before any launch, and the block runs its formulas in
+PyTorch on the CPU."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from openfold3_triangle_kernel_amd import (
+    CompressedActivation,
+    CrossAttention,
+    compress_activation,
+    cross_attention,
+    decompress_activation,
+    layer_norm,
+    linear,
+    set_turbopairformer_strict,
+    stock_invocation_count,
+)
+
+
+def _qkv(B=1, H=2, Hk=2, Nq=4, Nk=8, D=64, dtype=torch.bfloat16):
+    return [torch.zeros(B, h, n, D, dtype=dtype) for h, n in ((H, Nq), (Hk, Nk), (Hk, Nk))]
+
+
+@pytest.mark.parametrize("args,match", [
+    ((*_qkv(),), "GPU"),
+    ((_qkv()[0], _qkv()[1], None), "torch.Tensor"),
+    ((*(t[0, 0] for t in _qkv()),), "shape"),
+    ((*_qkv(dtype=torch.float32),), "BF16 or FP16"),
+    ((*_qkv(D=129),), "D<=128"),
+    ((*_qkv(H=3),), "multiple"),
+    ((_qkv()[0], _qkv()[1], _qkv(Nk=9)[2]), "one shape"),
+    ((_qkv(B=2)[0], *_qkv()[1:]), "batch prefix"),
+    ((_qkv(D=32)[0], *_qkv()[1:]), "head dimension"),
+    ((*_qkv(), torch.zeros(7)), "broadcast"),
+    ((*_qkv(), torch.zeros(3, 8)), "broadcast"),
+    ((*_qkv(), torch.zeros(1)), "broadcast"),
+    ((*_qkv(), torch.zeros(8, dtype=torch.int64)), "boolean"),
+    ((*_qkv(), torch.zeros(8, requires_grad=True)), "must not require"),
+    ((*_qkv(), None, -1.0), "scale"),
+    ((*_qkv(), None, float("nan")), "scale"),
+])
+def test_cross_attention_refuses(args, match):
+    with pytest.raises(ValueError, match=match):
+        cross_attention(*args)
+
+
+def test_rows_operators_refuse():
+    x, w = torch.zeros(4, 16), torch.ones(16)
+    for call, match in ((lambda: layer_norm(x, w), "GPU"),
+                        (lambda: layer_norm(x.long()), "BF16"),
+                        (lambda: layer_norm(x, save="fp8"), "save"),
+                        (lambda: layer_norm(None), "torch.Tensor"),
+                        (lambda: compress_activation(x), "GPU"),
+                        (lambda: compress_activation(torch.tensor(1.0)), "channels"),
+                        (lambda: decompress_activation(None), "CompressedActivation"),
+                        (lambda: linear(x.bfloat16(), x.bfloat16()), "GPU"),
+                        (lambda: linear(x, x, save="half"), "save")):
+        with pytest.raises(ValueError, match=match):
+            call()
+
+
+def test_decompress_checks_what_it_is_given():
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8)
+    for args in ((codes, scales, (4, 33), torch.float32), (codes, scales[:3], (4, 20), torch.float32),
+                 (codes.int(), scales, (4, 20), torch.float32), (codes, scales, (4, 0), torch.float32),
+                 (codes, scales, (), torch.float32), (codes, scales, (4, 20), torch.int32),
+                 (codes, scales, (4, 20), torch.float32)):
+        with pytest.raises(ValueError):
+            decompress_activation(CompressedActivation(*args))
+
+
+def _shape(**kw):
+    v = dict(B=1, H=2, Hk=2, Nq=4, Nk=8, D=64, dtype=0, kind=0, ms=0, q=(512, 256, 64),
+             k=(1024, 512, 64), v=(1024, 512, 64))
+    v.update(kw)
+    return (ctypes.c_int64 * 18)(v["B"], v["H"], v["Hk"], v["Nq"], v["Nk"], v["D"], v["dtype"],
+                                 v["kind"], v["ms"], *v["q"], *v["k"], *v["v"])
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(D=60), "bad shape"), (dict(D=136), "bad shape"), (dict(D=0), "bad shape"),
+    (dict(Nq=0), "bad shape"), (dict(Nk=0), "bad shape"), (dict(H=3), "bad shape"),
+    (dict(Nq=1 << 31), "too many"), (dict(k=(1024, 512, 60)), "strides"),
+    (dict(q=(512, -256, 64)), "strides"), (dict(k=(1024, 512, 1 << 23)), "stride too large"),
+    (dict(dtype=2), "dtype"), (dict(kind=3), "bad mask"), (dict(kind=1), "disagree"),
+])
+def test_c_abi_cross_attention_shapes(kw, match):
+    from openfold3_triangle_kernel_amd import _native
+
+    with pytest.raises(RuntimeError, match=match):
+        _native.call("tpf_xattn_forward", 16, 16, 16, None, 16, None, 16, 1 << 30, _shape(**kw), 0.125,
+                     None)
+    if match != "disagree":
+        assert _native.query("tpf_xattn_forward_workspace_bytes", _shape(**kw)) == -1
+
+
+def test_c_abi_arguments():
+    from openfold3_triangle_kernel_amd import _native
+
+    def refused(match, name, *args):
+        with pytest.raises(RuntimeError, match=match):
+            _native.call(name, *args)
+
+    s, g = _shape(), (ctypes.c_int64 * 9)(512, 256, 64, 1024, 512, 64, 1024, 512, 64)
+    refused("null pointer", "tpf_xattn_forward", None, 16, 16, None, 16, None, 16, 0, s, 0.1, None)
+    refused("16 bytes", "tpf_xattn_forward", 8, 16, 16, None, 16, None, 16, 0, s, 0.1, None)
+    refused("scale", "tpf_xattn_forward", 16, 16, 16, None, 16, None, 16, 0, s, 0.0, None)
+    refused("workspace", "tpf_xattn_forward", 16, 16, 16, None, 16, None, 16, 8, _shape(Nk=4096), 0.1,
+            None)
+    refused("workspace", "tpf_xattn_backward_bf16", *([16] * 3), None, *([16] * 7), 8, s, g, 0.1, None)
+    refused("BF16 only", "tpf_xattn_backward_bf16", *([16] * 3), None, *([16] * 7), 1 << 20,
+            _shape(dtype=1), g, 0.1, None)
+    bad = (ctypes.c_int64 * 9)(512, 256, 63, 1024, 512, 64, 1024, 512, 64)
+    refused("gradient strides", "tpf_xattn_backward_bf16", *([16] * 3), None, *([16] * 7), 1 << 20, s,
+            bad, 0.1, None)
+    refused("bad shape", "tpf_norm_forward", 16, 8, 0, 8, 0, None, None, 0, 1e-5, 16, None, None, None,
+            None, None)
+    refused("unknown type", "tpf_norm_forward", 16, 8, 4, 8, 3, None, None, 0, 1e-5, 16, None, None,
+            None, None, None)
+    refused("both given or both null", "tpf_norm_forward", 16, 8, 4, 8, 0, None, None, 0, 1e-5, 16,
+            None, None, 16, None, None)
+    refused("means or the codes", "tpf_norm_backward", 16, None, 8, None, None, None, 16, 4, 8, 0, None,
+            0, 16, 8, None, None, None, 0, None)
+    refused("workspace", "tpf_norm_backward", 16, 16, 8, None, None, 16, 16, 4, 8, 0, None, 0, 16, 8,
+            16, None, 16, 4, None)
+    refused("8 bytes", "tpf_act8_pack", 16, 8, 4, 8, 0, 12, 16, None)
+    refused("null pointer", "tpf_act8_unpack", None, 16, 4, 8, 16, 8, 0, None)
+    refused("bad shape", "tpf_wgrad_act8", 16, 12, 16, 16, 4, 12, 8, 16, 0, 16, 0, None)
+    refused("BF16 or FP32", "tpf_wgrad_act8", 16, 16, 16, 16, 4, 16, 8, 16, 1, 16, 0, None)
+    refused("workspace", "tpf_wgrad_act8", 16, 16, 16, 16, 1 << 16, 16, 8, 16, 0, 16, 4, None)
+    refused("bad shape", "tpf_row_gemm_bf16", 16, 8, 16, 1, 16, 0, 8, 8, None)
+
+
+def test_block_runs_its_formulas_on_the_cpu():
+    torch.manual_seed(0)
+    block = CrossAttention(24, 40, 8, 4, no_kv_heads=2).double()
+    x = torch.randn(2, 5, 24, dtype=torch.float64, requires_grad=True)
+    kv = torch.randn(2, 7, 40, dtype=torch.float64)
+    mask = torch.ones(2, 7, dtype=torch.bool)
+    mask[0, 4:] = False
+    mask[1] = False
+    before = stock_invocation_count()
+    out = block(x, kv, mask)
+    assert stock_invocation_count() == before + 2  # the states' projection and the call
+    assert out.shape == x.shape and not out[1].any()  # no state: nothing attended
+    s = torch.nn.functional.layer_norm(kv[:, :4].float(), (40,), block.layer_norm_kv.weight.float(),
+                                       block.layer_norm_kv.bias.float()).double()
+    q = torch.nn.functional.layer_norm(x.float(), (24,), block.layer_norm_q.weight.float(),
+                                       block.layer_norm_q.bias.float()).double()
+    heads = lambda t, h: t.reshape(2, -1, h, 8).transpose(1, 2)  # noqa: E731
+    k, v = (heads(m(s), 2).repeat_interleave(2, 1) for m in (block.linear_k, block.linear_v))
+    p = torch.softmax(heads(block.linear_q(q), 4) @ k.transpose(-1, -2) / math.sqrt(8), -1)
+    want = (p @ v).transpose(1, 2).reshape(2, 5, 32) * torch.sigmoid(block.linear_g(q))
+    # The norms and the attention run in FP32 here.
+    assert (out[0] - block.linear_o(want)[0]).abs().max() <= 1e-5
+    states = block.project_states(kv)
+    assert torch.equal(block(x, key_mask=mask, states=states), out)
+    out.sum().backward()
+    assert torch.isfinite(x.grad).all() and not x.grad[1].any()
+    with pytest.raises(ValueError, match="either kv or states"):
+        block(x)
+    set_turbopairformer_strict(True)
+    try:
+        with pytest.raises(RuntimeError, match="strict"):
+            block(x, kv)
+    finally:
+        set_turbopairformer_strict(False)
+    for bad in (dict(no_heads=3, no_kv_heads=2), dict(no_heads=2, activation_save="int4")):
+        with pytest.raises(ValueError):
+            CrossAttention(8, 8, 8, **bad)
