@@ -241,7 +241,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, save: str = "int8") -> torch.T
     if weight.dtype not in (torch.bfloat16, torch.float32) or weight.device != x.device:
         raise ValueError("linear needs a BF16 or FP32 weight on the input's device")
     N, K = weight.shape
-    if N < 8 or N % 8 or K % 8 or max(N, K) * K * 2 > _GEMM_SPAN:
+    if N < 8 or N % 8 or K % 8 or N * K * 2 > _GEMM_SPAN:
         raise ValueError("linear needs feature counts that are multiples of 8, the weight below 2 GiB")
     if x.numel() == 0:
         return x.matmul(weight.to(x.dtype).t())

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import numbers
 
 import torch
 
@@ -50,8 +51,8 @@ def _check(q, k, v, key_mask, scale) -> None:
     heads, kv_heads = q.shape[-3], k.shape[-3]
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise _unsupported("the query heads must be a positive multiple of the kv heads")
-    if scale is not None and not (0.0 < scale < 1e30):
-        raise _unsupported("scale must be positive and finite")
+    if scale is not None and not (isinstance(scale, numbers.Real) and 0.0 < scale < 1e30):
+        raise _unsupported("scale must be a positive finite number")
     tensors = [q, k, v]
     if key_mask is not None:
         if not isinstance(key_mask, torch.Tensor):
@@ -89,6 +90,14 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
             return t
         return t.clone(memory_format=torch.contiguous_format)
     return t
+
+
+def _grad_like(t: torch.Tensor) -> torch.Tensor:
+    """A gradient in the operand's storage order, where that keeps its channels
+    contiguous (a broadcast operand's order may not)."""
+    g = torch.empty_like(t)
+    return g if g.stride(3) == 1 and all(s % 8 == 0 for s in g.stride()[:3]) else torch.empty(
+        t.shape, device=t.device, dtype=t.dtype)
 
 
 def _strides(t: torch.Tensor):
@@ -152,9 +161,7 @@ class _CrossAttentionFn(torch.autograd.Function):
         q, k, v, mask, out, lse = ctx.saved_tensors
         kind, mask_stride, scale = ctx.args
         d_out = _native.aligned(d_out.to(q.dtype).contiguous())
-        dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
-        for name, t in (("dq", dq), ("dk", dk), ("dv", dv)):
-            assert t.stride(-1) == 1, name
+        dq, dk, dv = (_grad_like(t) for t in (q, k, v))
         shape = _shape(q, k, v, kind, mask_stride)
         grads = (ctypes.c_int64 * 9)(*_strides(dq), *_strides(dk), *_strides(dv))
         ws_bytes = int(_native.query("tpf_xattn_backward_workspace_bytes", shape))
@@ -180,7 +187,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     FP16 is for inference.  ``1 <= D <= 128`` (copied to a multiple of 8 where it is
     none).  Other cases raise ``ValueError`` before any launch.
     """
-    if host_path(q, k, v) and (key_mask is None or _native.host_eligible(key_mask)):
+    if (host_path(q, k, v) and (key_mask is None or _native.host_eligible(key_mask))
+            and (scale is None or type(scale) in (float, int))):
         # The common form entirely in C++; None (nothing launched) for any other.
         out = _native.host().cross_attention(q, k, v, key_mask, scale)
         if out is not None:

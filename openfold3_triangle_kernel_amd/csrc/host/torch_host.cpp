@@ -415,6 +415,15 @@ Tensor xattn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   return out;
 }
 
+// A gradient in the operand's storage order, where that keeps its channels
+// contiguous (a broadcast operand's order may not).
+Tensor grad_like(const Tensor& t) {
+  Tensor g = at::empty_like(t);
+  bool fine = g.stride(3) == 1;
+  for (int i = 0; i < 3; ++i) fine = fine && g.stride(i) % 8 == 0;
+  return fine ? g : at::empty(t.sizes(), t.options());
+}
+
 struct XattnFn : torch::autograd::Function<XattnFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const std::optional<Tensor>& mask_in, int64_t kind, int64_t mask_stride,
@@ -435,7 +444,7 @@ struct XattnFn : torch::autograd::Function<XattnFn> {
     const tpf_xattn_shape s = xattn_shape(q, k, v, ctx->saved_data["kind"].toInt(),
                                           ctx->saved_data["stride"].toInt());
     const Tensor dout = kernel_grad(grads[0]);
-    Tensor d[3] = {at::empty_like(q), at::empty_like(k), at::empty_like(v)};
+    Tensor d[3] = {grad_like(q), grad_like(k), grad_like(v)};
     int64_t gs[9];
     for (int i = 0; i < 3; ++i) strides3(d[i], gs + 3 * i);
     const int64_t n = tpf_xattn_backward_workspace_bytes(&s);
@@ -666,9 +675,7 @@ std::optional<Tensor> linear(const Tensor& x, const Tensor& w) {
       return std::nullopt;
   if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1)) return std::nullopt;
   const int64_t N = w.size(0), K = w.size(1), R = x.numel() / K, most = (int64_t(1) << 30) - 1;
-  if (N % 8 || K % 8 || R > most / (N > K ? N : K) || N > most / (N > K ? N : K) ||
-      K > most / (N > K ? N : K))
-    return std::nullopt;
+  if (N % 8 || K % 8 || R > most / (N > K ? N : K) || N > most / K) return std::nullopt;
   const Tensor x2 = x.dim() == 2 ? x : x.view({R, K});
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
   const Tensor y = grad ? LinearFn::apply(x2, w) : row_gemm(x2, w, true);

@@ -297,6 +297,30 @@ def test_broadcast_and_offset_operands(gpu):
         assert torch.equal(cross_attention(q, wide[..., :64], v), cross_attention(q, k, v))
 
 
+@pytest.mark.parametrize("axis", ["batch", "head", "position", "all"])
+def test_gradients_of_broadcast_operands(gpu, axis):
+    """Operands broadcast along any axis: the gradients are those of their copies,
+    summed (in BF16, 2^-8 of the terms for each of the additions)."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    full = {"batch": (3, 1, 1), "head": (1, 4, 1), "position": (1, 1, 70), "all": (3, 4, 70)}[axis]
+    shape = tuple(1 if n > 1 else m for n, m in zip(full, (3, 4, 70)))
+    g = torch.Generator().manual_seed(12)
+    base = [torch.randn(*shape, 64, generator=g).bfloat16().to(gpu).requires_grad_(True) for _ in range(3)]
+    dout = torch.randn(3, 70, 4, 64, generator=g).bfloat16().to(gpu)
+    wide = [t.expand(3, 4, 70, 64) for t in base]
+    got = torch.autograd.grad(cross_attention(*wide), base, dout)
+    dense = [t.detach().contiguous().requires_grad_(True) for t in wide]
+    out = cross_attention(*dense)
+    assert torch.equal(out, cross_attention(*wide))
+    dims = tuple(i for i in range(3) if shape[i] == 1)
+    n = math.prod(full)
+    for a, b in zip(got, torch.autograd.grad(out, dense, dout)):
+        want = b.double().sum(dims, keepdim=True)
+        bound = 2.0 ** -8 * min(n, 32) * b.double().abs().sum(dims, keepdim=True)
+        assert ((a.double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("Nq,Nk", [(0, 5), (5, 0), (0, 0)])
 def test_empty_axes(gpu, Nq, Nk):
     from openfold3_triangle_kernel_amd import cross_attention
@@ -380,7 +404,8 @@ def test_refusals(gpu):
             ((*ops(), torch.zeros(8)), "one device"),
             ((*ops(), torch.zeros(8, device=gpu, requires_grad=True)), "must not require"),
             ((*ops(), None, 0.0), "scale"),
-            ((*ops(), None, float("inf")), "scale")):
+            ((*ops(), None, float("inf")), "scale"),
+            ((*ops(), None, torch.ones((), device=gpu)), "scale")):
         with pytest.raises(ValueError, match=match):
             cross_attention(*args)
     half = [t.requires_grad_(True) for t in ops(dtype=torch.float16)]
