@@ -15,6 +15,7 @@
 namespace tpf {
 
 constexpr float kXaLow = -3.402823466e38f;
+constexpr int kXaMaxSplits = 256;  // threads of the workgroup that joins a row's splits
 
 // Running softmax state of a wave's rows; scores and maxima m are in raw units
 // (before the scale).  The maximum is raised only once a row's scores pass it by
@@ -429,6 +430,63 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
   if (a.lse && d == 0) xa_store_stats(a, row, m, l);
 }
 
+// The same for many splits (eight or more; fewer do better with a thread a row and
+// four channels): a workgroup joins one row, its 256 threads 32 groups of four
+// channels by eight ranges of splits (s mod 8), the ranges meeting in LDS in order.
+// One token of 32 heads, 16384 states in 32 splits: 19.5 us in all against 30.
+template <bool F16>
+__global__ __launch_bounds__(256) void xattn_join_few_kernel(XAttnArgs a) {
+  __shared__ float wt[kXaMaxSplits], part[8][32][4], red[4][2];
+  const int64_t row = blockIdx.x, bh = row / a.R;
+  const int r = (int)(row - bh * a.R), tid = threadIdx.x, w = tid >> 6;
+  const float* ml = a.part_ml + 2 * (bh * a.splits * a.R + r);
+  float m0 = kXaLow, l0 = 0.f;  // this thread's split (at most 256)
+  if (tid < a.splits) {
+    m0 = ml[2 * (int64_t)tid * a.R];
+    l0 = ml[2 * (int64_t)tid * a.R + 1];
+  }
+  float m = m0;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if ((tid & 63) == 0) red[w][0] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  const float f = tid < a.splits ? fast_exp2((m0 - m) * a.c) : 0.f;
+  wt[tid] = f;
+  const float ls = lanes_sum<64>(f * l0);
+  if ((tid & 63) == 0) red[w][1] = ls;
+  __syncthreads();
+  const float l = red[0][1] + red[1][1] + red[2][1] + red[3][1];
+  const int dg = tid & 31, q = tid >> 5, d = 4 * dg;
+  f32x4 o = (f32x4)0.f;
+  if (d < a.D) {
+    const float* po = a.part_o + (bh * a.splits * a.R + r) * a.D + d;
+#pragma unroll 4
+    for (int s = q; s < a.splits; s += 8) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(po + (int64_t)s * a.R * a.D);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += wt[s] * v[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) part[q][dg][e] = o[e];
+  __syncthreads();
+  if (q || d >= a.D) return;
+#pragma unroll
+  for (int x = 1; x < 8; ++x)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += part[x][dg][e];
+  const float inv = xa_inverse(l);
+  int g, i;
+  xa_row(a, r, g, i);
+  const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
+  uint2 v;
+  v.x = xa_pair<F16>(o[0] * inv, o[1] * inv);
+  v.y = xa_pair<F16>(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d) = v;
+  if (a.lse && tid == 0) xa_store_stats(a, row, m, l);
+}
+
 // Up to 64 rows run on the streaming kernel, 32 or 64 at once; more on the tile
 // kernel, 128 rows a workgroup, or 256 up to 64 channels where those fill the
 // chip twice (512): each K and V fragment then feeds two products (64 channels,
@@ -436,16 +494,21 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
 // twice the workgroups (512 x 1500, 128 heads: 40 us against 45).  Either kernel
 // splits the states only while it has less than one workgroup a CU: further
 // splits cost more in prologues and partials than they level (16 tokens of 32
-// heads, 8191 ragged states: 86 us at 256 workgroups, 90 at 512, 117 at 2048).
+// heads, 8191 ragged states: 86 us at 256 workgroups, 90 at 512, 117 at 2048).  A
+// split has 256 states (four tiles for every two waves) or 128 (two tiles) at least
+// and there are four or none (one token, 8 heads: 512 states in 7.4 us unsplit, 10.2
+// split; one kv head of 65536 states in 13.5 us, with at most 64 splits 16; 128 rows
+// of 8192 states in 12.4 us, from 512 states a split 18.4).
 static void xattn_plan(XAttnArgs& a) {
   const bool few = a.R <= 64;
   const int64_t BH = (int64_t)a.B * a.Hk;
   a.qb = few ? (a.R > 32 ? 2 : 1) : a.D <= 64 && BH * ((a.R + 255) / 256) >= 512 ? 2 : 1;
   a.tiles = few ? 1 : (int)((a.R + 128 * a.qb - 1) / (128 * a.qb));
   int64_t s = 256 / (BH * a.tiles);
-  const int64_t most = (a.Nk + 511) / 512;  // a split is worth 512 states
+  const int64_t step = few ? 256 : 128;
+  const int64_t most = a.Nk < 4 * step ? 1 : a.Nk / step;
   if (s > most) s = most;
-  if (s > 64) s = 64;
+  if (s > kXaMaxSplits) s = kXaMaxSplits;
   if (s < 1) s = 1;
   const int64_t tiles = (a.Nk + 63) / 64;
   a.chunk = (int)((tiles + s - 1) / s) * 64;
@@ -522,8 +585,11 @@ static void xattn_forward(const XAttnArgs& a, hipStream_t s) {
   else if (a.D <= 96) xattn_launch<96, F16>(a, s);
   else xattn_launch<128, F16>(a, s);
   if (a.splits > 1) {
-    const int64_t n = (int64_t)a.B * a.Hk * a.R * (a.D / 4);
-    hipLaunchKernelGGL(xattn_join_kernel<F16>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    const int64_t rows = (int64_t)a.B * a.Hk * a.R, n = rows * (a.D / 4);
+    if (a.splits >= 8)
+      hipLaunchKernelGGL(xattn_join_few_kernel<F16>, dim3((unsigned)rows), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL(xattn_join_kernel<F16>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
   }
 }
 

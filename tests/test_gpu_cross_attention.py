@@ -133,6 +133,12 @@ FORWARD = [
     (2, 2, 2, 70, 63, 20, "bf16", "head", "tail"),
     (1, 1, 1, 64, 2500, 72, "fp16", "head", "none"),
     (1, 2, 1, 130, 6000, 128, "bf16", "head", "tail"),
+    (1, 2, 2, 1, 1100, 64, "bf16", "seq", "random"),  # a few splits
+    (1, 2, 2, 100, 650, 96, "bf16", "head", "empty"),
+    (1, 1, 1, 1, 70001, 32, "bf16", "head", "none"),  # as many as there may be
+    (1, 8, 1, 5, 1500, 128, "fp16", "head", "add"),
+    (1, 64, 64, 300, 70, 64, "bf16", "head", "tail"),  # 256 rows a workgroup needs 512 of them
+    (4, 64, 64, 513, 65, 48, "fp16", "seq", "random"),
 ]
 _T = {"bf16": torch.bfloat16, "fp16": torch.float16}
 
