@@ -35,6 +35,7 @@ struct XAttnArgs {
   float mask_floor; // lowest finite raw mask value
   int splits, chunk, tiles;  // state splits, states per split (a multiple of 64), row tiles
   int qb;           // blocks of 32 rows a wave
+  int kw;           // groups of four waves that share a row tile's states
   float* part_o;    // [B*Hk, splits, R, D] unnormalised outputs of the splits
   float* part_ml;   // [B*Hk, splits, R, 2] their raw maxima and sums
 };
@@ -190,6 +191,71 @@ __device__ __forceinline__ void xa_mask32(f32x16& s, uint32_t live, const float*
 #pragma unroll
   for (int r = 0; r < 16; ++r)
     if (!((w >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = -__builtin_inff();
+}
+
+// The tiles of 64 states that a workgroup walks over, KW at a time (one for each
+// group of four waves), in the order of the states; rounds without a live state are
+// passed over.  Every wave keeps the same state, so all take the same turns.
+template <int KW>
+struct XTiles {
+  XMask mask;
+  int k0, kend;
+  uint32_t raw[KW];
+  uint64_t live[KW];
+  bool values[KW];
+  __device__ __forceinline__ void init(const XAttnArgs& a, int batch, int kbeg, int kend_) {
+    mask.init(a, batch);
+    k0 = kbeg - 64 * KW;
+    kend = kend_;
+#pragma unroll
+    for (int t = 0; t < KW; ++t) raw[t] = mask.load(kbeg + 64 * t, kend);
+  }
+  // To the next round with a live state; false past the end.
+  __device__ __forceinline__ bool advance() {
+    for (;;) {
+      k0 += 64 * KW;
+      if (k0 >= kend) return false;
+      uint64_t any = 0;
+#pragma unroll
+      for (int t = 0; t < KW; ++t) {
+        live[t] = mask.live(raw[t]);
+        values[t] = mask.values(raw[t]);
+        raw[t] = mask.load(k0 + 64 * (KW + t), kend);
+        any |= live[t];
+      }
+      if (any) return true;
+    }
+  }
+};
+
+// Hands N blocks of a wave's accumulators from the second group of four waves to
+// the first through LDS (4 waves x N x 4 KiB); `w`: the wave's number in its group.
+template <int N>
+__device__ __forceinline__ void xa_give(char* lds, int w, const f32x16 (&o)[N]) {
+  f32x4* p = reinterpret_cast<f32x4*>(lds) + w * N * 256 + (threadIdx.x & 63);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = o[n][4 * q + e];
+      p[(4 * n + q) * 64] = v;
+    }
+}
+// o = mine * o + other * (what the second group's wave gave).
+template <int N>
+__device__ __forceinline__ void xa_take(const char* lds, int w, f32x16 (&o)[N], float mine,
+                                        float other) {
+  const f32x4* p = reinterpret_cast<const f32x4*>(lds) + w * N * 256 + (threadIdx.x & 63);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 v = p[(4 * n + q) * 64];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][4 * q + e] = mine * o[n][4 * q + e] + other * v[e];
+    }
 }
 
 // Address of row r (already split) in a [B, H, Nq, D] operand.

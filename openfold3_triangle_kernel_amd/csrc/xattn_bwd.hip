@@ -29,6 +29,7 @@ struct XAttnGrad {
   float* part_q;         // [splits, B*Hk, R, D], null when unsplit
   float *part_k, *part_v;  // [rsplits, B*Hk, Nk, D]
   int rsplits, rchunk;   // row splits of the dK / dV launch, rows per split
+  int rkw;               // its groups of four waves
   int ktiles;            // state tiles of the dK / dV launch
 };
 
@@ -70,13 +71,15 @@ __device__ __forceinline__ void xg_store(const f32x16 (&o)[DB], int D, u16* dst,
     }
 }
 
-// dQ and delta: four waves of 32 rows share K and V tiles of 64 states.
-template <int DP, bool ADD>
-__global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XAttnGrad ga) {
+// dQ and delta: four waves of 32 rows share K and V tiles of 64 states.  KW = 2:
+// two groups of four waves take the row tile's states in turn and add their sums in
+// LDS, for grids that give a CU one workgroup (as in the forward).
+template <int DP, bool ADD, int KW>
+__global__ __launch_bounds__(256 * KW, 2) void xattn_dq_kernel(XAttnGrad ga) {
   constexpr int KT = 64, TILE = KT * DP, DS = DP / 16, DB = DP / 32;
-  __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
+  __shared__ __attribute__((aligned(1024))) u16 smem[KW][2][2][TILE];
   const XAttnArgs& a = ga.f;
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int group = threadIdx.x >> 8, w = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63;
   const int64_t T = xcd_order((int64_t)a.B * a.Hk * a.splits * a.tiles);
   if (T < 0) return;
   const int tile = (int)(T % a.tiles);
@@ -89,8 +92,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XAttnGrad ga) {
   const u16* kp = a.k + b * a.k_sb + hk * a.k_sh;
   const u16* vp = a.v + b * a.v_sb + hk * a.v_sh;
 
-  XMask mask;
-  mask.init(a, b);
+  XTiles<KW> t;
+  t.init(a, b, kbeg, kend);
   XTileLoader<DP, KT, 4> lk, lv;
   lk.init(w, a.k_sn, a.D);
   lv.init(w, a.v_sn, a.D);
@@ -115,44 +118,34 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XAttnGrad ga) {
   }
   delta = xor32_sum(delta);
   const float lse = ga.lse[bh * a.R + rc], top = ADD ? ga.top[bh * a.R + rc] : 0.f;
-  if (split == 0 && lane < 32 && r < a.R) ga.delta[bh * a.R + r] = delta;
+  if (split == 0 && group == 0 && lane < 32 && r < a.R) ga.delta[bh * a.R + r] = delta;
 
   f32x16 dq[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dq[db] = zero16();
 
-  int k0 = kbeg - KT;
-  uint64_t live = 0;
-  bool values = false;
-  uint32_t raw = mask.load(kbeg, kend);
-  auto advance = [&]() {
-    for (;;) {
-      k0 += KT;
-      if (k0 >= kend) return false;
-      live = mask.live(raw);
-      values = mask.values(raw);
-      raw = mask.load(k0 + KT, kend);
-      if (live) return true;
+  auto issue = [&](int st) {
+    const uint64_t live = KW == 2 && group ? t.live[KW - 1] : t.live[0];
+    const int64_t k = t.k0 + KT * group;
+    if (live) {
+      lk.issue(kp + k * a.k_sn, live, w, smem[group][st][0]);
+      lv.issue(vp + k * a.v_sn, live, w, smem[group][st][1]);
     }
   };
-  bool more = advance();
-  if (more) {
-    lk.issue(kp + (int64_t)k0 * a.k_sn, live, w, smem[0][0]);
-    lv.issue(vp + (int64_t)k0 * a.v_sn, live, w, smem[0][1]);
-  }
+  bool more = t.advance();
+  if (more) issue(0);
   int st = 0;
   while (more) {
-    const int kc = k0;
-    const uint64_t lc = live;
-    const bool vc = values;
+    const int kc = t.k0 + KT * group;
+    const uint64_t lc = KW == 2 && group ? t.live[KW - 1] : t.live[0];
+    const bool vc = KW == 2 && group ? t.values[KW - 1] : t.values[0];
     wait_vmcnt<0>();
     lds_barrier();
-    more = advance();
-    if (more) {
-      lk.issue(kp + (int64_t)k0 * a.k_sn, live, w, smem[st ^ 1][0]);
-      lv.issue(vp + (int64_t)k0 * a.v_sn, live, w, smem[st ^ 1][1]);
-    }
-    const u16 *K = smem[st][0], *V = smem[st][1];
+    more = t.advance();
+    if (more) issue(st ^ 1);
+    const u16 *K = smem[group][st][0], *V = smem[group][st][1];
+    st ^= 1;
+    if (!lc) continue;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       f32x16 s = zero16(), dp = zero16();
@@ -161,7 +154,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XAttnGrad ga) {
 #pragma unroll
       for (int d = 0; d < DS; ++d) dp = mfma32(xa_frag<DP>(V, 32 * kb, d), dO[d], dp);
       if (lc != ~0ull || vc)
-        xa_mask32(s, (uint32_t)(lc >> (32 * kb)), vc ? mask.f : nullptr, kc + 32 * kb, a.Nk,
+        xa_mask32(s, (uint32_t)(lc >> (32 * kb)), vc ? t.mask.f : nullptr, kc + 32 * kb, a.Nk,
                   a.inv_scale, a.mask_floor);
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -173,7 +166,15 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XAttnGrad ga) {
         dq[db] = mfma32(xa_frag_t<DP>(K, 32 * kb, 1, db), p1, dq[db]);
       }
     }
-    st ^= 1;
+  }
+  if constexpr (KW == 2) {
+    static_assert(sizeof(smem) >= 4 * DB * 4096, "the join fits");
+    char* lds = reinterpret_cast<char*>(&smem[0][0][0][0]);
+    __syncthreads();
+    if (group) xa_give<DB>(lds, w, dq);
+    __syncthreads();
+    if (group) return;
+    xa_take<DB>(lds, w, dq, 1.f, 1.f);
   }
   if (r >= a.R) return;
   const int64_t BH = (int64_t)a.B * a.Hk;
@@ -189,18 +190,20 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XAttnGrad ga) {
 // V stays in LDS (and at 128 the tiles have 32 rows), so that a wave fits 256
 // registers and two run on a SIMD.  A tile inside one query head (all of them when Nq is a
 // multiple of RT) is loaded at fixed lane offsets from its first row; others
-// find each row's address.
-template <int DP, bool ADD>
-__global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
+// find each row's address.  KW = 2: two groups of four waves take the row tiles in
+// turn for the same states and add their sums in LDS.
+template <int DP, bool ADD, int KW>
+__global__ __launch_bounds__(256 * KW, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
   constexpr bool VLDS = DP > 64;
   constexpr int RT = DP == 128 ? 32 : 64, TILE = RT * DP, DS = DP / 16, DB = DP / 32, CPR = DP / 8;
   constexpr int NI = RT * CPR / 256;
   static_assert(RT * CPR % 256 == 0, "whole instructions");
-  __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
-  __shared__ __attribute__((aligned(1024))) float stats[2][ADD ? 3 : 2][64];
+  __shared__ __attribute__((aligned(1024))) u16 smem[KW][2][2][TILE];
+  __shared__ __attribute__((aligned(1024))) float stats[KW][2][ADD ? 3 : 2][64];
   __shared__ __attribute__((aligned(1024))) u16 vs[VLDS ? 128 * DP : 8];
   const XAttnArgs& a = ga.f;
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
+  const int group = threadIdx.x >> 8, w = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63,
+            h = lane >> 5;
   const int64_t BH = (int64_t)a.B * a.Hk;
   const int64_t T = xcd_order(BH * ga.rsplits * ga.ktiles);
   if (T < 0) return;
@@ -232,7 +235,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
       const bool in = live && d < a.D;
       kf[s] = in ? *reinterpret_cast<const bf16x8*>(kp + d) : zero8();
       const bf16x8 x = in ? *reinterpret_cast<const bf16x8*>(vp + d) : zero8();
-      if constexpr (VLDS)
+      if constexpr (VLDS)  // (both groups write the same values)
         *reinterpret_cast<bf16x8*>(vs + row * DP + ((2 * s + h) ^ xa_swz<DP>(row)) * 8) = x;
       else
         vf[s] = x;
@@ -257,9 +260,9 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
   }
   const bool near = a.q_sn < (1 << 23) && o_sn < (1 << 23);  // 64 rows within 2 GiB
   auto issue = [&](int r0, int st) {
-    char* dst = reinterpret_cast<char*>(smem[st][0]) + NI * w * 1024;
+    char* dst = reinterpret_cast<char*>(smem[group][st][0]) + NI * w * 1024;
     int g0, i0;
-    xa_row(a, r0, g0, i0);
+    xa_row(a, min(r0, a.R - 1), g0, i0);
     if (near && i0 + RT <= a.Nq && r0 + RT <= rend) {
       const i32x4 qr = buffer_rsrc(a.q + b * a.q_sb + (int64_t)(hk * a.G + g0) * a.q_sh +
                                    (int64_t)i0 * a.q_sn);
@@ -289,19 +292,21 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
     if (w < (ADD ? 3 : 2)) {  // wave 0: lse, 1: delta, 2: maxima of the tile's rows
       const float* src = w == 0 ? ga.lse : w == 1 ? ga.delta : ga.top;
       g2lds4(lane < RT && r0 + lane < rend ? src + bh * a.R + r0 + lane : kXaNone + (w ? 0 : 4),
-             stats[st][w]);
+             stats[group][st][w]);
     }
   };
 
   const bool some = __syncthreads_or(live ? 1 : 0);
   if (some) {
-    issue(rbeg, 0);
+    // A group past the last row loads absent rows, whose p is 0: no branch.
+    const int mine = RT * group;
+    issue(rbeg + mine, 0);
     int st = 0;
-    for (int r0 = rbeg; r0 < rend; r0 += RT, st ^= 1) {
+    for (int r0 = rbeg; r0 < rend; r0 += RT * KW, st ^= 1) {
       wait_vmcnt<0>();
       lds_barrier();
-      if (r0 + RT < rend) issue(r0 + RT, st ^ 1);
-      const u16 *Q = smem[st][0], *dO = smem[st][1];
+      if (r0 + RT * KW < rend) issue(r0 + RT * KW + mine, st ^ 1);
+      const u16 *Q = smem[group][st][0], *dO = smem[group][st][1];
 #pragma unroll
       for (int rb = 0; rb < RT / 32; ++rb) {
         f32x16 s = zero16(), dp = zero16();
@@ -313,10 +318,10 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
                       VLDS ? xa_frag<DP>(vs, 32 * w, d) : vf[VLDS ? 0 : d], dp);
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
-          const f32x4 ls = *reinterpret_cast<const f32x4*>(&stats[st][0][32 * rb + 8 * g4 + 4 * h]);
-          const f32x4 de = *reinterpret_cast<const f32x4*>(&stats[st][1][32 * rb + 8 * g4 + 4 * h]);
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(&stats[group][st][0][32 * rb + 8 * g4 + 4 * h]);
+          const f32x4 de = *reinterpret_cast<const f32x4*>(&stats[group][st][1][32 * rb + 8 * g4 + 4 * h]);
           f32x4 tp;
-          if (ADD) tp = *reinterpret_cast<const f32x4*>(&stats[st][ADD ? 2 : 0][32 * rb + 8 * g4 + 4 * h]);
+          if (ADD) tp = *reinterpret_cast<const f32x4*>(&stats[group][st][ADD ? 2 : 0][32 * rb + 8 * g4 + 4 * h]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = ADD ? (s[4 * g4 + e] + add) - tp[e] : s[4 * g4 + e];
@@ -336,6 +341,19 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
         }
       }
     }
+  }
+  if constexpr (KW == 2) {
+    static_assert(sizeof(smem) >= 4 * DB * 4096, "the join fits");
+    char* lds = reinterpret_cast<char*>(&smem[0][0][0][0]);
+    __syncthreads();
+    if (group) xa_give<DB>(lds, w, dk);
+    __syncthreads();
+    if (!group) xa_take<DB>(lds, w, dk, 1.f, 1.f);
+    __syncthreads();
+    if (group) xa_give<DB>(lds, w, dv);
+    __syncthreads();
+    if (group) return;
+    xa_take<DB>(lds, w, dv, 1.f, 1.f);
   }
   if (k >= a.Nk) return;
   const int64_t po = (((int64_t)split * BH + bh) * a.Nk + k) * a.D;
@@ -384,16 +402,18 @@ __global__ __launch_bounds__(256) void xattn_fold_kernel(XAttnGrad ga, unsigned 
   *reinterpret_cast<uint2*>(dst + b * st[0] + head * st[1] + (int64_t)pos * st[2] + d) = x;
 }
 
-// Each launch is split once its tiles leave CUs idle: up to 512 workgroups (two
-// a CU), no split below 256 states or rows.
-static void split_axis(int64_t groups, int64_t n, int64_t tile, int* splits, int* chunk) {
-  int64_t s = 512 / groups;
+// A launch that leaves CUs without a workgroup is split, 256 states or rows at least
+// to a split; one workgroup a CU has two groups of waves (forward and backward of 32
+// heads, 1024 x 1024 x 128: 138 us against 165 with up to 512 workgroups of one).
+static void split_axis(int64_t groups, int64_t n, int64_t tile, int* splits, int* chunk, int* kw) {
+  int64_t s = 256 / groups;
   if (s > (n + 255) / 256) s = (n + 255) / 256;
   if (s > 16) s = 16;
   if (s < 1) s = 1;
   const int64_t t = (n + tile - 1) / tile;
   *chunk = (int)((t + s - 1) / s * tile);
   *splits = (int)((n + *chunk - 1) / *chunk);
+  *kw = groups * *splits <= 256 && *chunk >= 128 ? 2 : 1;
 }
 
 static void grad_plan(XAttnGrad& g) {
@@ -401,8 +421,8 @@ static void grad_plan(XAttnGrad& g) {
   const int64_t BH = (int64_t)a.B * a.Hk;
   a.tiles = (a.R + 127) / 128;
   g.ktiles = (a.Nk + 127) / 128;
-  split_axis(BH * a.tiles, a.Nk, 64, &a.splits, &a.chunk);
-  split_axis(BH * g.ktiles, a.R, 64, &g.rsplits, &g.rchunk);
+  split_axis(BH * a.tiles, a.Nk, 64, &a.splits, &a.chunk, &a.kw);
+  split_axis(BH * g.ktiles, a.R, 64, &g.rsplits, &g.rchunk, &g.rkw);
 }
 
 // Workspace in floats: delta, then the partials of the split launches, each
@@ -424,10 +444,11 @@ static void grad_launch(const XAttnGrad& g, hipStream_t s) {
   const XAttnArgs& a = g.f;
   const int64_t BH = (int64_t)a.B * a.Hk;
   const int64_t n1 = BH * a.splits * a.tiles, n2 = BH * g.rsplits * g.ktiles;
-  hipLaunchKernelGGL((xattn_dq_kernel<DP, ADD>), dim3((unsigned)((n1 + 7) / 8 * 8)), dim3(256), 0, s,
-                     g);
-  hipLaunchKernelGGL((xattn_dkdv_kernel<DP, ADD>), dim3((unsigned)((n2 + 7) / 8 * 8)), dim3(256), 0,
-                     s, g);
+  const dim3 g1((unsigned)((n1 + 7) / 8 * 8)), g2((unsigned)((n2 + 7) / 8 * 8));
+  if (a.kw == 2) hipLaunchKernelGGL((xattn_dq_kernel<DP, ADD, 2>), g1, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((xattn_dq_kernel<DP, ADD, 1>), g1, dim3(256), 0, s, g);
+  if (g.rkw == 2) hipLaunchKernelGGL((xattn_dkdv_kernel<DP, ADD, 2>), g2, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((xattn_dkdv_kernel<DP, ADD, 1>), g2, dim3(256), 0, s, g);
 }
 
 template <bool ADD>
