@@ -185,7 +185,8 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
   static_assert(KW == 1 || QB == 1, "a group's results fit its tiles");
   __shared__ __attribute__((aligned(1024))) u16 smem[KW][2][2][TILE];
   __shared__ float ml[KW == 2 ? 512 : 1];
-  const int group = threadIdx.x >> 8, w = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = KW == 2 ? wave >> 2 : 0, w = wave & 3, lane = threadIdx.x & 63;
   const int64_t total = (int64_t)a.B * a.Hk * a.splits * a.tiles;
   const int64_t T = xcd_order(total);
   if (T < 0) return;

@@ -79,7 +79,8 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_dq_kernel(XAttnGrad ga) {
   constexpr int KT = 64, TILE = KT * DP, DS = DP / 16, DB = DP / 32;
   __shared__ __attribute__((aligned(1024))) u16 smem[KW][2][2][TILE];
   const XAttnArgs& a = ga.f;
-  const int group = threadIdx.x >> 8, w = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = KW == 2 ? wave >> 2 : 0, w = wave & 3, lane = threadIdx.x & 63;
   const int64_t T = xcd_order((int64_t)a.B * a.Hk * a.splits * a.tiles);
   if (T < 0) return;
   const int tile = (int)(T % a.tiles);
@@ -202,8 +203,8 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
   __shared__ __attribute__((aligned(1024))) float stats[KW][2][ADD ? 3 : 2][64];
   __shared__ __attribute__((aligned(1024))) u16 vs[VLDS ? 128 * DP : 8];
   const XAttnArgs& a = ga.f;
-  const int group = threadIdx.x >> 8, w = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63,
-            h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = KW == 2 ? wave >> 2 : 0, w = wave & 3, lane = threadIdx.x & 63, h = lane >> 5;
   const int64_t BH = (int64_t)a.B * a.Hk;
   const int64_t T = xcd_order(BH * ga.rsplits * ga.ktiles);
   if (T < 0) return;
