@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_dq_kernel(XAttnGrad ga) {
   auto issue = [&](int st) {
     const uint64_t live = KW == 2 && group ? t.live[KW - 1] : t.live[0];
     const int64_t k = t.k0 + KT * group;
-    if (live) {
+    if (KW == 1 || live) {
       lk.issue(kp + k * a.k_sn, live, w, smem[group][st][0]);
       lv.issue(vp + k * a.v_sn, live, w, smem[group][st][1]);
     }
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_dq_kernel(XAttnGrad ga) {
     if (more) issue(st ^ 1);
     const u16 *K = smem[group][st][0], *V = smem[group][st][1];
     st ^= 1;
-    if (!lc) continue;
+    if (KW == 2 && !lc) continue;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       f32x16 s = zero16(), dp = zero16();
