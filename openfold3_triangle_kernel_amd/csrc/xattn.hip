@@ -286,14 +286,16 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
 
 // Few rows (at most 32 QB, one decoded token above all): the states' bytes are
 // the bound.  Every wave streams tiles of 32 states of its own, two stages deep
-// without a barrier, and the four waves' results meet in LDS at the end.
+// without a barrier, and the four waves' results meet in LDS at the end.  32 kv heads
+// of 4096 states, one row each, unsplit: 96 us, 5.6 TB/s.  16 tokens of 32 heads on 8
+// with 8191 ragged states (403 MB live) in two splits: 79 us with the join.
 template <int DP, int QB, bool F16>
 __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
   constexpr int KT = 32, TILE = KT * DP, NI = KT * DP / 512;
   constexpr int OP = DP + 4;  // pitch of the joined rows (f32)
   __shared__ __attribute__((aligned(1024))) u16 smem[4][2][2][TILE];
   static_assert(sizeof(smem) >= 4 * 32 * (OP + 2) * 4, "the join fits");
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t T = xcd_order((int64_t)a.B * a.Hk * a.splits);
   if (T < 0) return;
   const int64_t bh = T / a.splits;
@@ -511,7 +513,8 @@ __global__ __launch_bounds__(256) void xattn_join_few_kernel(XAttnArgs a) {
 // twice the workgroups (512 x 1500, 128 heads: 40 us against 45).  Either kernel
 // splits the states only while it has less than one workgroup a CU: further
 // splits cost more in prologues and partials than they level (16 tokens of 32
-// heads, 8191 ragged states: 86 us at 256 workgroups, 90 at 512, 117 at 2048).  A
+// heads, 8191 ragged states: 86 us at 256 workgroups, 90 at 512, 117 at 2048, before the
+// wave number moved to the scalar side: 79 now).  A
 // split has 256 states (four tiles for every two waves) or 128 (two tiles) at least
 // and there are four or none (one token, 8 heads: 512 states in 7.4 us unsplit, 10.2
 // split; one kv head of 65536 states in 13.5 us, with at most 64 splits 16; 128 rows
