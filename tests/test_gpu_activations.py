@@ -175,6 +175,39 @@ def test_linear_views(gpu):
     assert empty.shape == (0, 25, 48) and not w.grad.any()
 
 
+def test_rows_past_32_bits(gpu):
+    """dy and the codec's rows beyond 2^31 elements (and 4 GiB): rows are those of a call
+    on a few of them, the weight's gradient the sum of the parts'."""
+    from openfold3_triangle_kernel_amd import compress_activation, decompress_activation, linear
+
+    R, K, N = 4_250_000, 24, 512
+    g = torch.Generator(device=gpu).manual_seed(1)
+    x = torch.empty(R, K, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+    w = torch.empty(N, K, device=gpu, dtype=torch.bfloat16).normal_(generator=g).requires_grad_(True)
+    dy = torch.empty(R, N, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+
+    def run(x, dy):
+        xs = x.detach().requires_grad_(True)
+        y = linear(xs, w)
+        return [y.detach(), *torch.autograd.grad(y, (xs, w), dy)]
+
+    whole = run(x, dy)
+    for r in (0, 2_096_900, 4_194_200, R - 100):
+        part = run(x[r:r + 100], dy[r:r + 100])
+        assert torch.equal(whole[0][r:r + 100], part[0]) and torch.equal(whole[1][r:r + 100], part[1])
+    step = R // 8 + 1
+    total = sum(run(x[r:r + step], dy[r:r + step])[2].double() for r in range(0, R, step))
+    # Nine roundings to BF16 of parts no larger than their magnitudes' sum.
+    assert ((whole[2].double() - total).abs() <= 9 * 2.0 ** -8 * 5 * R ** 0.5).all()
+    saved = compress_activation(dy)
+    for r in (0, 2_096_900, 4_194_200, R - 100):
+        few = compress_activation(dy[r:r + 100])
+        assert torch.equal(saved.codes[r:r + 100], few.codes)
+        assert torch.equal(saved.scales[r:r + 100], few.scales)
+    back = decompress_activation(saved)
+    assert torch.equal(back[-100:], decompress_activation(few))
+
+
 def test_stream_and_graph(gpu):
     from openfold3_triangle_kernel_amd import compress_activation, decompress_activation, linear
 

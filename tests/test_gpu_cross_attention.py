@@ -139,6 +139,7 @@ FORWARD = [
     (1, 8, 1, 5, 1500, 128, "fp16", "head", "add"),
     (1, 64, 64, 300, 70, 64, "bf16", "head", "tail"),  # 256 rows a workgroup needs 512 of them
     (4, 64, 64, 513, 65, 48, "fp16", "seq", "random"),
+    (8, 64, 64, 260, 70, 32, "bf16", "seq", "add"),
 ]
 _T = {"bf16": torch.bfloat16, "fp16": torch.float16}
 
@@ -419,3 +420,49 @@ def test_refusals(gpu):
         cross_attention(*half)
     with torch.no_grad():
         cross_attention(*half)
+
+
+def test_prefixes_and_shared_operands(gpu):
+    """No batch axis, more than one, and one tensor in several places."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 6, 4, 2, 33, 70, 64, seed=13)
+    mask = _mask(gpu, "random", 6, 70, 13)
+    with torch.no_grad():
+        want = cross_attention(q, k, v, mask)
+        one = cross_attention(q[2], k[2], v[2], mask[2])
+        many = cross_attention(*(t.view(1, 2, 3, *t.shape[1:]) for t in (q, k, v)), mask.view(1, 2, 3, 70))
+    assert one.shape == (33, 4, 64) and torch.equal(one, want[2])
+    assert many.shape == (1, 2, 3, 33, 4, 64) and torch.equal(many.view_as(want), want)
+    dout = torch.randn(6, 33, 4, 64, generator=torch.Generator().manual_seed(3)).bfloat16().to(gpu)
+    s, qs = k.clone().requires_grad_(True), q.clone().requires_grad_(True)
+    gq, gs = torch.autograd.grad(cross_attention(qs, s, s, mask), (qs, s), dout)
+    parts = [t.clone().requires_grad_(True) for t in (q, k, k)]
+    dq, dk, dv = torch.autograd.grad(cross_attention(*parts, mask), parts, dout)
+    assert torch.equal(gq, dq) and torch.equal(gs, dk + dv)
+
+
+def test_two_calls_at_once(gpu):
+    """Calls that overlap on two streams, each with its own workspace."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    cases = [_make(gpu, 2, 16, 4, 200, 3000, 64, seed=s) for s in (1, 2)]
+    dout = torch.randn(2, 200, 16, 64, generator=torch.Generator().manual_seed(1)).bfloat16().to(gpu)
+
+    def step(ops):
+        leaves = [t.detach().requires_grad_(True) for t in ops]
+        out = cross_attention(*leaves)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    want = [step(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(cases[i]))
+    torch.cuda.synchronize()
+    for runs, w in zip(got, want):
+        for r in runs:
+            assert all(torch.equal(a, b) for a, b in zip(r, w))

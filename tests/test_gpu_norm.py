@@ -214,6 +214,37 @@ def test_layer_norm_special_rows(gpu):
         assert torch.equal(torch.isnan(dx).any(-1), bad) and torch.isfinite(dx[~bad]).all()
 
 
+@pytest.mark.parametrize("save", ["full", "int8"])
+def test_rows_past_32_bits(gpu, save):
+    """More than 2^31 elements: a row's results are those of a call on a few rows, the
+    parameters' gradients the sums of the parts'."""
+    from openfold3_triangle_kernel_amd import layer_norm
+
+    R, C = 2_150_000, 1001
+    g = torch.Generator(device=gpu).manual_seed(1)
+    x = torch.empty(R, C, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+    dy = torch.empty(R, C, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+    w = torch.linspace(0.5, 1.5, C, device=gpu).requires_grad_(True)
+    b = torch.zeros(C, device=gpu).requires_grad_(True)
+
+    def run(x, dy):
+        xs = x.detach().requires_grad_(True)
+        y = layer_norm(xs, w, b, save=save)
+        return [y.detach(), *torch.autograd.grad(y, (xs, w, b), dy)]
+
+    whole = run(x, dy)
+    for r in (0, 1_072_800, R - 100):
+        part = run(x[r:r + 100], dy[r:r + 100])
+        assert torch.equal(whole[0][r:r + 100], part[0]) and torch.equal(whole[1][r:r + 100], part[1])
+    step = R // 8 + 1
+    parts = [run(x[r:r + step], dy[r:r + step])[2:] for r in range(0, R, step)]
+    for i in (0, 1):
+        total = sum(p[i].double() for p in parts)
+        # Chains of R / 512 rows (plus folds) in 32 bits on either side; dy xh is at
+        # most of magnitude E|dy xh| < 1 a row.
+        assert ((whole[2 + i].double() - total).abs() <= 2 * (R / 512 + 64) * 2.0 ** -24 * R).all()
+
+
 def test_empty_rows(gpu):
     from openfold3_triangle_kernel_amd import layer_norm
 
