@@ -181,7 +181,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     ``key_mask`` broadcasts to ``[*B, Nk]``: boolean (True takes the state) or
     additive floating (added to the scores in 32 bits; -inf drops the state).  K and
-    V of a dropped state are never used, whatever they hold; a row without a state
+    V of a dropped state are never used, whatever they hold; a NaN that is not dropped,
+    in an additive mask too, reaches its rows.  A row without a state
     gives zeros, and zero gradients.  ``scale`` is 1/sqrt(D) unless given.  Returns
     ``[*B, Nq, H, D]`` of the operands' type.  BF16 operands have gradients (q, k, v);
     FP16 is for inference.  ``1 <= D <= 128`` (copied to a multiple of 8 where it is

@@ -141,11 +141,19 @@ struct XTileLoader {
   }
 };
 
-// A state's additive mask value; -inf is a dead state.
-__device__ __forceinline__ bool xa_dead(float m) { return __float_as_uint(m) == 0xff800000u; }
+// A live additive value in raw score units, finite ones not below floor_.  Compared as
+// bits (between floor_ and -inf), so that a NaN passes and makes its rows NaN; a
+// maximum would turn it into the floor, a state without weight.
+__device__ __forceinline__ float xa_raw_mask(float m, float inv_scale, float floor_) {
+  const float x = m * inv_scale;
+  const uint32_t lo = __float_as_uint(floor_);
+  return __float_as_uint(x) - lo <= 0xff800000u - lo ? floor_ : x;
+}
 
 // The masks of the 64 states from k0 on: lane l holds state k0 + l.  What a
-// dead or absent state gives is 0 in `live`.
+// dead or absent state gives is 0 in `live`.  Additive values are held as
+// bits: -inf is a dead state, a NaN is not (as floats, which the build takes for
+// never NaN, the two would pass one comparison).
 struct XMask {
   const uint8_t* b = nullptr;
   const float* f = nullptr;
@@ -184,7 +192,7 @@ __device__ __forceinline__ void xa_mask32(f32x16& s, uint32_t live, const float*
     for (int r = 0; r < 16; ++r) {
       const int k = k0 + 8 * (r >> 2) + 4 * h + (r & 3);
       const float m = k < Nk ? f[k] : 0.f;
-      s[r] += fmaxf(m * inv_scale, floor_);
+      s[r] += xa_raw_mask(m, inv_scale, floor_);
     }
   }
   const uint32_t w = live >> (4 * h);

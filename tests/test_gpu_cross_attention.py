@@ -236,6 +236,46 @@ def test_dropped_states_are_never_used(gpu, bad, Nq, D):
         assert not runs[1][2][dead.expand_as(k)].any() and not runs[1][3][dead.expand_as(v)].any()
 
 
+@pytest.mark.parametrize("Nq,Nk,D", [(1, 1, 64), (1, 300, 64), (3, 1000, 128), (130, 700, 64),
+                                     (300, 200, 96), (512, 1024, 128)])
+def test_nan_in_live_places_is_not_lost(gpu, Nq, Nk, D):
+    """NaN in q, k, v or an additive mask reaches all that the formula makes of it, and
+    nothing else: a row, a kv head, a channel of a kv head, a batch entry."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    nan = float("nan")
+    ops = _make(gpu, 2, 4, 2, Nq, Nk, D, seed=9)
+    zero = torch.zeros(2, Nk, device=gpu)
+
+    def run(q, k, v, mask):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+        out = cross_attention(*leaves, mask)
+        return (out, *torch.autograd.grad(out, leaves, torch.ones_like(out)))
+
+    clean = run(*ops, zero)
+    for what in range(4):
+        q, k, v, mask = (t.detach().clone() for t in (*ops, zero))
+        hit = torch.zeros(2, Nq, 4, D, dtype=torch.bool, device=gpu)  # of the output
+        if what == 0:
+            q[0, 1, Nq // 2, 5] = nan
+            hit[0, Nq // 2, 1] = True
+        elif what == 1:
+            k[0, 1, Nk // 2, 5] = nan
+            hit[0, :, 2:] = True
+        elif what == 2:
+            v[0, 1, Nk // 2, 5] = nan
+            hit[0, :, 2:, 5] = True
+        else:
+            mask[0, Nk // 2] = nan
+            hit[0] = True
+        out, dq, dk, dv = run(q, k, v, mask)
+        assert torch.equal(out.isnan(), hit)
+        assert torch.equal(out[~hit], clean[0][~hit])
+        if what == 3:
+            for g, c in zip((dq, dk, dv), clean[1:]):
+                assert g[0].isnan().all() and torch.equal(g[1], c[1])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("Nq", [1, 100])
 def test_lowest_finite_mask(gpu, dtype, Nq):
