@@ -568,8 +568,9 @@ int tpf_wgrad_act8(const void* dy, int64_t ld_dy, const void* codes, const void*
  * three axes (multiples of 8, 0 for a broadcast axis; channels contiguous);
  * out [B, Nq, H, D] contiguous.  D is a multiple of 8 up to 128.  mask, one
  * entry per state [B, Nk] with batch stride mask_stride (0: shared): bytes
- * (0 drops the state) or f32 added to the scores (-inf drops it).  K and V of a
- * dropped state are never used, whatever they hold.  A row without a state
+ * (0 drops the state) or f32 added to the scores (-inf drops it; finite values count as
+ * if within +-1.5e38 scale).  1e-30 < scale < 1e30.  K and V of a dropped state are
+ * never used, whatever they hold; a NaN that is not dropped reaches its rows.  A row without a state
  * gives 0, and gradients of 0.  Every tensor starts on 16 bytes.
  * lse: f32 [B, H, Nq], or [2, B, H, Nq] with an f32 mask: the rows' softmax
  * statistics for the backward; null when none follows.

@@ -51,8 +51,8 @@ def _check(q, k, v, key_mask, scale) -> None:
     heads, kv_heads = q.shape[-3], k.shape[-3]
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise _unsupported("the query heads must be a positive multiple of the kv heads")
-    if scale is not None and not (isinstance(scale, numbers.Real) and 0.0 < scale < 1e30):
-        raise _unsupported("scale must be a positive finite number")
+    if scale is not None and not (isinstance(scale, numbers.Real) and 1e-30 < scale < 1e30):
+        raise _unsupported("scale must be a number between 1e-30 and 1e30")
     tensors = [q, k, v]
     if key_mask is not None:
         if not isinstance(key_mask, torch.Tensor):
@@ -180,7 +180,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """Attention of ``q`` [*B, H, Nq, D] to the states ``k``, ``v`` [*B, Hk, Nk, D].
 
     ``key_mask`` broadcasts to ``[*B, Nk]``: boolean (True takes the state) or
-    additive floating (added to the scores in 32 bits; -inf drops the state).  K and
+    additive floating (added to the scores in 32 bits, finite values as if within
+    +-1.5e38 ``scale``; -inf drops the state).  K and
     V of a dropped state are never used, whatever they hold; a NaN that is not dropped,
     in an additive mask too, reaches its rows.  A row without a state
     gives zeros, and zero gradients.  ``scale`` is 1/sqrt(D) unless given.  Returns

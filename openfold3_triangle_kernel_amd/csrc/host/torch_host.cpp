@@ -483,7 +483,7 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
   for (const Tensor* t : {&q, &k, &v})
     if (!xattn_operand(*t)) return std::nullopt;
   const double scale = scale_in ? *scale_in : 1.0 / std::sqrt((double)D);
-  if (!(scale > 0.0 && scale < 1e30)) return std::nullopt;
+  if (!(scale > 1e-30 && scale < 1e30)) return std::nullopt;
   Tensor mask;
   int64_t kind = TPF_MASK_NONE, mask_stride = 0;
   if (mask_in) {

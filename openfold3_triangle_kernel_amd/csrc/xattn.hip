@@ -565,8 +565,8 @@ int xattn_check(XAttnArgs& a, const tpf_xattn_shape* s, double scale, const char
     return set_error(TPF_ERR_ARG, "%s: dtype must be TPF_BF16 or TPF_F16", fn);
   if (s->mask_kind < 0 || s->mask_kind > 2 || s->mask_stride < 0)
     return set_error(TPF_ERR_ARG, "%s: bad mask", fn);
-  if (!(scale > 0.0) || !(scale < 1e30))
-    return set_error(TPF_ERR_ARG, "%s: the scale must be positive", fn);
+  if (!(scale > 1e-30) || !(scale < 1e30))  // it and its reciprocal in FP32
+    return set_error(TPF_ERR_ARG, "%s: the scale must be between 1e-30 and 1e30", fn);
   a.q_sb = s->q_stride[0]; a.q_sh = s->q_stride[1]; a.q_sn = s->q_stride[2];
   a.k_sb = s->k_stride[0]; a.k_sh = s->k_stride[1]; a.k_sn = s->k_stride[2];
   a.v_sb = s->v_stride[0]; a.v_sh = s->v_stride[1]; a.v_sn = s->v_stride[2];

@@ -32,7 +32,7 @@ struct XAttnArgs {
   FastDiv div_nq;
   float c;          // scale * log2(e)
   float inv_scale;  // additive masks enter the raw scores divided by the scale
-  float mask_floor; // lowest finite raw mask value
+  float mask_floor; // lowest finite raw mask value, its negative the highest
   int splits, chunk, tiles;  // state splits, states per split (a multiple of 64), row tiles
   int qb;           // blocks of 32 rows a wave
   int kw;           // groups of four waves that share a row tile's states
@@ -141,13 +141,13 @@ struct XTileLoader {
   }
 };
 
-// A live additive value in raw score units, finite ones not below floor_.  Compared as
-// bits (between floor_ and -inf), so that a NaN passes and makes its rows NaN; a
-// maximum would turn it into the floor, a state without weight.
-__device__ __forceinline__ float xa_raw_mask(float m, float inv_scale, float floor_) {
-  const float x = m * inv_scale;
-  const uint32_t lo = __float_as_uint(floor_);
-  return __float_as_uint(x) - lo <= 0xff800000u - lo ? floor_ : x;
+// A live additive value, given by its bits, in raw score units: finite ones within
+// +-floor_, so that they stay finite beside any score.  NaN and infinity are told by the
+// bits and pass as they are: their rows are NaN, as the formula's.  (A clamp alone would
+// turn a NaN into the floor, a state without weight.)
+__device__ __forceinline__ float xa_raw_mask(uint32_t m, float inv_scale, float floor_) {
+  const float x = __builtin_amdgcn_fmed3f(__uint_as_float(m) * inv_scale, floor_, -floor_);
+  return (m & 0x7fffffffu) < 0x7f800000u ? x : __uint_as_float(m);
 }
 
 // The masks of the 64 states from k0 on: lane l holds state k0 + l.  What a
@@ -191,7 +191,7 @@ __device__ __forceinline__ void xa_mask32(f32x16& s, uint32_t live, const float*
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int k = k0 + 8 * (r >> 2) + 4 * h + (r & 3);
-      const float m = k < Nk ? f[k] : 0.f;
+      const uint32_t m = k < Nk ? reinterpret_cast<const uint32_t*>(f)[k] : 0u;
       s[r] += xa_raw_mask(m, inv_scale, floor_);
     }
   }

@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_dkdv_kernel(XAttnGrad ga) {
   } else if (a.mask_kind == kMaskF32) {
     const uint32_t m = ((const uint32_t*)a.mask)[(int64_t)b * a.mask_sb + kc];
     live = live && m != 0xff800000u;
-    add = live ? xa_raw_mask(__uint_as_float(m), a.inv_scale, a.mask_floor) : 0.f;
+    add = live ? xa_raw_mask(m, a.inv_scale, a.mask_floor) : 0.f;
   }
   bf16x8 kf[DS], vf[VLDS ? 1 : DS];
   {

@@ -301,6 +301,27 @@ def test_lowest_finite_mask(gpu, dtype, Nq):
     assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("Nq", [1, 100])
+def test_highest_finite_mask(gpu, Nq):
+    """States with the type's highest value outweigh all others: the row is their mean
+    (the scores vanish beside it), and the others' gradients are 0."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = (t.requires_grad_(True) for t in _make(gpu, 2, 2, 2, Nq, 130, 64, seed=8))
+    mask = torch.randn(2, 130, generator=torch.Generator().manual_seed(8)).to(gpu)
+    mask[0, 70:72] = mask[1, 5:7] = torch.finfo(torch.float32).max
+    out = cross_attention(q, k, v, mask)
+    dv, = torch.autograd.grad(out, v, torch.ones_like(out))
+    for b, top in ((0, slice(70, 72)), (1, slice(5, 7))):
+        pair = v[b, :, top].double()
+        # p = 1 / 2 is exact, the output rounded once; dv sums Nq halves, rounded once.
+        assert ((out[b].double() - pair.mean(-2)).abs() <= 2.0 ** -8 * pair.abs().sum(-2)).all()
+        assert ((dv[b, :, top].double() - Nq / 2).abs() <= 2.0 ** -8 * Nq / 2).all()
+        rest = torch.ones(130, dtype=torch.bool, device=gpu)
+        rest[top] = False
+        assert not dv[b][:, rest].any()
+
+
 def test_masks_that_broadcast(gpu):
     from openfold3_triangle_kernel_amd import cross_attention
 
@@ -452,6 +473,7 @@ def test_refusals(gpu):
             ((*ops(), torch.zeros(8, device=gpu, requires_grad=True)), "must not require"),
             ((*ops(), None, 0.0), "scale"),
             ((*ops(), None, float("inf")), "scale"),
+            ((*ops(), None, 1e-31), "scale"),
             ((*ops(), None, torch.ones((), device=gpu)), "scale")):
         with pytest.raises(ValueError, match=match):
             cross_attention(*args)
