@@ -24,6 +24,7 @@ from .attention import _device_supported, _is_gfx950
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # TPF_BF16, TPF_F16, TPF_F32
 _BLOCK = 32
 _GEMM_SPAN = (1 << 31) - 1  # bytes of a GEMM operand
+_MAX_FEATURES = 1 << 23  # and elements between rows: 64 of them lie within 32-bit offsets
 
 
 class CompressedActivation:
@@ -165,8 +166,10 @@ def _row_gemm(a: torch.Tensor, b: torch.Tensor, b_kc: bool) -> torch.Tensor:
 
 
 def _gemm_rows(x: torch.Tensor) -> torch.Tensor:
-    """[R, C] rows as the GEMM reads them: 16-byte aligned rows of whole vectors."""
-    if x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < x.shape[1])):
+    """[R, C] rows as the GEMM reads them: 16-byte aligned rows of whole vectors, 64 of
+    them within 32-bit offsets."""
+    ld = x.stride(0)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and (ld % 8 or not x.shape[1] <= ld <= _MAX_FEATURES)):
         x = x.contiguous()
     return _native.aligned(x)
 
@@ -224,7 +227,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, save: str = "int8") -> torch.T
 
     For the gradient of ``weight`` the input is kept in 8 bits (``save="int8"``, about
     half of BF16) or as it is (``"full"``).  ``x`` is BF16, ``weight`` BF16 or FP32 (used
-    in BF16, its gradient from FP32 sums in its own type); K and N are multiples of 8.
+    in BF16, its gradient from FP32 sums in its own type); K and N are multiples of 8 up
+    to 2^23.
     """
     if save not in ("int8", "full"):
         raise ValueError('save must be "int8" or "full"')
@@ -241,8 +245,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, save: str = "int8") -> torch.T
     if weight.dtype not in (torch.bfloat16, torch.float32) or weight.device != x.device:
         raise ValueError("linear needs a BF16 or FP32 weight on the input's device")
     N, K = weight.shape
-    if N < 8 or N % 8 or K % 8 or N * K * 2 > _GEMM_SPAN:
-        raise ValueError("linear needs feature counts that are multiples of 8, the weight below 2 GiB")
+    if N < 8 or N % 8 or K % 8 or max(N, K) > _MAX_FEATURES or N * K * 2 > _GEMM_SPAN:
+        raise ValueError("linear needs feature counts that are multiples of 8 up to 2^23, "
+                         "the weight below 2 GiB")
     if x.numel() == 0:
         return x.matmul(weight.to(x.dtype).t())
     return _LinearFn.apply(x.reshape(-1, K), weight, save).view(x.shape[:-1] + (N,))

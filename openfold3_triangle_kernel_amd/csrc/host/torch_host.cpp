@@ -675,7 +675,8 @@ std::optional<Tensor> linear(const Tensor& x, const Tensor& w) {
       return std::nullopt;
   if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1)) return std::nullopt;
   const int64_t N = w.size(0), K = w.size(1), R = x.numel() / K, most = (int64_t(1) << 30) - 1;
-  if (N % 8 || K % 8 || R > most / (N > K ? N : K) || N > most / K) return std::nullopt;
+  const int64_t wide = N > K ? N : K;
+  if (N % 8 || K % 8 || wide > (1 << 23) || R > most / wide || N > most / K) return std::nullopt;
   const Tensor x2 = x.dim() == 2 ? x : x.view({R, K});
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
   const Tensor y = grad ? LinearFn::apply(x2, w) : row_gemm(x2, w, true);

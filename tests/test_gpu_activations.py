@@ -242,11 +242,32 @@ def test_stream_and_graph(gpu):
         assert all(torch.equal(p, q) for p, q in zip(held, step(new)))
 
 
+@pytest.mark.parametrize("save", ["int8", "full"])
+def test_linear_of_far_rows(gpu, save):
+    """Rows further apart than the GEMM's 32-bit offsets serve, in the input and in the
+    gradient: as of their contiguous copies."""
+    from openfold3_triangle_kernel_amd import linear
+
+    g = torch.Generator().manual_seed(5)
+    far = torch.zeros(3, (1 << 24) + 8, device=gpu, dtype=torch.bfloat16)
+    x, dy = far[:, :64], far[:, 64:64 + 24]
+    x.copy_(torch.randn(3, 64, generator=g))
+    dy.copy_(torch.randn(3, 24, generator=g))
+    runs = []
+    for rows, grad in ((x, dy), (x.contiguous(), dy.contiguous())):
+        rows = rows.detach().requires_grad_(True)
+        w = torch.randn(24, 64, generator=torch.Generator().manual_seed(6)).to(gpu).requires_grad_(True)
+        y = linear(rows, w, save=save)
+        runs.append((y, *torch.autograd.grad(y, (rows, w), grad)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
 def test_refusals(gpu):
     from openfold3_triangle_kernel_amd import compress_activation, decompress_activation, linear
 
     x = torch.zeros(4, 16, device=gpu, dtype=torch.bfloat16)
     w = torch.zeros(8, 16, device=gpu, dtype=torch.bfloat16)
+    big = torch.zeros((1 << 23) + 8, 8, device=gpu, dtype=torch.bfloat16)
     for call, match in ((lambda: compress_activation(x.cpu()), "GPU"),
                         (lambda: compress_activation(x.double()), "BF16"),
                         (lambda: compress_activation(x[:, :0]), "channels"),
@@ -256,6 +277,7 @@ def test_refusals(gpu):
                         (lambda: linear(x, w[:, :8]), "weight"),
                         (lambda: linear(x, w[:4]), "multiples of 8"),
                         (lambda: linear(x[:, :12], w[:, :12]), "multiples of 8"),
+                        (lambda: linear(x[:, :8], big), "2\\^23"),
                         (lambda: linear(x, w.cpu()), "device"),
                         (lambda: linear(x, w.half()), "weight"),
                         (lambda: linear(x, w, save="none"), "save")):
