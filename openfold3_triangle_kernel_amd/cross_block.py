@@ -132,7 +132,8 @@ def _stock_cross_attention(q, k, v, key_mask):
     if key_mask is not None:
         drop = key_mask[..., None, None, :]
         s = s.masked_fill(~drop, float("-inf")) if drop.dtype == torch.bool else s + drop.float()
-    top = s.amax(-1, keepdim=True)
+    # The maximum only guards the exponentials; 0 for a row without a state.
+    top = s.detach().amax(-1, keepdim=True) if s.shape[-1] else s.new_zeros(s.shape[:-1] + (1,))
     p = torch.exp(s - top.masked_fill(torch.isneginf(top), 0.0))
     total = p.sum(-1, keepdim=True)
     p = p / total.masked_fill(total == 0, 1.0)

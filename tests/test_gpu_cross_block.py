@@ -168,3 +168,16 @@ def test_second_derivatives_are_refused(gpu):
         g, = torch.autograd.grad(out, wrt, torch.ones_like(out), create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.sum().backward()
+
+
+@pytest.mark.parametrize("Nq,Nk", [(3, 0), (0, 5), (0, 0)])
+def test_block_of_empty_axes(gpu, Nq, Nk):
+    block = _make(gpu).bfloat16()
+    x = torch.randn(2, Nq, 128, device=gpu).bfloat16().requires_grad_(True)
+    kv = torch.randn(2, Nk, 192, device=gpu).bfloat16().requires_grad_(True)
+    for mask in (None, torch.ones(2, Nk, dtype=torch.bool, device=gpu), torch.zeros(2, Nk, device=gpu)):
+        out = block(x, kv, mask)
+        assert out.shape == x.shape and not out.any()  # no state: nothing attended
+        params = list(block.parameters())
+        grads = torch.autograd.grad(out, [x, kv, *params], torch.ones_like(out), allow_unused=True)
+        assert not any(g.any() for g in grads if g is not None)

@@ -173,3 +173,14 @@ def test_block_runs_its_formulas_on_the_cpu():
     for bad in (dict(no_heads=3, no_kv_heads=2), dict(no_heads=2, activation_save="int4")):
         with pytest.raises(ValueError):
             CrossAttention(8, 8, 8, **bad)
+
+
+@pytest.mark.parametrize("Nq,Nk", [(3, 0), (0, 5), (0, 0)])
+def test_block_of_empty_axes_on_the_cpu(Nq, Nk):
+    block = CrossAttention(16, 24, 8, 4, no_kv_heads=2)
+    x, kv = torch.randn(2, Nq, 16, requires_grad=True), torch.randn(2, Nk, 24, requires_grad=True)
+    for mask in (None, torch.ones(2, Nk, dtype=torch.bool), torch.zeros(2, Nk)):
+        out = block(x, kv, mask)
+        assert out.shape == x.shape and not out.any()  # no state: nothing attended
+        for g in torch.autograd.grad(out, [x, kv, *block.parameters()], torch.ones_like(out)):
+            assert not g.any()
