@@ -575,6 +575,11 @@ int tpf_wgrad_act8(const void* dy, int64_t ld_dy, const void* codes, const void*
  * lse: f32 [B, H, Nq], or [2, B, H, Nq] with an f32 mask: the rows' softmax
  * statistics for the backward; null when none follows.
  * The forward serves BF16 and FP16, the backward BF16.
+ *
+ * The _shadow entry points carry what the rounding of out drops: residual, BF16 laid
+ * out as out, which the backward adds to out in delta = rowsum(dout * out), as the
+ * triangle attention's do.  dout v^T and delta nearly cancel in what the states' V
+ * have in common; from the rounded out alone, that rounding is left in the gradients.
  * ---------------------------------------------------------------------- */
 enum { TPF_MASK_NONE = 0, TPF_MASK_BYTES = 1, TPF_MASK_F32 = 2 };
 typedef struct tpf_xattn_shape {
@@ -586,6 +591,10 @@ int64_t tpf_xattn_forward_workspace_bytes(const tpf_xattn_shape* shape);
 int tpf_xattn_forward(const void* q, const void* k, const void* v, const void* mask, void* out,
                       float* lse, void* workspace, int64_t workspace_bytes,
                       const tpf_xattn_shape* shape, double scale, void* stream);
+int tpf_xattn_forward_shadow_bf16(const void* q, const void* k, const void* v, const void* mask,
+                                  void* out, float* lse, void* residual, void* workspace,
+                                  int64_t workspace_bytes, const tpf_xattn_shape* shape, double scale,
+                                  void* stream);
 /* Gradients of q, k and v from the forward's out and lse and the upstream
  * gradient dout [B, Nq, H, D] (contiguous).  grad_strides: the element strides
  * (batch, head, position) of dq, dk and dv, nine values. */
@@ -595,6 +604,11 @@ int tpf_xattn_backward_bf16(const void* q, const void* k, const void* v, const v
                             void* dv, void* workspace, int64_t workspace_bytes,
                             const tpf_xattn_shape* shape, const int64_t* grad_strides,
                             double scale, void* stream);
+int tpf_xattn_backward_shadow_bf16(const void* q, const void* k, const void* v, const void* mask,
+                                   const void* out, const void* residual, const void* dout,
+                                   const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                   int64_t workspace_bytes, const tpf_xattn_shape* shape,
+                                   const int64_t* grad_strides, double scale, void* stream);
 
 #ifdef __cplusplus
 }

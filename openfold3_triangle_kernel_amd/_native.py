@@ -158,8 +158,10 @@ SIGNATURES: dict[str, tuple] = {
         _I32, [_P, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
     "tpf_xattn_forward_workspace_bytes": (_I64, [_P]),
     "tpf_xattn_forward": (_I32, [_P] * 7 + [_I64, _P, _F64, _P]),
+    "tpf_xattn_forward_shadow_bf16": (_I32, [_P] * 8 + [_I64, _P, _F64, _P]),
     "tpf_xattn_backward_workspace_bytes": (_I64, [_P]),
     "tpf_xattn_backward_bf16": (_I32, [_P] * 11 + [_I64, _P, _P, _F64, _P]),
+    "tpf_xattn_backward_shadow_bf16": (_I32, [_P] * 12 + [_I64, _P, _P, _F64, _P]),
 }
 
 _LOCK = threading.Lock()

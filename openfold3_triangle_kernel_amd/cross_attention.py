@@ -21,7 +21,7 @@ import torch
 
 from . import _native
 from .activations import differentiable_once, host_path
-from .attention import _device_supported
+from .attention import _device_supported, shadow_enabled
 
 _MAX_HEAD_DIM = 128
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # TPF_BF16, TPF_F16
@@ -130,7 +130,8 @@ def _shape(q, k, v, kind, mask_stride):
                   *_strides(k), *_strides(v))
 
 
-def _forward(q, k, v, mask, kind, mask_stride, scale, want_lse):
+def _forward(q, k, v, mask, kind, mask_stride, scale, want_lse, shadow=False):
+    """(out, lse, what out's rounding drops); what is not asked for is None."""
     B, H, Nq, D = q.shape
     out = torch.empty((B, Nq, H, D), device=q.device, dtype=q.dtype)
     lse = torch.empty((2 if kind == _MASK_F32 else 1, B, H, Nq), device=q.device,
@@ -138,27 +139,30 @@ def _forward(q, k, v, mask, kind, mask_stride, scale, want_lse):
     shape = _shape(q, k, v, kind, mask_stride)
     ws_bytes = int(_native.query("tpf_xattn_forward_workspace_bytes", shape))
     ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes > 0 else None
+    residual = torch.empty_like(out) if shadow else None
+    name, kept = ("tpf_xattn_forward", ()) if residual is None else (
+        "tpf_xattn_forward_shadow_bf16", (residual.data_ptr(),))
     with _native.device_ctx(q.device):
-        _native.call("tpf_xattn_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                     _native.ptr(mask), out.data_ptr(), _native.ptr(lse), _native.ptr(ws),
+        _native.call(name, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                     _native.ptr(mask), out.data_ptr(), _native.ptr(lse), *kept, _native.ptr(ws),
                      max(ws_bytes, 0), shape, scale, _native.stream_of(q))
-    return out, lse
+    return out, lse, residual
 
 
 class _CrossAttentionFn(torch.autograd.Function):
     """Operands as the kernels read them: q [B, H, Nq, D], k and v [B, Hk, Nk, D]."""
 
     @staticmethod
-    def forward(ctx, q, k, v, mask, kind, mask_stride, scale):
-        out, lse = _forward(q, k, v, mask, kind, mask_stride, scale, True)
-        ctx.save_for_backward(q, k, v, mask, out, lse)
+    def forward(ctx, q, k, v, mask, kind, mask_stride, scale, shadow):
+        out, lse, residual = _forward(q, k, v, mask, kind, mask_stride, scale, True, shadow)
+        ctx.save_for_backward(q, k, v, mask, out, lse, residual)
         ctx.args = (kind, mask_stride, scale)
         return out
 
     @staticmethod
     @differentiable_once
     def backward(ctx, d_out):
-        q, k, v, mask, out, lse = ctx.saved_tensors
+        q, k, v, mask, out, lse, residual = ctx.saved_tensors
         kind, mask_stride, scale = ctx.args
         d_out = _native.aligned(d_out.to(q.dtype).contiguous())
         dq, dk, dv = (_grad_like(t) for t in (q, k, v))
@@ -166,12 +170,14 @@ class _CrossAttentionFn(torch.autograd.Function):
         grads = (ctypes.c_int64 * 9)(*_strides(dq), *_strides(dk), *_strides(dv))
         ws_bytes = int(_native.query("tpf_xattn_backward_workspace_bytes", shape))
         ws = torch.empty(max(ws_bytes, 16), device=q.device, dtype=torch.uint8)
+        name, kept = ("tpf_xattn_backward_bf16", ()) if residual is None else (
+            "tpf_xattn_backward_shadow_bf16", (residual.data_ptr(),))
         with _native.device_ctx(q.device):
-            _native.call("tpf_xattn_backward_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                         _native.ptr(mask), out.data_ptr(), d_out.data_ptr(), lse.data_ptr(),
+            _native.call(name, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                         _native.ptr(mask), out.data_ptr(), *kept, d_out.data_ptr(), lse.data_ptr(),
                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes,
                          shape, grads, scale, _native.stream_of(q))
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -186,8 +192,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     in an additive mask too, reaches its rows.  A row without a state
     gives zeros, and zero gradients.  ``scale`` is 1/sqrt(D) unless given.  Returns
     ``[*B, Nq, H, D]`` of the operands' type.  BF16 operands have gradients (q, k, v);
-    FP16 is for inference.  ``1 <= D <= 128`` (copied to a multiple of 8 where it is
-    none).  Other cases raise ``ValueError`` before any launch.
+    FP16 is for inference.  With the policy of ``attention.shadow_enabled`` (the default)
+    a training forward also keeps what the output's rounding drops, a tensor of the
+    output's size: no rounding of the output then enters the gradients, however much the
+    states' values have in common.  ``1 <= D <= 128`` (copied to a multiple of 8 where it
+    is none).  Other cases raise ``ValueError`` before any launch.
     """
     if (host_path(q, k, v) and (key_mask is None or _native.host_eligible(key_mask))
             and (scale is None or type(scale) in (float, int))):
@@ -216,7 +225,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     q, k, v = _operand(q), _operand(k), _operand(v)
     mask, kind, mask_stride = _mask_operand(key_mask, prefix, batch, Nk)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out = _CrossAttentionFn.apply(q, k, v, mask, kind, mask_stride, float(scale))
+        out = _CrossAttentionFn.apply(q, k, v, mask, kind, mask_stride, float(scale),
+                                      shadow_enabled())
     else:
         out = _forward(q, k, v, mask, kind, mask_stride, float(scale), False)[0]
     if pad:

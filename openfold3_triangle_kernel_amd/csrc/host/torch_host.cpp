@@ -402,16 +402,24 @@ tpf_xattn_shape xattn_shape(const Tensor& q, const Tensor& k, const Tensor& v, i
 }
 
 Tensor xattn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask,
-                     int64_t kind, int64_t mask_stride, double scale, Tensor* lse) {
+                     int64_t kind, int64_t mask_stride, double scale, Tensor* lse, Tensor* res) {
   const tpf_xattn_shape s = xattn_shape(q, k, v, kind, mask_stride);
   Tensor out = at::empty({s.B, s.Nq, s.H, s.D}, q.options());
   if (lse) *lse = at::empty({kind == TPF_MASK_F32 ? 2 : 1, s.B, s.H, s.Nq}, like(q, at::kFloat));
   const int64_t n = tpf_xattn_forward_workspace_bytes(&s);
   const Tensor ws = bytes(q, n);
-  check(tpf_xattn_forward(cptr(q), cptr(k), cptr(v), cptr(mask), out.data_ptr(),
-                          lse ? (float*)lse->data_ptr() : nullptr, mptr(ws), n < 0 ? 0 : n, &s, scale,
-                          stream()),
-        "tpf_xattn_forward");
+  if (res) {
+    *res = at::empty_like(out);
+    check(tpf_xattn_forward_shadow_bf16(cptr(q), cptr(k), cptr(v), cptr(mask), out.data_ptr(),
+                                        (float*)lse->data_ptr(), res->data_ptr(), mptr(ws),
+                                        n < 0 ? 0 : n, &s, scale, stream()),
+          "tpf_xattn_forward_shadow_bf16");
+  } else {
+    check(tpf_xattn_forward(cptr(q), cptr(k), cptr(v), cptr(mask), out.data_ptr(),
+                            lse ? (float*)lse->data_ptr() : nullptr, mptr(ws), n < 0 ? 0 : n, &s, scale,
+                            stream()),
+          "tpf_xattn_forward");
+  }
   return out;
 }
 
@@ -427,11 +435,11 @@ Tensor grad_like(const Tensor& t) {
 struct XattnFn : torch::autograd::Function<XattnFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const std::optional<Tensor>& mask_in, int64_t kind, int64_t mask_stride,
-                        double scale) {
+                        double scale, bool shadow) {
     const Tensor mask = mask_in.value_or(Tensor());
-    Tensor lse;
-    Tensor out = xattn_forward(q, k, v, mask, kind, mask_stride, scale, &lse);
-    ctx->save_for_backward({q, k, v, mask, out, lse});
+    Tensor lse, res;
+    Tensor out = xattn_forward(q, k, v, mask, kind, mask_stride, scale, &lse, shadow ? &res : nullptr);
+    ctx->save_for_backward({q, k, v, mask, out, lse, res});
     ctx->saved_data["kind"] = kind;
     ctx->saved_data["stride"] = mask_stride;
     ctx->saved_data["scale"] = scale;
@@ -440,7 +448,7 @@ struct XattnFn : torch::autograd::Function<XattnFn> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list sv = ctx->get_saved_variables();
-    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &mask = sv[3], &out = sv[4], &lse = sv[5];
+    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &mask = sv[3], &out = sv[4], &lse = sv[5], &res = sv[6];
     const tpf_xattn_shape s = xattn_shape(q, k, v, ctx->saved_data["kind"].toInt(),
                                           ctx->saved_data["stride"].toInt());
     const Tensor dout = kernel_grad(grads[0]);
@@ -449,11 +457,18 @@ struct XattnFn : torch::autograd::Function<XattnFn> {
     for (int i = 0; i < 3; ++i) strides3(d[i], gs + 3 * i);
     const int64_t n = tpf_xattn_backward_workspace_bytes(&s);
     const Tensor ws = bytes(q, n < 16 ? 16 : n);
-    check(tpf_xattn_backward_bf16(cptr(q), cptr(k), cptr(v), cptr(mask), cptr(out), cptr(dout),
-                                  (const float*)cptr(lse), mptr(d[0]), mptr(d[1]), mptr(d[2]),
-                                  mptr(ws), n, &s, gs, ctx->saved_data["scale"].toDouble(), stream()),
-          "tpf_xattn_backward_bf16");
-    return once({d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor()});
+    const double scale = ctx->saved_data["scale"].toDouble();
+    if (res.defined())
+      check(tpf_xattn_backward_shadow_bf16(cptr(q), cptr(k), cptr(v), cptr(mask), cptr(out), cptr(res),
+                                           cptr(dout), (const float*)cptr(lse), mptr(d[0]), mptr(d[1]),
+                                           mptr(d[2]), mptr(ws), n, &s, gs, scale, stream()),
+            "tpf_xattn_backward_shadow_bf16");
+    else
+      check(tpf_xattn_backward_bf16(cptr(q), cptr(k), cptr(v), cptr(mask), cptr(out), cptr(dout),
+                                    (const float*)cptr(lse), mptr(d[0]), mptr(d[1]), mptr(d[2]),
+                                    mptr(ws), n, &s, gs, scale, stream()),
+            "tpf_xattn_backward_bf16");
+    return once({d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -464,9 +479,10 @@ bool xattn_operand(const Tensor& t) {
   return true;
 }
 
+// sh: the policy variable of the shadow residual (env_flag).
 std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v,
                                       const std::optional<Tensor>& mask_in,
-                                      std::optional<double> scale_in) {
+                                      std::optional<double> scale_in, const std::string& sh) {
   if (transforms_active() || !q.is_cuda()) return std::nullopt;
   const c10::DeviceIndex dev = c10::hip::current_device();
   for (const Tensor* t : {&q, &k, &v})
@@ -476,6 +492,7 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
   const bool grad = at::GradMode::is_enabled() &&
                     (q.requires_grad() || k.requires_grad() || v.requires_grad());
   if (type != at::kBFloat16 && (type != at::kHalf || grad)) return std::nullopt;
+  if (grad && sh != "0" && sh != "1") return std::nullopt;
   const int64_t B = q.size(0), D = q.size(3), Nk = k.size(2);
   if (k.sizes() != v.sizes() || k.size(0) != B || k.size(3) != D || D % 8 || D > 128 ||
       q.size(1) % k.size(1))
@@ -496,8 +513,8 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
     kind = mt == at::kBool ? TPF_MASK_BYTES : TPF_MASK_F32;
     mask_stride = mask.dim() == 2 && mask.size(0) > 1 ? Nk : 0;
   }
-  if (grad) return XattnFn::apply(q, k, v, mask_in, kind, mask_stride, scale);
-  return xattn_forward(q, k, v, mask, kind, mask_stride, scale, nullptr);
+  if (grad) return XattnFn::apply(q, k, v, mask_in, kind, mask_stride, scale, sh == "1");
+  return xattn_forward(q, k, v, mask, kind, mask_stride, scale, nullptr, nullptr);
 }
 
 // ---------------------------------------------------------------- layer norm
@@ -711,7 +728,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return attention(q, k, v, res_mask, pair_bias, backward, shadow);
   });
   m.def("trimul", &trimul, pybind11::call_guard<pybind11::gil_scoped_release>());
-  m.def("cross_attention", &cross_attention, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("cross_attention", [](const Tensor& q, const Tensor& k, const Tensor& v,
+                              const std::optional<Tensor>& mask, std::optional<double> scale) {
+    const std::string shadow = env_flag("TURBOPAIRFORMER_SR_SHADOW", "OPENFOLD3_SR_SHADOW");
+    pybind11::gil_scoped_release nogil;
+    return cross_attention(q, k, v, mask, scale, shadow);
+  });
   m.def("layer_norm", &layer_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("act8_pack", &act8_pack, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("act8_unpack", &act8_unpack, pybind11::call_guard<pybind11::gil_scoped_release>());

@@ -24,12 +24,21 @@ constexpr int kXaMaxSplits = 256;  // threads of the workgroup that joins a row'
 // tile.  p is one fused multiply-add and an exponential, 2^(c s - c m); where a
 // tile has additive values, which may be of any size, the maximum is taken off
 // first, 2^(c (s - m)).
-template <int DP, int QB, bool F16>
+//
+// p enters the second product rounded to the operands' type, and the outputs are
+// divided by n, the sum of the rounded p: they are means of V with weights that sum
+// to 1, so what the states' values have in common passes exactly (divided by the
+// unrounded sum, the roundings of p would scale it).  The backward's p come from
+// scores again and are divided by l, the sum of the unrounded ones, which only a
+// forward with statistics forms (32 heads, 4096 x 4096 x 128: 306 us with it and the
+// residual's stores against 289 without).  n is summed among the second product's steps,
+// whose time hides it (before them, 4096 x 4096 x 128 took 289 us instead of 272).
+template <int DP, int QB, bool F16, bool STATS>
 struct XRows {
   static constexpr int DS = DP / 16, DB = DP / 32;
   bf16x8 q[QB][DS];
   f32x16 o[QB][DB];
-  float m[QB], l[QB];
+  float m[QB], l[QB], n[QB];
 
   __device__ __forceinline__ void init(const XAttnArgs& a, int b, int hk, int r0) {
     const int lane = threadIdx.x & 63;
@@ -47,7 +56,7 @@ struct XRows {
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[qb][db] = zero16();
       m[qb] = kXaLow;
-      l[qb] = 0.f;
+      l[qb] = n[qb] = 0.f;
     }
   }
 
@@ -91,7 +100,8 @@ struct XRows {
       if (__ballot((t - m[qb]) * a.c > 8.f)) {
         const float mn = fmaxf(m[qb], t), al = fast_exp2((m[qb] - mn) * a.c);
         m[qb] = mn;
-        l[qb] *= al;
+        if constexpr (STATS) l[qb] *= al;
+        n[qb] *= al;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -110,24 +120,33 @@ struct XRows {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[qb][kb][r] = fast_exp2(fmaf(s[qb][kb][r], a.c, off));
-          sum += s[qb][kb][r];
+          if constexpr (STATS) sum += s[qb][kb][r];
         }
-        p[qb][2 * kb] = xa_pack8<F16>(s[qb][kb], 0);
-        p[qb][2 * kb + 1] = xa_pack8<F16>(s[qb][kb], 8);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          p[qb][2 * kb + t] = xa_pack8<F16>(s[qb][kb], 8 * t);
+        }
       }
-      l[qb] += sum;
+      if constexpr (STATS) l[qb] += sum;
     }
     if constexpr (DP > 96) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           const bf16x8 vf = xa_frag_t<DP>(V, 32 * kb, t, db);
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) o[qb][db] = xa_mfma<F16>(vf, p[qb][2 * kb + t], o[qb][db]);
         }
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          const u32x4 w = __builtin_bit_cast(u32x4, p[qb][2 * kb + t]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) n[qb] = xa_add_pair<F16>(w[e], n[qb]);
+        }
+      }
     if constexpr (DP > 96) __builtin_amdgcn_s_setprio(0);
   }
 };
@@ -150,6 +169,25 @@ __device__ __forceinline__ void xa_store_stats(const XAttnArgs& a, int64_t row, 
   }
 }
 
+// Writes four channels of a row's output at `at`, and what their rounding drops where
+// the backward wants it: its delta = dO . O takes O from both.
+template <bool F16>
+__device__ __forceinline__ void xa_store4(const XAttnArgs& a, int64_t at, float x0, float x1, float x2,
+                                          float x3) {
+  uint2 v;
+  v.x = xa_pair<F16>(x0, x1);
+  v.y = xa_pair<F16>(x2, x3);
+  *reinterpret_cast<uint2*>(a.out + at) = v;
+  if constexpr (!F16) {
+    if (a.res) {
+      uint2 r;
+      r.x = xa_pair<false>(x0 - __uint_as_float(v.x << 16), x1 - __uint_as_float(v.x & 0xffff0000u));
+      r.y = xa_pair<false>(x2 - __uint_as_float(v.y << 16), x3 - __uint_as_float(v.y & 0xffff0000u));
+      *reinterpret_cast<uint2*>(a.res + at) = r;
+    }
+  }
+}
+
 // Writes a row's outputs that this lane holds (channels 32 db + 8 g4 + 4 h + e).
 template <int DB, bool F16>
 __device__ __forceinline__ void xa_store_row(const XAttnArgs& a, int b, int hk, int r,
@@ -157,18 +195,15 @@ __device__ __forceinline__ void xa_store_row(const XAttnArgs& a, int b, int hk, 
   const int h = (threadIdx.x >> 5) & 1;
   int g, i;
   xa_row(a, r, g, i);
-  u16* p = a.out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D;
+  const int64_t at = (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int g4 = 0; g4 < 4; ++g4) {
       const int d = 32 * db + 8 * g4 + 4 * h;
-      if (d < a.D) {
-        uint2 v;
-        v.x = xa_pair<F16>(o[db][4 * g4] * inv, o[db][4 * g4 + 1] * inv);
-        v.y = xa_pair<F16>(o[db][4 * g4 + 2] * inv, o[db][4 * g4 + 3] * inv);
-        *reinterpret_cast<uint2*>(p + d) = v;
-      }
+      if (d < a.D)
+        xa_store4<F16>(a, at + d, o[db][4 * g4] * inv, o[db][4 * g4 + 1] * inv,
+                       o[db][4 * g4 + 2] * inv, o[db][4 * g4 + 3] * inv);
     }
 }
 
@@ -179,12 +214,12 @@ __device__ __forceinline__ void xa_store_row(const XAttnArgs& a, int b, int hk, 
 // heads on 4, 4 x 509 x 1021 x 80: 24.5 us against 28.6 with two splits in memory).
 // 32 heads, 4096 x 4096 x 128 in 288 us (954 TFLOP/s, the matrix and the vector units
 // busy about half the time each), 64 channels in 172.
-template <int DP, int QB, bool F16, int KW>
+template <int DP, int QB, bool F16, int KW, bool STATS>
 __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
   constexpr int KT = 64, TILE = KT * DP, DB = DP / 32;
   static_assert(KW == 1 || QB == 1, "a group's results fit its tiles");
   __shared__ __attribute__((aligned(1024))) u16 smem[KW][2][2][TILE];
-  __shared__ float ml[KW == 2 ? 512 : 1];
+  __shared__ float ml[KW == 2 ? 768 : 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = KW == 2 ? wave >> 2 : 0, w = wave & 3, lane = threadIdx.x & 63;
   const int64_t total = (int64_t)a.B * a.Hk * a.splits * a.tiles;
@@ -205,7 +240,7 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
   XTileLoader<DP, KT, 4> lk, lv;
   lk.init(w, a.k_sn, a.D);
   lv.init(w, a.v_sn, a.D);
-  XRows<DP, QB, F16> rows;
+  XRows<DP, QB, F16, STATS> rows;
   rows.init(a, b, hk, r0);
 
   // With one group a round always has a live state (no branch then: with it, 4096 x
@@ -240,32 +275,36 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
     __syncthreads();
     if (group) {
       xa_give<DB>(lds, w, rows.o[0]);
-      ml[2 * (64 * w + lane)] = rows.m[0];
-      ml[2 * (64 * w + lane) + 1] = rows.l[0];
+      ml[3 * (64 * w + lane)] = rows.m[0];
+      ml[3 * (64 * w + lane) + 1] = rows.l[0];
+      ml[3 * (64 * w + lane) + 2] = rows.n[0];
     }
     __syncthreads();
     if (group) return;
-    const float m1 = ml[2 * (64 * w + lane)], l1 = ml[2 * (64 * w + lane) + 1];
+    const float m1 = ml[3 * (64 * w + lane)], l1 = ml[3 * (64 * w + lane) + 1];
+    const float n1 = ml[3 * (64 * w + lane) + 2];
     const float m = fmaxf(rows.m[0], m1);
     const float f0 = fast_exp2((rows.m[0] - m) * a.c), f1 = fast_exp2((m1 - m) * a.c);
     xa_take<DB>(lds, w, rows.o[0], f0, f1);
     rows.l[0] = f0 * rows.l[0] + f1 * l1;
+    rows.n[0] = f0 * rows.n[0] + f1 * n1;
     rows.m[0] = m;
   }
 
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int r = r0 + 32 * qb + (lane & 31);
-    const float l = xor32_sum(rows.l[qb]);
+    const float l = xor32_sum(rows.l[qb]), n = xor32_sum(rows.n[qb]);
     if (r >= a.R) continue;
     if (a.splits == 1) {
-      xa_store_row<DP / 32, F16>(a, b, hk, r, rows.o[qb], xa_inverse(l));
+      xa_store_row<DP / 32, F16>(a, b, hk, r, rows.o[qb], xa_inverse(n));
       if (a.lse && lane < 32) xa_store_stats(a, bh * a.R + r, rows.m[qb], l);
     } else {
       const int64_t pr = (bh * a.splits + split) * a.R + r;
       if (lane < 32) {
-        a.part_ml[2 * pr] = rows.m[qb];
-        a.part_ml[2 * pr + 1] = l;
+        a.part_ml[3 * pr] = rows.m[qb];
+        a.part_ml[3 * pr + 1] = l;
+        a.part_ml[3 * pr + 2] = n;
       }
       float* p = a.part_o + pr * a.D;
 #pragma unroll
@@ -289,12 +328,12 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
 // without a barrier, and the four waves' results meet in LDS at the end.  32 kv heads
 // of 4096 states, one row each, unsplit: 96 us, 5.6 TB/s.  16 tokens of 32 heads on 8
 // with 8191 ragged states (403 MB live) in two splits: 79 us with the join.
-template <int DP, int QB, bool F16>
+template <int DP, int QB, bool F16, bool STATS>
 __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
   constexpr int KT = 32, TILE = KT * DP, NI = KT * DP / 512;
   constexpr int OP = DP + 4;  // pitch of the joined rows (f32)
   __shared__ __attribute__((aligned(1024))) u16 smem[4][2][2][TILE];
-  static_assert(sizeof(smem) >= 4 * 32 * (OP + 2) * 4, "the join fits");
+  static_assert(sizeof(smem) >= 4 * 32 * (OP + 3) * 4, "the join fits");
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t T = xcd_order((int64_t)a.B * a.Hk * a.splits);
   if (T < 0) return;
@@ -310,7 +349,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
   XTileLoader<DP, KT, 1> lk, lv;
   lk.init(0, a.k_sn, a.D);
   lv.init(0, a.v_sn, a.D);
-  XRows<DP, QB, F16> rows;
+  XRows<DP, QB, F16, STATS> rows;
   rows.init(a, b, hk, 0);
 
   int k0 = kbeg + KT * (w - 4);
@@ -355,7 +394,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     __syncthreads();
-    const float lw = xor32_sum(rows.l[qb]);
+    const float lw = xor32_sum(rows.l[qb]), nw = xor32_sum(rows.n[qb]);
     float* ow = O + (w * 32 + (lane & 31)) * OP;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
@@ -367,22 +406,24 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
         *reinterpret_cast<f32x4*>(ow + 32 * db + 8 * g4 + 4 * (lane >> 5)) = v;
       }
     if (lane < 32) {
-      ML[2 * (w * 32 + lane)] = rows.m[qb];
-      ML[2 * (w * 32 + lane) + 1] = lw;
+      ML[3 * (w * 32 + lane)] = rows.m[qb];
+      ML[3 * (w * 32 + lane) + 1] = lw;
+      ML[3 * (w * 32 + lane) + 2] = nw;
     }
     __syncthreads();
     const int rl = threadIdx.x >> 3, r = 32 * qb + rl;
     if (r >= a.R) continue;
-    float m = kXaLow, l = 0.f, f[4];
+    float m = kXaLow, l = 0.f, n = 0.f, f[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) m = fmaxf(m, ML[2 * (x * 32 + rl)]);
+    for (int x = 0; x < 4; ++x) m = fmaxf(m, ML[3 * (x * 32 + rl)]);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      f[x] = fast_exp2((ML[2 * (x * 32 + rl)] - m) * a.c);
-      l += f[x] * ML[2 * (x * 32 + rl) + 1];
+      f[x] = fast_exp2((ML[3 * (x * 32 + rl)] - m) * a.c);
+      l += f[x] * ML[3 * (x * 32 + rl) + 1];
+      n += f[x] * ML[3 * (x * 32 + rl) + 2];
     }
     const int64_t pr = (bh * a.splits + split) * a.R + r;
-    const float inv = xa_inverse(l);
+    const float inv = xa_inverse(n);
     int g, i;
     xa_row(a, r, g, i);
     for (int d = 4 * (threadIdx.x & 7); d < a.D; d += 32) {
@@ -394,11 +435,8 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
         for (int e = 0; e < 4; ++e) o[e] += f[x] * v[e];
       }
       if (a.splits == 1) {
-        uint2 v;
-        v.x = xa_pair<F16>(o[0] * inv, o[1] * inv);
-        v.y = xa_pair<F16>(o[2] * inv, o[3] * inv);
-        *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d) =
-            v;
+        xa_store4<F16>(a, (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d, o[0] * inv,
+                       o[1] * inv, o[2] * inv, o[3] * inv);
       } else {
         *reinterpret_cast<f32x4*>(a.part_o + pr * a.D + d) = o;
       }
@@ -407,14 +445,15 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
       if (a.splits == 1) {
         if (a.lse) xa_store_stats(a, bh * a.R + r, m, l);
       } else {
-        a.part_ml[2 * pr] = m;
-        a.part_ml[2 * pr + 1] = l;
+        a.part_ml[3 * pr] = m;
+        a.part_ml[3 * pr + 1] = l;
+        a.part_ml[3 * pr + 2] = n;
       }
     }
   }
 }
 
-// Joins the key splits: o = sum_s 2^(c (m_s - m)) o_s / sum_s 2^(c (m_s - m)) l_s
+// Joins the key splits: o = sum_s 2^(c (m_s - m)) o_s / sum_s 2^(c (m_s - m)) n_s
 // in ascending order.  A thread forms four channels of one row.
 template <bool F16>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
@@ -425,27 +464,26 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
   const int d = 4 * (int)(t - row * dv);
   const int64_t bh = row / a.R;
   const int r = (int)(row - bh * a.R);
-  const float* ml = a.part_ml + 2 * (bh * a.splits * a.R + r);
+  const float* ml = a.part_ml + 3 * (bh * a.splits * a.R + r);
   const float* po = a.part_o + (bh * a.splits * a.R + r) * a.D + d;
   float m = kXaLow;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[2 * (int64_t)s * a.R]);
-  float l = 0.f;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[3 * (int64_t)s * a.R]);
+  float l = 0.f, n = 0.f;
   f32x4 o = (f32x4)0.f;
   for (int s = 0; s < a.splits; ++s) {
-    const float w = fast_exp2((ml[2 * (int64_t)s * a.R] - m) * a.c);
-    l += w * ml[2 * (int64_t)s * a.R + 1];
+    const float w = fast_exp2((ml[3 * (int64_t)s * a.R] - m) * a.c);
+    l += w * ml[3 * (int64_t)s * a.R + 1];
+    n += w * ml[3 * (int64_t)s * a.R + 2];
     const f32x4 v = *reinterpret_cast<const f32x4*>(po + (int64_t)s * a.R * a.D);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += w * v[e];
   }
-  const float inv = xa_inverse(l);
+  const float inv = xa_inverse(n);
   int g, i;
   xa_row(a, r, g, i);
   const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
-  uint2 v;
-  v.x = xa_pair<F16>(o[0] * inv, o[1] * inv);
-  v.y = xa_pair<F16>(o[2] * inv, o[3] * inv);
-  *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d) = v;
+  xa_store4<F16>(a, (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d, o[0] * inv, o[1] * inv,
+                 o[2] * inv, o[3] * inv);
   if (a.lse && d == 0) xa_store_stats(a, row, m, l);
 }
 
@@ -455,14 +493,15 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
 // One token of 32 heads, 16384 states in 32 splits: 19.5 us in all against 30.
 template <bool F16>
 __global__ __launch_bounds__(256) void xattn_join_few_kernel(XAttnArgs a) {
-  __shared__ float wt[kXaMaxSplits], part[8][32][4], red[4][2];
+  __shared__ float wt[kXaMaxSplits], part[8][32][4], red[4][3];
   const int64_t row = blockIdx.x, bh = row / a.R;
   const int r = (int)(row - bh * a.R), tid = threadIdx.x, w = tid >> 6;
-  const float* ml = a.part_ml + 2 * (bh * a.splits * a.R + r);
-  float m0 = kXaLow, l0 = 0.f;  // this thread's split (at most 256)
+  const float* ml = a.part_ml + 3 * (bh * a.splits * a.R + r);
+  float m0 = kXaLow, l0 = 0.f, n0 = 0.f;  // this thread's split (at most 256)
   if (tid < a.splits) {
-    m0 = ml[2 * (int64_t)tid * a.R];
-    l0 = ml[2 * (int64_t)tid * a.R + 1];
+    m0 = ml[3 * (int64_t)tid * a.R];
+    l0 = ml[3 * (int64_t)tid * a.R + 1];
+    n0 = ml[3 * (int64_t)tid * a.R + 2];
   }
   float m = m0;
 #pragma unroll
@@ -472,10 +511,14 @@ __global__ __launch_bounds__(256) void xattn_join_few_kernel(XAttnArgs a) {
   m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
   const float f = tid < a.splits ? fast_exp2((m0 - m) * a.c) : 0.f;
   wt[tid] = f;
-  const float ls = lanes_sum<64>(f * l0);
-  if ((tid & 63) == 0) red[w][1] = ls;
+  const float ls = lanes_sum<64>(f * l0), ns = lanes_sum<64>(f * n0);
+  if ((tid & 63) == 0) {
+    red[w][1] = ls;
+    red[w][2] = ns;
+  }
   __syncthreads();
   const float l = red[0][1] + red[1][1] + red[2][1] + red[3][1];
+  const float n = red[0][2] + red[1][2] + red[2][2] + red[3][2];
   const int dg = tid & 31, q = tid >> 5, d = 4 * dg;
   f32x4 o = (f32x4)0.f;
   if (d < a.D) {
@@ -495,14 +538,12 @@ __global__ __launch_bounds__(256) void xattn_join_few_kernel(XAttnArgs a) {
   for (int x = 1; x < 8; ++x)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += part[x][dg][e];
-  const float inv = xa_inverse(l);
+  const float inv = xa_inverse(n);
   int g, i;
   xa_row(a, r, g, i);
   const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
-  uint2 v;
-  v.x = xa_pair<F16>(o[0] * inv, o[1] * inv);
-  v.y = xa_pair<F16>(o[2] * inv, o[3] * inv);
-  *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d) = v;
+  xa_store4<F16>(a, (((int64_t)b * a.Nq + i) * a.H + hk * a.G + g) * a.D + d, o[0] * inv, o[1] * inv,
+                 o[2] * inv, o[3] * inv);
   if (a.lse && tid == 0) xa_store_stats(a, row, m, l);
 }
 
@@ -537,7 +578,7 @@ static void xattn_plan(XAttnArgs& a) {
 }
 
 static int64_t xattn_part_floats(const XAttnArgs& a) {
-  return a.splits > 1 ? (int64_t)a.B * a.Hk * a.splits * a.R * (a.D + 2) : 0;
+  return a.splits > 1 ? (int64_t)a.B * a.Hk * a.splits * a.R * (a.D + 3) : 0;
 }
 
 // Sizes and strides as the kernels need them; 0 or an error code.
@@ -581,31 +622,37 @@ int xattn_check(XAttnArgs& a, const tpf_xattn_shape* s, double scale, const char
   return TPF_OK;
 }
 
-template <int DP, bool F16>
+template <int DP, bool F16, bool STATS>
 static void xattn_launch(const XAttnArgs& a, hipStream_t s) {
   const int64_t groups = (int64_t)a.B * a.Hk * a.splits;
   const dim3 grid((unsigned)((groups * a.tiles + 7) / 8 * 8));
   if (a.R <= 64) {
-    if (a.qb == 1) hipLaunchKernelGGL((xattn_few_kernel<DP, 1, F16>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((xattn_few_kernel<DP, 2, F16>), grid, dim3(256), 0, s, a);
+    if (a.qb == 1) hipLaunchKernelGGL((xattn_few_kernel<DP, 1, F16, STATS>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((xattn_few_kernel<DP, 2, F16, STATS>), grid, dim3(256), 0, s, a);
     return;
   }
   if constexpr (DP <= 64) {
     if (a.qb == 2) {
-      hipLaunchKernelGGL((xattn_fwd_kernel<DP, 2, F16, 1>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((xattn_fwd_kernel<DP, 2, F16, 1, STATS>), grid, dim3(256), 0, s, a);
       return;
     }
   }
-  if (a.kw == 2) hipLaunchKernelGGL((xattn_fwd_kernel<DP, 1, F16, 2>), grid, dim3(512), 0, s, a);
-  else hipLaunchKernelGGL((xattn_fwd_kernel<DP, 1, F16, 1>), grid, dim3(256), 0, s, a);
+  if (a.kw == 2) hipLaunchKernelGGL((xattn_fwd_kernel<DP, 1, F16, 2, STATS>), grid, dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((xattn_fwd_kernel<DP, 1, F16, 1, STATS>), grid, dim3(256), 0, s, a);
+}
+
+template <bool F16, bool STATS>
+static void xattn_pick(const XAttnArgs& a, hipStream_t s) {
+  if (a.D <= 32) xattn_launch<32, F16, STATS>(a, s);
+  else if (a.D <= 64) xattn_launch<64, F16, STATS>(a, s);
+  else if (a.D <= 96) xattn_launch<96, F16, STATS>(a, s);
+  else xattn_launch<128, F16, STATS>(a, s);
 }
 
 template <bool F16>
 static void xattn_forward(const XAttnArgs& a, hipStream_t s) {
-  if (a.D <= 32) xattn_launch<32, F16>(a, s);
-  else if (a.D <= 64) xattn_launch<64, F16>(a, s);
-  else if (a.D <= 96) xattn_launch<96, F16>(a, s);
-  else xattn_launch<128, F16>(a, s);
+  if (a.lse) xattn_pick<F16, true>(a, s);
+  else xattn_pick<F16, false>(a, s);
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.B * a.Hk * a.R, n = rows * (a.D / 4);
     if (a.splits >= 8)
@@ -624,26 +671,45 @@ extern "C" int64_t tpf_xattn_forward_workspace_bytes(const tpf_xattn_shape* shap
   return tpf::xattn_part_floats(a) * 4;
 }
 
-extern "C" int tpf_xattn_forward(const void* q, const void* k, const void* v, const void* mask,
-                                 void* out, float* lse, void* workspace, int64_t workspace_bytes,
-                                 const tpf_xattn_shape* shape, double scale, void* stream) {
-  const char* fn = "tpf_xattn_forward";
+static int xattn_forward_entry(const void* q, const void* k, const void* v, const void* mask, void* out,
+                               float* lse, void* residual, void* workspace, int64_t workspace_bytes,
+                               const tpf_xattn_shape* shape, double scale, void* stream,
+                               const char* fn) {
   if (!q || !k || !v || !out) return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
   tpf::XAttnArgs a{};
   if (int rc = tpf::xattn_check(a, shape, scale, fn)) return rc;
   if ((a.mask_kind != 0) != (mask != nullptr))
     return tpf::set_error(TPF_ERR_ARG, "%s: mask pointer and mask kind disagree", fn);
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)workspace) % 16)
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)residual |
+       (uintptr_t)workspace) % 16)
     return tpf::set_error(TPF_ERR_ARG, "%s: tensors must start on 16 bytes", fn);
   tpf::xattn_plan(a);
   const int64_t floats = tpf::xattn_part_floats(a);
   if (floats && (!workspace || workspace_bytes < floats * 4))
     return tpf::set_error(TPF_ERR_ARG, "%s: workspace too small", fn);
   a.q = (const tpf::u16*)q; a.k = (const tpf::u16*)k; a.v = (const tpf::u16*)v;
-  a.mask = mask; a.out = (tpf::u16*)out; a.lse = lse;
+  a.mask = mask; a.out = (tpf::u16*)out; a.res = (tpf::u16*)residual; a.lse = lse;
   a.part_o = (float*)workspace;
   a.part_ml = floats ? a.part_o + (int64_t)a.B * a.Hk * a.splits * a.R * a.D : nullptr;
   if (shape->dtype == TPF_F16) tpf::xattn_forward<true>(a, (hipStream_t)stream);
   else tpf::xattn_forward<false>(a, (hipStream_t)stream);
   return tpf::check_launch(fn);
+}
+
+extern "C" int tpf_xattn_forward(const void* q, const void* k, const void* v, const void* mask,
+                                 void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                 const tpf_xattn_shape* shape, double scale, void* stream) {
+  return xattn_forward_entry(q, k, v, mask, out, lse, nullptr, workspace, workspace_bytes, shape, scale,
+                             stream, "tpf_xattn_forward");
+}
+
+extern "C" int tpf_xattn_forward_shadow_bf16(const void* q, const void* k, const void* v,
+                                             const void* mask, void* out, float* lse, void* residual,
+                                             void* workspace, int64_t workspace_bytes,
+                                             const tpf_xattn_shape* shape, double scale, void* stream) {
+  const char* fn = "tpf_xattn_forward_shadow_bf16";
+  if (!lse || !residual) return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
+  if (shape && shape->dtype != TPF_BF16) return tpf::set_error(TPF_ERR_ARG, "%s: BF16 only", fn);
+  return xattn_forward_entry(q, k, v, mask, out, lse, residual, workspace, workspace_bytes, shape, scale,
+                             stream, fn);
 }

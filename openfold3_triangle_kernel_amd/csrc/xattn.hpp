@@ -27,6 +27,7 @@ struct XAttnArgs {
   int64_t mask_sb;
   int mask_kind;
   u16* out;    // [B, Nq, H, D]
+  u16* res;    // what its rounding drops, laid out the same; null when not wanted
   float* lse;  // the rows' statistics (xa_store_stats); null when no backward follows
   int B, H, Hk, G, Nq, Nk, D, R;
   FastDiv div_nq;
@@ -37,7 +38,7 @@ struct XAttnArgs {
   int qb;           // blocks of 32 rows a wave
   int kw;           // groups of four waves that share a row tile's states
   float* part_o;    // [B*Hk, splits, R, D] unnormalised outputs of the splits
-  float* part_ml;   // [B*Hk, splits, R, 2] their raw maxima and sums
+  float* part_ml;   // [B*Hk, splits, R, 3] their raw maxima and the two sums (XRows)
 };
 
 template <int DP>
@@ -82,6 +83,19 @@ __device__ __forceinline__ bf16x8 xa_pack8(const f32x16& c, int r0) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] = xa_pair<F16>(c[r0 + 2 * e], c[r0 + 2 * e + 1]);
   return __builtin_bit_cast(bf16x8, o);
+}
+
+// Adds the two 16-bit values of a pair to acc, in 32 bits.
+template <bool F16>
+__device__ __forceinline__ float xa_add_pair(uint32_t pair, float acc) {
+  if constexpr (F16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair),
+                                  __builtin_bit_cast(f16x2, 0x3c003c00u), acc, false);
+  } else {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair),
+                                           __builtin_bit_cast(bf16x2, 0x3f803f80u), acc, false);
+  }
 }
 
 // Row-wise fragment: row rbase + lane % 32, channels 16 s + 8 (lane / 32) .. + 8.

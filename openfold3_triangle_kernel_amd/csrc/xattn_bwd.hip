@@ -2,6 +2,8 @@
 //
 //   p_ij = 2^(c s_ij - lse_i) (with additive masks 2^(c (s_ij + m_j - max_i) -
 //   log2 sum_i), whatever the masks' size),  delta_i = dO_i . O_i,  dS = p (dO V^T - delta)
+// (O with what its rounding dropped where the forward kept that: dO V^T and delta
+// nearly cancel in what the states' values have in common)
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = p^T dO
 //
 // over the rows and states of xattn.hpp, in two launches that each rebuild p
@@ -21,7 +23,7 @@ namespace tpf {
 
 struct XAttnGrad {
   XAttnArgs f;           // operands; f.splits / f.chunk: states of the dQ launch
-  const u16 *o, *dout;   // [B, Nq, H, D]
+  const u16 *o, *res, *dout;  // [B, Nq, H, D]; res null when not kept
   const float *lse, *top;  // log-sum-exp; with additive masks log2 of the sum and the maximum
   float* delta;          // [B, Hk, R]
   u16 *dq, *dk, *dv;
@@ -116,6 +118,11 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_dq_kernel(XAttnGrad ga) {
       const bf16x8 o = in ? *reinterpret_cast<const bf16x8*>(ga.o + oo + d) : zero8();
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta = fmaf(bf2f(dO[s][e]), bf2f(o[e]), delta);
+      if (ga.res && in) {
+        const bf16x8 x = *reinterpret_cast<const bf16x8*>(ga.res + oo + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf(bf2f(dO[s][e]), bf2f(x[e]), delta);
+      }
     }
   }
   delta = xor32_sum(delta);
@@ -470,12 +477,12 @@ extern "C" int64_t tpf_xattn_backward_workspace_bytes(const tpf_xattn_shape* sha
   return tpf::GradSpace(g).total * 4;
 }
 
-extern "C" int tpf_xattn_backward_bf16(const void* q, const void* k, const void* v, const void* mask,
-                                       const void* out, const void* dout, const float* lse, void* dq,
-                                       void* dk, void* dv, void* workspace, int64_t workspace_bytes,
-                                       const tpf_xattn_shape* shape, const int64_t* grad_strides,
-                                       double scale, void* stream) {
-  const char* fn = "tpf_xattn_backward_bf16";
+static int xattn_backward_entry(const void* q, const void* k, const void* v, const void* mask,
+                                const void* out, const void* residual, const void* dout,
+                                const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                int64_t workspace_bytes, const tpf_xattn_shape* shape,
+                                const int64_t* grad_strides, double scale, void* stream,
+                                const char* fn) {
   if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !workspace || !grad_strides)
     return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
   tpf::XAttnGrad g{};
@@ -484,7 +491,7 @@ extern "C" int tpf_xattn_backward_bf16(const void* q, const void* k, const void*
   if (shape->dtype != TPF_BF16) return tpf::set_error(TPF_ERR_ARG, "%s: BF16 only", fn);
   if ((a.mask_kind != 0) != (mask != nullptr))
     return tpf::set_error(TPF_ERR_ARG, "%s: mask pointer and mask kind disagree", fn);
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout |
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)residual | (uintptr_t)dout |
        (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) % 16)
     return tpf::set_error(TPF_ERR_ARG, "%s: tensors must start on 16 bytes", fn);
   for (int i = 0; i < 9; ++i)
@@ -495,7 +502,7 @@ extern "C" int tpf_xattn_backward_bf16(const void* q, const void* k, const void*
   if (workspace_bytes < ws.total * 4)
     return tpf::set_error(TPF_ERR_ARG, "%s: workspace too small", fn);
   a.q = (const tpf::u16*)q; a.k = (const tpf::u16*)k; a.v = (const tpf::u16*)v; a.mask = mask;
-  g.o = (const tpf::u16*)out; g.dout = (const tpf::u16*)dout; g.lse = lse;
+  g.o = (const tpf::u16*)out; g.res = (const tpf::u16*)residual; g.dout = (const tpf::u16*)dout; g.lse = lse;
   g.top = a.mask_kind == tpf::kMaskF32 ? lse + (int64_t)a.B * a.Hk * a.R : nullptr;
   g.dq = (tpf::u16*)dq; g.dk = (tpf::u16*)dk; g.dv = (tpf::u16*)dv;
   for (int i = 0; i < 3; ++i) {
@@ -519,4 +526,26 @@ extern "C" int tpf_xattn_backward_bf16(const void* q, const void* k, const void*
     hipLaunchKernelGGL(tpf::xattn_fold_kernel, dim3((unsigned)(nq + 2 * nk)), dim3(256), 0, s, g,
                        (unsigned)nq, (unsigned)(nq + nk));
   return tpf::check_launch(fn);
+}
+
+extern "C" int tpf_xattn_backward_bf16(const void* q, const void* k, const void* v, const void* mask,
+                                       const void* out, const void* dout, const float* lse, void* dq,
+                                       void* dk, void* dv, void* workspace, int64_t workspace_bytes,
+                                       const tpf_xattn_shape* shape, const int64_t* grad_strides,
+                                       double scale, void* stream) {
+  return xattn_backward_entry(q, k, v, mask, out, nullptr, dout, lse, dq, dk, dv, workspace,
+                              workspace_bytes, shape, grad_strides, scale, stream,
+                              "tpf_xattn_backward_bf16");
+}
+
+extern "C" int tpf_xattn_backward_shadow_bf16(const void* q, const void* k, const void* v,
+                                              const void* mask, const void* out, const void* residual,
+                                              const void* dout, const float* lse, void* dq, void* dk,
+                                              void* dv, void* workspace, int64_t workspace_bytes,
+                                              const tpf_xattn_shape* shape, const int64_t* grad_strides,
+                                              double scale, void* stream) {
+  const char* fn = "tpf_xattn_backward_shadow_bf16";
+  if (!residual) return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
+  return xattn_backward_entry(q, k, v, mask, out, residual, dout, lse, dq, dk, dv, workspace,
+                              workspace_bytes, shape, grad_strides, scale, stream, fn);
 }

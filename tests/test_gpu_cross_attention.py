@@ -528,3 +528,114 @@ def test_two_calls_at_once(gpu):
     for runs, w in zip(got, want):
         for r in runs:
             assert all(torch.equal(a, b) for a, b in zip(r, w))
+
+
+COMMON = [
+    # B, H, Hk, Nq, Nk, D, mask, what K and V have in common (of the operands' deviation)
+    (1, 2, 1, 30, 700, 64, "none", 0.0), (1, 2, 1, 30, 700, 64, "none", 1.0),
+    (2, 4, 1, 16, 1500, 128, "tail", 1.0),  # few rows, splits joined in memory
+    (1, 1, 1, 40, 3000, 64, "add", 5.0),
+    (2, 4, 2, 200, 333, 128, "tail", 1.0), (2, 4, 2, 200, 333, 80, "add", 5.0),  # two wave groups
+    (1, 1, 1, 300, 2000, 96, "none", 5.0), (1, 1, 1, 140, 9000, 32, "random", 2.0),  # splits
+    (2, 64, 64, 520, 65, 64, "none", 2.0),  # 256 rows a workgroup
+    (2, 40, 40, 260, 190, 128, "tail", 2.0),
+]
+
+
+def _heads_in_common(dev, B, H, Hk, Nq, Nk, D, off, seed):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(B, H, Nq, D, generator=g)
+    k, v = (torch.randn(B, Hk, Nk, D, generator=g) + off * torch.randn(1, Hk, 1, D, generator=g)
+            for _ in range(2))
+    return [t.bfloat16().to(dev) for t in (q, k, v)]
+
+
+def _rounding_variances(q, k, v, mask, scale, do):
+    """Outputs and gradients in 64 bits, and the squared errors to expect of them when
+    P, dS and every result are rounded to BF16, each rounding an error of its own of
+    mean square u^2 / 3 (uniform at the largest step of a value).  The output is a mean
+    of V with weights that sum to 1, so an error d_j of p_j gives p_j d_j (v_j - o) in the
+    output and p_j d_j (dP_j - delta) = d_j dS_j in delta; no rounding of the output
+    enters delta."""
+    B, H, Nq, D = q.shape
+    Hk, Nk = k.shape[1:3]
+    u3 = (2.0 ** -8) ** 2 / 3
+    q, k, v, do = (t.detach().double().cpu() for t in (q, k, v, do))
+    do = do.transpose(1, 2)
+    ke, ve = (t.repeat_interleave(H // Hk, 1) for t in (k, v))
+    s = scale * q @ ke.transpose(-1, -2)
+    if mask is not None:
+        m = mask.cpu().expand(B, Nk)[:, None, None]
+        s = s.masked_fill(~m, float("-inf")) if m.dtype == torch.bool else s + m.double()
+    p = torch.softmax(s, -1)
+    o = p @ ve
+    ds = p * (do @ ve.transpose(-1, -2) - (do * o).sum(-1, keepdim=True))
+    group = lambda t: t.reshape(B, Hk, H // Hk, Nk, D).sum(2)  # noqa: E731
+    dq, dk = scale * ds @ ke, group(scale * ds.transpose(-1, -2) @ q)
+    dv = group(p.transpose(-1, -2) @ do)
+    p2, ds2 = p.square(), ds.square()
+    delta = ds2.sum(-1, keepdim=True)  # of u^2 / 3
+    # sum_j p_j^2 (v_j - o)^2
+    spread = p2 @ ve.square() - 2 * o * (p2 @ ve) + o.square() * p2.sum(-1, keepdim=True)
+    eo = o.square() + spread.clamp_min(0)
+    edq = dq.square() + scale ** 2 * (ds2 @ ke.square() + delta * (p @ ke).square())
+    edk = dk.square() + group(scale ** 2 * (ds2 + delta * p2).transpose(-1, -2) @ q.square())
+    edv = dv.square() + group(p2.transpose(-1, -2) @ do.square())
+    return ([o.transpose(1, 2), dq, dk, dv], [u3 * t.sum().item() for t in (eo, edq, edk, edv)])
+
+
+@pytest.mark.parametrize("host", [True, False], ids=["cpp", "python"])
+@pytest.mark.parametrize("case", COMMON, ids=str)
+def test_gradients_beside_common_components(gpu, monkeypatch, case, host):
+    """What keys and values have in common cancels between dO V^T and delta, and leaves
+    no rounding of the output in the gradients.  Root mean squares over all elements
+    against those expected; a quarter more for the sample's scatter and the 32-bit sums
+    (the expected ones are 1.2 to 1.4 times too high already: a value's last place is
+    smaller against it than u, but for powers of two)."""
+    from openfold3_triangle_kernel_amd import _native, cross_attention
+
+    if not host:
+        monkeypatch.setattr(_native, "_HOST", False)
+    B, H, Hk, Nq, Nk, D, mk, off = case
+    q, k, v = (t.requires_grad_(True) for t in _heads_in_common(gpu, B, H, Hk, Nq, Nk, D, off, 31))
+    mask = _mask(gpu, mk, B, Nk, 31)
+    do = torch.randn(B, Nq, H, D, generator=torch.Generator().manual_seed(32)).bfloat16().to(gpu)
+    want, expected = _rounding_variances(q, k, v, mask, 1 / math.sqrt(D), do)
+    out = cross_attention(q, k, v, mask)
+    got = [out.detach(), *torch.autograd.grad(out, (q, k, v), do)]
+    for g, w, e, name in zip(got, want, expected, ("out", "dq", "dk", "dv")):
+        err = (g.double().cpu() - w).square().sum().item()
+        assert err <= 1.25 ** 2 * e, f"{name}: {(err / e) ** 0.5:.2f} of the expected error"
+
+
+def test_shadow_policy(gpu, monkeypatch):
+    """Without the residual (TURBOPAIRFORMER_SR_SHADOW=0) the same output and dV, delta
+    from the rounded output, on both host paths; another value is refused."""
+    from openfold3_triangle_kernel_amd import _native, cross_attention
+
+    q, k, v = (t.requires_grad_(True) for t in _heads_in_common(gpu, 1, 2, 1, 130, 200, 64, 2.0, 33))
+    do = torch.randn(1, 130, 2, 64, generator=torch.Generator().manual_seed(34)).bfloat16().to(gpu)
+
+    def run():
+        out = cross_attention(q, k, v)
+        return [out.detach(), *torch.autograd.grad(out, (q, k, v), do)]
+
+    want, tol = _reference(q, k, v, None, 1 / 8.0, do)  # its delta counts the output's rounding
+    runs = {}
+    for shadow in ("1", "0"):
+        monkeypatch.setenv("TURBOPAIRFORMER_SR_SHADOW", shadow)
+        for host in (None, False):
+            with monkeypatch.context() as m:
+                if host is False:
+                    m.setattr(_native, "_HOST", False)
+                runs[shadow, host] = run()
+        assert all(torch.equal(a, b) for a, b in zip(runs[shadow, None], runs[shadow, False]))
+    with_, without = runs["1", None], runs["0", None]
+    _check(without, want, tol)
+    assert torch.equal(with_[0], without[0]) and torch.equal(with_[3], without[3])
+    assert not torch.equal(with_[1], without[1])
+    monkeypatch.setenv("TURBOPAIRFORMER_SR_SHADOW", "2")
+    with pytest.raises(ValueError, match="must be 0 or 1"):
+        cross_attention(q, k, v)
+    with torch.no_grad():
+        assert torch.equal(cross_attention(q, k, v), with_[0])

@@ -184,3 +184,19 @@ def test_block_of_empty_axes_on_the_cpu(Nq, Nk):
         assert out.shape == x.shape and not out.any()  # no state: nothing attended
         for g in torch.autograd.grad(out, [x, kv, *block.parameters()], torch.ones_like(out)):
             assert not g.any()
+
+
+def test_c_abi_shadow_arguments():
+    from openfold3_triangle_kernel_amd import _native
+
+    s, g = _shape(), (ctypes.c_int64 * 9)(512, 256, 64, 1024, 512, 64, 1024, 512, 64)
+    for match, args in (("null pointer", (16, 16, 16, None, 16, None, 16, 16, 0, s, 0.1, None)),
+                        ("null pointer", (16, 16, 16, None, 16, 16, None, 16, 0, s, 0.1, None)),
+                        ("16 bytes", (16, 16, 16, None, 16, 16, 8, 16, 0, s, 0.1, None)),
+                        ("BF16 only", (16, 16, 16, None, 16, 16, 16, 16, 0, _shape(dtype=1), 0.1, None))):
+        with pytest.raises(RuntimeError, match=match):
+            _native.call("tpf_xattn_forward_shadow_bf16", *args)
+    for match, residual in (("null pointer", None), ("16 bytes", 8), ("workspace", 16)):
+        with pytest.raises(RuntimeError, match=match):
+            _native.call("tpf_xattn_backward_shadow_bf16", 16, 16, 16, None, 16, residual, *([16] * 6), 8,
+                         s, g, 0.1, None)
