@@ -157,14 +157,12 @@ class _LayerNormFn(torch.autograd.Function):
         dev = dy.device
         dy = dy.to(dtype).contiguous()
         dx = torch.empty((R, C), device=dev, dtype=dtype)
-        # The fold writes the gradients in the parameters' type where both share one.
-        types = {t for t, n in ((wtype, 1), (btype, 2)) if t is not None and ctx.needs_input_grad[n]}
-        ptype = types.pop() if len(types) == 1 else torch.float32
+        # The fold writes the gradients in the type of the weight as the forward read it
+        # (FP32 beside a bias of another type): dx needs that weight, not a rounding of it.
+        ptype = w.dtype if w is not None else torch.float32 if btype is None else btype
         dw = torch.empty(C, device=dev, dtype=ptype) if ctx.needs_input_grad[1] else None
         db = torch.empty(C, device=dev, dtype=ptype) if ctx.needs_input_grad[2] else None
         ws, ws_bytes = None, 0
-        if w is not None and w.dtype != ptype:
-            w = w.to(ptype)
         if dw is not None or db is not None:
             ws_bytes = int(_native.query("tpf_norm_backward_workspace_bytes", R, C))
             ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)

@@ -300,3 +300,28 @@ def test_refusals(gpu):
                             ((x[:, :0],), {}, "channels")):
         with pytest.raises(ValueError, match=match):
             layer_norm(*args, **kw)
+
+
+@pytest.mark.parametrize("save", ["full", "int8"])
+@pytest.mark.parametrize("t,wt,bt,size", [("fp32", "fp32", "bf16", 1.0), ("fp32", "fp32", "fp16", 1e6),
+                                          ("bf16", "bf16", "fp16", 1e6), ("fp32", "fp16", "bf16", 1.0)])
+def test_frozen_weight_beside_a_bias_of_another_type(gpu, save, t, wt, bt, size):
+    """The backward uses the weight that the forward used, whatever the type of the
+    parameters that want a gradient."""
+    from openfold3_triangle_kernel_amd import layer_norm
+    from openfold3_triangle_kernel_amd.layernorm import _norm_forward
+
+    x, w, b, dy = _inputs(gpu, 60, 200, t, "fp32", seed=6)
+    x.requires_grad_(True)
+    w, b = (size * w).to(_T[wt]), b.to(_T[bt]).requires_grad_(True)
+    dx, db = torch.autograd.grad(layer_norm(x, w, b, save=save), (x, b), dy)
+    xd, wd, dyd = (v.detach().double().cpu() for v in (x, w, dy))
+    xh, rstd, e, tt = _xh(xd)
+    if save == "int8":
+        _, _, _, codes, scales = _norm_forward(x.detach(), None, None, 1e-5, "int8")
+        xh, e = _decode(codes.cpu(), scales.cpu(), 200), xh * 0
+    (want, tol), _, (wdb, tdb) = _backward_bound(dyd, xh, rstd, e, tt, wd, x.dtype, b.dtype)
+    if save == "int8":
+        tol = tol + want.abs() * rstd * tt * xd.abs().mean(-1, keepdim=True)  # rstd's, from the mean's
+    _near(dx, want, tol, "dx")
+    _near(db, wdb, tdb, "db")
