@@ -190,6 +190,19 @@ def weight_grad(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cha
     return dw.to(dtype)
 
 
+def _weight_grad_full(dy: torch.Tensor, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """dW [N, K] = dy^T x of BF16 rows; rows beyond an operand's 2 GiB in further products,
+    whose FP32 sums are added in order."""
+    from .modules import _wgrad
+
+    R, pitch = dy.shape[0], max(dy.stride(0), x.stride(0))
+    step = max(1, _GEMM_SPAN // (2 * pitch))
+    dw = _wgrad(dy[:step], x[:step], dtype if R <= step else torch.float32)
+    for r in range(step, R, step):
+        dw += _wgrad(dy[r:r + step], x[r:r + step], torch.float32)
+    return dw.to(dtype)
+
+
 class _LinearFn(torch.autograd.Function):
     """y = x w^T over rows x [R, K]; w [N, K] in its own type, used in BF16."""
 
@@ -216,9 +229,7 @@ class _LinearFn(torch.autograd.Function):
             if ctx.save == "int8":
                 dw = weight_grad(dy, *kept, w.shape[1], ctx.weight_dtype)
             else:
-                from .modules import _wgrad
-
-                dw = _wgrad(dy, kept[0], ctx.weight_dtype)
+                dw = _weight_grad_full(dy, kept[0], ctx.weight_dtype)
         return dx, dw, None
 
 

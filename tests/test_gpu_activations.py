@@ -283,3 +283,52 @@ def test_refusals(gpu):
                         (lambda: linear(x, w, save="none"), "save")):
         with pytest.raises(ValueError, match=match):
             call()
+
+
+@pytest.mark.parametrize("save", ["int8", "full"])
+def test_weight_gradient_of_rows_past_2_gib(gpu, save):
+    """dy beyond 2 GiB: both modes give the sum of the parts' gradients, in 32 bits.
+
+    With an FP32 weight either side is a sum in 32 bits of products exact in it.  Terms are
+    independent of mean 0 (x and dy normal), so n of them sum to less than 6 sqrt(n) in
+    magnitude.  A split (128 of them) adds its R / 128 rows 16 at a time, two roundings of
+    the running sum a time: 2^-23 sum_i 6 sqrt(16 i) = 2^-23 16 (R / 2048)^1.5; the folds add
+    300 sums of at most 6 sqrt(R).  The parts' own splits are shorter."""
+    from openfold3_triangle_kernel_amd import linear
+
+    R, K, N = 4_250_000, 24, 512
+    g = torch.Generator(device=gpu).manual_seed(3)
+    x = torch.empty(R, K, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+    dy = torch.empty(R, N, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+    w = torch.empty(N, K, device=gpu).normal_(generator=g).requires_grad_(True)
+
+    def grad(x, dy):
+        return torch.autograd.grad(linear(x, w, save=save), w, dy)[0]
+
+    whole = grad(x, dy)
+    step = R // 8 + 1
+    total = sum(grad(x[r:r + step], dy[r:r + step]).double() for r in range(0, R, step))
+    bound = 2 * (128 * 2.0 ** -23 * 16 * (R / 2048) ** 1.5 + 300 * 2.0 ** -24 * 6 * R ** 0.5)
+    assert bound < 0.3 * (R / 128) ** 0.5  # a split's rows left out would show
+    assert ((whole.double() - total).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("save", ["int8", "full"])
+@pytest.mark.parametrize("pitch", [64, 75, 72, (1 << 24) + 8])
+def test_linear_of_one_row(gpu, save, pitch):
+    """A single row's stride addresses nothing and may be anything, in the input and in
+    the gradient."""
+    from openfold3_triangle_kernel_amd import linear
+
+    g = torch.Generator().manual_seed(7)
+    wide = torch.zeros(pitch, device=gpu, dtype=torch.bfloat16)
+    x, dy = wide.as_strided((1, 64), (pitch, 1)), wide.clone().as_strided((1, 24), (pitch, 1))
+    x.copy_(torch.randn(1, 64, generator=g))
+    dy.copy_(torch.randn(1, 24, generator=g))
+    runs = []
+    for rows, grad in ((x, dy), (x.clone().contiguous(), dy.clone().contiguous())):
+        rows = rows.detach().requires_grad_(True)
+        w = torch.randn(24, 64, generator=torch.Generator().manual_seed(8)).to(gpu).requires_grad_(True)
+        y = linear(rows, w, save=save)
+        runs.append((y, *torch.autograd.grad(y, (rows, w), grad)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
