@@ -152,10 +152,10 @@ def _row_gemm(a: torch.Tensor, b: torch.Tensor, b_kc: bool) -> torch.Tensor:
     """``a [R, K] @ b.t()`` (b_kc: b [N, K]) or ``a @ b`` (b [K, N]) on the BF16 GEMM;
     rows beyond an operand's 2 GiB in further calls (a row's result does not depend
     on the row count)."""
-    R, K = a.shape
-    N = b.shape[0] if b_kc else b.shape[1]
+    R, K = map(int, a.shape)  # (tensors in a trace)
+    N = int(b.shape[0] if b_kc else b.shape[1])
     out = torch.empty((R, N), device=a.device, dtype=torch.bfloat16)
-    ld = a.stride(0) if R > 1 else K
+    ld = int(a.stride(0)) if R > 1 else K
     step = max(1, _GEMM_SPAN // (2 * ld))
     with _native.device_ctx(a.device):
         for r in range(0, R, step):

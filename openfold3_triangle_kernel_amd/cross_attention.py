@@ -114,7 +114,7 @@ def _mask_operand(mask: torch.Tensor | None, prefix, batch: int, Nk: int):
         kind = _MASK_BYTES
     else:
         kind = _MASK_F32
-        mask = mask.detach().to(torch.float32)
+        mask = mask.to(torch.float32)
     lead = mask.shape[:-1]
     if all(n == 1 for n in lead):
         return mask.reshape(Nk).contiguous(), kind, 0
@@ -180,6 +180,19 @@ class _CrossAttentionFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
+class _CrossAttentionInference(torch.autograd.Function):
+    """The forward alone.  A Function all the same, so that forward-mode AD and function
+    transforms, which the native calls would hide, are refused, and a trace records it."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, mask, kind, mask_stride, scale):
+        return _forward(q, k, v, mask, kind, mask_stride, scale, False)[0]
+
+    @staticmethod
+    def backward(ctx, d_out):  # pragma: no cover - only called without gradients
+        raise RuntimeError("the inference call has no backward")
+
+
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                     key_mask: torch.Tensor | None = None,
                     scale: float | None = None) -> torch.Tensor:
@@ -228,7 +241,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         out = _CrossAttentionFn.apply(q, k, v, mask, kind, mask_stride, float(scale),
                                       shadow_enabled())
     else:
-        out = _forward(q, k, v, mask, kind, mask_stride, float(scale), False)[0]
+        out = _CrossAttentionInference.apply(q, k, v, mask, kind, mask_stride, float(scale))
     if pad:
         out = out[..., :head_dim].contiguous()
     return out if len(prefix) == 1 else out.reshape(tuple(prefix) + out.shape[1:])

@@ -177,6 +177,19 @@ class _LayerNormFn(torch.autograd.Function):
                 None, None, None)
 
 
+class _LayerNormInference(torch.autograd.Function):
+    """The forward alone.  A Function all the same, so that forward-mode AD and function
+    transforms, which the native calls would hide, are refused, and a trace records it."""
+
+    @staticmethod
+    def forward(ctx, x2, w, b, eps):
+        return _norm_forward(x2, w, b, eps, None)[0]
+
+    @staticmethod
+    def backward(ctx, dy):  # pragma: no cover - only called without gradients
+        raise RuntimeError("the inference call has no backward")
+
+
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
                bias: torch.Tensor | None = None, eps: float = 1e-5,
                save: str = "full") -> torch.Tensor:
@@ -211,15 +224,16 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
         for p, op in ((weight, torch.mul), (bias, torch.add)):
             out = out if p is None else op(out, p.to(x.dtype))
         return out.clone() if out is x else out
-    w, b = (None if p is None else p.detach().contiguous() for p in (weight, bias))
+    w, b = (None if p is None else p.contiguous() for p in (weight, bias))
     if w is not None and b is not None and w.dtype != b.dtype:
         w, b = w.float(), b.float()
     grad = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, weight, bias))
     if grad:
+        w, b = (None if p is None else p.detach() for p in (w, b))
         y = _LayerNormFn.apply(as_rows(x), weight, bias, w, b, float(eps), save)
     else:
-        y = _norm_forward(as_rows(x.detach()), w, b, float(eps), None)[0]
+        y = _LayerNormInference.apply(as_rows(x), w, b, float(eps))
     return y.view(x.shape)
 
 
