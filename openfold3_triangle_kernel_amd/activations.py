@@ -103,6 +103,32 @@ def _pack(x2: torch.Tensor):
     return codes, scales
 
 
+class _PackFn(torch.autograd.Function):
+    """The codes and scales of rows x [R, C].  A Function for traces to record and function
+    transforms to be refused; its outputs are whole numbers, without derivatives."""
+
+    @staticmethod
+    def forward(ctx, x2):
+        codes, scales = _pack(x2)
+        ctx.mark_non_differentiable(codes, scales)
+        return codes, scales
+
+
+class _UnpackFn(torch.autograd.Function):
+    """The tensor of ``shape`` and ``dtype`` that codes and scales stand for."""
+
+    @staticmethod
+    def forward(ctx, codes, scales, shape, dtype):
+        out = torch.empty(shape, device=codes.device, dtype=dtype)
+        if out.numel():
+            C = shape[-1]
+            with _native.device_ctx(out.device):
+                _native.call("tpf_act8_unpack", codes.data_ptr(), scales.data_ptr(),
+                             out.numel() // C, C, out.data_ptr(), C, _DTYPES[dtype],
+                             _native.stream_of(out))
+        return out
+
+
 def compress_activation(x: torch.Tensor) -> CompressedActivation:
     """``x`` [*, C] (BF16, FP16 or FP32) in 8 bits; no gradient passes through."""
     if host_path(x):
@@ -111,7 +137,7 @@ def compress_activation(x: torch.Tensor) -> CompressedActivation:
         if packed is not None:
             return CompressedActivation(*packed, x.shape, x.dtype)
     check_rows("compress_activation", x)
-    return CompressedActivation(*_pack(as_rows(x.detach())), x.shape, x.dtype)
+    return CompressedActivation(*_PackFn.apply(as_rows(x.detach())), x.shape, x.dtype)
 
 
 def decompress_activation(saved: CompressedActivation,
@@ -139,13 +165,8 @@ def decompress_activation(saved: CompressedActivation,
     ok, reason = _device_supported(saved.codes)
     if not ok:
         raise ValueError(f"decompress_activation: {reason}")
-    out = torch.empty(saved.shape, device=saved.codes.device, dtype=dtype)
-    if out.numel():
-        with _native.device_ctx(out.device):
-            _native.call("tpf_act8_unpack", saved.codes.data_ptr(), saved.scales.data_ptr(),
-                         out.numel() // C, C, out.data_ptr(), C, _DTYPES[dtype],
-                         _native.stream_of(out))
-    return out
+    shape = tuple(map(int, saved.shape))  # (tensors in a trace)
+    return _UnpackFn.apply(saved.codes, saved.scales, shape, dtype)
 
 
 def _row_gemm(a: torch.Tensor, b: torch.Tensor, b_kc: bool) -> torch.Tensor:

@@ -95,3 +95,26 @@ def test_traces_compute(gpu):
         traced = torch.jit.trace(call, first[name], check_trace=False)
         want = call(*second[name])
         assert torch.equal(traced(*second[name]), want), name
+
+
+def _there_and_back(x):
+    return decompress_activation(compress_activation(x), torch.float32)
+
+
+def test_codec_takes_values_only(fake):
+    """No derivative passes through the codec, forward mode included; a trace holds it."""
+    x = torch.randn(30, 64)
+    with forward_ad.dual_level():
+        out = _there_and_back(forward_ad.make_dual(x, torch.ones_like(x)))
+        assert forward_ad.unpack_dual(out).tangent is None
+    graph = str(torch.jit.trace(_there_and_back, (x,), check_trace=False).graph)
+    assert graph.count("^_") == 2, graph
+    with pytest.raises(RuntimeError, match="functorch|vmap|data pointer"):
+        torch.vmap(_there_and_back)(x[None])
+
+
+@pytest.mark.gpu
+def test_traced_codec_computes(gpu):
+    x, y = (torch.randn(30, 64, generator=torch.Generator().manual_seed(s)).to(gpu) for s in (1, 2))
+    traced = torch.jit.trace(_there_and_back, (x,), check_trace=False)
+    assert torch.equal(traced(y), _there_and_back(y)) and not torch.equal(traced(y), traced(x))
