@@ -41,12 +41,12 @@ DEVICE_FLAGS = [
 ]
 
 
-# Per-source extra flags.  The attention kernels: they never test for NaN
+# Per-source extra flags.  attention.hip: the kernels never test for NaN
 # and take scores that are finite or -inf, so fmaxf needs no NaN quieting
 # (without the flag every v_max of an MFMA result is preceded by a
 # canonicalising v_max: six VALU instructions per 32 x 32 score block).
-FILE_FLAGS = {name: ["-fno-honor-nans"]
-              for name in ("attention.hip", "xattn.hip", "xattn_bwd.hip")}
+# Not for the cross-attention sources, which answer for NaN in their operands.
+FILE_FLAGS = {"attention.hip": ["-fno-honor-nans"]}
 
 
 def _hipcc() -> str:

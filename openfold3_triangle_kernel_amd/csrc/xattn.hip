@@ -95,10 +95,10 @@ struct XRows {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) t = fmaxf(t, s[qb][kb][r]);
-      t = xor32_max(t);
+        for (int r = 0; r < 16; ++r) t = xa_max(t, s[qb][kb][r]);
+      t = xa_max32(t);
       if (__ballot((t - m[qb]) * a.c > 8.f)) {
-        const float mn = fmaxf(m[qb], t), al = fast_exp2((m[qb] - mn) * a.c);
+        const float mn = xa_max(m[qb], t), al = fast_exp2((m[qb] - mn) * a.c);
         m[qb] = mn;
         if constexpr (STATS) l[qb] *= al;
         n[qb] *= al;
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
     if (group) return;
     const float m1 = ml[3 * (64 * w + lane)], l1 = ml[3 * (64 * w + lane) + 1];
     const float n1 = ml[3 * (64 * w + lane) + 2];
-    const float m = fmaxf(rows.m[0], m1);
+    const float m = xa_max(rows.m[0], m1);
     const float f0 = fast_exp2((rows.m[0] - m) * a.c), f1 = fast_exp2((m1 - m) * a.c);
     xa_take<DB>(lds, w, rows.o[0], f0, f1);
     rows.l[0] = f0 * rows.l[0] + f1 * l1;
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
     if (r >= a.R) continue;
     float m = kXaLow, l = 0.f, n = 0.f, f[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) m = fmaxf(m, ML[3 * (x * 32 + rl)]);
+    for (int x = 0; x < 4; ++x) m = xa_max(m, ML[3 * (x * 32 + rl)]);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       f[x] = fast_exp2((ML[3 * (x * 32 + rl)] - m) * a.c);
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
   const float* ml = a.part_ml + 3 * (bh * a.splits * a.R + r);
   const float* po = a.part_o + (bh * a.splits * a.R + r) * a.D + d;
   float m = kXaLow;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[3 * (int64_t)s * a.R]);
+  for (int s = 0; s < a.splits; ++s) m = xa_max(m, ml[3 * (int64_t)s * a.R]);
   float l = 0.f, n = 0.f;
   f32x4 o = (f32x4)0.f;
   for (int s = 0; s < a.splits; ++s) {
@@ -505,10 +505,10 @@ __global__ __launch_bounds__(256) void xattn_join_few_kernel(XAttnArgs a) {
   }
   float m = m0;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  for (int o = 32; o; o >>= 1) m = xa_max(m, __shfl_xor(m, o));
   if ((tid & 63) == 0) red[w][0] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  m = xa_max(xa_max(red[0][0], red[1][0]), xa_max(red[2][0], red[3][0]));
   const float f = tid < a.splits ? fast_exp2((m0 - m) * a.c) : 0.f;
   wt[tid] = f;
   const float ls = lanes_sum<64>(f * l0), ns = lanes_sum<64>(f * n0);

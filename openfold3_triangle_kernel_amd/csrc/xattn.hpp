@@ -85,6 +85,17 @@ __device__ __forceinline__ bf16x8 xa_pack8(const f32x16& c, int r0) {
   return __builtin_bit_cast(bf16x8, o);
 }
 
+// The larger of two values, NaN where one is (v_maximum3_f32: three values a step, and
+// no quieting of its operands first): a NaN score makes its row's maximum NaN.
+__device__ __forceinline__ float xa_max(float x, float y) {
+  return __builtin_elementwise_maximum(x, y);
+}
+// The larger of a lane's and lane ^ 32's value.
+__device__ __forceinline__ float xa_max32(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return xa_max(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // Adds the two 16-bit values of a pair to acc, in 32 bits.
 template <bool F16>
 __device__ __forceinline__ float xa_add_pair(uint32_t pair, float acc) {
@@ -166,8 +177,7 @@ __device__ __forceinline__ float xa_raw_mask(uint32_t m, float inv_scale, float 
 
 // The masks of the 64 states from k0 on: lane l holds state k0 + l.  What a
 // dead or absent state gives is 0 in `live`.  Additive values are held as
-// bits: -inf is a dead state, a NaN is not (as floats, which the build takes for
-// never NaN, the two would pass one comparison).
+// bits: -inf is a dead state, a NaN is not.
 struct XMask {
   const uint8_t* b = nullptr;
   const float* f = nullptr;

@@ -200,3 +200,10 @@ def test_c_abi_shadow_arguments():
         with pytest.raises(RuntimeError, match=match):
             _native.call("tpf_xattn_backward_shadow_bf16", 16, 16, 16, None, 16, residual, *([16] * 6), 8,
                          s, g, 0.1, None)
+
+
+def test_nan_is_honoured_where_it_is_answered_for():
+    """No source whose kernels carry NaN to their results is built as if there were none."""
+    from openfold3_triangle_kernel_amd.build import FILE_FLAGS
+
+    assert {name for name, flags in FILE_FLAGS.items() if any("nan" in f for f in flags)} <= {"attention.hip"}
