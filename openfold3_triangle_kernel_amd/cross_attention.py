@@ -106,6 +106,14 @@ def _strides(t: torch.Tensor):
     return (sb if nb > 1 else 0, sh if nh > 1 else 0, sn if nn > 1 else 0)
 
 
+def additive_f32(mask: torch.Tensor) -> torch.Tensor:
+    """An additive mask in FP32: finite values of FP64 stay finite."""
+    if mask.dtype == torch.float64:
+        ends = torch.finfo(torch.float32)
+        mask = torch.where(torch.isfinite(mask), mask.clamp(ends.min, ends.max), mask)
+    return mask.to(torch.float32)
+
+
 def _mask_operand(mask: torch.Tensor | None, prefix, batch: int, Nk: int):
     """(tensor, kind, batch stride) of the mask as the kernels read it."""
     if mask is None:
@@ -114,7 +122,7 @@ def _mask_operand(mask: torch.Tensor | None, prefix, batch: int, Nk: int):
         kind = _MASK_BYTES
     else:
         kind = _MASK_F32
-        mask = mask.to(torch.float32)
+        mask = additive_f32(mask)
     lead = mask.shape[:-1]
     if all(n == 1 for n in lead):
         return mask.reshape(Nk).contiguous(), kind, 0

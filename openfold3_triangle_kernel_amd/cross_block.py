@@ -22,7 +22,7 @@ from torch import nn
 from . import routing
 from .activations import linear
 from .attention import _device_supported
-from .cross_attention import cross_attention
+from .cross_attention import additive_f32, cross_attention
 from .layernorm import layer_norm
 
 
@@ -131,7 +131,7 @@ def _stock_cross_attention(q, k, v, key_mask):
     s = q.float() @ k.float().transpose(-1, -2).contiguous() / math.sqrt(q.shape[-1])
     if key_mask is not None:
         drop = key_mask[..., None, None, :]
-        s = s.masked_fill(~drop, float("-inf")) if drop.dtype == torch.bool else s + drop.float()
+        s = s.masked_fill(~drop, float("-inf")) if drop.dtype == torch.bool else s + additive_f32(drop)
     # The maximum only guards the exponentials; 0 for a row without a state.
     top = s.detach().amax(-1, keepdim=True) if s.shape[-1] else s.new_zeros(s.shape[:-1] + (1,))
     p = torch.exp(s - top.masked_fill(torch.isneginf(top), 0.0))

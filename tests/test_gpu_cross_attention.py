@@ -639,3 +639,26 @@ def test_shadow_policy(gpu, monkeypatch):
         cross_attention(q, k, v)
     with torch.no_grad():
         assert torch.equal(cross_attention(q, k, v), with_[0])
+
+
+@pytest.mark.parametrize("Nq", [1, 100])
+def test_masks_in_64_bits(gpu, Nq):
+    """Finite values past the 32-bit range are finite still: at the lowest a state is not
+    dropped, at the highest it does not make its rows NaN."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 2, 2, 2, Nq, 130, 64, seed=8)
+    ends = torch.finfo(torch.float64).min, torch.finfo(torch.float64).max
+    wide = torch.randn(2, 130, dtype=torch.float64, generator=torch.Generator().manual_seed(8)).to(gpu)
+    wide[0, 7], wide[0, 9], wide[1] = float("-inf"), ends[0], ends[0]
+    narrow = wide.clamp(torch.finfo(torch.float32).min, torch.finfo(torch.float32).max).float()
+    narrow[0, 7] = float("-inf")
+    with torch.no_grad():
+        out = cross_attention(q, k, v, wide)
+        assert torch.equal(out, cross_attention(q, k, v, narrow))
+        assert out[1].any()  # live states, not a row of zeros
+        wide[1, 5], narrow[1, 5] = ends[1], torch.finfo(torch.float32).max
+        out = cross_attention(q, k, v, wide)
+        assert torch.equal(out, cross_attention(q, k, v, narrow)) and torch.isfinite(out).all()
+        wide[1, 6] = float("nan")
+        assert cross_attention(q, k, v, wide)[1].isnan().all()

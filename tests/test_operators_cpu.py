@@ -207,3 +207,15 @@ def test_nan_is_honoured_where_it_is_answered_for():
     from openfold3_triangle_kernel_amd.build import FILE_FLAGS
 
     assert {name for name, flags in FILE_FLAGS.items() if any("nan" in f for f in flags)} <= {"attention.hip"}
+
+
+def test_block_takes_masks_in_64_bits():
+    """Finite values past the 32-bit range leave a state live, as in the kernels."""
+    torch.manual_seed(0)
+    block = CrossAttention(16, 24, 8, 4)
+    x, kv = torch.randn(2, 3, 16), torch.randn(2, 5, 24)
+    mask = torch.zeros(2, 5, dtype=torch.float64)
+    mask[0, 2], mask[1] = torch.finfo(torch.float64).max, torch.finfo(torch.float64).min
+    narrow = mask.clamp(torch.finfo(torch.float32).min, torch.finfo(torch.float32).max).float()
+    out = block(x, kv, mask)
+    assert torch.equal(out, block(x, kv, narrow)) and torch.isfinite(out).all() and out[1].any()
