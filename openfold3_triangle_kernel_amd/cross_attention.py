@@ -138,14 +138,24 @@ def _shape(q, k, v, kind, mask_stride):
                   *_strides(k), *_strides(v))
 
 
+def _workspace_bytes(shape, backward: bool) -> int:
+    """Bytes of the forward's workspace; sizes that its launches (or the backward's) do
+    not hold are refused."""
+    ws_bytes = int(_native.query("tpf_xattn_forward_workspace_bytes", shape))
+    if ws_bytes < 0 or (backward and int(
+            _native.query("tpf_xattn_backward_workspace_bytes", shape)) < 0):
+        raise _unsupported(_native.query("tpf_last_error").decode(errors="replace"))
+    return ws_bytes
+
+
 def _forward(q, k, v, mask, kind, mask_stride, scale, want_lse, shadow=False):
     """(out, lse, what out's rounding drops); what is not asked for is None."""
     B, H, Nq, D = q.shape
+    shape = _shape(q, k, v, kind, mask_stride)
+    ws_bytes = _workspace_bytes(shape, want_lse)
     out = torch.empty((B, Nq, H, D), device=q.device, dtype=q.dtype)
     lse = torch.empty((2 if kind == _MASK_F32 else 1, B, H, Nq), device=q.device,
                       dtype=torch.float32) if want_lse else None
-    shape = _shape(q, k, v, kind, mask_stride)
-    ws_bytes = int(_native.query("tpf_xattn_forward_workspace_bytes", shape))
     ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes > 0 else None
     residual = torch.empty_like(out) if shadow else None
     name, kept = ("tpf_xattn_forward", ()) if residual is None else (
@@ -153,7 +163,7 @@ def _forward(q, k, v, mask, kind, mask_stride, scale, want_lse, shadow=False):
     with _native.device_ctx(q.device):
         _native.call(name, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                      _native.ptr(mask), out.data_ptr(), _native.ptr(lse), *kept, _native.ptr(ws),
-                     max(ws_bytes, 0), shape, scale, _native.stream_of(q))
+                     ws_bytes, shape, scale, _native.stream_of(q))
     return out, lse, residual
 
 

@@ -72,7 +72,8 @@ __global__ __launch_bounds__(256) void act8_kernel(ActArgs a) {
 template <bool PACK>
 static int act8_launch(ActArgs a, int64_t dt, hipStream_t s, const char* fn) {
   const int64_t n = (a.R * a.chunks.d + 511) / 512;
-  if (n > INT32_MAX) return set_error(TPF_ERR_SHAPE, "%s: too many values", fn);
+  if (n >= (int64_t)1 << 24)  // 2^32 threads
+    return set_error(TPF_ERR_SHAPE, "%s: too many values", fn);
   const dim3 grid((unsigned)n), block(256);
   if (dt == TPF_BF16) hipLaunchKernelGGL((act8_kernel<0, PACK>), grid, block, 0, s, a);
   else if (dt == TPF_F16) hipLaunchKernelGGL((act8_kernel<1, PACK>), grid, block, 0, s, a);

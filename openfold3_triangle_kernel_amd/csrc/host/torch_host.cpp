@@ -412,11 +412,11 @@ Tensor xattn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Te
     *res = at::empty_like(out);
     check(tpf_xattn_forward_shadow_bf16(cptr(q), cptr(k), cptr(v), cptr(mask), out.data_ptr(),
                                         (float*)lse->data_ptr(), res->data_ptr(), mptr(ws),
-                                        n < 0 ? 0 : n, &s, scale, stream()),
+                                        n, &s, scale, stream()),
           "tpf_xattn_forward_shadow_bf16");
   } else {
     check(tpf_xattn_forward(cptr(q), cptr(k), cptr(v), cptr(mask), out.data_ptr(),
-                            lse ? (float*)lse->data_ptr() : nullptr, mptr(ws), n < 0 ? 0 : n, &s, scale,
+                            lse ? (float*)lse->data_ptr() : nullptr, mptr(ws), n, &s, scale,
                             stream()),
           "tpf_xattn_forward");
   }
@@ -513,6 +513,10 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
     kind = mt == at::kBool ? TPF_MASK_BYTES : TPF_MASK_F32;
     mask_stride = mask.dim() == 2 && mask.size(0) > 1 ? Nk : 0;
   }
+  // Sizes that the launches do not hold (of the backward too, before the forward).
+  const tpf_xattn_shape s = xattn_shape(q, k, v, kind, mask_stride);
+  if (tpf_xattn_forward_workspace_bytes(&s) < 0 || (grad && tpf_xattn_backward_workspace_bytes(&s) < 0))
+    return std::nullopt;
   if (grad) return XattnFn::apply(q, k, v, mask_in, kind, mask_stride, scale, sh == "1");
   return xattn_forward(q, k, v, mask, kind, mask_stride, scale, nullptr, nullptr);
 }

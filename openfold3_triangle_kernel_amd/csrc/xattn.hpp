@@ -296,6 +296,9 @@ __device__ __forceinline__ void xa_row(const XAttnArgs& a, int r, int& g, int& i
   i = r - g * a.Nq;
 }
 
+// Workgroups of 256 threads a launch may have: below 2^32 threads, a multiple of 8.
+constexpr int64_t kXaMaxGroups = ((int64_t)1 << 24) - 8;
+
 // Sizes, strides and scale of a call into `a` (xattn.hip); 0 or an error code.
 int xattn_check(XAttnArgs& a, const tpf_xattn_shape* s, double scale, const char* fn);
 

@@ -425,13 +425,16 @@ static void split_axis(int64_t groups, int64_t n, int64_t tile, int* splits, int
   *kw = groups * *splits <= 256 && *chunk >= 128 ? 2 : 1;
 }
 
-static void grad_plan(XAttnGrad& g) {
+static int grad_plan(XAttnGrad& g, const char* fn) {
   XAttnArgs& a = g.f;
   const int64_t BH = (int64_t)a.B * a.Hk;
+  if (BH * (((int64_t)a.Nk + 127) / 128) > kXaMaxGroups)
+    return set_error(TPF_ERR_SHAPE, "%s: too many states", fn);
   a.tiles = (a.R + 127) / 128;
   g.ktiles = (a.Nk + 127) / 128;
   split_axis(BH * a.tiles, a.Nk, 64, &a.splits, &a.chunk, &a.kw);
   split_axis(BH * g.ktiles, a.R, 64, &g.rsplits, &g.rchunk, &g.rkw);
+  return TPF_OK;
 }
 
 // Workspace in floats: delta, then the partials of the split launches, each
@@ -472,8 +475,8 @@ static void grad_pick(const XAttnGrad& g, hipStream_t s) {
 
 extern "C" int64_t tpf_xattn_backward_workspace_bytes(const tpf_xattn_shape* shape) {
   tpf::XAttnGrad g{};
-  if (tpf::xattn_check(g.f, shape, 1.0, "tpf_xattn_backward_workspace_bytes")) return -1;
-  tpf::grad_plan(g);
+  const char* fn = "tpf_xattn_backward_workspace_bytes";
+  if (tpf::xattn_check(g.f, shape, 1.0, fn) || tpf::grad_plan(g, fn)) return -1;
   return tpf::GradSpace(g).total * 4;
 }
 
@@ -497,7 +500,7 @@ static int xattn_backward_entry(const void* q, const void* k, const void* v, con
   for (int i = 0; i < 9; ++i)
     if (grad_strides[i] < 0 || grad_strides[i] % 8)
       return tpf::set_error(TPF_ERR_SHAPE, "%s: gradient strides must be multiples of 8 elements", fn);
-  tpf::grad_plan(g);
+  if (int rc = tpf::grad_plan(g, fn)) return rc;
   const tpf::GradSpace ws(g);
   if (workspace_bytes < ws.total * 4)
     return tpf::set_error(TPF_ERR_ARG, "%s: workspace too small", fn);

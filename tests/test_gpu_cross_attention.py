@@ -662,3 +662,18 @@ def test_masks_in_64_bits(gpu, Nq):
         assert torch.equal(out, cross_attention(q, k, v, narrow)) and torch.isfinite(out).all()
         wide[1, 6] = float("nan")
         assert cross_attention(q, k, v, wide)[1].isnan().all()
+
+
+@pytest.mark.parametrize("host", [True, False], ids=["cpp", "python"])
+def test_more_rows_than_a_launch_holds_are_refused(gpu, monkeypatch, host):
+    from openfold3_triangle_kernel_amd import _native, cross_attention
+
+    if not host:
+        monkeypatch.setattr(_native, "_HOST", False)
+    one = torch.zeros(1, 1, 1, 8, device=gpu, dtype=torch.bfloat16)
+    wide = one.expand(1 << 24, -1, -1, -1)
+    with pytest.raises(ValueError, match="too many"):
+        cross_attention(wide, wide, wide)
+    states = one.expand(1 << 11, -1, 1 << 20, -1)  # the dK / dV launch
+    with pytest.raises(ValueError, match="too many states"):
+        cross_attention(one.expand(1 << 11, -1, -1, -1).clone().requires_grad_(True), states, states)

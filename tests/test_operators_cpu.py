@@ -219,3 +219,30 @@ def test_block_takes_masks_in_64_bits():
     narrow = mask.clamp(torch.finfo(torch.float32).min, torch.finfo(torch.float32).max).float()
     out = block(x, kv, mask)
     assert torch.equal(out, block(x, kv, narrow)) and torch.isfinite(out).all() and out[1].any()
+
+
+def test_sizes_that_a_launch_does_not_hold():
+    """A launch has less than 2^32 threads: more workgroups are refused, of the backward's
+    too before the forward."""
+    from openfold3_triangle_kernel_amd import _native
+    from openfold3_triangle_kernel_amd.cross_attention import _workspace_bytes
+
+    most = (1 << 24) - 8
+    one = dict(H=1, Hk=1, D=8, q=(8, 8, 8), k=(8, 8, 8), v=(8, 8, 8))
+    for kw, forward, backward in ((dict(B=most, Nq=1, Nk=1), True, True),
+                                  (dict(B=most + 1, Nq=1, Nk=1), False, False),
+                                  (dict(B=most // 2, Nq=256, Nk=1), False, False),
+                                  (dict(B=most // 8, Nq=64, Nk=1024), True, True),
+                                  (dict(B=most // 8, Nq=64, Nk=1025), True, False)):
+        shape = _shape(**one, **kw)
+        for ok, name in ((forward, "tpf_xattn_forward_workspace_bytes"),
+                         (backward, "tpf_xattn_backward_workspace_bytes")):
+            assert (_native.query(name, shape) >= 0) == ok, (kw, name)
+        for ok, grad in ((forward, False), (backward, True)):
+            if ok:
+                assert _workspace_bytes(shape, grad) >= 0
+            else:
+                with pytest.raises(ValueError, match="too many"):
+                    _workspace_bytes(shape, grad)
+    with pytest.raises(RuntimeError, match="too many values"):
+        _native.call("tpf_act8_pack", 16, 32, 1 << 31, 32, 0, 16, 16, None)
