@@ -677,3 +677,36 @@ def test_more_rows_than_a_launch_holds_are_refused(gpu, monkeypatch, host):
     states = one.expand(1 << 11, -1, 1 << 20, -1)  # the dK / dV launch
     with pytest.raises(ValueError, match="too many states"):
         cross_attention(one.expand(1 << 11, -1, -1, -1).clone().requires_grad_(True), states, states)
+
+
+@pytest.mark.parametrize("mk", ["none", "random", "add"])
+@pytest.mark.parametrize("scale", [0.02, 1, 4.0])
+@pytest.mark.parametrize("B,H,Hk,Nq,Nk,D", [(2, 4, 2, 3, 400, 64), (2, 2, 1, 130, 150, 40)])
+def test_explicit_scales(gpu, B, H, Hk, Nq, Nk, D, scale, mk):
+    """Scales other than the default in both directions, whole numbers too; additive
+    values are added after the scale."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = (t.requires_grad_(True)
+               for t in _make(gpu, B, H, Hk, Nq, Nk, D, seed=14, qscale=0.5))
+    mask = _mask(gpu, mk, B, Nk, 14)
+    dout = torch.randn(B, Nq, H, D, generator=torch.Generator().manual_seed(15)).bfloat16().to(gpu)
+    want, tol = _reference(q, k, v, mask, scale, dout)
+    out = cross_attention(q, k, v, mask, scale)
+    _check([out, *torch.autograd.grad(out, (q, k, v), dout)], want, tol)
+
+
+@pytest.mark.parametrize("scale", [1e-29, 1e-10, 1e6, 1e29])
+def test_scales_of_the_whole_range(gpu, scale):
+    """q carries the scale's inverse: the products are those of the default scale."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 1, 2, 1, 70, 90, 64, seed=16)
+    mask = _mask(gpu, "add", 1, 90, 16)
+    power = round(math.log2(0.125 / scale))
+    qs = (q.float() * 2.0 ** power).bfloat16().requires_grad_(True)
+    k, v = k.requires_grad_(True), v.requires_grad_(True)
+    dout = torch.randn(1, 70, 2, 64, generator=torch.Generator().manual_seed(17)).bfloat16().to(gpu)
+    want, tol = _reference(qs, k, v, mask, scale, dout)
+    out = cross_attention(qs, k, v, mask, scale)
+    _check([out, *torch.autograd.grad(out, (qs, k, v), dout)], want, tol)

@@ -325,3 +325,45 @@ def test_frozen_weight_beside_a_bias_of_another_type(gpu, save, t, wt, bt, size)
         tol = tol + want.abs() * rstd * tt * xd.abs().mean(-1, keepdim=True)  # rstd's, from the mean's
     _near(dx, want, tol, "dx")
     _near(db, wdb, tdb, "db")
+
+
+@pytest.mark.parametrize("save", ["full", "int8"])
+def test_parameter_gradients_of_many_rows(gpu, save):
+    """Column sums over 2 150 000 rows against sums in 64 bits, by a bound that a
+    workgroup's rows left out would pass.
+
+    Inputs and upstream gradients are independent normal values, so n terms sum to less
+    than 6 sqrt(n) in magnitude.  A thread adds n = R / 4096 rows (1024 workgroups of four
+    rows), each addition off by at most 2^-24 of the running sum: 2^-24 sum_i 6 sqrt(i) =
+    2^-24 4 n^1.5, for 4096 threads; the fold adds 64 + 16 + 4 sums of at most 6 sqrt(R).
+    dw also has the error of xh, e a term, which is independent of dy: 6 sqrt(R) e."""
+    from openfold3_triangle_kernel_amd import layer_norm
+    from openfold3_triangle_kernel_amd.layernorm import _norm_forward
+
+    R, C, u = 2_150_000, 1001, 2.0 ** -24
+    g = torch.Generator(device=gpu).manual_seed(2)
+    x = torch.empty(R, C, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+    dy = torch.empty(R, C, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+    w = torch.ones(C, device=gpu).requires_grad_(True)
+    b = torch.zeros(C, device=gpu).requires_grad_(True)
+    dw, db = torch.autograd.grad(layer_norm(x, w, b, save=save), (w, b), dy)
+    chain = 4096 * u * 4 * (R / 4096) ** 1.5 + u * 6 * R ** 0.5 * (64 + 16 + 4)
+    e = 2 * (C / 32 + 32 + 8) * u  # of xh, whose mean square is 1 (|xh| below 6)
+    tol_b, tol_w = chain, chain + 6 * R ** 0.5 * 6 * e
+    sums = torch.zeros(2, C, device=gpu, dtype=torch.float64)
+    share = 4 * -(-R // 4096)  # rows of a workgroup
+    step = 25 * share
+    for r in range(0, R, step):
+        xs, d = x[r:r + step].double(), dy[r:r + step].double()
+        if save == "int8":
+            _, _, _, codes, scales = _norm_forward(x[r:r + step], None, None, 1e-5, "int8")
+            k = torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+            xh = ((codes.double() - 128) * k)[:, :C]
+        else:
+            xh = torch.nn.functional.layer_norm(xs, (C,), eps=1e-5)
+        part = torch.stack([(d * xh)[:share].sum(0), d[:share].sum(0)])
+        assert part.abs().amax() > tol_w > tol_b  # what a workgroup's rows add is seen
+        sums[0] += (d * xh).sum(0)
+        sums[1] += d.sum(0)
+    assert ((dw.double() - sums[0]).abs() <= tol_w).all()
+    assert ((db.double() - sums[1]).abs() <= tol_b).all()
