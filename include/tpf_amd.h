@@ -571,7 +571,7 @@ int tpf_wgrad_act8(const void* dy, int64_t ld_dy, const void* codes, const void*
  * (0 drops the state) or f32 added to the scores (-inf drops it; finite values count as
  * if within +-1.5e38 scale).  1e-30 < scale < 1e30.  K and V of a dropped state are
  * never used, whatever they hold; a NaN that is not dropped reaches its rows.  A row without a state
- * gives 0, and gradients of 0.  Every tensor starts on 16 bytes.
+ * gives 0, and gradients of 0; one whose states all score -inf is NaN.  Every tensor starts on 16 bytes.
  * lse: f32 [B, H, Nq], or [2, B, H, Nq] with an f32 mask: the rows' softmax
  * statistics for the backward; null when none follows.
  * The forward serves BF16 and FP16, the backward BF16.

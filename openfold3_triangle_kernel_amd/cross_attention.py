@@ -221,7 +221,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     +-1.5e38 ``scale``; -inf drops the state).  K and
     V of a dropped state are never used, whatever they hold; a NaN that is not dropped,
     in an additive mask too, reaches its rows.  A row without a state
-    gives zeros, and zero gradients.  ``scale`` is 1/sqrt(D) unless given.  Returns
+    gives zeros, and zero gradients; one whose states all score -inf is NaN.  ``scale`` is 1/sqrt(D) unless given.  Returns
     ``[*B, Nq, H, D]`` of the operands' type.  BF16 operands have gradients (q, k, v);
     FP16 is for inference.  With the policy of ``attention.shadow_enabled`` (the default)
     a training forward also keeps what the output's rounding drops, a tensor of the

@@ -132,11 +132,14 @@ def _stock_cross_attention(q, k, v, key_mask):
     if key_mask is not None:
         drop = key_mask[..., None, None, :]
         s = s.masked_fill(~drop, float("-inf")) if drop.dtype == torch.bool else s + additive_f32(drop)
-    # The maximum only guards the exponentials; 0 for a row without a state.
+    # The maximum only guards the exponentials; 0 for scores of -inf alone.
     top = s.detach().amax(-1, keepdim=True) if s.shape[-1] else s.new_zeros(s.shape[:-1] + (1,))
     p = torch.exp(s - top.masked_fill(torch.isneginf(top), 0.0))
     total = p.sum(-1, keepdim=True)
-    p = p / total.masked_fill(total == 0, 1.0)
+    if key_mask is not None:
+        # Rows without a state give 0; rows whose scores are all -inf otherwise 0 / 0.
+        total = total.masked_fill(dead.all(-2, keepdim=True), 1.0)
+    p = p / total
     return (p @ v.float()).transpose(-2, -3).to(q.dtype)
 
 

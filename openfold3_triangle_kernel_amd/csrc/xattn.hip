@@ -14,7 +14,9 @@
 
 namespace tpf {
 
-constexpr float kXaLow = -3.402823466e38f;
+// The maximum of a row before its first live state, and the least one after it: a row
+// whose scores are all -inf (infinite operands) is told from a row without a state.
+constexpr float kXaLow = -3.402823466e38f, kXaSeen = -3.3e38f;
 constexpr int kXaMaxSplits = 256;  // threads of the workgroup that joins a row's splits
 
 // Running softmax state of a wave's rows; scores and maxima m are in raw units
@@ -91,7 +93,7 @@ struct XRows {
     bf16x8 p[QB][2 * KB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      float t = s[qb][0][0];
+      float t = kXaSeen;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -107,7 +109,7 @@ struct XRows {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[qb][db][r] *= al;
       }
-      float off = -m[qb] * a.c, sum = 0.f;
+      float off = xa_min(-m[qb] * a.c, -kXaLow), sum = 0.f;  // (finite beside a score of -inf)
       if (fmask) {
         off = 0.f;
 #pragma unroll
@@ -151,10 +153,10 @@ struct XRows {
   }
 };
 
-// 1 / sum, and 0 for a row without a live state (compared by bits: a sum that
-// is NaN stays NaN).
-__device__ __forceinline__ float xa_inverse(float l) {
-  return __float_as_uint(l) == 0u ? 0.f : 1.f / l;
+// 1 / sum of a row with the maximum m; 0 for a row without a live state, NaN for one
+// whose scores are all -inf.
+__device__ __forceinline__ float xa_inverse(float n, float m) {
+  return n == 0.f ? (m == kXaLow ? 0.f : __builtin_nanf("")) : 1.f / n;
 }
 
 // A row's statistics for the backward: log2 of the sum and the raw maximum, or
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
     const float l = xor32_sum(rows.l[qb]), n = xor32_sum(rows.n[qb]);
     if (r >= a.R) continue;
     if (a.splits == 1) {
-      xa_store_row<DP / 32, F16>(a, b, hk, r, rows.o[qb], xa_inverse(n));
+      xa_store_row<DP / 32, F16>(a, b, hk, r, rows.o[qb], xa_inverse(n, rows.m[qb]));
       if (a.lse && lane < 32) xa_store_stats(a, bh * a.R + r, rows.m[qb], l);
     } else {
       const int64_t pr = (bh * a.splits + split) * a.R + r;
@@ -423,7 +425,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
       n += f[x] * ML[3 * (x * 32 + rl) + 2];
     }
     const int64_t pr = (bh * a.splits + split) * a.R + r;
-    const float inv = xa_inverse(n);
+    const float inv = xa_inverse(n, m);
     int g, i;
     xa_row(a, r, g, i);
     for (int d = 4 * (threadIdx.x & 7); d < a.D; d += 32) {
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XAttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += w * v[e];
   }
-  const float inv = xa_inverse(n);
+  const float inv = xa_inverse(n, m);
   int g, i;
   xa_row(a, r, g, i);
   const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
@@ -538,7 +540,7 @@ __global__ __launch_bounds__(256) void xattn_join_few_kernel(XAttnArgs a) {
   for (int x = 1; x < 8; ++x)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += part[x][dg][e];
-  const float inv = xa_inverse(n);
+  const float inv = xa_inverse(n, m);
   int g, i;
   xa_row(a, r, g, i);
   const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);

@@ -90,6 +90,9 @@ __device__ __forceinline__ bf16x8 xa_pack8(const f32x16& c, int r0) {
 __device__ __forceinline__ float xa_max(float x, float y) {
   return __builtin_elementwise_maximum(x, y);
 }
+__device__ __forceinline__ float xa_min(float x, float y) {
+  return __builtin_elementwise_minimum(x, y);
+}
 // The larger of a lane's and lane ^ 32's value.
 __device__ __forceinline__ float xa_max32(float x) {
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

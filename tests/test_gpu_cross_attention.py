@@ -710,3 +710,38 @@ def test_scales_of_the_whole_range(gpu, scale):
     want, tol = _reference(qs, k, v, mask, scale, dout)
     out = cross_attention(qs, k, v, mask, scale)
     _check([out, *torch.autograd.grad(out, (qs, k, v), dout)], want, tol)
+
+
+@pytest.mark.parametrize("scale", [0.125, 4.0])
+@pytest.mark.parametrize("Nq,Nk", [(1, 90), (5, 1500), (1, 6000), (130, 200), (200, 3000)])
+def test_scores_of_minus_infinity(gpu, Nq, Nk, scale):
+    """A live state whose score is -inf has no weight; a row that has only such is NaN, as
+    0 / 0 is, and no row without a state (which is 0)."""
+    from openfold3_triangle_kernel_amd import cross_attention
+
+    q, k, v = _make(gpu, 2, 4, 2, Nq, Nk, 64, seed=18)
+    q[..., 0], k[..., 0] = q[..., 0].abs() + 0.5, -k[..., 0].abs() - 0.5
+    whole = _mask(gpu, "random", 2, Nk, 18)
+    whole[:, 0] = True
+    add = torch.where(whole, 0.25, float("-inf"))
+    with torch.no_grad():
+        # The first states (whole tiles of them among many), and some of the others.
+        far = torch.zeros(2, 2, Nk, dtype=torch.bool, device=gpu)
+        far[:, :, :Nk // 3] = True
+        far[:, :, -1] = True
+        ks = k.clone()
+        ks[..., 0] = torch.where(far, float("-inf"), ks[..., 0])
+        for mask in (None, whole, add):
+            kept = torch.ones(2, Nk, dtype=torch.bool, device=gpu) if mask is None else whole
+            want, tol = _reference(q, k, v, kept & ~far[:, 0], scale)
+            _check([cross_attention(q, ks, v, mask, scale)], want, tol)
+        for mask in (None, whole, add):
+            qi = q.clone()
+            qi[1, 2, Nq // 2, 0] = float("inf")
+            out, clean = cross_attention(qi, k, v, mask, scale), cross_attention(q, k, v, mask, scale)
+            hit = torch.zeros(2, Nq, 4, dtype=torch.bool, device=gpu)
+            hit[1, Nq // 2, 2] = True
+            assert out[hit].isnan().all() and torch.equal(out[~hit], clean[~hit])
+        none = whole.clone()
+        none[1] = False
+        assert not cross_attention(qi, k, v, none, scale)[1].any()

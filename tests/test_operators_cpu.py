@@ -246,3 +246,21 @@ def test_sizes_that_a_launch_does_not_hold():
                     _workspace_bytes(shape, grad)
     with pytest.raises(RuntimeError, match="too many values"):
         _native.call("tpf_act8_pack", 16, 32, 1 << 31, 32, 0, 16, 16, None)
+
+
+def test_block_formulas_of_infinite_scores():
+    """In the PyTorch route as in the kernels: no weight for a score of -inf, NaN for a row
+    that has only such, 0 for a row without a state."""
+    from openfold3_triangle_kernel_amd.cross_block import _stock_cross_attention
+
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(2, 2, n, 8, generator=g) for n in (3, 5, 5))
+    q[..., 0], k[..., 0] = q[..., 0].abs() + 0.5, -k[..., 0].abs() - 0.5
+    for mask in (None, torch.ones(2, 5, dtype=torch.bool), torch.zeros(2, 5)):
+        ks = k.clone()
+        ks[:, :, 2:, 0] = float("-inf")
+        part = _stock_cross_attention(q, k[:, :, :2], v[:, :, :2], None)
+        assert (_stock_cross_attention(q, ks, v, mask) - part).abs().max() <= 1e-6
+        ks[..., 0] = float("-inf")
+        assert _stock_cross_attention(q, ks, v, mask).isnan().all()
+    assert not _stock_cross_attention(q, ks, v, torch.zeros(2, 5, dtype=torch.bool)).any()
