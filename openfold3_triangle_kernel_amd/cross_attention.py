@@ -81,15 +81,12 @@ def _check(q, k, v, key_mask, scale) -> None:
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """``t`` [B, H, N, D], or a contiguous copy where the kernels cannot read it."""
-    sb, sh, sn, sd = t.stride()
-    if sd != 1 or (sb | sh | sn) % 8 or sn >= _MAX_STATE_STRIDE or t.data_ptr() % 16:
-        # Strides of axes of one entry address nothing and may be anything.
-        if sd == 1 and t.data_ptr() % 16 == 0 and all(
-                n <= 1 or (s % 8 == 0 and s < _MAX_STATE_STRIDE)
-                for n, s in zip(t.shape[:3], (sb, sh, sn))):
-            return t
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    # Strides of axes of one entry address nothing and may be anything.
+    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
+            and all(n <= 1 or s % 8 == 0 for n, s in zip(t.shape[:3], t.stride()))
+            and (t.shape[2] <= 1 or t.stride(2) < _MAX_STATE_STRIDE)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _grad_like(t: torch.Tensor) -> torch.Tensor:

@@ -475,8 +475,8 @@ struct XattnFn : torch::autograd::Function<XattnFn> {
 bool xattn_operand(const Tensor& t) {
   if (t.stride(3) != 1 || !aligned16(t)) return false;
   for (int i = 0; i < 3; ++i)
-    if (t.size(i) > 1 && (t.stride(i) % 8 || t.stride(i) >= (int64_t(1) << 23))) return false;
-  return true;
+    if (t.size(i) > 1 && t.stride(i) % 8) return false;
+  return t.size(2) <= 1 || t.stride(2) < (int64_t(1) << 23);
 }
 
 // sh: the policy variable of the shadow residual (env_flag).

@@ -745,3 +745,28 @@ def test_scores_of_minus_infinity(gpu, Nq, Nk, scale):
         none = whole.clone()
         none[1] = False
         assert not cross_attention(qi, k, v, none, scale)[1].any()
+
+
+@pytest.mark.parametrize("host", [True, False], ids=["cpp", "python"])
+def test_sequences_far_apart(gpu, monkeypatch, host):
+    """Caches whose sequences or heads lie 2^24 elements apart are read in place, and by the
+    C++ host path where it is there."""
+    import sys
+
+    from openfold3_triangle_kernel_amd import _native, cross_attention
+
+    module = sys.modules["openfold3_triangle_kernel_amd.cross_attention"]
+    q, k, v = _make(gpu, 2, 4, 2, 3, 200, 64, seed=19)
+    far = torch.zeros(2, 1 << 24, device=gpu, dtype=torch.bfloat16)
+    kc, vc = (far[:, at:at + 2 * 200 * 64].view(2, 2, 200, 64) for at in (0, 1 << 16))
+    kc.copy_(k), vc.copy_(v)
+    with torch.no_grad():
+        want = cross_attention(q, k, v)
+        if host:
+            monkeypatch.setattr(module, "_check", lambda *args: pytest.fail("not the C++ host path"))
+        else:
+            monkeypatch.setattr(_native, "_HOST", False)
+        assert torch.equal(cross_attention(q, kc, vc), want)
+        heads = [t.transpose(0, 1) for t in (kc, vc)]
+        assert torch.equal(cross_attention(q[:, :2], *heads),
+                           cross_attention(q[:, :2], *(t.contiguous() for t in heads)))

@@ -264,3 +264,21 @@ def test_block_formulas_of_infinite_scores():
         ks[..., 0] = float("-inf")
         assert _stock_cross_attention(q, ks, v, mask).isnan().all()
     assert not _stock_cross_attention(q, ks, v, torch.zeros(2, 5, dtype=torch.bool)).any()
+
+
+@pytest.mark.parametrize("shape,strides,read", [
+    ((2, 4, 100, 64), (1 << 24, 6400, 64, 1), True),  # sequences far apart
+    ((2, 4, 100, 64), (64, 1 << 24, 256, 1), True),
+    ((2, 1, 100, 64), (1 << 24, 3, 64, 1), True),  # an axis of one entry
+    ((1, 1, 1, 64), (1, 3, 1 << 24, 1), True),
+    ((1, 4, 1, 64), (1, 64, (1 << 23) + 1, 1), True),
+    ((2, 4, 100, 64), (1 << 30, 64, (1 << 23) - 8, 1), True),
+    ((2, 4, 100, 64), (1 << 30, 64, 1 << 23, 1), False),
+    ((2, 4, 100, 64), (25600 + 4, 6400, 64, 1), False),
+    ((2, 4, 100, 64), (51200, 12800, 128, 2), False),
+])
+def test_cross_attention_reads_operands_in_place(shape, strides, read):
+    from openfold3_triangle_kernel_amd.cross_attention import _operand
+
+    t = torch.empty(1 << 32, dtype=torch.bfloat16, device="meta").as_strided(shape, strides)
+    assert (_operand(t) is t) == read
