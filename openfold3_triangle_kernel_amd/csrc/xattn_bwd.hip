@@ -118,11 +118,18 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_dq_kernel(XAttnGrad ga) {
       const bf16x8 o = in ? *reinterpret_cast<const bf16x8*>(ga.o + oo + d) : zero8();
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta = fmaf(bf2f(dO[s][e]), bf2f(o[e]), delta);
-      if (ga.res && in) {
-        const bf16x8 x = *reinterpret_cast<const bf16x8*>(ga.res + oo + d);
+    }
+    if (ga.res) {  // (a loop of its own: its loads go out together)
+      bf16x8 x[DS];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) delta = fmaf(bf2f(dO[s][e]), bf2f(x[e]), delta);
+      for (int s = 0; s < DS; ++s) {
+        const int d = 16 * s + 8 * (lane >> 5);
+        x[s] = d < a.D ? *reinterpret_cast<const bf16x8*>(ga.res + oo + d) : zero8();
       }
+#pragma unroll
+      for (int s = 0; s < DS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf(bf2f(dO[s][e]), bf2f(x[s][e]), delta);
     }
   }
   delta = xor32_sum(delta);
