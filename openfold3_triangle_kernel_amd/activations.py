@@ -4,7 +4,7 @@
 from -120 on for which ``round(max / 2^k)`` is at most 127 (and at most 121, 9 for
 FP16: a larger quotient is held as 127, so decoded values are finite); a value ``x`` is held as
 ``round(x / 2^k)`` (ties to even) in one byte: 33/32 byte a value, an error of at
-most 1/127.5 of the block's largest magnitude.  A decoded value has seven bits and is
+most 1/127.5 of the block's largest magnitude (or 2^-121, half the smallest step).  A decoded value has seven bits and is
 exact in BF16, so the matrix cores take it as it is.  A block that holds an
 infinity or NaN decodes to NaN.
 
@@ -258,7 +258,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, save: str = "int8") -> torch.T
     """``x`` [*, K] times ``weight``^T (``weight`` [N, K]) on the BF16 GEMM.
 
     For the gradient of ``weight`` the input is kept in 8 bits (``save="int8"``, about
-    half of BF16) or as it is (``"full"``).  ``x`` is BF16, ``weight`` BF16 or FP32 (used
+    half of BF16; a channel below 1/255 of the largest among its 32 is kept as 0 and gives
+    its column no gradient) or as it is (``"full"``).  ``x`` is BF16, ``weight`` BF16 or FP32 (used
     in BF16, its gradient from FP32 sums in its own type); K and N are multiples of 8 up
     to 2^23.
     """

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(NormArg
     }
     load(r + step);
     row_sum<TPR, 1>(s, 0);
-    const float mean = s[0] / (float)a.C;  // divided: a constant row's mean is its value
+    const float mean = s[0] / (float)a.C;  // divided: exact where the sum is
     s[0] = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_wide_kernel(NormArgs a) {
       for (int i = 0; i < 8; ++i) s[0] += f[i];
     }
     row_sum<1024, 1>(s, 0);
-    const float mean = s[0] / (float)a.C;  // divided: a constant row's mean is its value
+    const float mean = s[0] / (float)a.C;  // divided: exact where the sum is
     s[0] = 0.f;
     for (int j = threadIdx.x; 8 * j < a.C; j += 1024) {
       to_f32<DT>(load8<DT>(x + 8 * j * EB, min(8, a.C - 8 * j)), f);

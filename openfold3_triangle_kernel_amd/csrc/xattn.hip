@@ -32,8 +32,8 @@ constexpr int kXaMaxSplits = 256;  // threads of the workgroup that joins a row'
 // to 1, so what the states' values have in common passes exactly (divided by the
 // unrounded sum, the roundings of p would scale it).  The backward's p come from
 // scores again and are divided by l, the sum of the unrounded ones, which only a
-// forward with statistics forms (32 heads, 4096 x 4096 x 128: 306 us with it and the
-// residual's stores against 289 without).  n is summed among the second product's steps,
+// forward with statistics forms (32 heads, 4096 x 4096 x 128: 305 us with it and the
+// residual's stores against 284 without).  n is summed among the second product's steps,
 // whose time hides it (before them, 4096 x 4096 x 128 took 289 us instead of 272).
 template <int DP, int QB, bool F16, bool STATS>
 struct XRows {
@@ -214,8 +214,8 @@ __device__ __forceinline__ void xa_store_row(const XAttnArgs& a, int b, int hk, 
 // take a row tile's states in turn (64 each of every 128) and join their results in
 // LDS, for grids that give a CU one workgroup: the SIMDs then have two waves (16
 // heads on 4, 4 x 509 x 1021 x 80: 24.5 us against 28.6 with two splits in memory).
-// 32 heads, 4096 x 4096 x 128 in 288 us (954 TFLOP/s, the matrix and the vector units
-// busy about half the time each), 64 channels in 172.
+// 32 heads, 4096 x 4096 x 128 in 268 to 289 us from card to card (950 to 1025 TFLOP/s, the
+// matrix and the vector units busy about half the time each), 64 channels in 154 to 173.
 template <int DP, int QB, bool F16, int KW, bool STATS>
 __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
   constexpr int KT = 64, TILE = KT * DP, DB = DP / 32;
@@ -327,8 +327,8 @@ __global__ __launch_bounds__(256 * KW, 2) void xattn_fwd_kernel(XAttnArgs a) {
 
 // Few rows (at most 32 QB, one decoded token above all): the states' bytes are
 // the bound.  Every wave streams tiles of 32 states of its own, two stages deep
-// without a barrier, and the four waves' results meet in LDS at the end.  32 kv heads
-// of 4096 states, one row each, unsplit: 96 us, 5.6 TB/s.  16 tokens of 32 heads on 8
+// without a barrier, and the four waves' results meet in LDS at the end.  8 sequences of
+// 32 kv heads with 4096 states, one row each (537 MB, unsplit): 96 us, 5.6 TB/s.  16 tokens of 32 heads on 8
 // with 8191 ragged states (403 MB live) in two splits: 79 us with the join.
 template <int DP, int QB, bool F16, bool STATS>
 __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XAttnArgs a) {
