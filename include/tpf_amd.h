@@ -610,6 +610,75 @@ int tpf_xattn_backward_shadow_bf16(const void* q, const void* k, const void* v, 
                                    int64_t workspace_bytes, const tpf_xattn_shape* shape,
                                    const int64_t* grad_strides, double scale, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Norms of queries and keys for each head with the rotation by position, in one pass.
+ *
+ * x^ = x / sqrt(mean(x^2) + eps) (norm; else x), z = x^ w (w [D] of weight_dtype, null
+ * for 1); the first 2 half channels are turned in pairs by the angles position *
+ * frequencies[c] (f64 [half], radians): y_a = z_a cos - z_b sin, y_b = z_b cos + z_a
+ * sin, pairs (c, c + half) or interleaved (2 c, 2 c + 1); the others pass.  q [B, H, N,
+ * D] and k [B, Hk, N, D] (H or Hk may be 0), outputs the same, each through its element
+ * strides of the first three axes, channels contiguous, aligned to the element; D up to
+ * 256.  positions: whole numbers of position_bits (32 or 64) [B, N] through
+ * position_stride, null for 0 .. N - 1.  Sums and angles in 32 bits, an angle's turns
+ * in 64.
+ *
+ * The backward takes the upstream gradients through grad_strides (six values: of dq_out,
+ * then dk_out), q and k as the forward read them (null without a norm) and writes dq and
+ * dk through the out strides; dq_weight, dk_weight [D] of weight_dtype, null when not
+ * wanted (with both null no workspace is needed).
+ * ---------------------------------------------------------------------- */
+typedef struct tpf_rotary_shape {
+  int64_t B, N, H, Hk, D, half;
+  int64_t dtype, weight_dtype, norm, interleaved, position_bits;
+  int64_t position_stride[2];
+  int64_t q_stride[3], k_stride[3], out_q_stride[3], out_k_stride[3]; /* batch, head, position */
+} tpf_rotary_shape;
+int tpf_rotary_forward(const void* q, const void* k, const void* positions,
+                       const double* frequencies, const void* q_weight, const void* k_weight,
+                       double eps, void* q_out, void* k_out, const tpf_rotary_shape* shape,
+                       void* stream);
+int64_t tpf_rotary_backward_workspace_bytes(const tpf_rotary_shape* shape);
+int tpf_rotary_backward(const void* q, const void* k, const void* dq_out, const void* dk_out,
+                        const void* positions, const double* frequencies, const void* q_weight,
+                        const void* k_weight, double eps, void* dq, void* dk, void* dq_weight,
+                        void* dk_weight, void* workspace, int64_t workspace_bytes,
+                        const tpf_rotary_shape* shape, const int64_t* grad_strides, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Sequences over a paged cache.  k_cache and v_cache are [pages, Hk, page, D]
+ * contiguous; a batch packs the new tokens of S sequences into T rows: those of sequence
+ * s are the rows starts[s] .. starts[s + 1] (ascending from 0; rows from starts[S] on
+ * belong to none) and the last of its lengths[s] states.  State j lies in page
+ * tables[s][j / page] at place j % page.  The three arrays are int32 on the device and
+ * read there alone: starts are held to [0, T], lengths to the table's width, and a page
+ * outside [0, pages) holds no state (it is neither written nor read).
+ *
+ * tpf_paged_row: page * page size + place of a state, -1 where there is none (host
+ * arrays; the kernels' own rule).
+ *
+ * tpf_paged_append: norm and rotation (as above, by the states' numbers) of the new keys
+ * k [T, Hk, D] on the way into the cache, their values v as they are, and the queries q
+ * [T, H, D] into q_out (contiguous; rows of no sequence are 0; H may be 0).  strides:
+ * token, head.  No two sequences may append to one page.
+ * ---------------------------------------------------------------------- */
+typedef struct tpf_paged_batch {
+  const int32_t* tables;
+  const int32_t* starts;
+  const int32_t* lengths;
+  int64_t S, T, width, table_stride, page, pages;
+} tpf_paged_batch;
+typedef struct tpf_append_shape {
+  int64_t H, Hk, D, half;
+  int64_t dtype, weight_dtype, norm, interleaved;
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+} tpf_append_shape;
+int64_t tpf_paged_row(const tpf_paged_batch* batch, int64_t s, int64_t state);
+int tpf_paged_append(const void* q, const void* k, const void* v, const double* frequencies,
+                     const void* q_weight, const void* k_weight, double eps, void* q_out,
+                     void* k_cache, void* v_cache, const tpf_append_shape* shape,
+                     const tpf_paged_batch* batch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -81,3 +81,11 @@ __all__ += ["cross_attention"]
 from .cross_block import CrossAttention  # noqa: E402
 
 __all__ += ["CrossAttention"]
+
+from .rotary import qk_norm_rotary  # noqa: E402
+
+__all__ += ["qk_norm_rotary"]
+
+from .paged import PagedCache, append_kv  # noqa: E402
+
+__all__ += ["PagedCache", "append_kv"]

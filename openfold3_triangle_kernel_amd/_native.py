@@ -162,6 +162,11 @@ SIGNATURES: dict[str, tuple] = {
     "tpf_xattn_backward_workspace_bytes": (_I64, [_P]),
     "tpf_xattn_backward_bf16": (_I32, [_P] * 11 + [_I64, _P, _P, _F64, _P]),
     "tpf_xattn_backward_shadow_bf16": (_I32, [_P] * 12 + [_I64, _P, _P, _F64, _P]),
+    "tpf_rotary_forward": (_I32, [_P] * 6 + [_F64] + [_P] * 4),
+    "tpf_rotary_backward_workspace_bytes": (_I64, [_P]),
+    "tpf_rotary_backward": (_I32, [_P] * 8 + [_F64] + [_P] * 5 + [_I64] + [_P] * 3),
+    "tpf_paged_row": (_I64, [_P, _I64, _I64]),
+    "tpf_paged_append": (_I32, [_P] * 6 + [_F64] + [_P] * 6),
 }
 
 _LOCK = threading.Lock()

@@ -1,0 +1,136 @@
+"""Refusals of self-attention's operators without a GPU: host tensors and bad arguments
+raise before any native call, the C ABI answers bad shapes with a status before any
+launch, and the rule of a paged cache's places on host arrays."""
+
+import ctypes
+
+import pytest
+import torch
+
+from openfold3_triangle_kernel_amd import PagedCache, _native, append_kv, qk_norm_rotary
+from openfold3_triangle_kernel_amd.paged import batch_struct
+
+
+def _qk(B=1, H=2, Hk=2, N=4, D=16, dtype=torch.bfloat16):
+    return torch.zeros(B, H, N, D, dtype=dtype), torch.zeros(B, Hk, N, D, dtype=dtype)
+
+
+_F = torch.ones(8)
+
+
+@pytest.mark.parametrize("args,match", [
+    ((*_qk(),), "GPU"),
+    ((_qk()[0], None), "torch.Tensor"),
+    ((*(t[0, 0] for t in _qk()),), "shape"),
+    ((*_qk(dtype=torch.float64),), "BF16, FP16 or FP32"),
+    ((_qk()[0], _qk(dtype=torch.float16)[1]), "share one type"),
+    ((_qk(N=5)[0], _qk()[1]), "positions"),
+    ((_qk(B=2)[0], _qk()[1]), "prefix"),
+    ((*_qk(D=257),), "D<=256"),
+    ((*_qk(), torch.zeros(4)), "int32 or int64"),
+    ((*_qk(), torch.zeros(3, dtype=torch.int64)), "broadcast"),
+    ((*_qk(), torch.zeros(2, 4, dtype=torch.int64)), "broadcast"),
+    ((*_qk(), None, torch.ones(9)), "more pairs"),
+    ((*_qk(), None, torch.ones(8, dtype=torch.int64)), "floating"),
+    ((*_qk(), None, torch.ones(2, 4)), "one axis"),
+    ((*_qk(), None, torch.ones(8, requires_grad=True)), "must not require"),
+    ((*_qk(), None, _F, torch.ones(16)), "give eps"),
+    ((*_qk(), None, _F, torch.ones(15), None, 1e-6), "shape"),
+    ((*_qk(), None, _F, torch.ones(16, dtype=torch.float64), None, 1e-6), "BF16, FP16 or FP32"),
+    ((*_qk(), None, _F, None, None, -1e-6), "eps"),
+    ((*_qk(), None, _F, None, None, float("nan")), "eps"),
+])
+def test_rotary_refuses(args, match):
+    with pytest.raises(ValueError, match=match):
+        qk_norm_rotary(*args)
+
+
+def _paged(S=2, T=3, Hk=2, D=16, width=2, page=4, pages=5):
+    cache = PagedCache(pages, Hk, page, D, device="cpu")
+    tables = torch.zeros(S, width, dtype=torch.int32)
+    starts, lengths = torch.zeros(S + 1, dtype=torch.int32), torch.zeros(S, dtype=torch.int32)
+    return cache, torch.zeros(T, Hk, D).bfloat16(), tables, starts, lengths
+
+
+def test_cache_refuses():
+    good = torch.zeros(3, 2, 4, 16).bfloat16()
+    for k, v, match in ((good, good[:2], "alike"), (good.float(), good.float(), "BF16 or FP16"),
+                        (good[0], good[0], r"\[pages"), (good, good.half(), "alike"),
+                        (good[..., :12], good[..., :12], "contiguous"),
+                        (good[..., :4].contiguous(), good[..., :4].contiguous(), "multiple of 8"),
+                        (None, good, r"\[pages"),
+                        (good.clone().requires_grad_(True), good, "gradients")):
+        with pytest.raises(ValueError, match=match):
+            PagedCache.of(k, v)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        PagedCache(3, 2, 4, 136, device="cpu")
+    cache = PagedCache.of(good, good)
+    assert (cache.pages, cache.kv_heads, cache.page, cache.head_dim) == (3, 2, 4, 16)
+
+
+def test_append_refuses():
+    cache, x, tables, starts, lengths = _paged()
+    cases = [((cache, x, x, tables, starts, lengths), "GPU"),
+             ((None, x, x, tables, starts, lengths), "PagedCache"),
+             ((cache, x, x, tables.long(), starts, lengths), "int32"),
+             ((cache, x, x, tables[0], starts, lengths), "2 axes"),
+             ((cache, x, x, tables, starts[:2], lengths), "S, S"),
+             ((cache, x, x, tables[:1], starts, lengths), "S, S"),
+             ((cache, x, x, tables.t().contiguous().t(), starts, lengths), "contiguous"),
+             ((cache, x[:, :1], x, tables, starts, lengths), "kv heads"),
+             ((cache, x, x[:2], tables, starts, lengths), "shape"),
+             ((cache, x, x.half(), tables, starts, lengths), "type"),
+             ((cache, x[..., :8], x, tables, starts, lengths), "shape"),
+             ((cache, x, x, tables, starts, lengths, x[0]), "shape"),
+             ((cache, x.clone().requires_grad_(True), x, tables, starts, lengths), "no_grad"),
+             ((cache, x, x, tables, starts, lengths, None, torch.ones(9)), "more pairs"),
+             ((cache, x, x, tables, starts, lengths, None, None, torch.ones(16)), "give eps"),
+             ((cache, x, x, torch.zeros(2, 1 << 29, dtype=torch.int32), starts, lengths), "2\\^30")]
+    for args, match in cases:
+        with pytest.raises(ValueError, match=match):
+            append_kv(*args)
+
+
+def test_places_of_a_cache():
+    """``tpf_paged_row`` on host arrays: the rule that the kernels share."""
+    cache, _, tables, starts, lengths = _paged(S=3, width=3, page=4, pages=7)
+    tables.copy_(torch.tensor([[6, 0, 3], [7, -1, 2], [1, 2 ** 31 - 1, 5]]))
+    batch = batch_struct(cache, tables, starts, lengths, 5)
+    row = lambda s, j: _native.query("tpf_paged_row", ctypes.byref(batch), s, j)  # noqa: E731
+    for s in range(3):
+        for j in range(12):
+            p = int(tables[s, j // 4])
+            assert row(s, j) == (p * 4 + j % 4 if 0 <= p < 7 else -1)
+        assert row(s, -1) == row(s, 12) == row(s, 1 << 40) == -1
+    assert row(3, 0) == row(-1, 0) == -1
+
+
+def test_c_abi_answers_before_a_launch():
+    shape = (ctypes.c_int64 * 25)(1, 4, 2, 2, 16, 9, 0, 2, 1, 0, 64)
+    with pytest.raises(RuntimeError, match="half=9"):
+        _native.call("tpf_rotary_forward", 16, 16, None, 16, None, None, 1e-6, 16, 16, shape, None)
+    shape[5] = 8
+    with pytest.raises(RuntimeError, match="null pointer"):
+        _native.call("tpf_rotary_forward", 16, 16, None, None, None, None, 1e-6, 16, 16, shape, None)
+    with pytest.raises(RuntimeError, match="eps"):
+        _native.call("tpf_rotary_forward", 16, 16, None, 16, None, None, -1.0, 16, 16, shape, None)
+    shape[10] = 16
+    with pytest.raises(RuntimeError, match="32 or 64"):
+        _native.call("tpf_rotary_forward", 16, 16, None, 16, None, None, 1e-6, 16, 16, shape, None)
+    shape[10] = 64
+    with pytest.raises(RuntimeError, match="workspace"):
+        _native.call("tpf_rotary_backward", 16, 16, 16, 16, None, 16, 16, 16, 1e-6, 16, 16, 16, 16,
+                     16, 8, shape, (ctypes.c_int64 * 6)(), None)
+    assert _native.query("tpf_rotary_backward_workspace_bytes", shape) == 1 * 2 * 16 * 4
+    shape[4] = 257
+    assert _native.query("tpf_rotary_backward_workspace_bytes", shape) == -1
+    cache, x, tables, starts, lengths = _paged()
+    batch = batch_struct(cache, tables, starts, lengths, 3)
+    append = (ctypes.c_int64 * 14)(0, 2, 16, 0, 2, 2)
+    with pytest.raises(RuntimeError, match="TPF_BF16 or TPF_F16"):
+        _native.call("tpf_paged_append", None, 16, 16, None, None, None, 0.0, None, 16, 16, append,
+                     ctypes.byref(batch), None)
+    batch.page = 0
+    with pytest.raises(RuntimeError, match="bad batch"):
+        _native.call("tpf_paged_append", None, 16, 16, None, None, None, 0.0, None, 16, 16, append,
+                     ctypes.byref(batch), None)
