@@ -661,6 +661,11 @@ int tpf_rotary_backward(const void* q, const void* k, const void* dq_out, const 
  * k [T, Hk, D] on the way into the cache, their values v as they are, and the queries q
  * [T, H, D] into q_out (contiguous; rows of no sequence are 0; H may be 0).  strides:
  * token, head.  No two sequences may append to one page.
+ *
+ * tpf_paged_attention: the new tokens' queries q [T, H, D] (strides token, head) over
+ * their sequences' states, out [T, H, D] contiguous, by the rules of tpf_window_forward; a
+ * row of no sequence is 0.  The cache and out start on 16 bytes, D is a multiple of 8 up
+ * to 128.
  * ---------------------------------------------------------------------- */
 typedef struct tpf_paged_batch {
   const int32_t* tables;
@@ -678,6 +683,43 @@ int tpf_paged_append(const void* q, const void* k, const void* v, const double* 
                      const void* q_weight, const void* k_weight, double eps, void* q_out,
                      void* k_cache, void* v_cache, const tpf_append_shape* shape,
                      const tpf_paged_batch* batch, void* stream);
+typedef struct tpf_paged_shape {
+  int64_t H, Hk, D, dtype, window, sinks;
+  int64_t q_stride[2];
+} tpf_paged_shape;
+int64_t tpf_paged_attention_workspace_bytes(const tpf_paged_shape* shape, const tpf_paged_batch* batch);
+int tpf_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out,
+                        void* workspace, int64_t workspace_bytes, const tpf_paged_shape* shape,
+                        const tpf_paged_batch* batch, double scale, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Causal self-attention with a window and sinks over a batch's own tokens.
+ *
+ * q [B, H, N, D], k and v [B, Hk, N, D] (BF16 or FP16, H a multiple of Hk, D a multiple of
+ * 8 up to 128, strides of batch, head, token, multiples of 8; on 16 bytes), out [B, N, H, D]
+ * contiguous.  Token i sees the states j <= i with i - j < window (0: all) or j < sinks,
+ * where mask [B, N] (bytes, mask_stride apart; null: all) is not 0.  A row that sees none
+ * is 0; one whose states all score -inf is NaN.  What a row does not see never reaches
+ * it, whatever K and V hold there.
+ *
+ * lse [B, Hk, N H / Hk] (rows token by token) and residual (what out's rounding drops, laid
+ * out as out; may be null) are for the backward, BF16 alone; both null without one.
+ * ---------------------------------------------------------------------- */
+typedef struct tpf_window_shape {
+  int64_t B, H, Hk, N, D, dtype, window, sinks, mask_stride;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+} tpf_window_shape;
+int64_t tpf_window_forward_workspace_bytes(const tpf_window_shape* shape);
+int tpf_window_forward(const void* q, const void* k, const void* v, const void* mask, void* out,
+                       float* lse, void* residual, void* workspace, int64_t workspace_bytes,
+                       const tpf_window_shape* shape, double scale, void* stream);
+/* residual as the forward kept it, or null; grad_strides as tpf_xattn_backward_bf16's. */
+int64_t tpf_window_backward_workspace_bytes(const tpf_window_shape* shape);
+int tpf_window_backward_bf16(const void* q, const void* k, const void* v, const void* mask,
+                             const void* out, const void* residual, const void* dout,
+                             const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                             int64_t workspace_bytes, const tpf_window_shape* shape,
+                             const int64_t* grad_strides, double scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -86,6 +86,10 @@ from .rotary import qk_norm_rotary  # noqa: E402
 
 __all__ += ["qk_norm_rotary"]
 
-from .paged import PagedCache, append_kv  # noqa: E402
+from .window_attention import window_attention  # noqa: E402
 
-__all__ += ["PagedCache", "append_kv"]
+__all__ += ["window_attention"]
+
+from .paged import PagedCache, append_kv, paged_attention  # noqa: E402
+
+__all__ += ["PagedCache", "append_kv", "paged_attention"]

@@ -1,0 +1,256 @@
+// Shared pieces of causal self-attention (sattn.hip, sattn_bwd.hip): over a batch's own
+// tokens, or the new tokens of sequences over a paged cache.
+//
+// Rows and states.  The queries of the G query heads on a kv head are one row axis, token
+// by token: row r is token r / G under query head hk * G + r % G.  A tile of rows then
+// spans few tokens, and its states end close behind the last of them.  The token that is
+// state p sees the states j <= p with p - j < window or j < sinks, of those that live (the
+// key mask; a page that the cache has).  A tile of rows passes over the 64-state tiles
+// that any of its tokens may see: those of the sinks, then those from the first token's
+// window to the last token.
+//
+// Operand tiles in LDS are cross attention's (xattn.hpp).  A row's scores of states that it
+// does not see are -inf by bit, whatever they are.  Such a state's V is another matter: a
+// product takes 0 p times it, which infinities and NaN survive.  Blocks that some row sees
+// in part are looked over for them first, and they are kept from those rows.
+#pragma once
+
+#include "gemm_core.hpp"  // xcd_order
+#include "paged.hpp"
+#include "tpf_status.hpp"
+#include "xattn.hpp"
+
+namespace tpf {
+
+// The maximum of a row before its first visible state, and the least one after it.
+constexpr float kSaLow = -3.402823466e38f, kSaSeen = -3.3e38f;
+
+struct SAttnArgs {
+  const u16 *q, *k, *v;
+  int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn;  // element strides
+  const uint8_t* mask;  // [B, N], null without
+  int64_t mask_sb;
+  u16* out;    // [tokens, H, D]
+  u16* res;    // what its rounding drops, laid out the same; null when not wanted
+  float* lse;  // [B, Hk, R] log-sum-exp of the rows; null when no backward follows
+  int B, H, Hk, G, N, D, R;  // R = G * N rows of a kv head
+  FastDiv div_g;
+  float c;             // scale * log2(e)
+  int window, sinks;   // window above every position where there is none, then no sinks
+  int splits, tiles;   // most parts of a tile's states; row tiles of a batch entry
+  int order;           // sub-sequences of a batch entry's tiles (sa_tile)
+  int64_t rows;        // rows of a kv head in all
+  float* part_o;       // [Hk, rows, splits, D] unnormalised outputs of the parts
+  float* part_ml;      // the same by 3: their maxima and the two sums (SRows)
+  PagedTables t;
+};
+
+// ones(n): the n + 1 lowest bits, none below 0.
+__device__ __forceinline__ uint64_t sa_ones(int n) {
+  return n < 0 ? 0 : n >= 63 ? ~0ull : (2ull << n) - 1;
+}
+__device__ __forceinline__ uint32_t sa_ones32(int n) {
+  return n < 0 ? 0 : n >= 31 ? ~0u : (2u << n) - 1;
+}
+
+// The states that rows at positions pmin .. pmax may see, as tiles of 64: `n` in all, the
+// first `heads` of them the sinks' (from state 0), the others from state `low` on.
+struct SSpan {
+  int low, heads, n;
+  __host__ __device__ __forceinline__ SSpan(int pmin, int pmax, int window, int sinks) {
+    const int first = pmin - window + 1;  // (both below 2^30)
+    low = first > 0 ? first / 64 * 64 : 0;
+    heads = (sinks + 63) / 64;
+    if (heads > low / 64) heads = low / 64;
+    n = heads + (pmax >= low ? (pmax - low) / 64 + 1 : 0);
+    if (pmax < 0) n = 0;
+  }
+  __host__ __device__ __forceinline__ int state(int t) const { return t < heads ? 64 * t : low + 64 * (t - heads); }
+};
+
+// Parts of a tile's n state tiles: `per` each, the last one shorter; `live` of them.
+struct SParts {
+  int per, live;
+  __host__ __device__ __forceinline__ SParts(int n, int splits, int least) {
+    per = (n + splits - 1) / splits;
+    if (per < least) per = least;
+    live = (n + per - 1) / per;
+  }
+};
+constexpr int kSaLeast = 4;  // state tiles of a part, at least
+
+// The bits of the 64 states from k0 on that the row at position p sees, of the `live`.
+__device__ __forceinline__ uint64_t sa_sees(const SAttnArgs& a, int p, int k0, uint64_t live) {
+  const int rel = p - k0;
+  return live & sa_ones(rel) & (~sa_ones(rel - a.window) | sa_ones(a.sinks - 1 - k0));
+}
+
+// Whether rows at positions pmin .. pmax see all of the `count` states from k0 on.
+__device__ __forceinline__ bool sa_whole(const SAttnArgs& a, int pmin, int pmax, int k0, int count) {
+  return k0 + count - 1 <= pmin && (k0 > pmax - a.window || k0 + count <= a.sinks);
+}
+
+// Order of the tiles of a batch entry's rows.  Later tiles have more states, so they go
+// first; an XCD's share of the work is a run of the list, so where it is a part of an
+// entry (`order` parts), each part has every order-th tile.
+__device__ __forceinline__ int sa_tile(int i, int tiles, int order) {
+  // Part x of the list has the tiles tiles - 1 - x - y * order.
+  int x = 0, before = 0, size = (tiles + order - 1) / order;
+  while (i >= before + size) {
+    before += size;
+    ++x;
+    size = (tiles - x + order - 1) / order;
+  }
+  return tiles - 1 - x - (i - before) * order;
+}
+
+// Where states lie in the pages of sequence s under kv head hk: lane l holds the page of
+// table entry `first + l`, read once for 64 entries.
+template <int ROWS>
+struct SPages {
+  const int32_t* table;
+  int first, page, hk;
+  uint32_t row;  // of the lane's state: (page Hk + hk) P + place
+  __device__ __forceinline__ void init(const SAttnArgs& a, int s, int hk_) {
+    table = a.t.tables + s * a.t.table_ld;
+    first = -1 - 64;
+    page = -1;
+    hk = hk_;
+  }
+  // The states k0 + lane % ROWS below `end`: their rows, and which live.
+  __device__ __forceinline__ uint64_t at(const SAttnArgs& a, int k0, int end) {
+    const int lane = threadIdx.x & 63;
+    const int e0 = (int)fdiv((uint32_t)k0, a.t.div_page);
+    const int e1 = (int)fdiv((uint32_t)min(k0 + ROWS - 1, end - 1), a.t.div_page);
+    if (e0 < first || e1 > first + 63) {
+      first = e0;
+      page = first + lane < a.t.width ? table[first + lane] : -1;
+    }
+    const int j = min(k0 + lane % ROWS, end - 1);
+    const int e = (int)fdiv((uint32_t)j, a.t.div_page);
+    const int p = __shfl(page, e - first);
+    row = ((uint32_t)p * (uint32_t)a.Hk + (uint32_t)hk) * (uint32_t)a.t.page + (uint32_t)(j - e * a.t.page);
+    return __ballot(lane < ROWS && k0 + lane < end && p >= 0 && p < a.t.pages);
+  }
+};
+
+// The tiles of 64 states (or of 32: ROWS) that a wave walks over, from part [t, t1) of a
+// span; ones without a live state are passed over.
+template <bool PAGED, int ROWS, int STEP>
+struct STiles {
+  SPages<ROWS> pages;
+  const uint8_t* mask;
+  int t, t1, end, k0;
+  uint32_t raw;
+  uint64_t live;
+  __device__ __forceinline__ int state(const SSpan& span, int i) const {
+    if constexpr (ROWS == 64) return span.state(i);
+    else return span.state(i >> 1) + 32 * (i & 1);
+  }
+  __device__ __forceinline__ uint32_t load(const SSpan& span, int i) const {
+    const int k = state(span, i) + (int)(threadIdx.x & 63);
+    return i < t1 && k < end ? mask[k] : 0;
+  }
+  __device__ __forceinline__ void init(const SSpan& span, int t_, int t1_, int end_) {
+    t = t_ - STEP;
+    t1 = t1_;
+    end = end_;
+    if (!PAGED && mask) raw = load(span, t_);
+  }
+  __device__ __forceinline__ bool advance(const SAttnArgs& a, const SSpan& span) {
+    for (;;) {
+      t += STEP;
+      if (t >= t1) return false;
+      k0 = state(span, t);
+      if constexpr (PAGED) {
+        live = k0 < end ? pages.at(a, k0, end) : 0;
+      } else if (mask) {
+        live = __ballot(raw != 0);
+        raw = load(span, t + STEP);
+      } else {
+        live = sa_ones(end - 1 - k0);
+      }
+      if (live) return true;
+    }
+  }
+};
+
+// Whether a value in the 32 BLOCKS tile rows from rbase on is not finite: their product with
+// zeros is NaN then.
+template <int DP, bool F16, int BLOCKS>
+__device__ __forceinline__ bool sa_not_finite(const u16* T, int rbase) {
+  f32x16 bad = zero16();
+#pragma unroll
+  for (int t = 0; t < 2 * BLOCKS; ++t)
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) bad = xa_mfma<F16>(xa_frag_t<DP>(T, rbase, t, db), zero8(), bad);
+  float any = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) any += bad[e];
+  return __ballot(any != any) != 0;
+}
+
+// acc += T^T w over the 32 tile rows from rbase on, some of whose values are not finite: w
+// the pair of operands that a C tile's registers pack to, `sees` the bits of the tile rows
+// that count for this lane.  The product takes zeros in their place; products of marks
+// (this value is one, this lane sees its row) then add them where they belong: as they are
+// (POSITIVE: weights of a softmax), otherwise as NaN.
+template <int DP, bool F16, bool POSITIVE>
+__device__ __forceinline__ void sa_guarded(f32x16 (&acc)[DP / 32], const u16* T, int rbase, bf16x8 w0,
+                                           bf16x8 w1, uint32_t sees) {
+  constexpr uint32_t top = F16 ? 0x7c00u : 0x7f80u, one = F16 ? 0x3c00u : 0x3f80u;
+  const uint32_t mine = sees >> (4 * ((threadIdx.x >> 5) & 1));
+  bf16x8 marks[2];  // of the rows that this lane sees
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    u32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t two = mine >> (16 * t + 8 * (e >> 1) + 2 * (e & 1));
+      x[e] = (two & 1) * one + ((two >> 1) & 1) * (one << 16);
+    }
+    marks[t] = __builtin_bit_cast(bf16x8, x);
+  }
+  // The fragment's values turned by f, as a product with b.
+  auto product = [&](int db, f32x16 c, bf16x8 b0, bf16x8 b1, auto f) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      u32x4 x = __builtin_bit_cast(u32x4, xa_frag_t<DP>(T, rbase, t, db));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = f(x[e] & 0xffffu) | f(x[e] >> 16) << 16;
+      c = xa_mfma<F16>(__builtin_bit_cast(bf16x8, x), t ? b1 : b0, c);
+    }
+    return c;
+  };
+  auto add = [&](int db, float v, auto f) {
+    const f32x16 c = product(db, zero16(), marks[0], marks[1], f);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[db][e] += c[e] > 0.f ? v : 0.f;
+  };
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) {
+    acc[db] = product(db, acc[db], w0, w1, [](uint32_t x) { return (x & top) == top ? 0u : x; });
+    if constexpr (POSITIVE) {
+      add(db, __builtin_inff(), [](uint32_t x) { return x == top ? one : 0u; });
+      add(db, -__builtin_inff(), [](uint32_t x) { return x == (top | 0x8000u) ? one : 0u; });
+      add(db, __builtin_nanf(""), [](uint32_t x) { return (x & 0x7fffu) > top ? one : 0u; });
+    } else {
+      add(db, __builtin_nanf(""), [](uint32_t x) { return (x & top) == top ? one : 0u; });
+    }
+  }
+}
+
+// Sizes, strides and scale of a windowed call into `a` (sattn.hip); 0 or an error code.
+int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const char* fn);
+
+// Parts of a batch entry's tile list, so that every XCD's run of it is a whole number.
+inline int sa_order(int64_t entries) {
+  int k = 8;
+  while (k > 1 && entries % 2 == 0) {
+    entries /= 2;
+    k /= 2;
+  }
+  return k;
+}
+
+}  // namespace tpf

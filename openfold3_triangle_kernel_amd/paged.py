@@ -14,12 +14,14 @@ that is no page of the cache holds no state: it is neither written nor read.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
 from . import _native
 from .attention import _device_supported
 from .rotary import _weight_type, check_rotation, rotation_operands
+from .window_attention import check_limits, limits
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # TPF_BF16, TPF_F16
 _MAX_HEAD_DIM = 128
@@ -193,4 +195,66 @@ def append_kv(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, tables: torch
     return None if q is None else out
 
 
-__all__ = ["PagedCache", "append_kv"]
+def _attention_unsupported(reason: str):
+    return ValueError(f"unsupported paged attention case: {reason}")
+
+
+_PagedShape = ctypes.c_int64 * 8  # tpf_paged_shape
+
+
+class _PagedFn(torch.autograd.Function):
+    """A Function, so that forward-mode AD and function transforms, which the native call
+    would hide, are refused."""
+
+    @staticmethod
+    def forward(ctx, q, cache, tables, starts, lengths, window, sinks, scale):
+        T, H, D = q.shape
+        out = q.new_empty((T, H, D))
+        strides = (s if n > 1 else 0 for n, s in zip(q.shape[:2], q.stride()))
+        shape = _PagedShape(H, cache.kv_heads, D, _DTYPES[q.dtype], window, sinks, *strides)
+        batch = ctypes.byref(batch_struct(cache, tables, starts, lengths, T))
+        ws_bytes = int(_native.query("tpf_paged_attention_workspace_bytes", shape, batch))
+        if ws_bytes < 0:
+            raise _attention_unsupported(_native.query("tpf_last_error").decode(errors="replace"))
+        ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes > 0 else None
+        ptr = _native.ptr
+        with _native.device_ctx(q.device):
+            _native.call("tpf_paged_attention", ptr(q), ptr(cache.k), ptr(cache.v), ptr(out), ptr(ws),
+                         ws_bytes, shape, batch, scale, _native.stream_of(q))
+        ctx.mark_non_differentiable(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, d_out):  # pragma: no cover - nothing is differentiable
+        raise RuntimeError("no gradients pass through a cache")
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, starts: torch.Tensor,
+                    lengths: torch.Tensor, window: int | None = None, sinks: int = 0,
+                    scale: float | None = None) -> torch.Tensor:
+    """Attention of the new tokens' queries ``q`` [T, H, D] over their sequences' states in
+    ``cache`` (module text; ``append_kv`` puts the new ones there): a token that is state
+    ``p`` sees the states ``j <= p`` by the rules of ``window_attention``.  One new token
+    for each sequence, chunks of them, or both at once.
+
+    H is a multiple of the cache's kv heads; ``scale`` is 1/sqrt(D) unless given.  Returns
+    [T, H, D], contiguous: a row that sees no state, or is of no sequence, is zeros.  Other
+    cases raise ``ValueError`` before any launch.
+    """
+    check_batch(_attention_unsupported, cache, tables, starts, lengths, [("q", q, None)])
+    check_limits(_attention_unsupported, window, sinks, scale)
+    if q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
+        raise _attention_unsupported("the query heads must be a positive multiple of the kv heads")
+    ok, reason = _device_supported(q)
+    if not ok:
+        raise _attention_unsupported(reason)
+    if q.shape[0] == 0:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if (q.stride(2) != 1 or q.data_ptr() % 16
+            or any(n > 1 and s % 8 for n, s in zip(q.shape[:2], q.stride()))):
+        q = q.clone(memory_format=torch.contiguous_format)
+    scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
+    return _PagedFn.apply(q, cache, tables, starts, lengths, *limits(window, sinks), scale)
+
+
+__all__ = ["PagedCache", "append_kv", "paged_attention"]

@@ -125,3 +125,201 @@ def test_append_replays(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, want) and torch.equal(cache.k, other.k) and torch.equal(cache.v, other.v)
+
+
+ATTEND = [
+    # new tokens, lengths with them, page, H, Hk, D, window, sinks, type, rows behind
+    ([1], [1], 1, 1, 1, 8, 0, 0, "bf16", 0),
+    ([1], [77], 16, 8, 8, 64, 0, 0, "bf16", 0),
+    ([1, 1, 1], [700, 3, 1300], 16, 8, 2, 128, 0, 0, "bf16", 2),
+    ([1, 1, 1, 1], [2500, 64, 65, 1], 64, 16, 4, 64, 300, 4, "fp16", 0),
+    ([1, 0, 1], [5000, 9, 33], 7, 4, 1, 128, 0, 0, "fp16", 1),  # pages that end inside a tile
+    ([2, 1, 7], [500, 1, 7], 100, 8, 1, 96, 33, 100, "bf16", 0),
+    ([130, 1, 60], [400, 700, 60], 48, 4, 2, 96, 0, 0, "bf16", 5),
+    ([300, 5], [1000, 1100], 8, 6, 2, 80, 129, 3, "fp16", 40),
+    ([64, 64], [64, 2100], 256, 3, 3, 128, 0, 0, "bf16", 0),
+    ([700], [9000], 32, 1, 1, 32, 0, 0, "bf16", 0),
+    ([1], [40000], 16, 2, 1, 40, 0, 0, "bf16", 0),  # many parts
+    ([1] * 70, [30 + 11 * s for s in range(70)], 8, 2, 1, 64, 50, 1, "bf16", 1),
+    ([0, 0, 0], [4, 0, 1], 4, 2, 2, 32, 0, 0, "bf16", 3),
+    ([40], [40], 16, 40, 1, 64, 0, 0, "bf16", 0),
+]
+
+
+def _attended(q, cache, tables, news, lengths, window, sinks):
+    """The reference of every sequence: (rows, outputs, bounds)."""
+    from test_gpu_window_attention import reference, seen
+
+    page, first = cache.page, 0
+    for s, (m, n) in enumerate(zip(news, lengths)):
+        if m:
+            p = tables[s, :-(-n // page)].long()
+            k, v = (t[p].transpose(0, 1).reshape(cache.kv_heads, -1, cache.head_dim)[:, :n]
+                    for t in (cache.k, cache.v))
+            (out,), (err,) = reference(q[first:first + m].transpose(0, 1), k, v,
+                                       seen(torch.arange(n - m, n), n, window, sinks),
+                                       cache.head_dim ** -0.5)
+            yield slice(first, first + m), out.transpose(0, 1), err.transpose(0, 1)
+        first += m
+
+
+@pytest.mark.parametrize("case", ATTEND, ids=str)
+def test_attention(gpu, case):
+    from test_gpu_window_attention import check
+
+    from openfold3_triangle_kernel_amd import paged_attention
+
+    news, lengths, page, H, Hk, D, window, sinks, t, behind = case
+    cache, tables, starts, lens, T, g = _batch(gpu, news, lengths, page, Hk, D, _T[t], behind)
+    q = (1.5 * torch.randn(T, 2 * H, D, generator=g)).to(_T[t]).to(gpu)[:, H:]
+    out = paged_attention(q, cache, tables, starts, lens, window or None, sinks)
+    assert out.shape == q.shape and out.is_contiguous() and not out[sum(news):].any()
+    for rows, want, err in _attended(q, cache, tables, news, lengths, window, sinks):
+        check([out[rows]], [want], [err])
+    wide = torch.nn.functional.pad(tables, (0, 60), value=-1)  # a longer table splits otherwise
+    again = paged_attention(q, cache, wide[:, :-1], starts, lens, window or None, sinks)
+    for rows, want, err in _attended(q, cache, tables, news, lengths, window, sinks):
+        check([again[rows]], [want], [err])
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("new", [1, 60])
+def test_attention_never_reads_what_is_not_there(gpu, bad, new):
+    """Places behind a sequence, other pages, pages that the cache does not have and states
+    before the window never reach an output, whatever they hold; a later token of the
+    chunk never reaches an earlier one."""
+    from openfold3_triangle_kernel_amd import PagedCache, paged_attention
+
+    news, lengths = [new, new], [333, 200]
+    cache, tables, starts, lens, T, g = _batch(gpu, news, lengths, 12, 2, 64, torch.bfloat16)
+    q = torch.randn(T, 4, 64, generator=g).bfloat16().to(gpu)
+    live = torch.zeros(cache.pages, 12, dtype=torch.bool)
+    for s, n in enumerate(lengths):
+        for j in range(n):
+            live[tables[s, j // 12].item(), j % 12] = True
+    dead = ~live.to(gpu)[:, None, :, None]
+    clean = PagedCache.of(cache.k.masked_fill(dead, 0), cache.v.masked_fill(dead, 0))
+    dirty = PagedCache.of(cache.k.masked_fill(dead, bad), cache.v.masked_fill(dead, bad))
+    for window in (None, 40):
+        want = paged_attention(q, clean, tables, starts, lens, window)
+        got = paged_attention(q, dirty, tables, starts, lens, window)
+        assert torch.isfinite(want).all() and torch.equal(got, want)
+    # Pages freed behind the window: no entry, or another sequence's page.
+    freed = tables.clone()
+    for s, n in enumerate(lengths):
+        freed[s, :max(0, n - new - 40) // 12] = -1 if s else cache.pages + 7
+    assert torch.equal(paged_attention(q, dirty, freed, starts, lens, 40), want)
+    # The chunk's last token.
+    for t in (dirty.k, dirty.v):
+        t[tables[0, 332 // 12].item(), :, 332 % 12] = bad
+    got = paged_attention(q, dirty, tables, starts, lens, None)
+    want = paged_attention(q, clean, tables, starts, lens, None)
+    rows = torch.ones(T, dtype=torch.bool, device=gpu)
+    rows[new - 1] = False
+    assert torch.equal(got[rows], want[rows]) and not torch.isfinite(got[new - 1]).all()
+
+
+def test_attention_without_pages_or_states(gpu):
+    """Sequences whose pages the cache does not have, lengths of zero, lengths below the
+    new tokens and past the table: zeros, or the states that are there."""
+    from openfold3_triangle_kernel_amd import PagedCache, paged_attention
+
+    cache, tables, starts, lens, T, g = _batch(gpu, [3, 3], [40, 50], 8, 1, 32, torch.bfloat16)
+    q = torch.randn(T, 2, 32, generator=g).bfloat16().to(gpu)
+    want = paged_attention(q, cache, tables, starts, lens)
+    none = tables.clone()
+    none[0] = 1 << 30
+    got = paged_attention(q, cache, none, starts, lens)
+    assert not got[:3].any() and torch.equal(got[3:], want[3:])
+    for n in (0, -7):
+        lens[0] = n
+        got = paged_attention(q, cache, tables, starts, lens)
+        assert not got[:3].any() and torch.equal(got[3:], want[3:])
+    lens[0] = 2  # three tokens, two states: the first token sees none
+    got = paged_attention(q, cache, tables, starts, lens)
+    assert not got[0].any() and got[1].any() and got[2].any()
+    lens[1] = 1 << 30  # held to the table's 56 states: page -1 for the last of them
+    assert torch.isfinite(paged_attention(q, cache, tables, starts, lens)).all()
+    empty = PagedCache.of(cache.k[:0], cache.v[:0])
+    assert not paged_attention(q, empty, tables, starts, lens).any()
+    assert not paged_attention(q, cache, tables[:, :0], starts, lens).any()
+    assert not paged_attention(q, cache, tables[:0], starts[:1], lens[:0]).any()
+    assert paged_attention(q[:0], cache, tables, starts, lens).shape == (0, 2, 32)
+
+
+def test_attention_far_pages(gpu):
+    """Pages past 32-bit byte offsets."""
+    from openfold3_triangle_kernel_amd import PagedCache, paged_attention
+
+    pages = 140000  # of 16 states of 2 kv heads of 128: 1.1 GB... times 2 bytes each
+    k, v = (torch.zeros(pages, 2, 16, 128, device=gpu, dtype=torch.bfloat16) for _ in range(2))
+    g = torch.Generator().manual_seed(4)
+    small = [torch.randn(6, 2, 16, 128, generator=g).bfloat16().to(gpu) for _ in range(2)]
+    at = torch.tensor([3, pages - 1, 131072, 70001, 139990, 65535], device=gpu)
+    k[at], v[at] = small
+    starts, lens = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0, 5], [90]))
+    q = torch.randn(5, 4, 128, generator=g).bfloat16().to(gpu)
+    table = torch.arange(6, dtype=torch.int32, device=gpu)[None]
+    want = paged_attention(q, PagedCache.of(*small), table, starts, lens)
+    assert torch.equal(paged_attention(q, PagedCache.of(k, v), at[None].int(), starts, lens), want)
+
+
+def test_attention_replays_and_overlaps(gpu):
+    """A captured call on other tables, lengths and tokens; calls on two streams."""
+    from openfold3_triangle_kernel_amd import paged_attention
+
+    cache, tables, starts, lens, T, g = _batch(gpu, [1, 1, 1], [3000, 700, 1500], 16, 2, 64,
+                                               torch.bfloat16, behind=1)
+    q = torch.randn(T, 8, 64, generator=g).bfloat16().to(gpu)
+    run = lambda: paged_attention(q, cache, tables, starts, lens)  # noqa: E731
+    run()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = run()
+    for n in ([3000, 700, 1500], [1, 688, 0], [2999, 1, 1024]):
+        lens.copy_(torch.tensor(n))
+        q.copy_(torch.randn(T, 8, 64, generator=g).bfloat16())
+        tables.copy_(tables[:, torch.randperm(tables.shape[1], generator=g).to(gpu)])
+        want = run()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+
+
+def test_prompt_then_tokens(gpu):
+    """A prompt in chunks and tokens one by one through the cache give the rows of one call
+    over all the tokens, to the roundings of both."""
+    from test_gpu_window_attention import check, reference, seen
+
+    from openfold3_triangle_kernel_amd import PagedCache, append_kv, paged_attention, qk_norm_rotary
+
+    N, H, Hk, D, window, sinks = 75, 4, 2, 64, 30, 3
+    g = torch.Generator().manual_seed(8)
+    q, k, v = (torch.randn(N, h, D, generator=g).bfloat16().to(gpu) for h in (H, Hk, Hk))
+    w = (1 + 0.3 * torch.randn(D, generator=g)).to(gpu)
+    freq = 100.0 ** (-torch.arange(16, device=gpu) / 16)
+    cache = PagedCache(12, Hk, 8, D)
+    table = torch.randperm(12, generator=g).int()[None, :10].to(gpu)
+    heads = lambda t: t.transpose(0, 1)  # noqa: E731
+    tq, tk = qk_norm_rotary(heads(q)[None], heads(k)[None], None, freq, w, w, 1e-6)
+    see = seen(torch.arange(N), N, window, sinks)
+    want, err = reference(tq[0], tk[0], heads(v), see, D ** -0.5)
+    at = 0
+    for new in (33, 1, 30, 1, 1, 1, 8):
+        rows = slice(at, at + new)
+        at += new
+        starts, lens = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0, new], [at]))
+        turned = append_kv(cache, k[rows], v[rows], table, starts, lens, q[rows], freq, w, w, 1e-6)
+        assert torch.equal(turned, heads(tq[0])[rows])
+        out = paged_attention(turned, cache, table, starts, lens, window, sinks)
+        check([heads(out)], [want[0][:, rows]], [err[0][:, rows]])

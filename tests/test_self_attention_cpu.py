@@ -7,7 +7,8 @@ import ctypes
 import pytest
 import torch
 
-from openfold3_triangle_kernel_amd import PagedCache, _native, append_kv, qk_norm_rotary
+from openfold3_triangle_kernel_amd import (PagedCache, _native, append_kv, paged_attention, qk_norm_rotary,
+                                           window_attention)
 from openfold3_triangle_kernel_amd.paged import batch_struct
 
 
@@ -134,3 +135,86 @@ def test_c_abi_answers_before_a_launch():
     with pytest.raises(RuntimeError, match="bad batch"):
         _native.call("tpf_paged_append", None, 16, 16, None, None, None, 0.0, None, 16, 16, append,
                      ctypes.byref(batch), None)
+
+
+def _qkv(B=1, H=2, Hk=2, N=4, D=64, dtype=torch.bfloat16):
+    return [torch.zeros(B, h, N, D, dtype=dtype) for h in (H, Hk, Hk)]
+
+
+@pytest.mark.parametrize("args,match", [
+    ((*_qkv(),), "GPU"),
+    ((_qkv()[0], _qkv()[1], None), "torch.Tensor"),
+    ((*(t[0, 0] for t in _qkv()),), "shape"),
+    ((*_qkv(dtype=torch.float32),), "BF16 or FP16"),
+    ((*_qkv(D=129),), "D<=128"),
+    ((*_qkv(H=3),), "multiple"),
+    ((_qkv()[0], _qkv()[1], _qkv(N=5)[2]), "one shape"),
+    ((_qkv(N=5)[0], *_qkv()[1:]), "tokens"),
+    ((_qkv(B=2)[0], *_qkv()[1:]), "batch prefix"),
+    ((*_qkv(), 0), "window"),
+    ((*_qkv(), 2.0), "window"),
+    ((*_qkv(), 2, -1), "sinks"),
+    ((*_qkv(), 2, None), "sinks"),
+    ((*_qkv(), 2, 1, torch.zeros(4)), "boolean"),
+    ((*_qkv(), 2, 1, torch.zeros(3, dtype=torch.bool)), "broadcast"),
+    ((*_qkv(), 2, 1, torch.zeros(2, 4, dtype=torch.bool)), "broadcast"),
+    ((*_qkv(), 2, 1, torch.zeros(1, dtype=torch.bool)), "broadcast"),
+    ((*_qkv(), None, 0, None, 0.0), "scale"),
+    ((*_qkv(), None, 0, None, float("nan")), "scale"),
+])
+def test_window_attention_refuses(args, match):
+    with pytest.raises(ValueError, match=match):
+        window_attention(*args)
+
+
+def test_paged_attention_refuses():
+    cache, x, tables, starts, lengths = _paged()
+    q = torch.zeros(3, 4, 16).bfloat16()
+    for args, match in (((q, cache, tables, starts, lengths), "GPU"),
+                        ((q, None, tables, starts, lengths), "PagedCache"),
+                        ((q[:, :3], cache, tables, starts, lengths), "multiple"),
+                        ((q[:, :0], cache, tables, starts, lengths), "multiple"),
+                        ((q[0], cache, tables, starts, lengths), "shape"),
+                        ((q.half(), cache, tables, starts, lengths), "type"),
+                        ((q, cache, tables.long(), starts, lengths), "int32"),
+                        ((q, cache, tables, starts, lengths[:1]), "S, S"),
+                        ((q.clone().requires_grad_(True), cache, tables, starts, lengths), "no_grad"),
+                        ((q, cache, tables, starts, lengths, 0), "window"),
+                        ((q, cache, tables, starts, lengths, 4, -1), "sinks"),
+                        ((q, cache, tables, starts, lengths, 4, 1, -1.0), "scale")):
+        with pytest.raises(ValueError, match=match):
+            paged_attention(*args)
+
+
+def test_attention_c_abi_answers_before_a_launch():
+    shape = (ctypes.c_int64 * 18)(1, 4, 2, 100, 64, 0, 10, 2, 0)
+    q = lambda name, *args: _native.query(name, *args)  # noqa: E731
+    assert q("tpf_window_forward_workspace_bytes", shape) == 0
+    assert q("tpf_window_backward_workspace_bytes", shape) == 4 * 100 * 4
+    call = lambda s=shape, fn="tpf_window_forward": _native.call(  # noqa: E731
+        fn, *([16] * (4 if fn == "tpf_window_forward" else 12)), *(
+            [16, None, None, None, 0] if fn == "tpf_window_forward" else [8]), s, *(
+            [] if fn == "tpf_window_forward" else [(ctypes.c_int64 * 9)()]), 0.125, None)
+    for at, value, match in ((1, 3, "H=3"), (4, 136, "D=136"), (4, 12, "D=12"), (3, 0, "rows"),
+                             (3, 1 << 40, "rows"), (5, 2, "TPF_BF16"), (6, -1, "window"), (7, -1, "window"),
+                             (9, 4, "multiples of 8"), (14, 1 << 23, "state stride")):
+        bad = (ctypes.c_int64 * 18)(*shape)
+        bad[at] = value
+        with pytest.raises(RuntimeError, match=match):
+            call(bad)
+        assert q("tpf_window_forward_workspace_bytes", bad) == -1
+    with pytest.raises(RuntimeError, match="workspace"):
+        call(fn="tpf_window_backward_bf16")
+    cache, x, tables, starts, lengths = _paged()
+    batch = batch_struct(cache, tables, starts, lengths, 3)
+    paged = (ctypes.c_int64 * 8)(4, 2, 16, 0, 0, 0, 64, 16)
+    size = lambda s=paged: q("tpf_paged_attention_workspace_bytes", s, ctypes.byref(batch))  # noqa: E731
+    assert size() == 0
+    batch.width, batch.page, batch.pages = 64, 64, 100
+    assert size() > 0
+    for at, value in ((0, 3), (2, 12), (3, 2), (4, -1), (5, -1), (6, 4)):
+        bad = (ctypes.c_int64 * 8)(*paged)
+        bad[at] = value
+        assert size(bad) == -1
+    batch.pages = 1 << 25
+    assert size() == -1
