@@ -70,11 +70,12 @@ struct SRows {
   }
 
   // KB blocks of 32 states from k0 on; `whole`: every row sees them all.
+  // `poison`: the wave's rows' words of SPoison.
   template <int KB>
   __device__ __forceinline__ void step(const SAttnArgs& a, const u16* K, const u16* V, uint64_t live,
-                                       int k0, bool whole) {
+                                       int k0, bool whole, uint32_t* poison) {
     uint64_t sees[QB];
-    bool guard = false;
+    uint32_t bad[KB] = {};
     if (!whole) {
       bool some = false;
 #pragma unroll
@@ -83,7 +84,16 @@ struct SRows {
         some = some || sees[qb] != 0;
       }
       if (__ballot(some) == 0) return;
-      guard = sa_not_finite<DP, F16, KB>(V, 0);
+      #pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        bad[kb] = sa_bad_rows<DP, F16>(V, 32 * kb);
+        if (bad[kb]) {
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb)
+            SPoison<DP>::template note<F16>(poison + (32 * qb + (threadIdx.x & 31)) * SPoison<DP>::WORDS, V,
+                                            32 * kb, bad[kb], (uint32_t)(sees[qb] >> (32 * kb)));
+        }
+      }
     }
     f32x16 s[QB][KB];
 #pragma unroll
@@ -145,22 +155,6 @@ struct SRows {
       }
       if constexpr (STATS) l[qb] += sum;
     }
-    if (guard) {
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          sa_guarded<DP, F16, true>(o[qb], V, 32 * kb, pr[qb][2 * kb], pr[qb][2 * kb + 1],
-                                    (uint32_t)(sees[qb] >> (32 * kb)));
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const u32x4 w = __builtin_bit_cast(u32x4, pr[qb][2 * kb + t]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) n[qb] = xa_add_pair<F16>(w[e], n[qb]);
-          }
-        }
-      return;
-    }
     if constexpr (DP > 96) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -168,7 +162,8 @@ struct SRows {
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          const bf16x8 vf = xa_frag_t<DP>(V, 32 * kb, t, db);
+          bf16x8 vf = xa_frag_t<DP>(V, 32 * kb, t, db);
+          if (bad[kb]) vf = sa_finite<F16>(vf);
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) o[qb][db] = xa_mfma<F16>(vf, pr[qb][2 * kb + t], o[qb][db]);
         }
@@ -239,7 +234,9 @@ struct STile {
 template <int DP, int QB, bool F16, bool STATS, bool PAGED>
 __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
   constexpr int KT = 64, TILE = KT * DP, RT = 128 * QB;
+  typedef SPoison<DP> Poison;
   __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
+  __shared__ uint32_t poison[RT * Poison::WORDS];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t T = xcd_order((int64_t)(PAGED ? 1 : a.B) * a.Hk * a.splits * a.tiles);
   if (T < 0) return;
@@ -289,6 +286,8 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
       lv.issue(vp + (int64_t)t.k0 * a.v_sn, t.live, w, smem[st][1]);
     }
   };
+  // (A wave's rows are its own: no barrier.)
+  for (int i = lane; i < 32 * QB * Poison::WORDS; i += 64) poison[w * 32 * QB * Poison::WORDS + i] = 0;
   bool more = t.advance(a, span);
   if (more) issue(0);
   int st = 0;
@@ -300,7 +299,8 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
     more = t.advance(a, span);
     if (more) issue(st ^ 1);
     if (r0 < at.R)
-      rows.template step<2>(a, smem[st][0], smem[st][1], lc, kc, lc == ~0ull && sa_whole(a, p0, p1, kc, KT));
+      rows.template step<2>(a, smem[st][0], smem[st][1], lc, kc, lc == ~0ull && sa_whole(a, p0, p1, kc, KT),
+                            poison + w * 32 * QB * Poison::WORDS);
     st ^= 1;
   }
 
@@ -309,6 +309,18 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
     const int r = r0 + 32 * qb + (lane & 31);
     const float l = xor32_sum(rows.l[qb]), n = xor32_sum(rows.n[qb]);
     if (r >= at.R) continue;
+    const uint32_t* hurt = poison + (w * 32 * QB + 32 * qb + (lane & 31)) * Poison::WORDS;
+    uint32_t any = 0;
+#pragma unroll
+    for (int x = 0; x < Poison::WORDS; ++x) any |= hurt[x];
+    if (__ballot(any != 0)) {
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          rows.o[qb][db][e] =
+              Poison::apply(hurt, 32 * db + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), rows.o[qb][db][e]);
+    }
     const int i = (int)fdiv((uint32_t)r, a.div_g), g = r - i * a.G;
     if (a.splits == 1) {
       const float inv = sa_inverse(n, rows.m[qb]);
@@ -355,7 +367,9 @@ template <int DP, bool F16>
 __global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
   constexpr int KT = 32, RT = 32, TILE = KT * DP, NI = KT * DP / 512;
   constexpr int OP = DP + 4;  // pitch of the joined rows (f32)
+  typedef SPoison<DP> Poison;
   __shared__ __attribute__((aligned(1024))) u16 smem[4][2][2][TILE];
+  __shared__ uint32_t poison[RT * Poison::WORDS];
   static_assert(sizeof(smem) >= 4 * 32 * (OP + 2) * 4, "the join fits");
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t T = xcd_order((int64_t)a.Hk * a.splits * a.tiles);
@@ -379,6 +393,8 @@ __global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
     SPageLoader<DP, KT, 1>::issue(a, a.k, t.live, t.pages.row, 0, smem[w][st][0]);
     SPageLoader<DP, KT, 1>::issue(a, a.v, t.live, t.pages.row, 0, smem[w][st][1]);
   };
+  for (int i = threadIdx.x; i < RT * Poison::WORDS; i += 256) poison[i] = 0;
+  lds_barrier();
   bool more = t.advance(a, span);
   if (more) issue(0);
   int st = 0;
@@ -393,7 +409,7 @@ __global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
       wait_vmcnt<0>();
     }
     rows.template step<1>(a, smem[w][st][0], smem[w][st][1], lc, kc,
-                          lc == 0xffffffffull && sa_whole(a, p0, p1, kc, KT));
+                          lc == 0xffffffffull && sa_whole(a, p0, p1, kc, KT), poison);
     st ^= 1;
   }
 
@@ -438,6 +454,8 @@ __global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] += f[x] * v[e];
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = Poison::apply(poison + rl * Poison::WORDS, d + e, o[e]);
     if (a.splits == 1) sa_store4<F16>(a, out + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     else *reinterpret_cast<f32x4*>(a.part_o + pr * a.D + d) = o;
   }

@@ -175,70 +175,87 @@ struct STiles {
   }
 };
 
-// Whether a value in the 32 BLOCKS tile rows from rbase on is not finite: their product with
-// zeros is NaN then.
-template <int DP, bool F16, int BLOCKS>
-__device__ __forceinline__ bool sa_not_finite(const u16* T, int rbase) {
-  f32x16 bad = zero16();
+// Which of the 32 tile rows from rbase on hold a value that is not finite.
+template <int DP, bool F16>
+__device__ __forceinline__ uint32_t sa_bad_rows(const u16* T, int rbase) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  constexpr uint16_t top = F16 ? 0x7c00u : 0x7f80u;
+  u16x2 most = {0, 0};
 #pragma unroll
-  for (int t = 0; t < 2 * BLOCKS; ++t)
+  for (int s = 0; s < DP / 16; ++s) {
+    const u32x4 x = __builtin_bit_cast(u32x4, xa_frag<DP>(T, rbase, s));
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) bad = xa_mfma<F16>(xa_frag_t<DP>(T, rbase, t, db), zero8(), bad);
-  float any = 0.f;
+    for (int e = 0; e < 4; ++e)
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[e] & (top * 0x10001u)));
+  }
+  const uint64_t rows = __ballot(most[0] == top || most[1] == top);
+  return (uint32_t)(rows | rows >> 32);
+}
+// A fragment with zeros in the place of values that are not finite.
+template <bool F16>
+__device__ __forceinline__ bf16x8 sa_finite(bf16x8 f) {
+  constexpr uint32_t top = F16 ? 0x7c00u : 0x7f80u;
+  u32x4 x = __builtin_bit_cast(u32x4, f);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) any += bad[e];
-  return __ballot(any != any) != 0;
+  for (int e = 0; e < 4; ++e) {
+    if ((x[e] & top) == top) x[e] &= 0xffff0000u;
+    if (((x[e] >> 16) & top) == top) x[e] &= 0xffffu;
+  }
+  return __builtin_bit_cast(bf16x8, x);
 }
 
-// acc += T^T w over the 32 tile rows from rbase on, some of whose values are not finite: w
-// the pair of operands that a C tile's registers pack to, `sees` the bits of the tile rows
-// that count for this lane.  The product takes zeros in their place; products of marks
-// (this value is one, this lane sees its row) then add them where they belong: as they are
-// (POSITIVE: weights of a softmax), otherwise as NaN.
-template <int DP, bool F16, bool POSITIVE>
-__device__ __forceinline__ void sa_guarded(f32x16 (&acc)[DP / 32], const u16* T, int rbase, bf16x8 w0,
-                                           bf16x8 w1, uint32_t sees) {
-  constexpr uint32_t top = F16 ? 0x7c00u : 0x7f80u, one = F16 ? 0x3c00u : 0x3f80u;
-  const uint32_t mine = sees >> (4 * ((threadIdx.x >> 5) & 1));
-  bf16x8 marks[2];  // of the rows that this lane sees
+// Zeros in the place of the values of a tile of T's chunks (64 (n w + t) + lane, as its loader
+// put them there) that are not finite; mark(row) for their rows.
+template <int DP, int NI, typename F>
+__device__ __forceinline__ void sa_clean(u16* T, int w, F mark) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    u32x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t two = mine >> (16 * t + 8 * (e >> 1) + 2 * (e & 1));
-      x[e] = (two & 1) * one + ((two >> 1) & 1) * (one << 16);
-    }
-    marks[t] = __builtin_bit_cast(bf16x8, x);
-  }
-  // The fragment's values turned by f, as a product with b.
-  auto product = [&](int db, f32x16 c, bf16x8 b0, bf16x8 b1, auto f) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      u32x4 x = __builtin_bit_cast(u32x4, xa_frag_t<DP>(T, rbase, t, db));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = f(x[e] & 0xffffu) | f(x[e] >> 16) << 16;
-      c = xa_mfma<F16>(__builtin_bit_cast(bf16x8, x), t ? b1 : b0, c);
-    }
-    return c;
-  };
-  auto add = [&](int db, float v, auto f) {
-    const f32x16 c = product(db, zero16(), marks[0], marks[1], f);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[db][e] += c[e] > 0.f ? v : 0.f;
-  };
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db) {
-    acc[db] = product(db, acc[db], w0, w1, [](uint32_t x) { return (x & top) == top ? 0u : x; });
-    if constexpr (POSITIVE) {
-      add(db, __builtin_inff(), [](uint32_t x) { return x == top ? one : 0u; });
-      add(db, -__builtin_inff(), [](uint32_t x) { return x == (top | 0x8000u) ? one : 0u; });
-      add(db, __builtin_nanf(""), [](uint32_t x) { return (x & 0x7fffu) > top ? one : 0u; });
-    } else {
-      add(db, __builtin_nanf(""), [](uint32_t x) { return (x & top) == top ? one : 0u; });
+  for (int t = 0; t < NI; ++t) {
+    const int p = 64 * (NI * w + t) + (int)(threadIdx.x & 63);
+    bf16x8* at = reinterpret_cast<bf16x8*>(T) + p;
+    const u32x4 x = __builtin_bit_cast(u32x4, *at), y = __builtin_bit_cast(u32x4, sa_finite<false>(*at));
+    if (x[0] != y[0] || x[1] != y[1] || x[2] != y[2] || x[3] != y[3]) {
+      *at = __builtin_bit_cast(bf16x8, y);
+      mark(p / (DP / 8));
     }
   }
 }
+
+// What rows see that is not finite, beside their sums: two bits a channel, 1 +inf, 2 -inf,
+// both NaN, 16 channels a word.
+template <int DP>
+struct SPoison {
+  static constexpr int WORDS = DP / 16;  // a row
+  // Adds what the lane's row sees (`sees`) of the tile rows `bad` from rbase on.
+  template <bool F16>
+  static __device__ __forceinline__ void note(uint32_t* row, const u16* T, int rbase, uint32_t bad,
+                                              uint32_t sees) {
+    constexpr uint32_t top = F16 ? 0x7c00u : 0x7f80u;
+    const int h = (threadIdx.x >> 5) & 1;
+    while (bad) {  // (uniform)
+      const int r = __builtin_ctz(bad);
+      bad &= bad - 1;
+#pragma unroll 1
+      for (int d = 4 * h; d < DP; d += 8) {
+        const int slot = (d >> 3) ^ xa_swz<DP>(rbase + r);
+        const uint2 x = *reinterpret_cast<const uint2*>(T + (rbase + r) * DP + slot * 8 + (d & 7));
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t v = ((e & 2 ? x.y : x.x) >> (16 * (e & 1))) & 0xffffu;
+          if ((v & top) == top) bits |= ((v & 0x7fffu) > top ? 3u : v & 0x8000u ? 2u : 1u) << (2 * e);
+        }
+        if (bits && ((sees >> r) & 1)) atomicOr(row + (d >> 4), bits << (2 * (d & 15)));
+      }
+    }
+  }
+  // The value x of channel d of a row.
+  static __device__ __forceinline__ float apply(const uint32_t* row, int d, float x) {
+    const uint32_t b = (row[d >> 4] >> (2 * (d & 15))) & 3;
+    if (b & 1) x += __builtin_inff();
+    if (b & 2) x -= __builtin_inff();
+    return x;
+  }
+};
 
 // Sizes, strides and scale of a windowed call into `a` (sattn.hip); 0 or an error code.
 int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const char* fn);

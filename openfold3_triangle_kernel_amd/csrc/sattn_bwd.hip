@@ -132,8 +132,13 @@ __global__ __launch_bounds__(256, 2) void sattn_dq_kernel(SAttnGrad ga) {
     lds_barrier();
     more = t.advance(a, span);
     if (more) issue(st ^ 1);
-    const u16 *K = smem[st][0], *V = smem[st][1];
+    u16 *K = smem[st][0], *V = smem[st][1];
     st ^= 1;
+    if (!sa_whole(a, position(t0), pmax, kc, KT)) {
+      // A state whose K is not finite: its V makes dO V^T, and so dS, NaN.
+      sa_clean<DP, XTileLoader<DP, KT, 4>::NI>(K, w, [&](int row) { V[row * DP + xa_swz<DP>(row) * 8] = 0x7fc0; });
+      lds_barrier();
+    }
     if (r0 >= a.R) continue;
     const bool whole = lc == ~0ull && sa_whole(a, p0, p1, kc, KT);
     uint64_t sees = ~0ull;
@@ -145,7 +150,6 @@ __global__ __launch_bounds__(256, 2) void sattn_dq_kernel(SAttnGrad ga) {
     for (int kb = 0; kb < 2; ++kb) {
       const uint32_t bits = (uint32_t)(sees >> (32 * kb));
       if (!whole && __ballot(bits != 0) == 0) continue;
-      const bool guard = !whole && sa_not_finite<DP, false, 1>(K, 32 * kb);
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int d = 0; d < DS; ++d) s = mfma32(xa_frag<DP>(K, 32 * kb, d), q[d], s);
@@ -159,10 +163,6 @@ __global__ __launch_bounds__(256, 2) void sattn_dq_kernel(SAttnGrad ga) {
           if (!((bits >> (8 * (e >> 2) + 4 * h + (e & 3))) & 1)) s[e] = 0.f;
       }
       const bf16x8 x0 = xa_pack8<false>(s, 0), x1 = xa_pack8<false>(s, 8);
-      if (guard) {
-        sa_guarded<DP, false, false>(dq, K, 32 * kb, x0, x1, bits);
-        continue;
-      }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
         dq[db] = mfma32(xa_frag_t<DP>(K, 32 * kb, 0, db), x0, dq[db]);
@@ -231,6 +231,9 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
   const int wfrom = min(kw + 31, a.N - 1) * a.G;
   const int wto = a.window >= a.N || kw + 31 < a.sinks
                       ? a.R : (int)min((int64_t)a.R, ((int64_t)min(kw, a.N - 1) + a.window) * a.G);
+
+  const int tfrom = min(k0 + 127, a.N - 1) * a.G;  // and of the tile's
+  const int tto = a.window >= a.N || k0 + 127 < a.sinks ? a.R : (int)min((int64_t)a.R, ((int64_t)k0 + a.window) * a.G);
 
   bool live = k < a.N;
   if (a.mask) live = live && a.mask[b * a.mask_sb + kc] != 0;
@@ -312,18 +315,22 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
       wait_vmcnt<0>();
       lds_barrier();
       if (r0 + RT < rend) issue(r0 + RT, st ^ 1);
-      const u16 *Q = smem[st][0], *dO = smem[st][1];
+      u16 *Q = smem[st][0], *dO = smem[st][1];
+      if (r0 < tfrom || r0 + RT > tto) {
+        // A row whose Q or dO is not finite: its statistic makes p and dS NaN.
+        auto mark = [&](int row) { stats[st][0][row] = __builtin_nanf(""); };
+        sa_clean<DP, NI>(Q, w, mark);
+        sa_clean<DP, NI>(dO, w, mark);
+        lds_barrier();
+      }
 #pragma unroll
       for (int rb = 0; rb < RT / 32; ++rb) {
         const int rr = r0 + 32 * rb;
         const bool whole = rr >= wfrom && rr + 32 <= wto;
         uint32_t bits = ~0u;
-        bool gq = false, go = false;
         if (!whole) {
           bits = sa_ones32(to - 1 - rr) & ~sa_ones32(from - 1 - rr);
           if (__ballot(bits != 0) == 0) continue;
-          gq = sa_not_finite<DP, false, 1>(Q, 32 * rb);
-          go = sa_not_finite<DP, false, 1>(dO, 32 * rb);
         }
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -353,11 +360,6 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
         for (int t = 0; t < 2; ++t) {
           pb[t] = xa_pack8<false>(s, 8 * t);
           sb[t] = xa_pack8<false>(dp, 8 * t);
-        }
-        if (gq || go) {
-          sa_guarded<DP, false, true>(dv, dO, 32 * rb, pb[0], pb[1], bits);
-          sa_guarded<DP, false, false>(dk, Q, 32 * rb, sb[0], sb[1], bits);
-          continue;
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
