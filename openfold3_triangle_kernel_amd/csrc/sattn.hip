@@ -69,13 +69,20 @@ struct SRows {
     }
   }
 
+  // Notes what the rows see of the states `bad` from k0 on (SPoison), whose V is not finite.
+  __device__ __forceinline__ void note(const SAttnArgs& a, const u16* V, uint64_t bad, uint64_t live, int k0,
+                                       uint32_t* poison) const {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+      SPoison<DP>::template note<F16>(poison + (32 * qb + (threadIdx.x & 31)) * SPoison<DP>::WORDS, V, bad,
+                                      sa_sees(a, p[qb], k0, live));
+  }
+
   // KB blocks of 32 states from k0 on; `whole`: every row sees them all.
-  // `poison`: the wave's rows' words of SPoison.
   template <int KB>
   __device__ __forceinline__ void step(const SAttnArgs& a, const u16* K, const u16* V, uint64_t live,
-                                       int k0, bool whole, uint32_t* poison) {
+                                       int k0, bool whole) {
     uint64_t sees[QB];
-    uint32_t bad[KB] = {};
     if (!whole) {
       bool some = false;
 #pragma unroll
@@ -84,17 +91,7 @@ struct SRows {
         some = some || sees[qb] != 0;
       }
       if (__ballot(some) == 0) return;
-      #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        bad[kb] = sa_bad_rows<DP, F16>(V, 32 * kb);
-        if (bad[kb]) {
-#pragma unroll
-          for (int qb = 0; qb < QB; ++qb)
-            SPoison<DP>::template note<F16>(poison + (32 * qb + (threadIdx.x & 31)) * SPoison<DP>::WORDS, V,
-                                            32 * kb, bad[kb], (uint32_t)(sees[qb] >> (32 * kb)));
-        }
-      }
-    }
+          }
     f32x16 s[QB][KB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb)
@@ -162,8 +159,7 @@ struct SRows {
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          bf16x8 vf = xa_frag_t<DP>(V, 32 * kb, t, db);
-          if (bad[kb]) vf = sa_finite<F16>(vf);
+          const bf16x8 vf = xa_frag_t<DP>(V, 32 * kb, t, db);
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) o[qb][db] = xa_mfma<F16>(vf, pr[qb][2 * kb + t], o[qb][db]);
         }
@@ -215,14 +211,15 @@ struct STile {
   // has the tiles from starts[s] G / RT + s on, which are enough for its rows whatever its
   // length; the rows behind the last one are those of a sequence S without states.
   __device__ __forceinline__ bool find(const SAttnArgs& a, int tile, int rt) {
-    auto before = [&](int x) { return (int)((uint64_t)paged_start(a.t, x) * a.G / (uint32_t)rt) + x; };
+    // (T G is below 2^30, rt a power of two.)
+    auto before = [&](int x) { return (int)((uint32_t)paged_start(a.t, x) * (uint32_t)a.G / (uint32_t)rt) + x; };
     s = __builtin_amdgcn_readfirstlane(paged_search(a.t.S, [&](int x) { return before(x) <= tile; }));
     token = paged_start(a.t, s);
     const int64_t next = s < a.t.S ? paged_start(a.t, s + 1) : a.t.T;
     const int fresh = (int)(next > token ? next - token : 0);
-    R = fresh * a.G;
-    r0 = (tile - before(s)) * rt;
-    pos = s < a.t.S ? (int)paged_length(a.t, s) - fresh : -fresh;
+    R = sa_scalar(fresh * a.G);
+    r0 = sa_scalar((tile - before(s)) * rt);
+    pos = sa_scalar(s < a.t.S ? (int)paged_length(a.t, s) - fresh : -fresh);
     return r0 < R;
   }
   __device__ __forceinline__ int position(const SAttnArgs& a, int r) const {
@@ -236,31 +233,30 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
   constexpr int KT = 64, TILE = KT * DP, RT = 128 * QB;
   typedef SPoison<DP> Poison;
   __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
-  __shared__ uint32_t poison[RT * Poison::WORDS];
+  __shared__ uint32_t poison[RT * Poison::WORDS], bad[2];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t T = xcd_order((int64_t)(PAGED ? 1 : a.B) * a.Hk * a.splits * a.tiles);
-  if (T < 0) return;
-  const int64_t u = T / a.tiles;
-  const int split = (int)(u % a.splits);
-  const int64_t bh = u / a.splits;
-  const int b = PAGED ? 0 : (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
+  int64_t bh;
+  int unit;
+  if (!sa_unit(a.order, &bh, &unit)) return;
+  const int tile = (int)sa_div(unit, a.splits), split = unit - tile * a.splits;
+  const int b = PAGED ? 0 : (int)sa_div((uint32_t)bh, a.Hk), hk = (int)bh - b * a.Hk;
   STile at;
   if constexpr (PAGED) {
-    if (!at.find(a, (int)(T % a.tiles), RT)) return;
+    if (!at.find(a, tile, RT)) return;
   } else {
     at.s = b;
-    at.r0 = sa_tile((int)(T % a.tiles), a.tiles, a.order) * RT;
+    at.r0 = (a.tiles - 1 - tile) * RT;  // (later rows see more states)
     at.R = a.R;
     at.pos = 0;
     at.token = (int64_t)b * a.N;
   }
-  const int pmax = at.position(a, at.r0 + RT - 1);
-  const SSpan span(at.position(a, at.r0), pmax, a.window, a.sinks);
+  const int pmin = sa_scalar(at.position(a, at.r0)), pmax = sa_scalar(at.position(a, at.r0 + RT - 1));
+  const SSpan span(pmin, pmax, a.window, a.sinks);
   const SParts parts(span.n, a.splits, kSaLeast);
   if (a.splits > 1 && split >= parts.live) return;
 
   const int r0 = at.r0 + w * 32 * QB;
-  const int p0 = at.position(a, r0), p1 = at.position(a, r0 + 32 * QB - 1);
+  const int p0 = sa_scalar(at.position(a, r0)), p1 = sa_scalar(at.position(a, r0 + 32 * QB - 1));
   STiles<PAGED, KT, 1> t;
   const u16 *kp = a.k, *vp = a.v;
   XTileLoader<DP, KT, 4> lk, lv;
@@ -268,8 +264,8 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
     t.pages.init(a, at.s, hk);
   } else {
     t.mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
-    kp += b * a.k_sb + hk * a.k_sh;
-    vp += b * a.v_sb + hk * a.v_sh;
+    kp = sa_scalar(kp + b * a.k_sb + hk * a.k_sh);
+    vp = sa_scalar(vp + b * a.v_sb + hk * a.v_sh);
     lk.init(w, a.k_sn, a.D);
     lv.init(w, a.v_sn, a.D);
   }
@@ -288,6 +284,7 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
   };
   // (A wave's rows are its own: no barrier.)
   for (int i = lane; i < 32 * QB * Poison::WORDS; i += 64) poison[w * 32 * QB * Poison::WORDS + i] = 0;
+  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
   bool more = t.advance(a, span);
   if (more) issue(0);
   int st = 0;
@@ -298,9 +295,23 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
     lds_barrier();
     more = t.advance(a, span);
     if (more) issue(st ^ 1);
+    if (!sa_whole(a, pmin, pmax, kc, KT)) {
+      // Rows that do not see a state must not meet its V: it is looked over first.
+      constexpr int NI = XTileLoader<DP, KT, 4>::NI;
+      u16* V = smem[st][1];
+      sa_look<DP, NI, F16, false>(V, w, [&](int row) { atomicOr(&bad[row >> 5], 1u << (row & 31)); });
+      lds_barrier();
+      const uint64_t rows_ = (uint64_t)(uint32_t)sa_scalar((int)bad[1]) << 32 | (uint32_t)sa_scalar((int)bad[0]);
+      if (rows_) {
+        rows.note(a, V, rows_, lc, kc, poison + w * 32 * QB * Poison::WORDS);
+        lds_barrier();
+        sa_look<DP, NI, F16, true>(V, w, [](int) {});
+        if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+        lds_barrier();
+      }
+    }
     if (r0 < at.R)
-      rows.template step<2>(a, smem[st][0], smem[st][1], lc, kc, lc == ~0ull && sa_whole(a, p0, p1, kc, KT),
-                            poison + w * 32 * QB * Poison::WORDS);
+      rows.template step<2>(a, smem[st][0], smem[st][1], lc, kc, lc == ~0ull && sa_whole(a, p0, p1, kc, KT));
     st ^= 1;
   }
 
@@ -372,13 +383,13 @@ __global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
   __shared__ uint32_t poison[RT * Poison::WORDS];
   static_assert(sizeof(smem) >= 4 * 32 * (OP + 2) * 4, "the join fits");
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t T = xcd_order((int64_t)a.Hk * a.splits * a.tiles);
-  if (T < 0) return;
-  const int64_t u = T / a.tiles;
-  const int split = (int)(u % a.splits), hk = (int)(u / a.splits);
+  int64_t head;
+  int unit;
+  if (!sa_unit(a.order, &head, &unit)) return;
+  const int hk = (int)head, tile = (int)sa_div(unit, a.splits), split = unit - tile * a.splits;
   STile at;
-  if (!at.find(a, (int)(T % a.tiles), RT)) return;
-  const int p0 = at.position(a, at.r0), p1 = at.position(a, at.r0 + RT - 1);
+  if (!at.find(a, tile, RT)) return;
+  const int p0 = sa_scalar(at.position(a, at.r0)), p1 = sa_scalar(at.position(a, at.r0 + RT - 1));
   const SSpan span(p0, p1, a.window, a.sinks);
   const SParts parts(span.n, a.splits, kSaLeast);
   if (a.splits > 1 && split >= parts.live) return;
@@ -408,8 +419,16 @@ __global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
     } else {
       wait_vmcnt<0>();
     }
-    rows.template step<1>(a, smem[w][st][0], smem[w][st][1], lc, kc,
-                          lc == 0xffffffffull && sa_whole(a, p0, p1, kc, KT), poison);
+    const bool whole = lc == 0xffffffffull && sa_whole(a, p0, p1, kc, KT);
+    if (!whole) {  // (as in the tile kernel; the tile is this wave's own)
+      u16* V = smem[w][st][1];
+      const uint32_t bad = sa_bad_rows<DP, F16>(V, 0);
+      if (bad) {
+        rows.note(a, V, bad, lc, kc, poison);
+        sa_look<DP, NI, F16, true>(V, 0, [](int) {});
+      }
+    }
+    rows.template step<1>(a, smem[w][st][0], smem[w][st][1], lc, kc, whole);
     st ^= 1;
   }
 
@@ -560,7 +579,7 @@ int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const ch
   const int64_t lim = (int64_t)1 << 30;
   if (s->B < 1 || s->N < 1 || s->B > lim || s->N > lim || a.G * s->N > lim ||
       (double)s->B * s->Hk * ((double)(a.G * s->N) / 64 + 1) * 64 > 2e9 ||
-      s->B * s->Hk * ((a.G * s->N + 127) / 128) > kXaMaxGroups)
+      s->B * s->Hk * ((a.G * s->N + 127) / 128 + 8) > kXaMaxGroups)
     return set_error(TPF_ERR_SHAPE, "%s: too many rows (B=%lld N=%lld)", fn, (long long)s->B, (long long)s->N);
   for (int i = 0; i < 3; ++i) {
     const int64_t* st = i == 0 ? s->q_stride : i == 1 ? s->k_stride : s->v_stride;
@@ -579,7 +598,6 @@ int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const ch
   a.mask_sb = s->mask_stride;
   a.B = (int)s->B; a.N = (int)s->N; a.R = (int)(a.G * s->N);
   a.rows = (int64_t)a.B * a.R;
-  a.order = sa_order((int64_t)a.B * a.Hk);
   return TPF_OK;
 }
 
@@ -601,13 +619,13 @@ static int window_plan(SAttnArgs& a) {
   const int qb = a.D <= 64 && BH * ((a.R + 255) / 256) >= 512 ? 2 : 1;
   a.tiles = (a.R + 128 * qb - 1) / (128 * qb);
   a.splits = sattn_splits(BH * a.tiles, 256, a.N);
+  a.order = sa_order(BH, (int64_t)a.tiles * a.splits);
   return qb;
 }
 
 template <int DP, bool F16, bool STATS>
 static void window_launch(const SAttnArgs& a, int qb, hipStream_t s) {
-  const int64_t n = (int64_t)a.B * a.Hk * a.splits * a.tiles;
-  const dim3 grid((unsigned)((n + 7) / 8 * 8));
+  const dim3 grid((unsigned)a.order.groups);
   if constexpr (DP <= 64) {
     if (qb == 2) {
       hipLaunchKernelGGL((sattn_fwd_kernel<DP, 2, F16, STATS, false>), grid, dim3(256), 0, s, a);
@@ -647,7 +665,7 @@ static int paged_attn_check(SAttnArgs& a, const tpf_paged_shape* s, const tpf_pa
   a.q_sn = s->q_stride[0]; a.q_sh = s->q_stride[1];
   a.B = a.t.S;
   a.rows = a.t.T * a.G;
-  if (a.rows > ((int64_t)1 << 30) || ((double)a.rows / 32 + a.t.S + 1) * a.Hk > (double)kXaMaxGroups ||
+  if (a.rows > ((int64_t)1 << 30) || ((double)a.rows / 32 + a.t.S + 9) * a.Hk > (double)kXaMaxGroups / 2 ||
       (double)a.rows * a.Hk / 4 + 1 > (double)kXaMaxGroups)
     return set_error(TPF_ERR_SHAPE, "%s: too many rows", fn);
   return TPF_OK;
@@ -661,14 +679,14 @@ static int paged_plan(SAttnArgs& a) {
   int64_t units = a.rows / rt > a.t.S ? a.rows / rt : a.t.S;
   units *= a.Hk;
   a.splits = sattn_splits(units < 1 ? 1 : units, 512, (int64_t)a.t.width * a.t.page);
-  while (a.splits > 1 && (double)a.tiles * a.Hk * a.splits > (double)kXaMaxGroups) a.splits /= 2;
+  while (a.splits > 1 && (double)a.tiles * a.Hk * a.splits > (double)kXaMaxGroups / 2) a.splits /= 2;
+  a.order = sa_order(a.Hk, (int64_t)a.tiles * a.splits);
   return rt;
 }
 
 template <int DP, bool F16>
 static void paged_launch(const SAttnArgs& a, int rt, hipStream_t s) {
-  const int64_t n = (int64_t)a.Hk * a.splits * a.tiles;
-  const dim3 grid((unsigned)((n + 7) / 8 * 8));
+  const dim3 grid((unsigned)a.order.groups);
   if (rt == 32) hipLaunchKernelGGL((sattn_few_kernel<DP, F16>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((sattn_fwd_kernel<DP, 1, F16, false, true>), grid, dim3(256), 0, s, a);
 }

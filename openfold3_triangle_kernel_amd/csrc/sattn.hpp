@@ -25,6 +25,14 @@ namespace tpf {
 // The maximum of a row before its first visible state, and the least one after it.
 constexpr float kSaLow = -3.402823466e38f, kSaSeen = -3.3e38f;
 
+// Order of `units` units of work of every head over the XCDs (sa_unit): 2^shift sub-sequences of
+// a head's units; those of an XCD, and how many of them at a time; units of a sub-sequence.
+struct SOrder {
+  int units;
+  uint32_t shift, subs, together, each;
+  int64_t groups;  // workgroups in all
+};
+
 struct SAttnArgs {
   const u16 *q, *k, *v;
   int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn;  // element strides
@@ -38,7 +46,7 @@ struct SAttnArgs {
   float c;             // scale * log2(e)
   int window, sinks;   // window above every position where there is none, then no sinks
   int splits, tiles;   // most parts of a tile's states; row tiles of a batch entry
-  int order;           // sub-sequences of a batch entry's tiles (sa_tile)
+  SOrder order;        // of the forward's or dQ's units
   int64_t rows;        // rows of a kv head in all
   float* part_o;       // [Hk, rows, splits, D] unnormalised outputs of the parts
   float* part_ml;      // the same by 3: their maxima and the two sums (SRows)
@@ -90,18 +98,35 @@ __device__ __forceinline__ bool sa_whole(const SAttnArgs& a, int pmin, int pmax,
   return k0 + count - 1 <= pmin && (k0 > pmax - a.window || k0 + count <= a.sinks);
 }
 
-// Order of the tiles of a batch entry's rows.  Later tiles have more states, so they go
-// first; an XCD's share of the work is a run of the list, so where it is a part of an
-// entry (`order` parts), each part has every order-th tile.
-__device__ __forceinline__ int sa_tile(int i, int tiles, int order) {
-  // Part x of the list has the tiles tiles - 1 - x - y * order.
-  int x = 0, before = 0, size = (tiles + order - 1) / order;
-  while (i >= before + size) {
-    before += size;
-    ++x;
-    size = (tiles - x + order - 1) / order;
-  }
-  return tiles - 1 - x - (i - before) * order;
+// A quotient of uniform values, on the scalar side (the compiler forms it in vector registers
+// and leaves all that follows from it there).
+__device__ __forceinline__ uint32_t sa_div(uint32_t n, uint32_t d) {
+  return __builtin_amdgcn_readfirstlane(n / d);
+}
+
+__device__ __forceinline__ int sa_scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+template <typename T>
+__device__ __forceinline__ const T* sa_scalar(const T* p) {
+  const uint64_t x = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return (const T*)(uintptr_t)((uint64_t)hi << 32 | lo);
+}
+
+// This workgroup's kv head of a batch entry, and its unit of work there, of those that the
+// host counted (SOrder); false past the last one.  Units are numbered from the longest on
+// and start in that order; an XCD (workgroup L runs on XCD L % 8) has whole heads, whose
+// K and V its L2 then holds, one after the other or two at a time, or, where their number
+// is none of eight's, every second, fourth or eighth unit of one.
+__device__ __forceinline__ bool sa_unit(const SOrder& o, int64_t* head, int* unit) {
+  const uint32_t x = blockIdx.x & 7, j = blockIdx.x >> 3;
+  const uint32_t run = o.together * o.each, group = sa_div(j, run), rest = j - group * run;
+  const uint32_t at = o.together == 2 ? rest / 2 : rest;
+  const uint32_t sub = x * o.subs + group * o.together + (rest - at * o.together);
+  const uint32_t bh = sub >> o.shift;
+  *head = bh;
+  *unit = (int)((at << o.shift) + (sub - (bh << o.shift)));
+  return *unit < o.units;
 }
 
 // Where states lie in the pages of sequence s under kv head hk: lane l holds the page of
@@ -204,17 +229,17 @@ __device__ __forceinline__ bf16x8 sa_finite(bf16x8 f) {
   return __builtin_bit_cast(bf16x8, x);
 }
 
-// Zeros in the place of the values of a tile of T's chunks (64 (n w + t) + lane, as its loader
-// put them there) that are not finite; mark(row) for their rows.
-template <int DP, int NI, typename F>
-__device__ __forceinline__ void sa_clean(u16* T, int w, F mark) {
+// Calls mark(row) for the rows of a tile's chunks (64 (n w + t) + lane, as its loader put them
+// there) that hold a value that is not finite; CLEAN: and puts zeros in the values' place.
+template <int DP, int NI, bool F16, bool CLEAN, typename F>
+__device__ __forceinline__ void sa_look(u16* T, int w, F mark) {
 #pragma unroll
   for (int t = 0; t < NI; ++t) {
     const int p = 64 * (NI * w + t) + (int)(threadIdx.x & 63);
     bf16x8* at = reinterpret_cast<bf16x8*>(T) + p;
-    const u32x4 x = __builtin_bit_cast(u32x4, *at), y = __builtin_bit_cast(u32x4, sa_finite<false>(*at));
+    const u32x4 x = __builtin_bit_cast(u32x4, *at), y = __builtin_bit_cast(u32x4, sa_finite<F16>(*at));
     if (x[0] != y[0] || x[1] != y[1] || x[2] != y[2] || x[3] != y[3]) {
-      *at = __builtin_bit_cast(bf16x8, y);
+      if constexpr (CLEAN) *at = __builtin_bit_cast(bf16x8, y);
       mark(p / (DP / 8));
     }
   }
@@ -225,19 +250,18 @@ __device__ __forceinline__ void sa_clean(u16* T, int w, F mark) {
 template <int DP>
 struct SPoison {
   static constexpr int WORDS = DP / 16;  // a row
-  // Adds what the lane's row sees (`sees`) of the tile rows `bad` from rbase on.
+  // Adds what the lane's row sees (`sees`) of the tile rows `bad`.
   template <bool F16>
-  static __device__ __forceinline__ void note(uint32_t* row, const u16* T, int rbase, uint32_t bad,
-                                              uint32_t sees) {
+  static __device__ __forceinline__ void note(uint32_t* row, const u16* T, uint64_t bad, uint64_t sees) {
     constexpr uint32_t top = F16 ? 0x7c00u : 0x7f80u;
     const int h = (threadIdx.x >> 5) & 1;
     while (bad) {  // (uniform)
-      const int r = __builtin_ctz(bad);
+      const int r = __builtin_ctzll(bad);
       bad &= bad - 1;
 #pragma unroll 1
       for (int d = 4 * h; d < DP; d += 8) {
-        const int slot = (d >> 3) ^ xa_swz<DP>(rbase + r);
-        const uint2 x = *reinterpret_cast<const uint2*>(T + (rbase + r) * DP + slot * 8 + (d & 7));
+        const int slot = (d >> 3) ^ xa_swz<DP>(r);
+        const uint2 x = *reinterpret_cast<const uint2*>(T + r * DP + slot * 8 + (d & 7));
         uint32_t bits = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -260,14 +284,17 @@ struct SPoison {
 // Sizes, strides and scale of a windowed call into `a` (sattn.hip); 0 or an error code.
 int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const char* fn);
 
-// Parts of a batch entry's tile list, so that every XCD's run of it is a whole number.
-inline int sa_order(int64_t entries) {
-  int k = 8;
-  while (k > 1 && entries % 2 == 0) {
-    entries /= 2;
-    k /= 2;
-  }
-  return k;
+inline SOrder sa_order(int64_t heads, int64_t units) {
+  int64_t shared = 8;
+  while (heads % shared) shared /= 2;
+  SOrder o;
+  o.units = (int)units;
+  o.shift = shared == 8 ? 0 : shared == 4 ? 1 : shared == 2 ? 2 : 3;
+  o.subs = (uint32_t)(heads / shared);
+  o.together = o.subs == 2 ? 2 : 1;
+  o.each = (uint32_t)((units + (8 / shared) - 1) / (8 / shared));
+  o.groups = 8 * (int64_t)o.subs * o.each;
+  return o;
 }
 
 }  // namespace tpf

@@ -23,9 +23,13 @@ struct SAttnGrad {
   u16 *dq, *dk, *dv;
   int64_t dq_s[3], dk_s[3], dv_s[3];
   float scale;
-  int ktiles;          // tiles of 128 states
-  int sunk, splits, rchunk;  // tiles with sinks, parts of their rows, rows of a part
-  float *part_k, *part_v;    // [splits, B*Hk, 128 sunk, D], null when there are no parts
+  // The dK / dV launch: tiles of 128 states, the first `sunk` of them with sinks, whose rows
+  // are in `splits` parts of rchunk, those of the others in `parts`; without a window parts
+  // are the same runs of chunk_tiles tiles' rows for every tile (grad_unit).
+  int ktiles, sunk, splits, rchunk, parts, chunk_tiles;
+  SOrder order;
+  float *part_k, *part_v;  // [parts, B*Hk, N, D], null without parts
+  float *sunk_k, *sunk_v;  // [splits, B*Hk, 128 sunk, D]
 };
 
 // Four consecutive channels of a lane's row or state, as f32 partial or rounded with
@@ -62,11 +66,11 @@ __global__ __launch_bounds__(256, 2) void sattn_dq_kernel(SAttnGrad ga) {
   __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
   const SAttnArgs& a = ga.f;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-  const int64_t T = xcd_order((int64_t)a.B * a.Hk * a.tiles);
-  if (T < 0) return;
-  const int64_t bh = T / a.tiles;
-  const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
-  const int t0 = sa_tile((int)(T - bh * a.tiles), a.tiles, a.order) * RT, r0 = t0 + w * 32;
+  int64_t bh;
+  int unit;
+  if (!sa_unit(a.order, &bh, &unit)) return;
+  const int b = (int)sa_div((uint32_t)bh, a.Hk), hk = (int)bh - b * a.Hk;
+  const int t0 = (a.tiles - 1 - unit) * RT, r0 = t0 + w * 32;  // (later rows see more states)
   auto position = [&](int r) { return (int)fdiv((uint32_t)min(r, a.R - 1), a.div_g); };
   const int pmax = position(t0 + RT - 1), p0 = position(r0), p1 = position(r0 + 31);
   const SSpan span(position(t0), pmax, a.window, a.sinks);
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(256, 2) void sattn_dq_kernel(SAttnGrad ga) {
     st ^= 1;
     if (!sa_whole(a, position(t0), pmax, kc, KT)) {
       // A state whose K is not finite: its V makes dO V^T, and so dS, NaN.
-      sa_clean<DP, XTileLoader<DP, KT, 4>::NI>(K, w, [&](int row) { V[row * DP + xa_swz<DP>(row) * 8] = 0x7fc0; });
+      sa_look<DP, XTileLoader<DP, KT, 4>::NI, false, true>(K, w, [&](int row) { V[row * DP + xa_swz<DP>(row) * 8] = 0x7fc0; });
       lds_barrier();
     }
     if (r0 >= a.R) continue;
@@ -158,9 +162,10 @@ __global__ __launch_bounds__(256, 2) void sattn_dq_kernel(SAttnGrad ga) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], a.c, -lse)) * (dp[e] - delta);
       if (!whole) {
+        const uint32_t mine = bits >> (4 * h);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (!((bits >> (8 * (e >> 2) + 4 * h + (e & 3))) & 1)) s[e] = 0.f;
+          if (!((mine >> (8 * (e >> 2) + (e & 3))) & 1)) s[e] = 0.f;
       }
       const bf16x8 x0 = xa_pack8<false>(s, 0), x1 = xa_pack8<false>(s, 8);
 #pragma unroll
@@ -176,15 +181,68 @@ __global__ __launch_bounds__(256, 2) void sattn_dq_kernel(SAttnGrad ga) {
                nullptr, ga.scale, false);
 }
 
-// Direct 4-byte global -> LDS load: lane i writes dst_base + 4 i.
-__device__ __forceinline__ void sg_lds4(const void* src, void* dst_base) {
+// Direct 4-byte buffer -> LDS load: lane i writes dst_base + 4 i with element i of the n at src,
+// zero past them.  (The lane's number is formed on the spot: with 128 channels one kept from
+// before is a spilled one, whose return from memory would wait for every load under way.)
+__device__ __forceinline__ void sg_lds4(const float* src, int n, void* dst_base) {
   const unsigned lds = __builtin_amdgcn_readfirstlane(lds_offset(dst_base));
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
-               :: "v"(src), "s"(lds) : "memory", "m0");
+  i32x4 rsrc = buffer_rsrc(src);
+  rsrc[2] = __builtin_amdgcn_readfirstlane(4 * n);
+  uint32_t at;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0\n\t"
+               "v_lshlrev_b32 %0, 2, %0" : "=&v"(at));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(lds), "v"(at), "s"(rsrc) : "memory", "m0");
 }
 
-// 16 zero bytes, then the log-sum-exp of an absent row: its p is 0.
-__device__ const float kSaNone[8] = {0.f, 0.f, 0.f, 0.f, __builtin_inff(), 0.f, 0.f, 0.f};
+// 16 zero bytes.
+__device__ const uint32_t kSaNone[4] = {0, 0, 0, 0};
+
+// Unit `unit` of a head: its tile of states, which part of the rows that see it, and those
+// rows (from a whole tile of rows on).  Without a window tile t is seen by all rows from
+// 128 t G on; these run in the chunks that all tiles share: first the tiles' whole chunks, then
+// each chunk's own tiles, the longest first.
+__device__ __forceinline__ bool grad_unit(const SAttnGrad& ga, int unit, int* tile, int* part, int* rbeg,
+                                          int* rend) {
+  const SAttnArgs& a = ga.f;
+  if (a.window >= a.N) {
+    const int per = ga.chunk_tiles, whole = ga.parts * (ga.parts - 1) / 2 * per;
+    int c, t;
+    if (unit < whole) {
+      c = 1;
+      t = unit;
+      while (t >= c * per) t -= c++ * per;
+    } else {
+      const int i = (int)sa_div(unit - whole, ga.parts);
+      c = unit - whole - i * ga.parts;
+      t = c * per + i;
+      if (t >= ga.ktiles) return false;
+    }
+    *tile = t;
+    *part = c;
+    *rbeg = max(t, c * per) * 128 * a.G;
+    *rend = (int)min((int64_t)a.R, ((int64_t)c + 1) * per * 128 * a.G);
+    return true;
+  }
+  const int sinks = ga.sunk * ga.splits;
+  int t, p, n;
+  if (unit < sinks) {
+    t = (int)sa_div(unit, ga.splits);
+    p = unit - t * ga.splits;
+    n = a.R;
+  } else {
+    t = (int)sa_div(unit - sinks, ga.parts);
+    p = unit - sinks - t * ga.parts;
+    t += ga.sunk;
+    n = (int)min((int64_t)a.R, ((int64_t)min(t * 128 + 127, a.N - 1) + a.window) * a.G);
+  }
+  const int64_t from = (int64_t)t * 128 * a.G + (int64_t)p * ga.rchunk;
+  *tile = t;
+  *part = p;
+  *rbeg = (int)min(from, (int64_t)n);
+  *rend = (int)min(from + ga.rchunk, (int64_t)n);
+  return true;
+}
 
 // dK and dV: four waves of 32 states each pass over tiles of RT of the rows that see them.
 // A state's column of the tiles depends on that state alone, so dead states are left to run
@@ -199,41 +257,29 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
   __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
   __shared__ __attribute__((aligned(1024))) float stats[2][2][64];
   __shared__ __attribute__((aligned(1024))) u16 vs[VLDS ? 128 * DP : 8];
+  // What each thread keeps here instead of in registers: above 64 channels none are left, and a
+  // spilled one's return from memory would wait for every load under way.
+  constexpr int KEPT = DP == 128 ? 2 + 2 * NI : DP > 64 ? 2 : 0;
+  __shared__ int kept[KEPT ? KEPT : 1][256];
   const SAttnArgs& a = ga.f;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int64_t BH = (int64_t)a.B * a.Hk;
-  const int units = ga.sunk * ga.splits + ga.ktiles - ga.sunk;
-  const int64_t T = xcd_order(BH * units);
-  if (T < 0) return;
-  const int64_t bh = T / units;
-  const int b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
-  // The sinks' parts first, then the tiles, the earlier ones (which have more rows) first.
-  int unit = (int)(T - bh * units), tile, split = 0;
-  if (unit < ga.sunk * ga.splits) {
-    tile = unit / ga.splits;
-    split = unit - tile * ga.splits;
-  } else {
-    tile = ga.ktiles - 1 - sa_tile(unit - ga.sunk * ga.splits, ga.ktiles - ga.sunk, a.order);
-  }
+  int64_t bh;
+  int unit, tile, part, rbeg, rend;
+  if (!sa_unit(ga.order, &bh, &unit) || !grad_unit(ga, unit, &tile, &part, &rbeg, &rend)) return;
+  const int b = (int)sa_div((uint32_t)bh, a.Hk), hk = (int)bh - b * a.Hk;
+  rbeg = sa_scalar(rbeg);
+  rend = sa_scalar(rend);
+  tile = sa_scalar(tile);
   const int k0 = tile * 128, kw = k0 + w * 32, k = kw + (lane & 31), kc = min(k, a.N - 1);
-  // Rows that see the tile's states, from a whole tile of rows on, and those of this part.
-  const bool all = tile < ga.sunk || a.window >= a.N;
-  int rbeg = (int)((int64_t)k0 * a.G / RT * RT);
-  int rend = all ? a.R : (int)min((int64_t)a.R, ((int64_t)min(k0 + 127, a.N - 1) + a.window) * a.G);
-  if (tile < ga.sunk) {
-    const int64_t from = rbeg + (int64_t)split * ga.rchunk;
-    rend = (int)min((int64_t)rend, from + ga.rchunk);
-    rbeg = (int)min(from, (int64_t)rend);
-  }
   // Rows that see this lane's state, and those that see all of the wave's.
   const int from = kc * a.G;
   const int to = a.window >= a.N || kc < a.sinks ? a.R : (int)min((int64_t)a.R, ((int64_t)kc + a.window) * a.G);
   const int wfrom = min(kw + 31, a.N - 1) * a.G;
-  const int wto = a.window >= a.N || kw + 31 < a.sinks
-                      ? a.R : (int)min((int64_t)a.R, ((int64_t)min(kw, a.N - 1) + a.window) * a.G);
-
+  const int wto = sa_scalar(a.window >= a.N || kw + 31 < a.sinks
+                      ? a.R : (int)min((int64_t)a.R, ((int64_t)min(kw, a.N - 1) + a.window) * a.G));
   const int tfrom = min(k0 + 127, a.N - 1) * a.G;  // and of the tile's
-  const int tto = a.window >= a.N || k0 + 127 < a.sinks ? a.R : (int)min((int64_t)a.R, ((int64_t)k0 + a.window) * a.G);
+  const int tto = sa_scalar(a.window >= a.N || k0 + 127 < a.sinks ? a.R : (int)min((int64_t)a.R, ((int64_t)k0 + a.window) * a.G));
 
   bool live = k < a.N;
   if (a.mask) live = live && a.mask[b * a.mask_sb + kc] != 0;
@@ -273,17 +319,30 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
     const bool in = near && 8 * chunk < a.D;
     qo[t] = in ? (uint32_t)(i * a.q_sn + g * a.q_sh + 8 * chunk) * 2u : kBufOOB;
     oo[t] = in ? (uint32_t)(i * o_sn + g * a.D + 8 * chunk) * 2u : kBufOOB;
+    if constexpr (KEPT > 2) {
+      kept[2 + 2 * t][threadIdx.x] = (int)qo[t];
+      kept[3 + 2 * t][threadIdx.x] = (int)oo[t];
+    }
   }
+  if constexpr (KEPT > 0) {
+    kept[0][threadIdx.x] = from;
+    kept[KEPT ? 1 : 0][threadIdx.x] = to;
+  }
+  const u16* qbase = sa_scalar(a.q + b * a.q_sb + (int64_t)hk * a.G * a.q_sh);
+  const u16* obase = sa_scalar(ga.dout + ((int64_t)b * a.N * a.H + hk * a.G) * a.D);
+  const float* sbase = sa_scalar((w == 0 ? ga.lse : ga.delta) + bh * a.R);
   auto issue = [&](int r0, int st) {
     char* dst = reinterpret_cast<char*>(smem[st][0]) + NI * w * 1024;
     if (near && r0 + RT <= rend) {
       const int i0 = (int)fdiv((uint32_t)r0, a.div_g);
-      const i32x4 qr = buffer_rsrc(a.q + b * a.q_sb + (int64_t)hk * a.G * a.q_sh + (int64_t)i0 * a.q_sn);
-      const i32x4 dr = buffer_rsrc(ga.dout + (((int64_t)b * a.N + i0) * a.H + hk * a.G) * a.D);
+      const i32x4 qr = buffer_rsrc(qbase + (int64_t)i0 * a.q_sn);
+      const i32x4 dr = buffer_rsrc(obase + (int64_t)i0 * o_sn);
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
-        buf2lds16(qr, qo[t], dst + t * 1024);
-        buf2lds16(dr, oo[t], dst + t * 1024 + TILE * 2);
+        const uint32_t qa = KEPT > 2 ? (uint32_t)kept[KEPT > 2 ? 2 + 2 * t : 0][threadIdx.x] : qo[t];
+        const uint32_t oa = KEPT > 2 ? (uint32_t)kept[KEPT > 2 ? 3 + 2 * t : 0][threadIdx.x] : oo[t];
+        buf2lds16(qr, qa, dst + t * 1024);
+        buf2lds16(dr, oa, dst + t * 1024 + TILE * 2);
       }
     } else {
 #pragma unroll
@@ -294,16 +353,16 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
         const u16 *qs = (const u16*)kSaNone, *os = (const u16*)kSaNone;
         if (r < rend && 8 * chunk < a.D) {
           const int i = (int)fdiv((uint32_t)r, a.div_g), g = r - i * a.G;
-          qs = a.q + b * a.q_sb + (int64_t)(hk * a.G + g) * a.q_sh + (int64_t)i * a.q_sn + 8 * chunk;
-          os = ga.dout + (((int64_t)b * a.N + i) * a.H + hk * a.G + g) * a.D + 8 * chunk;
+          qs = qbase + g * a.q_sh + (int64_t)i * a.q_sn + 8 * chunk;
+          os = obase + (int64_t)i * o_sn + g * a.D + 8 * chunk;
         }
         g2lds16(qs, dst + t * 1024);
         g2lds16(os, dst + t * 1024 + TILE * 2);
       }
     }
     if (w < 2) {  // wave 0: lse, 1: delta of the tile's rows
-      const float* src = w == 0 ? ga.lse : ga.delta;
-      sg_lds4(lane < RT && r0 + lane < rend ? src + bh * a.R + r0 + lane : kSaNone + (w ? 0 : 4), stats[st][w]);
+      // (Absent rows: no state sees them.)
+      sg_lds4(sbase + r0, min(RT, a.R - r0), stats[st][w]);
     }
   };
 
@@ -319,8 +378,8 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
       if (r0 < tfrom || r0 + RT > tto) {
         // A row whose Q or dO is not finite: its statistic makes p and dS NaN.
         auto mark = [&](int row) { stats[st][0][row] = __builtin_nanf(""); };
-        sa_clean<DP, NI>(Q, w, mark);
-        sa_clean<DP, NI>(dO, w, mark);
+        sa_look<DP, NI, false, true>(Q, w, mark);
+        sa_look<DP, NI, false, true>(dO, w, mark);
         lds_barrier();
       }
 #pragma unroll
@@ -329,7 +388,8 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
         const bool whole = rr >= wfrom && rr + 32 <= wto;
         uint32_t bits = ~0u;
         if (!whole) {
-          bits = sa_ones32(to - 1 - rr) & ~sa_ones32(from - 1 - rr);
+          const int first = KEPT ? kept[0][threadIdx.x] : from, end = KEPT ? kept[KEPT ? 1 : 0][threadIdx.x] : to;
+          bits = sa_ones32(end - 1 - rr) & ~sa_ones32(first - 1 - rr);
           if (__ballot(bits != 0) == 0) continue;
         }
         f32x16 s = zero16(), dp = zero16();
@@ -351,9 +411,10 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
           }
         }
         if (!whole) {
+          const uint32_t mine = bits >> (4 * h);
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (!((bits >> (8 * (e >> 2) + 4 * h + (e & 3))) & 1)) s[e] = dp[e] = 0.f;
+            if (!((mine >> (8 * (e >> 2) + (e & 3))) & 1)) s[e] = dp[e] = 0.f;
         }
         bf16x8 pb[2], sb[2];
 #pragma unroll
@@ -372,32 +433,38 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
     }
   }
   if (k >= a.N) return;
-  const bool part = ga.part_k && tile < ga.sunk;
-  const int64_t po = (((int64_t)split * BH + bh) * (128 * ga.sunk) + k) * a.D;
+  // A tile's only part is its sum.
+  const bool sunk = tile < ga.sunk;
+  const bool alone = sunk ? ga.splits == 1 : ga.parts == 1 || (a.window >= a.N && tile >= (ga.parts - 1) * ga.chunk_tiles);
+  const int64_t po = (((int64_t)part * BH + bh) * (sunk ? 128 * ga.sunk : a.N) + k) * a.D;
   sg_store<DB>(dk, a.D, ga.dk + b * ga.dk_s[0] + hk * ga.dk_s[1] + (int64_t)k * ga.dk_s[2],
-               part ? ga.part_k + po : nullptr, ga.scale, !live);
+               alone ? nullptr : (sunk ? ga.sunk_k : ga.part_k) + po, ga.scale, !live);
   sg_store<DB>(dv, a.D, ga.dv + b * ga.dv_s[0] + hk * ga.dv_s[1] + (int64_t)k * ga.dv_s[2],
-               part ? ga.part_v + po : nullptr, 1.f, !live);
+               alone ? nullptr : (sunk ? ga.sunk_v : ga.part_v) + po, 1.f, !live);
 }
 
-// Sums the parts [splits, BH, n, D] of the sinks' states in ascending order, four channels
-// a thread; blockIdx.y 0: dK, 1: dV.
-__global__ __launch_bounds__(256) void sattn_fold_kernel(SAttnGrad ga) {
+// Sums the parts of the states' gradients in ascending order, four channels a thread, of the
+// first n states; blockIdx.y 0: dK, 1: dV.
+__global__ __launch_bounds__(256) void sattn_fold_kernel(SAttnGrad ga, int n) {
   const SAttnArgs& a = ga.f;
-  const float* part = blockIdx.y ? ga.part_v : ga.part_k;
   u16* dst = blockIdx.y ? ga.dv : ga.dk;
   const int64_t* st = blockIdx.y ? ga.dv_s : ga.dk_s;
   const float scale = blockIdx.y ? 1.f : ga.scale;
-  const int n = 128 * ga.sunk, dv = a.D / 4;
+  const int dv = a.D / 4;
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, row = t / dv, BH = (int64_t)a.B * a.Hk;
   if (row >= BH * n) return;
   const int d = 4 * (int)(t - row * dv);
   const int64_t bh = row / n;
   const int k = (int)(row - bh * n), b = (int)(bh / a.Hk), hk = (int)(bh - (int64_t)b * a.Hk);
   if (k >= a.N) return;
+  const bool sunk = k < 128 * ga.sunk;
+  const int first = a.window >= a.N ? k / 128 / ga.chunk_tiles : 0, end = sunk ? ga.splits : ga.parts;
+  if (end - first == 1) return;  // (written at once)
+  const float* part = sunk ? (blockIdx.y ? ga.sunk_v : ga.sunk_k) : (blockIdx.y ? ga.part_v : ga.part_k);
+  const int64_t rows = sunk ? 128 * ga.sunk : a.N;
   f32x4 o = (f32x4)0.f;
-  for (int s = 0; s < ga.splits; ++s) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(part + ((int64_t)s * BH * n + row) * a.D + d);
+  for (int s = first; s < end; ++s) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(part + (((int64_t)s * BH + bh) * rows + k) * a.D + d);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += v[e];
   }
@@ -407,49 +474,64 @@ __global__ __launch_bounds__(256) void sattn_fold_kernel(SAttnGrad ga) {
   *reinterpret_cast<uint2*>(dst + b * st[0] + hk * st[1] + (int64_t)k * st[2] + d) = x;
 }
 
-// The sinks' tiles are split into parts of about as many rows as the other tiles have.
+// Parts of the rows, so that the dK / dV launch has two workgroups a CU and none of them is
+// much longer than the mean.
 static int window_grad_plan(SAttnGrad& g, const char* fn) {
   SAttnArgs& a = g.f;
   const int64_t BH = (int64_t)a.B * a.Hk;
   a.tiles = (a.R + 127) / 128;
   a.splits = 1;
   g.ktiles = (a.N + 127) / 128;
-  g.sunk = a.window < a.N ? (int)((((int64_t)a.sinks < a.N ? a.sinks : a.N) + 127) / 128) : 0;
-  g.splits = 1;
+  g.sunk = 0;
+  g.splits = g.parts = 1;
+  g.chunk_tiles = g.ktiles;
   g.rchunk = a.R;
-  if (g.sunk) {
-    int64_t rows = ((int64_t)a.window + 128) * a.G;
-    if (rows < 1024) rows = 1024;
-    rows = (rows + 63) / 64 * 64;
-    if (rows < a.R) {
-      g.rchunk = (int)rows;
-      g.splits = (int)((a.R + rows - 1) / rows);
+  int64_t units;
+  if (a.window >= a.N) {
+    int64_t parts = (1024 + BH * (g.ktiles + 1) - 1) / (BH * (g.ktiles + 1));
+    if (parts > 16) parts = 16;
+    if (parts > 1) {
+      g.chunk_tiles = (int)((g.ktiles + parts - 1) / parts);
+      g.parts = (g.ktiles + g.chunk_tiles - 1) / g.chunk_tiles;
     }
+    units = (int64_t)g.parts * (g.parts - 1) / 2 * g.chunk_tiles + (int64_t)g.parts * g.chunk_tiles;
+  } else {
+    g.sunk = (int)((((int64_t)a.sinks < a.N ? a.sinks : a.N) + 127) / 128);
+    int64_t rows = ((int64_t)a.window + 128) * a.G;
+    if (rows > a.R) rows = a.R;
+    int64_t parts = 1024 / (BH * g.ktiles);
+    if (parts > rows / 512) parts = rows / 512;
+    if (parts < 1) parts = 1;
+    rows = ((rows + parts - 1) / parts + 63) / 64 * 64;
+    g.parts = (int)parts;
+    if (g.sunk && rows < 512) rows = 512;
+    g.rchunk = (int)rows;
+    g.splits = (int)((a.R + rows - 1) / rows);
+    units = (int64_t)g.sunk * g.splits + (int64_t)(g.ktiles - g.sunk) * g.parts;
   }
-  if (BH * ((int64_t)g.sunk * g.splits + g.ktiles) > kXaMaxGroups ||
-      BH * g.sunk * 128 * (a.D / 4) / 256 + 1 > kXaMaxGroups / 2)
+  if (BH * (units + 8) > kXaMaxGroups || (double)BH * a.N * (a.D / 4) / 256 + 1 > (double)kXaMaxGroups / 2)
     return set_error(TPF_ERR_SHAPE, "%s: too many states", fn);
+  a.order = sa_order(BH, a.tiles);
+  g.order = sa_order(BH, units);
   return TPF_OK;
 }
 
 // Workspace in floats: delta, then the parts.
 struct WindowSpace {
-  int64_t delta, part, total;
+  int64_t delta, part, sunk, total;
   explicit WindowSpace(const SAttnGrad& g) {
     const int64_t BH = (int64_t)g.f.B * g.f.Hk;
     delta = (BH * g.f.R + 3) / 4 * 4;
-    part = g.splits > 1 ? g.splits * BH * g.sunk * 128 * g.f.D : 0;
-    total = delta + 2 * part;
+    part = g.parts > 1 ? g.parts * BH * g.f.N * g.f.D : 0;
+    sunk = g.sunk && g.splits > 1 ? g.splits * BH * g.sunk * 128 * g.f.D : 0;
+    total = delta + 2 * part + 2 * sunk;
   }
 };
 
 template <int DP>
 static void window_grad_launch(const SAttnGrad& g, hipStream_t s) {
-  const SAttnArgs& a = g.f;
-  const int64_t BH = (int64_t)a.B * a.Hk;
-  const int64_t n1 = BH * a.tiles, n2 = BH * ((int64_t)g.sunk * g.splits + g.ktiles - g.sunk);
-  hipLaunchKernelGGL((sattn_dq_kernel<DP>), dim3((unsigned)((n1 + 7) / 8 * 8)), dim3(256), 0, s, g);
-  hipLaunchKernelGGL((sattn_dkdv_kernel<DP>), dim3((unsigned)((n2 + 7) / 8 * 8)), dim3(256), 0, s, g);
+  hipLaunchKernelGGL((sattn_dq_kernel<DP>), dim3((unsigned)g.f.order.groups), dim3(256), 0, s, g);
+  hipLaunchKernelGGL((sattn_dkdv_kernel<DP>), dim3((unsigned)g.order.groups), dim3(256), 0, s, g);
 }
 
 }  // namespace tpf
@@ -495,16 +577,19 @@ extern "C" int tpf_window_backward_bf16(const void* q, const void* k, const void
   g.scale = (float)scale;
   float* w = (float*)workspace;
   g.delta = w;
-  g.part_k = ws.part ? w + ws.delta : nullptr;
-  g.part_v = ws.part ? w + ws.delta + ws.part : nullptr;
+  g.part_k = w + ws.delta;
+  g.part_v = g.part_k + ws.part;
+  g.sunk_k = g.part_v + ws.part;
+  g.sunk_v = g.sunk_k + ws.sunk;
   hipStream_t s = (hipStream_t)stream;
   if (a.D <= 32) tpf::window_grad_launch<32>(g, s);
   else if (a.D <= 64) tpf::window_grad_launch<64>(g, s);
   else if (a.D <= 96) tpf::window_grad_launch<96>(g, s);
   else tpf::window_grad_launch<128>(g, s);
-  if (ws.part) {
-    const int64_t n = ((int64_t)a.B * a.Hk * g.sunk * 128 * (a.D / 4) + 255) / 256;
-    hipLaunchKernelGGL(tpf::sattn_fold_kernel, dim3((unsigned)n, 2), dim3(256), 0, s, g);
+  if (ws.part || ws.sunk) {
+    const int states = ws.part || 128 * g.sunk > a.N ? a.N : 128 * g.sunk;
+    const int64_t n = ((int64_t)a.B * a.Hk * states * (a.D / 4) + 255) / 256;
+    hipLaunchKernelGGL(tpf::sattn_fold_kernel, dim3((unsigned)n, 2), dim3(256), 0, s, g, states);
   }
   return tpf::check_launch(fn);
 }
