@@ -38,6 +38,7 @@ struct RotArgs {
   int64_t N;
   int D, half, units;  // lanes of a row that hold channels
   int slices;      // waves that share a token's heads
+  FastDiv div_slices, div_n;
   float eps;
   int norm, inter;
   float* part;     // [groups, 2, D] partial gradients of the weights
@@ -49,26 +50,29 @@ template <> struct RotType<TPF_BF16> { typedef __bf16 E; };
 template <> struct RotType<TPF_F16> { typedef _Float16 E; };
 template <> struct RotType<TPF_F32> { typedef float E; };
 
-// Channel of entry i (0 .. 7) of a lane's first (e = 0) or second eight channels; -1
-// where there is none.  Lane u < nr has the pairs 8 u .. 8 u + 7, the others pass.
+// Where a lane's sixteen channels are: entries 0 .. 7 are the pairs' first channels, 8 .. 15
+// the second ones.  With halves lane u < nr has the pairs 8 u .. 8 u + 7 and the others
+// sixteen channels that pass; interleaved, lane u has the channels 16 u .. 16 u + 15 and pairs
+// past the last are turned by 0.
 struct RotUnit {
-  int a0, b0, na, nb, step;
-  bool turns;
+  int a0, b0, na, nb;
+  bool turns, inter;
   __device__ __forceinline__ RotUnit(const RotArgs& r, int u) {
+    inter = r.inter;
+    if (inter) {
+      a0 = 16 * u;
+      b0 = 16 * u + 1;
+      na = max(0, min(8, (r.D - 16 * u + 1) / 2));
+      nb = max(0, min(8, (r.D - 16 * u) / 2));
+      turns = 8 * u < r.half;
+      return;
+    }
     const int nr = (r.half + 7) / 8;
     turns = u < nr;
-    step = 1;
     if (turns) {
-      const int n = min(8, r.half - 8 * u);
-      na = nb = n;
-      if (r.inter) {
-        a0 = 16 * u;
-        b0 = 16 * u + 1;
-        step = 2;
-      } else {
-        a0 = 8 * u;
-        b0 = r.half + 8 * u;
-      }
+      na = nb = min(8, r.half - 8 * u);
+      a0 = 8 * u;
+      b0 = r.half + 8 * u;
     } else {
       a0 = 2 * r.half + 16 * (u - nr);
       b0 = a0 + 8;
@@ -76,86 +80,76 @@ struct RotUnit {
       nb = max(0, min(8, r.D - b0));
     }
   }
+  __device__ __forceinline__ bool has(int e) const { return e < 8 ? e < na : e - 8 < nb; }
+  __device__ __forceinline__ int channel(int e) const {
+    return inter ? a0 + 2 * (e & 7) + (e >> 3) : e < 8 ? a0 + e : b0 + e - 8;
+  }
 };
 
-// A lane's channels of a row as 32-bit values.  VEC: whole vectors of eight, on 16
-// bytes (half and D are multiples of 8); otherwise element by element.
-template <int TY, bool VEC>
+// A lane's channels of a row in memory's order: its sixteen channels, or eight and eight; in
+// vectors of W, which all strides, D and half are multiples of (interleaved: half may be any).
+template <int TY, int W>
 struct RotRow {
   typedef typename RotType<TY>::E E;
-  typedef E V8 __attribute__((ext_vector_type(8)));
-  V8 lo, hi;
+  typedef E V __attribute__((ext_vector_type(W > 1 ? W : 2)));
+  E x[16];
+  static __device__ __forceinline__ bool has(const RotUnit& u, int j) {
+    return u.inter ? j < u.na + u.nb : u.has(j);
+  }
+  static __device__ __forceinline__ int channel(const RotUnit& u, int j) {
+    return u.inter || j < 8 ? u.a0 + j : u.b0 + j - 8;
+  }
   __device__ __forceinline__ void load(const E* p, const RotUnit& u, bool in) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lo[i] = hi[i] = (E)0.f;
-    if (!in) return;
-    if constexpr (VEC) {
-      if (u.step == 2) {
-        if (u.na) {
-          lo = *reinterpret_cast<const V8*>(p + u.a0);
-          hi = *reinterpret_cast<const V8*>(p + u.a0 + 8);
-        }
-      } else {
-        if (u.na) lo = *reinterpret_cast<const V8*>(p + u.a0);
-        if (u.nb) hi = *reinterpret_cast<const V8*>(p + u.b0);
-      }
-    } else {
+    for (int j = 0; j < 16; j += W) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i < u.na) lo[i] = p[u.a0 + i * u.step];
-        if (i < u.nb) hi[i] = p[u.b0 + i * u.step];
+      for (int e = 0; e < W; ++e) x[j + e] = (E)0.f;
+      if (in && has(u, j)) {
+        if constexpr (W == 1) {
+          x[j] = p[channel(u, j)];
+        } else {
+          const V v = *reinterpret_cast<const V*>(p + channel(u, j));
+#pragma unroll
+          for (int e = 0; e < W; ++e) x[j + e] = v[e];
+        }
       }
     }
   }
   __device__ __forceinline__ void get(const RotUnit& u, float (&a)[8], float (&b)[8]) const {
-    if (VEC && u.step == 2) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = (float)lo[2 * i];
-        b[i] = (float)lo[2 * i + 1];
-        a[4 + i] = (float)hi[2 * i];
-        b[4 + i] = (float)hi[2 * i + 1];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] = (float)lo[i];
-        b[i] = (float)hi[i];
-      }
+    for (int i = 0; i < 8; ++i) {
+      a[i] = (float)(u.inter ? x[2 * i] : x[i]);
+      b[i] = (float)(u.inter ? x[2 * i + 1] : x[8 + i]);
     }
   }
   static __device__ __forceinline__ void store(E* p, const RotUnit& u, const float (&a)[8],
                                                const float (&b)[8]) {
-    if constexpr (VEC) {
-      V8 l, h;
-      if (u.step == 2) {
+    E y[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          l[2 * i] = (E)a[i];
-          l[2 * i + 1] = (E)b[i];
-          h[2 * i] = (E)a[4 + i];
-          h[2 * i + 1] = (E)b[4 + i];
-        }
-        if (u.na) {
-          *reinterpret_cast<V8*>(p + u.a0) = l;
-          *reinterpret_cast<V8*>(p + u.a0 + 8) = h;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          l[i] = (E)a[i];
-          h[i] = (E)b[i];
-        }
-        if (u.na) *reinterpret_cast<V8*>(p + u.a0) = l;
-        if (u.nb) *reinterpret_cast<V8*>(p + u.b0) = h;
-      }
-    } else {
+    for (int i = 0; i < 8; ++i) {
+      const E va = (E)a[i], vb = (E)b[i];
+      y[i] = va;
+      y[8 + i] = vb;
+    }
+    if (u.inter) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (i < u.na) p[u.a0 + i * u.step] = (E)a[i];
-        if (i < u.nb) p[u.b0 + i * u.step] = (E)b[i];
+        y[2 * i] = (E)a[i];
+        y[2 * i + 1] = (E)b[i];
       }
     }
+#pragma unroll
+    for (int j = 0; j < 16; j += W)
+      if (has(u, j)) {
+        if constexpr (W == 1) {
+          p[channel(u, j)] = y[j];
+        } else {
+          V v;
+#pragma unroll
+          for (int e = 0; e < W; ++e) v[e] = y[j + e];
+          *reinterpret_cast<V*>(p + channel(u, j)) = v;
+        }
+      }
   }
 };
 
@@ -164,13 +158,23 @@ __device__ __forceinline__ float rot_param(const void* p, int type, int c) {
   if (type == TPF_F16) return (float)((const _Float16*)p)[c];
   return bf2f(((const u16*)p)[c]);
 }
-// A lane's channels of side `s`'s weight (1 without one, 0 past the row).
-__device__ __forceinline__ void rot_weights(const RotArgs& r, int s, const RotUnit& u, float (&a)[8],
-                                            float (&b)[8]) {
+// Both sides' weights into LDS in the lanes' order (1 without one, 0 past the row); a barrier
+// has to follow.
+template <int L>
+__device__ __forceinline__ void rot_weights(const RotArgs& r, float (*w)[16 * L]) {
+  for (int i = threadIdx.x; i < 32 * L; i += 256) {
+    const int s = i / (16 * L), e = i % (16 * L);
+    const RotUnit u(r, e / 16);
+    const int x = e % 16;
+    w[s][e] = !u.has(x) ? 0.f : r.w[s] ? rot_param(r.w[s], r.w_type, u.channel(x)) : 1.f;
+  }
+}
+__device__ __forceinline__ void rot_eight(const float* p, float (&x)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    a[i] = i < u.na ? (r.w[s] ? rot_param(r.w[s], r.w_type, u.a0 + i * u.step) : 1.f) : 0.f;
-    b[i] = i < u.nb ? (r.w[s] ? rot_param(r.w[s], r.w_type, u.b0 + i * u.step) : 1.f) : 0.f;
+  for (int q = 0; q < 2; ++q) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p + 4 * q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * q + e] = v[e];
   }
 }
 
@@ -179,7 +183,7 @@ __device__ __forceinline__ void rot_weights(const RotArgs& r, int s, const RotUn
 __device__ __forceinline__ void rot_angles(const RotArgs& r, int64_t p, float* cs) {
   const int lane = threadIdx.x & 63;
   for (int c = lane; c < (r.half + 7) / 8 * 8; c += 64) {
-    float s = 0.f, co = 0.f;  // past the last pair: zeros, beside the lanes' zeros there
+    float s = 0.f, co = 1.f;  // past the last pair
     if (c < r.half) {
       double t = (double)p * (r.freq[c] * 0.15915494309189533577);  // turns
       t -= __builtin_rint(t);
@@ -189,18 +193,6 @@ __device__ __forceinline__ void rot_angles(const RotArgs& r, int64_t p, float* c
     cs[kRotMaxHalf + c] = s;
   }
   __builtin_amdgcn_wave_barrier();
-}
-__device__ __forceinline__ void rot_take(const float* cs, int u, float (&co)[8], float (&si)[8]) {
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const f32x4 c = *reinterpret_cast<const f32x4*>(cs + 8 * u + 4 * q);
-    const f32x4 s = *reinterpret_cast<const f32x4*>(cs + kRotMaxHalf + 8 * u + 4 * q);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      co[4 * q + e] = c[e];
-      si[4 * q + e] = s[e];
-    }
-  }
 }
 
 template <int L>
@@ -220,18 +212,23 @@ __device__ __forceinline__ int rot_side(const RotArgs& r, int hh, int& head) {
 }
 
 // Forward, and (PAGED) the way into the cache: a wave has a share of a token's heads.
-template <int TY, int L, bool VEC, bool PAGED>
+template <int TY, int L, int W, bool PAGED>
 __global__ __launch_bounds__(256) void rot_fwd_kernel(RotArgs r) {
-  typedef RotRow<TY, VEC> Row;
+  typedef RotRow<TY, W> Row;
   typedef typename Row::E E;
   __shared__ __attribute__((aligned(16))) float lds[4][2 * kRotMaxHalf];
+  __shared__ __attribute__((aligned(16))) float weights[2][16 * L];
   constexpr int RPW = 64 / L;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + w;
-  const int64_t token = item / r.slices;
+  if (r.norm) {
+    rot_weights<L>(r, weights);
+    __syncthreads();
+  }
+  const uint32_t item = blockIdx.x * 4 + w;  // (below 2^26)
+  const uint32_t token = fdiv(item, r.div_slices);
   const int slice = (int)(item - token * r.slices);
   if (token >= r.tokens) return;  // (no barrier follows)
-  const int64_t b = token / r.N, n = token - b * r.N;
+  const int64_t b = fdiv(token, r.div_n), n = token - b * r.N;
   const RotUnit u(r, lane % L);
   const int total = r.heads[0] + r.heads[1] + r.heads[2];
 
@@ -261,12 +258,10 @@ __global__ __launch_bounds__(256) void rot_fwd_kernel(RotArgs r) {
   float co[8], si[8];
   if (r.half) {
     rot_angles(r, p, lds[w]);
-    if (u.turns) rot_take(lds[w], lane % L, co, si);
-  }
-  float wa[2][8], wb[2][8];
-  if (r.norm) {
-    rot_weights(r, 0, u, wa[0], wb[0]);
-    rot_weights(r, 1, u, wa[1], wb[1]);
+    if (u.turns) {
+      rot_eight(lds[w] + 8 * (lane % L), co);
+      rot_eight(lds[w] + kRotMaxHalf + 8 * (lane % L), si);
+    }
   }
   const float inv_d = 1.f / (float)r.D;
 
@@ -281,10 +276,13 @@ __global__ __launch_bounds__(256) void rot_fwd_kernel(RotArgs r) {
     if (!PAGED || s < 2) {
       if (r.norm) {
         const float rstd = 1.f / sqrtf(fmaf(rot_squares<L>(a, c), inv_d, r.eps));
+        float wa[8], wb[8];
+        rot_eight(weights[s == 1] + 16 * (lane % L), wa);
+        rot_eight(weights[s == 1] + 16 * (lane % L) + 8, wb);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          a[i] = a[i] * rstd * (s ? wa[1][i] : wa[0][i]);
-          c[i] = c[i] * rstd * (s ? wb[1][i] : wb[0][i]);
+          a[i] = a[i] * rstd * wa[i];
+          c[i] = c[i] * rstd * wb[i];
         }
       }
       if (u.turns) {
@@ -315,29 +313,30 @@ __global__ __launch_bounds__(256) void rot_fwd_kernel(RotArgs r) {
 // Backward: a workgroup's waves take tokens in turn and keep the weights' gradients of
 // their channels in registers; what the rows, waves and workgroups have is added in a
 // fixed order.
-template <int TY, int L, bool VEC>
+template <int TY, int L, int W>
 __global__ __launch_bounds__(256) void rot_bwd_kernel(RotArgs r) {
-  typedef RotRow<TY, VEC> Row;
+  typedef RotRow<TY, W> Row;
   typedef typename Row::E E;
   __shared__ __attribute__((aligned(16))) float lds[4][2 * kRotMaxHalf];
+  __shared__ __attribute__((aligned(16))) float weights[2][16 * L];
   constexpr int RPW = 64 / L;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r.norm) {
+    rot_weights<L>(r, weights);
+    __syncthreads();
+  }
   const RotUnit u(r, lane % L);
   const int total = r.heads[0] + r.heads[1], step = RPW * r.slices;
   const float inv_d = 1.f / (float)r.D;
-  float wa[2][8], wb[2][8], ga[2][8], gb[2][8];
-  if (r.norm) {
-    rot_weights(r, 0, u, wa[0], wb[0]);
-    rot_weights(r, 1, u, wa[1], wb[1]);
-  }
+  float ga[2][8], gb[2][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) ga[0][i] = ga[1][i] = gb[0][i] = gb[1][i] = 0.f;
 
-  const int64_t items = r.tokens * r.slices;
-  for (int64_t item = (int64_t)blockIdx.x * 4 + w; item < items; item += (int64_t)gridDim.x * 4) {
-    const int64_t token = item / r.slices;
+  const uint32_t items = (uint32_t)(r.tokens * r.slices);  // (below 2^26)
+  for (uint32_t item = blockIdx.x * 4 + w; item < items; item += gridDim.x * 4) {
+    const uint32_t token = fdiv(item, r.div_slices);
     const int slice = (int)(item - token * r.slices);
-    const int64_t b = token / r.N, n = token - b * r.N;
+    const int64_t b = fdiv(token, r.div_n), n = token - b * r.N;
     Row nx, nd;
     int hh = slice * RPW + lane / L;
     auto load = [&](int h) {
@@ -355,7 +354,10 @@ __global__ __launch_bounds__(256) void rot_bwd_kernel(RotArgs r) {
     if (r.half) {
       __builtin_amdgcn_wave_barrier();
       rot_angles(r, p, lds[w]);
-      if (u.turns) rot_take(lds[w], lane % L, co, si);
+      if (u.turns) {
+        rot_eight(lds[w] + 8 * (lane % L), co);
+        rot_eight(lds[w] + kRotMaxHalf + 8 * (lane % L), si);
+      }
     }
     for (; hh - lane / L < total; hh += step) {
       const Row rx = nx, rd = nd;
@@ -376,7 +378,9 @@ __global__ __launch_bounds__(256) void rot_bwd_kernel(RotArgs r) {
         float xa[8], xb[8];
         rx.get(u, xa, xb);
         const float rstd = 1.f / sqrtf(fmaf(rot_squares<L>(xa, xb), inv_d, r.eps));
-        float dot = 0.f;
+        float dot = 0.f, wa[8], wb[8];
+        rot_eight(weights[s] + 16 * (lane % L), wa);
+        rot_eight(weights[s] + 16 * (lane % L) + 8, wb);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           xa[i] *= rstd;
@@ -391,8 +395,8 @@ __global__ __launch_bounds__(256) void rot_bwd_kernel(RotArgs r) {
               gb[0][i] += vb;
             }
           }
-          a[i] *= s ? wa[1][i] : wa[0][i];
-          c[i] *= s ? wb[1][i] : wb[0][i];
+          a[i] *= wa[i];
+          c[i] *= wb[i];
           dot = fmaf(a[i], xa[i], fmaf(c[i], xb[i], dot));
         }
         dot = lanes_sum<L>(dot) * inv_d;
@@ -427,31 +431,31 @@ __global__ __launch_bounds__(256) void rot_bwd_kernel(RotArgs r) {
   for (int t = threadIdx.x; t < 32 * L; t += 256) {
     const int s = t / (16 * L), e = t - s * 16 * L;
     const RotUnit v(r, e / 16);
-    const int i = e & 7;
-    const bool second = e & 8;
-    if (i < (second ? v.nb : v.na))
-      r.part[((int64_t)blockIdx.x * 2 + s) * r.D + (second ? v.b0 : v.a0) + i * v.step] =
+    if (v.has(e % 16))
+      r.part[((int64_t)blockIdx.x * 2 + s) * r.D + v.channel(e % 16)] =
           ((sums[0][s][e] + sums[1][s][e]) + sums[2][s][e]) + sums[3][s][e];
   }
 }
 
-// The weights' gradients from the workgroups' sums: 32 channels of a side a workgroup,
-// eight ranges of the sums that meet in LDS in order.
+// The weights' gradients from the workgroups' sums: sixteen channels of a side a workgroup,
+// sixteen ranges of the sums, whose partial sums meet in LDS in order.
 __global__ __launch_bounds__(256) void rot_fold_kernel(const float* part, int groups, int D, void* dq,
                                                        void* dk, int type) {
-  __shared__ float sums[8][32];
-  const int s = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), q = threadIdx.x >> 5;
+  __shared__ float sums[16][16];
+  const int s = blockIdx.y, c = blockIdx.x * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
   void* out = s ? dk : dq;
   if (!out) return;
-  const int per = (groups + 7) / 8;
+  const int per = (groups + 15) / 16, end = min(groups, (q + 1) * per);
   float v = 0.f;
-  if (c < D)
-    for (int g = q * per; g < min(groups, (q + 1) * per); ++g) v += part[((int64_t)g * 2 + s) * D + c];
-  sums[q][threadIdx.x & 31] = v;
+  if (c < D) {
+#pragma unroll 16
+    for (int g = q * per; g < end; ++g) v += part[((int64_t)g * 2 + s) * D + c];
+  }
+  sums[q][threadIdx.x & 15] = v;
   __syncthreads();
   if (q || c >= D) return;
 #pragma unroll
-  for (int x = 1; x < 8; ++x) v += sums[x][threadIdx.x & 31];
+  for (int x = 1; x < 16; ++x) v += sums[x][threadIdx.x & 15];
   if (type == TPF_F32) ((float*)out)[c] = v;
   else if (type == TPF_F16) ((_Float16*)out)[c] = (_Float16)v;
   else ((u16*)out)[c] = f2bf_bits(v);
@@ -463,6 +467,8 @@ static void rot_plan(RotArgs& r, int rows_per_wave) {
   const int most = (total + rows_per_wave - 1) / rows_per_wave;
   int64_t s = (8192 + r.tokens - 1) / r.tokens;
   r.slices = (int)(s < 1 ? 1 : s > most ? most : s);
+  r.div_slices = make_fastdiv((uint32_t)r.slices);
+  r.div_n = make_fastdiv((uint32_t)r.N);
 }
 
 static int rot_lanes(const RotArgs& r) {
@@ -478,34 +484,41 @@ static int64_t rot_groups(const RotArgs& r) {
   return n < kRotGroups ? n : kRotGroups;
 }
 
-template <int TY, int L, bool VEC>
+template <int TY, int L, int W>
 static void rot_launch(const RotArgs& r, int mode, hipStream_t s) {
   const dim3 all((unsigned)((r.tokens * r.slices + 3) / 4));
-  if (mode == 0) hipLaunchKernelGGL((rot_fwd_kernel<TY, L, VEC, false>), all, dim3(256), 0, s, r);
+  if (mode == 0) hipLaunchKernelGGL((rot_fwd_kernel<TY, L, W, false>), all, dim3(256), 0, s, r);
   if constexpr (TY != TPF_F32)
-    if (mode == 1) hipLaunchKernelGGL((rot_fwd_kernel<TY, L, VEC, true>), all, dim3(256), 0, s, r);
+    if (mode == 1) hipLaunchKernelGGL((rot_fwd_kernel<TY, L, W, true>), all, dim3(256), 0, s, r);
   if (mode == 2)
-    hipLaunchKernelGGL((rot_bwd_kernel<TY, L, VEC>), dim3((unsigned)rot_groups(r)), dim3(256), 0, s, r);
+    hipLaunchKernelGGL((rot_bwd_kernel<TY, L, W>), dim3((unsigned)rot_groups(r)), dim3(256), 0, s, r);
+}
+template <int TY, int L>
+static void rot_wide(const RotArgs& r, int mode, int w, hipStream_t s) {
+  if (w == 8 && TY != TPF_F32) rot_launch<TY, L, TY == TPF_F32 ? 4 : 8>(r, mode, s);
+  else if (w >= 4) rot_launch<TY, L, 4>(r, mode, s);
+  else if (w == 2) rot_launch<TY, L, 2>(r, mode, s);
+  else rot_launch<TY, L, 1>(r, mode, s);
 }
 template <int TY>
-static void rot_pick(const RotArgs& r, int mode, bool vec, hipStream_t s) {
+static void rot_pick(const RotArgs& r, int mode, int w, hipStream_t s) {
   switch (rot_lanes(r)) {
-    case 4: vec ? rot_launch<TY, 4, true>(r, mode, s) : rot_launch<TY, 4, false>(r, mode, s); break;
-    case 8: vec ? rot_launch<TY, 8, true>(r, mode, s) : rot_launch<TY, 8, false>(r, mode, s); break;
-    case 16: vec ? rot_launch<TY, 16, true>(r, mode, s) : rot_launch<TY, 16, false>(r, mode, s); break;
-    default: vec ? rot_launch<TY, 32, true>(r, mode, s) : rot_launch<TY, 32, false>(r, mode, s);
+    case 4: rot_wide<TY, 4>(r, mode, w, s); break;
+    case 8: rot_wide<TY, 8>(r, mode, w, s); break;
+    case 16: rot_wide<TY, 16>(r, mode, w, s); break;
+    default: rot_wide<TY, 32>(r, mode, w, s);
   }
 }
-static void rot_run(const RotArgs& r, int64_t type, int mode, bool vec, hipStream_t s) {
-  if (type == TPF_BF16) rot_pick<TPF_BF16>(r, mode, vec, s);
-  else if (type == TPF_F16) rot_pick<TPF_F16>(r, mode, vec, s);
-  else rot_pick<TPF_F32>(r, mode, vec, s);
+static void rot_run(const RotArgs& r, int64_t type, int mode, int w, hipStream_t s) {
+  if (type == TPF_BF16) rot_pick<TPF_BF16>(r, mode, w, s);
+  else if (type == TPF_F16) rot_pick<TPF_F16>(r, mode, w, s);
+  else rot_pick<TPF_F32>(r, mode, w, s);
 }
 
 // Sizes of a call into r; 0 or an error code.
 static int rot_check(RotArgs& r, int64_t B, int64_t N, int64_t H, int64_t Hk, int64_t Hv, int64_t D,
                      int64_t half, int64_t type, int64_t w_type, double eps, int norm,
-                     const char* fn) {
+                     int inter, const char* fn) {
   const int64_t lim = (int64_t)1 << 30;
   if (B < 1 || N < 1 || B > lim || N > lim || H < 0 || Hk < 0 || H + Hk < 1 || H > 65535 || Hk > 65535 ||
       D < 1 || D > 256 || half < 0 || 2 * half > D)
@@ -520,7 +533,8 @@ static int rot_check(RotArgs& r, int64_t B, int64_t N, int64_t H, int64_t Hk, in
   r.N = N;
   r.heads[0] = (int)H; r.heads[1] = (int)Hk; r.heads[2] = (int)Hv;
   r.D = (int)D; r.half = (int)half;
-  r.units = (int)((half + 7) / 8 + (D - 2 * half + 15) / 16);
+  r.inter = inter;
+  r.units = (int)(inter ? (D + 15) / 16 : (half + 7) / 8 + (D - 2 * half + 15) / 16);
   r.norm = norm;
   r.eps = (float)eps;
   r.w_type = (int)w_type;
@@ -530,9 +544,12 @@ static int rot_check(RotArgs& r, int64_t B, int64_t N, int64_t H, int64_t Hk, in
   return TPF_OK;
 }
 
-static bool rot_vec(const RotArgs& r, const void* p, const int64_t* strides) {
-  return r.half % 8 == 0 && r.D % 8 == 0 && (uintptr_t)p % 16 == 0 && strides[0] % 8 == 0 &&
-         strides[1] % 8 == 0 && strides[2] % 8 == 0;
+// Elements of the widest vectors (up to `w`) that the rows at p with these strides allow.
+static int rot_width(const RotArgs& r, int64_t type, int w, const void* p, const int64_t* strides) {
+  const int size = type == TPF_F32 ? 4 : 2;
+  const int64_t all = (r.inter ? 0 : r.half) | r.D | strides[0] | strides[1] | strides[2];
+  while (w > 1 && (all % w || (uintptr_t)p % (w * size))) w /= 2;
+  return w;
 }
 
 }  // namespace tpf
@@ -542,7 +559,7 @@ static int rot_entry(tpf::RotArgs& r, const tpf_rotary_shape* s, const void* pos
                      const char* fn) {
   if (!s) return tpf::set_error(TPF_ERR_ARG, "%s: null shape", fn);
   if (int rc = tpf::rot_check(r, s->B, s->N, s->H, s->Hk, 0, s->D, s->half, s->dtype, s->weight_dtype, eps,
-                              s->norm != 0, fn))
+                              s->norm != 0, s->interleaved != 0, fn))
     return rc;
   if (s->half && !frequencies) return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
   if (s->position_bits != 32 && s->position_bits != 64)
@@ -554,7 +571,6 @@ static int rot_entry(tpf::RotArgs& r, const tpf_rotary_shape* s, const void* pos
   r.freq = frequencies;
   r.w[0] = qw;
   r.w[1] = kw;
-  r.inter = s->interleaved != 0;
   for (int i = 0; i < 3; ++i) {
     r.x_s[0][i] = s->q_stride[i];
     r.x_s[1][i] = s->k_stride[i];
@@ -574,10 +590,13 @@ extern "C" int tpf_rotary_forward(const void* q, const void* k, const void* posi
   if ((shape->H && (!q || !q_out)) || (shape->Hk && (!k || !k_out)))
     return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
   r.x[0] = q; r.x[1] = k; r.y[0] = q_out; r.y[1] = k_out;
-  bool vec = true;
+  int w = 8;
   for (int i = 0; i < 2; ++i)
-    if (r.heads[i]) vec = vec && tpf::rot_vec(r, r.x[i], r.x_s[i]) && tpf::rot_vec(r, r.y[i], r.y_s[i]);
-  tpf::rot_run(r, shape->dtype, 0, vec, (hipStream_t)stream);
+    if (r.heads[i]) {
+      w = tpf::rot_width(r, shape->dtype, w, r.x[i], r.x_s[i]);
+      w = tpf::rot_width(r, shape->dtype, w, r.y[i], r.y_s[i]);
+    }
+  tpf::rot_run(r, shape->dtype, 0, w, (hipStream_t)stream);
   return tpf::check_launch(fn);
 }
 
@@ -609,15 +628,17 @@ extern "C" int tpf_rotary_backward(const void* q, const void* k, const void* dq_
   for (int i = 0; i < 2; ++i)
     for (int j = 0; j < 3; ++j) r.dy_s[i][j] = grad_strides[3 * i + j];
   r.part = want ? (float*)workspace : nullptr;
-  bool vec = true;
+  int w = 8;
   for (int i = 0; i < 2; ++i)
-    if (r.heads[i])
-      vec = vec && (!r.norm || tpf::rot_vec(r, r.x[i], r.x_s[i])) && tpf::rot_vec(r, r.dy[i], r.dy_s[i]) &&
-            tpf::rot_vec(r, r.y[i], r.y_s[i]);
+    if (r.heads[i]) {
+      if (r.norm) w = tpf::rot_width(r, shape->dtype, w, r.x[i], r.x_s[i]);
+      w = tpf::rot_width(r, shape->dtype, w, r.dy[i], r.dy_s[i]);
+      w = tpf::rot_width(r, shape->dtype, w, r.y[i], r.y_s[i]);
+    }
   hipStream_t st = (hipStream_t)stream;
-  tpf::rot_run(r, shape->dtype, 2, vec, st);
+  tpf::rot_run(r, shape->dtype, 2, w, st);
   if (want)
-    hipLaunchKernelGGL(tpf::rot_fold_kernel, dim3((r.D + 31) / 32, 2), dim3(256), 0, st, r.part,
+    hipLaunchKernelGGL(tpf::rot_fold_kernel, dim3((r.D + 15) / 16, 2), dim3(256), 0, st, r.part,
                        (int)tpf::rot_groups(r), r.D, dq_weight, dk_weight, r.w_type);
   return tpf::check_launch(fn);
 }
@@ -669,7 +690,7 @@ extern "C" int tpf_paged_append(const void* q, const void* k, const void* v, con
     return tpf::set_error(TPF_ERR_ARG, "%s: dtype must be TPF_BF16 or TPF_F16", fn);
   if (s->Hk < 1) return tpf::set_error(TPF_ERR_SHAPE, "%s: no kv heads", fn);
   if (int rc = tpf::rot_check(r, 1, batch->T, s->H, s->Hk, s->Hk, s->D, s->half, s->dtype, s->weight_dtype,
-                              eps, s->norm != 0, fn))
+                              eps, s->norm != 0, s->interleaved != 0, fn))
     return rc;
   if (!k || !v || !k_cache || !v_cache || (s->H && (!q || !q_out)) || (s->half && !frequencies))
     return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
@@ -677,9 +698,8 @@ extern "C" int tpf_paged_append(const void* q, const void* k, const void* v, con
   r.y[0] = q_out; r.y[1] = k_cache; r.y[2] = v_cache;
   r.w[0] = q_weight; r.w[1] = k_weight;
   r.freq = frequencies;
-  r.inter = s->interleaved != 0;
   const int64_t* in[3] = {s->q_stride, s->k_stride, s->v_stride};
-  bool vec = true;
+  int w = 8;
   for (int i = 0; i < 3; ++i) {
     r.x_s[i][1] = in[i][1];
     r.x_s[i][2] = in[i][0];
@@ -692,7 +712,10 @@ extern "C" int tpf_paged_append(const void* q, const void* k, const void* v, con
     r.y_s[i][2] = s->D;
   }
   for (int i = 0; i < 3; ++i)
-    if (r.heads[i]) vec = vec && tpf::rot_vec(r, r.x[i], r.x_s[i]) && tpf::rot_vec(r, r.y[i], r.y_s[i]);
-  tpf::rot_run(r, s->dtype, 1, vec, (hipStream_t)stream);
+    if (r.heads[i]) {
+      w = tpf::rot_width(r, s->dtype, w, r.x[i], r.x_s[i]);
+      w = tpf::rot_width(r, s->dtype, w, r.y[i], r.y_s[i]);
+    }
+  tpf::rot_run(r, s->dtype, 1, w, (hipStream_t)stream);
   return tpf::check_launch(fn);
 }
