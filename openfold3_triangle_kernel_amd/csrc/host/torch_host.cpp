@@ -521,6 +521,328 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
   return xattn_forward(q, k, v, mask, kind, mask_stride, scale, nullptr, nullptr);
 }
 
+// -------------------------------------------------------- norms and rotation
+
+Tensor or_none(const std::optional<Tensor>& t) { return t.value_or(Tensor()); }
+
+// Frequencies and weights as the kernels read them (D channels); nullopt-worthy ones are false.
+bool rotation_plain(int64_t D, const std::optional<Tensor>& freq, const std::optional<Tensor>& qw,
+                    const std::optional<Tensor>& kw, const std::optional<double>& eps,
+                    c10::DeviceIndex dev) {
+  if (freq && (!plain(*freq, dev) || freq->dim() != 1 || freq->numel() == 0 || 2 * freq->numel() > D ||
+               freq->scalar_type() != at::kDouble || !freq->is_contiguous() || freq->requires_grad()))
+    return false;
+  if (eps ? !(*eps >= 0.0 && *eps < 1e30) : qw.has_value() || kw.has_value()) return false;
+  for (const auto* w : {&qw, &kw})
+    if (*w && (!plain(**w, dev) || (*w)->dim() != 1 || (*w)->size(0) != D || !(*w)->is_contiguous() ||
+               type_code((*w)->scalar_type()) < 0))
+      return false;
+  return !(qw && kw) || qw->scalar_type() == kw->scalar_type();
+}
+at::ScalarType weight_type(const Tensor& qw, const Tensor& kw) {
+  return qw.defined() ? qw.scalar_type() : kw.defined() ? kw.scalar_type() : at::kFloat;
+}
+
+// A new tensor in t's storage order, its channels contiguous.
+Tensor rotary_like(const Tensor& t) {
+  Tensor out = at::empty_like(t);
+  return out.stride(3) == 1 ? out : at::empty(t.sizes(), t.options());
+}
+
+tpf_rotary_shape rotary_shape(const Tensor& q, const Tensor& k, const Tensor& out_q, const Tensor& out_k,
+                              const Tensor& positions, const Tensor& freq, at::ScalarType wtype, bool norm,
+                              bool interleaved) {
+  tpf_rotary_shape s{};
+  s.B = q.size(0); s.N = q.size(2); s.H = q.size(1); s.Hk = k.size(1); s.D = q.size(3);
+  s.half = freq.defined() ? freq.numel() : 0;
+  s.dtype = type_code(q.scalar_type());
+  s.weight_dtype = type_code(wtype);
+  s.norm = norm;
+  s.interleaved = interleaved;
+  s.position_bits = 64;
+  if (positions.defined()) {
+    s.position_bits = positions.scalar_type() == at::kLong ? 64 : 32;
+    for (int i = 0; i < 2; ++i) s.position_stride[i] = positions.size(i) > 1 ? positions.stride(i) : 0;
+  }
+  strides3(q, s.q_stride);
+  strides3(k, s.k_stride);
+  strides3(out_q, s.out_q_stride);
+  strides3(out_k, s.out_k_stride);
+  return s;
+}
+
+variable_list rotary_forward(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& freq,
+                             const Tensor& qw, const Tensor& kw, const std::optional<double>& eps,
+                             bool interleaved) {
+  Tensor oq = rotary_like(q), ok = rotary_like(k);
+  const tpf_rotary_shape s =
+      rotary_shape(q, k, oq, ok, positions, freq, weight_type(qw, kw), eps.has_value(), interleaved);
+  check(tpf_rotary_forward(cptr(q), cptr(k), cptr(positions), (const double*)cptr(freq), cptr(qw), cptr(kw),
+                           eps.value_or(0.0), mptr(oq), mptr(ok), &s, stream()),
+        "tpf_rotary_forward");
+  return {oq, ok};
+}
+
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                               const std::optional<Tensor>& qw, const std::optional<Tensor>& kw,
+                               const std::optional<Tensor>& positions, const std::optional<Tensor>& freq,
+                               std::optional<double> eps, bool interleaved) {
+    const Tensor p = or_none(positions), f = or_none(freq), wq = or_none(qw), wk = or_none(kw);
+    variable_list out = rotary_forward(q, k, p, f, wq, wk, eps, interleaved);
+    ctx->save_for_backward({eps ? q : Tensor(), eps ? k : Tensor(), p, f, wq, wk});
+    ctx->saved_data["eps"] = eps.value_or(-1.0);
+    ctx->saved_data["inter"] = interleaved;
+    ctx->saved_data["want"] = (int64_t)((wq.defined() && wq.requires_grad() ? 1 : 0) |
+                                        (wk.defined() && wk.requires_grad() ? 2 : 0));
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    const Tensor &q = sv[0], &k = sv[1], &p = sv[2], &f = sv[3], &qw = sv[4], &kw = sv[5];
+    const double eps = ctx->saved_data["eps"].toDouble();
+    const int64_t want = ctx->saved_data["want"].toInt();
+    Tensor dy[2], dx[2], dw[2];
+    int64_t gs[6];
+    for (int i = 0; i < 2; ++i) {
+      const Tensor& g = grads[i];
+      dy[i] = g.stride(3) == 1 || g.size(3) == 1 ? g : g.contiguous();
+      dx[i] = rotary_like(sv[i].defined() ? sv[i] : dy[i]);
+      strides3(dy[i], gs + 3 * i);
+    }
+    const auto wtype = weight_type(qw, kw);
+    for (int i = 0; i < 2; ++i)
+      if (want >> i & 1) dw[i] = at::empty({dx[0].size(3)}, like(dx[0], wtype));
+    const tpf_rotary_shape s =
+        rotary_shape(q.defined() ? q : dy[0], k.defined() ? k : dy[1], dx[0], dx[1], p, f, wtype, eps >= 0.0,
+                     ctx->saved_data["inter"].toBool());
+    const int64_t n = want ? tpf_rotary_backward_workspace_bytes(&s) : 0;
+    const Tensor ws = bytes(dx[0], n);
+    check(tpf_rotary_backward(cptr(q), cptr(k), cptr(dy[0]), cptr(dy[1]), cptr(p), (const double*)cptr(f),
+                              cptr(qw), cptr(kw), eps >= 0.0 ? eps : 0.0, mptr(dx[0]), mptr(dx[1]),
+                              mptr(dw[0]), mptr(dw[1]), mptr(ws), n, &s, gs, stream()),
+          "tpf_rotary_backward");
+    return once({dx[0], dx[1], dw[0], dw[1], Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+std::optional<std::tuple<Tensor, Tensor>> qk_norm_rotary(
+    const Tensor& q, const Tensor& k, const std::optional<Tensor>& positions_in,
+    const std::optional<Tensor>& freq, const std::optional<Tensor>& qw, const std::optional<Tensor>& kw,
+    std::optional<double> eps, bool interleaved) {
+  if (transforms_active() || !q.is_cuda()) return std::nullopt;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  for (const Tensor* t : {&q, &k})
+    if (!plain(*t, dev) || t->dim() != 4 || t->numel() == 0 || t->scalar_type() != q.scalar_type() ||
+        t->stride(3) != 1)
+      return std::nullopt;
+  const int64_t B = q.size(0), N = q.size(2), D = q.size(3);
+  if (type_code(q.scalar_type()) < 0 || k.size(0) != B || k.size(2) != N || k.size(3) != D || D > 256 ||
+      !rotation_plain(D, freq, qw, kw, eps, dev))
+    return std::nullopt;
+  std::optional<Tensor> positions = positions_in;
+  if (positions) {
+    const auto pt = positions->scalar_type();
+    if (!plain(*positions, dev) || (pt != at::kInt && pt != at::kLong) || !broadcasts(positions->sizes(), {B, N}))
+      return std::nullopt;
+    if (positions->dim() != 2 || positions->size(0) != B || positions->size(1) != N)
+      positions = positions->expand({B, N});
+  }
+  bool grad = false;
+  for (const Tensor* t : {&q, &k}) grad = grad || t->requires_grad();
+  for (const auto* w : {&qw, &kw}) grad = grad || (*w && (*w)->requires_grad());
+  const variable_list out =
+      grad && at::GradMode::is_enabled()
+          ? RotaryFn::apply(q, k, qw, kw, positions, freq, eps, interleaved)
+          : rotary_forward(q, k, or_none(positions), or_none(freq), or_none(qw), or_none(kw), eps, interleaved);
+  return std::make_tuple(out[0], out[1]);
+}
+
+// ---------------------------------------------------------- window attention
+
+tpf_window_shape window_shape(const Tensor& q, const Tensor& k, const Tensor& v, int64_t mask_stride,
+                              int64_t window, int64_t sinks) {
+  tpf_window_shape s{q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), type_code(q.scalar_type()),
+                     window, sinks, mask_stride, {}, {}, {}};
+  strides3(q, s.q_stride);
+  strides3(k, s.k_stride);
+  strides3(v, s.v_stride);
+  return s;
+}
+
+Tensor window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask,
+                      const tpf_window_shape& s, double scale, Tensor* lse, Tensor* res) {
+  Tensor out = at::empty({s.B, s.N, s.H, s.D}, q.options());
+  if (lse) *lse = at::empty({s.B, s.H, s.N}, like(q, at::kFloat));
+  if (res) *res = at::empty_like(out);
+  const int64_t n = tpf_window_forward_workspace_bytes(&s);
+  const Tensor ws = bytes(q, n);
+  check(tpf_window_forward(cptr(q), cptr(k), cptr(v), cptr(mask), out.data_ptr(),
+                           lse ? (float*)lse->data_ptr() : nullptr, res ? res->data_ptr() : nullptr, mptr(ws), n,
+                           &s, scale, stream()),
+        "tpf_window_forward");
+  return out;
+}
+
+struct WindowFn : torch::autograd::Function<WindowFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const std::optional<Tensor>& mask_in, int64_t mask_stride, int64_t window,
+                        int64_t sinks, double scale, bool shadow) {
+    const Tensor mask = or_none(mask_in);
+    Tensor lse, res;
+    Tensor out = window_forward(q, k, v, mask, window_shape(q, k, v, mask_stride, window, sinks), scale, &lse,
+                                shadow ? &res : nullptr);
+    ctx->save_for_backward({q, k, v, mask, out, lse, res});
+    ctx->saved_data["stride"] = mask_stride;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    const Tensor &q = sv[0], &k = sv[1], &v = sv[2];
+    const tpf_window_shape s =
+        window_shape(q, k, v, ctx->saved_data["stride"].toInt(), ctx->saved_data["window"].toInt(),
+                     ctx->saved_data["sinks"].toInt());
+    const Tensor dout = kernel_grad(grads[0]);
+    Tensor d[3] = {grad_like(q), grad_like(k), grad_like(v)};
+    int64_t gs[9];
+    for (int i = 0; i < 3; ++i) strides3(d[i], gs + 3 * i);
+    const int64_t n = tpf_window_backward_workspace_bytes(&s);
+    const Tensor ws = bytes(q, n < 16 ? 16 : n);
+    check(tpf_window_backward_bf16(cptr(q), cptr(k), cptr(v), cptr(sv[3]), cptr(sv[4]), cptr(sv[6]), cptr(dout),
+                                   (const float*)cptr(sv[5]), mptr(d[0]), mptr(d[1]), mptr(d[2]), mptr(ws), n,
+                                   &s, gs, ctx->saved_data["scale"].toDouble(), stream()),
+          "tpf_window_backward_bf16");
+    return once({d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+// window 0: none.  sh: the policy variable of the shadow residual (env_flag).
+std::optional<Tensor> window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
+                                       int64_t sinks, const std::optional<Tensor>& mask,
+                                       std::optional<double> scale_in, const std::string& sh) {
+  if (transforms_active() || !q.is_cuda()) return std::nullopt;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  for (const Tensor* t : {&q, &k, &v})
+    if (!plain(*t, dev) || t->dim() != 4 || t->numel() == 0 || t->scalar_type() != q.scalar_type())
+      return std::nullopt;
+  const auto type = q.scalar_type();
+  const bool grad = at::GradMode::is_enabled() &&
+                    (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  if (type != at::kBFloat16 && (type != at::kHalf || grad)) return std::nullopt;
+  if (grad && sh != "0" && sh != "1") return std::nullopt;
+  const int64_t B = q.size(0), N = q.size(2), D = q.size(3);
+  if (k.sizes() != v.sizes() || k.size(0) != B || k.size(2) != N || k.size(3) != D || D % 8 || D > 128 ||
+      q.size(1) % k.size(1))
+    return std::nullopt;
+  for (const Tensor* t : {&q, &k, &v})
+    if (!xattn_operand(*t)) return std::nullopt;
+  const double scale = scale_in ? *scale_in : 1.0 / std::sqrt((double)D);
+  if (!(scale > 1e-30 && scale < 1e30)) return std::nullopt;
+  int64_t mask_stride = 0;
+  if (mask) {
+    if (!plain(*mask, dev) || mask->scalar_type() != at::kBool || !mask->is_contiguous() || mask->dim() < 1 ||
+        mask->dim() > 2 || mask->size(-1) != N ||
+        (mask->dim() == 2 && mask->size(0) != B && mask->size(0) != 1))
+      return std::nullopt;
+    mask_stride = mask->dim() == 2 && mask->size(0) > 1 ? N : 0;
+  }
+  // Sizes that the launches do not hold (of the backward too, before the forward).
+  const tpf_window_shape s = window_shape(q, k, v, mask_stride, window, sinks);
+  if (tpf_window_forward_workspace_bytes(&s) < 0 || (grad && tpf_window_backward_workspace_bytes(&s) < 0))
+    return std::nullopt;
+  if (grad) return WindowFn::apply(q, k, v, mask, mask_stride, window, sinks, scale, sh == "1");
+  return window_forward(q, k, v, or_none(mask), s, scale, nullptr, nullptr);
+}
+
+// -------------------------------------------------------------- paged cache
+
+// The batch over a cache [pages, Hk, page, D] (checked when it was made) with T new tokens.
+std::optional<tpf_paged_batch> paged_batch(const Tensor& ck, const Tensor& tables, const Tensor& starts,
+                                           const Tensor& lengths, int64_t T, c10::DeviceIndex dev) {
+  for (const Tensor* t : {&tables, &starts, &lengths})
+    if (!plain(*t, dev) || t->scalar_type() != at::kInt || (t->numel() && t->stride(-1) != 1))
+      return std::nullopt;
+  if (tables.dim() != 2 || starts.dim() != 1 || lengths.dim() != 1) return std::nullopt;
+  const int64_t S = lengths.size(0), width = tables.size(1);
+  if (S < 1 || width < 1 || tables.size(0) != S || starts.size(0) != S + 1 || T < 1 || T >= (1 << 30) ||
+      width > (1 << 30) / ck.size(2))
+    return std::nullopt;
+  return tpf_paged_batch{(const int32_t*)cptr(tables), (const int32_t*)cptr(starts), (const int32_t*)cptr(lengths),
+                         S, T, width, S > 1 ? tables.stride(0) : width, ck.size(2), ck.size(0)};
+}
+// New tokens [T, heads, D] of the cache's type that a call without gradients takes.
+bool tokens_plain(const Tensor& t, const Tensor& ck, int64_t T, c10::DeviceIndex dev) {
+  return plain(t, dev) && t.dim() == 3 && t.size(0) == T && t.size(1) > 0 && t.size(2) == ck.size(3) &&
+         t.scalar_type() == ck.scalar_type() && t.stride(2) == 1 &&
+         !(t.requires_grad() && at::GradMode::is_enabled());
+}
+void strides2(const Tensor& t, int64_t* out) {
+  for (int i = 0; i < 2; ++i) out[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+std::optional<Tensor> append_kv(const Tensor& ck, const Tensor& cv, const Tensor& k, const Tensor& v,
+                                const Tensor& tables, const Tensor& starts, const Tensor& lengths,
+                                const std::optional<Tensor>& q, const std::optional<Tensor>& freq,
+                                const std::optional<Tensor>& qw, const std::optional<Tensor>& kw,
+                                std::optional<double> eps, bool interleaved) {
+  if (transforms_active() || !k.is_cuda() || k.dim() != 3) return std::nullopt;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  const int64_t T = k.size(0), Hk = ck.size(1), D = ck.size(3);
+  if (!plain(ck, dev) || !plain(cv, dev) || !tokens_plain(k, ck, T, dev) || !tokens_plain(v, ck, T, dev) ||
+      k.size(1) != Hk || v.size(1) != Hk || (q && !tokens_plain(*q, ck, T, dev)) ||
+      !rotation_plain(D, freq, qw, kw, eps, dev))
+    return std::nullopt;
+  for (const auto* w : {&qw, &kw})
+    if (*w && (*w)->requires_grad() && at::GradMode::is_enabled()) return std::nullopt;
+  const auto batch = paged_batch(ck, tables, starts, lengths, T, dev);
+  if (!batch) return std::nullopt;
+  const Tensor f = or_none(freq), wq = or_none(qw), wk = or_none(kw);
+  const int64_t H = q ? q->size(1) : 0;
+  Tensor out = at::empty({T, H, D}, k.options());
+  tpf_append_shape s{H, Hk, D, f.defined() ? f.numel() : 0, type_code(k.scalar_type()),
+                     type_code(weight_type(wq, wk)), eps.has_value(), interleaved, {}, {}, {}};
+  if (q) strides2(*q, s.q_stride);
+  strides2(k, s.k_stride);
+  strides2(v, s.v_stride);
+  check(tpf_paged_append(q ? cptr(*q) : nullptr, cptr(k), cptr(v), (const double*)cptr(f), cptr(wq), cptr(wk),
+                         eps.value_or(0.0), out.data_ptr(), ck.data_ptr(), cv.data_ptr(), &s, &*batch, stream()),
+        "tpf_paged_append");
+  for (const Tensor* t : {&ck, &cv})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
+// window 0: none.
+std::optional<Tensor> paged_attention(const Tensor& q, const Tensor& ck, const Tensor& cv, const Tensor& tables,
+                                      const Tensor& starts, const Tensor& lengths, int64_t window,
+                                      int64_t sinks, std::optional<double> scale_in) {
+  if (transforms_active() || !q.is_cuda() || q.dim() != 3) return std::nullopt;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  const int64_t T = q.size(0), Hk = ck.size(1), D = ck.size(3);
+  if (!plain(ck, dev) || !plain(cv, dev) || !tokens_plain(q, ck, T, dev) || q.size(1) % Hk || !aligned16(q) ||
+      (T > 1 && q.stride(0) % 8) || (q.size(1) > 1 && q.stride(1) % 8))
+    return std::nullopt;
+  const double scale = scale_in ? *scale_in : 1.0 / std::sqrt((double)D);
+  if (!(scale > 1e-30 && scale < 1e30)) return std::nullopt;
+  const auto batch = paged_batch(ck, tables, starts, lengths, T, dev);
+  if (!batch) return std::nullopt;
+  tpf_paged_shape s{q.size(1), Hk, D, type_code(q.scalar_type()), window, sinks, {}};
+  strides2(q, s.q_stride);
+  const int64_t n = tpf_paged_attention_workspace_bytes(&s, &*batch);
+  if (n < 0) return std::nullopt;
+  Tensor out = at::empty(q.sizes(), q.options());
+  const Tensor ws = bytes(q, n);
+  check(tpf_paged_attention(cptr(q), cptr(ck), cptr(cv), out.data_ptr(), mptr(ws), n, &s, &*batch, scale,
+                            stream()),
+        "tpf_paged_attention");
+  return out;
+}
+
 // ---------------------------------------------------------------- layer norm
 
 // Rows x2 [R, C]; what a backward needs of `keep` (0 nothing, 1 the rows, 2 the
@@ -738,6 +1060,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     pybind11::gil_scoped_release nogil;
     return cross_attention(q, k, v, mask, scale, shadow);
   });
+  m.def("window_attention", [](const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
+                               int64_t sinks, const std::optional<Tensor>& mask,
+                               std::optional<double> scale) {
+    const std::string shadow = env_flag("TURBOPAIRFORMER_SR_SHADOW", "OPENFOLD3_SR_SHADOW");
+    pybind11::gil_scoped_release nogil;
+    return window_attention(q, k, v, window, sinks, mask, scale, shadow);
+  });
+  m.def("qk_norm_rotary", &qk_norm_rotary, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("append_kv", &append_kv, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("paged_attention", &paged_attention, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("layer_norm", &layer_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("act8_pack", &act8_pack, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("act8_unpack", &act8_unpack, pybind11::call_guard<pybind11::gil_scoped_release>());

@@ -461,11 +461,13 @@ __global__ __launch_bounds__(256) void rot_fold_kernel(const float* part, int gr
   else ((u16*)out)[c] = f2bf_bits(v);
 }
 
-// Waves enough to fill the chip (32 a CU), as long as a token's heads divide.
-static void rot_plan(RotArgs& r, int rows_per_wave) {
+// A token's heads are shared by waves as long as there are fewer than 16384 (8192 backward,
+// whose workgroups take several tokens): 2 x 4096 tokens, 32 + 8 heads of 128 in 40 us forward
+// against 45 with 8192 and 43 with 40960; backward 71 against 79 with 16384.
+static void rot_plan(RotArgs& r, int rows_per_wave, bool backward) {
   const int total = r.heads[0] + r.heads[1] + r.heads[2];
   const int most = (total + rows_per_wave - 1) / rows_per_wave;
-  int64_t s = (8192 + r.tokens - 1) / r.tokens;
+  int64_t s = ((backward ? 8192 : 16384) + r.tokens - 1) / r.tokens;
   r.slices = (int)(s < 1 ? 1 : s > most ? most : s);
   r.div_slices = make_fastdiv((uint32_t)r.slices);
   r.div_n = make_fastdiv((uint32_t)r.N);
@@ -477,7 +479,9 @@ static int rot_lanes(const RotArgs& r) {
   return l;
 }
 
-constexpr int64_t kRotGroups = 1024;  // workgroups of a backward
+// Workgroups of a backward: three a CU, as many as its registers let run (the same tokens: 71 us
+// against 87 with 1024, a third of which had to wait).
+constexpr int64_t kRotGroups = 768;
 
 static int64_t rot_groups(const RotArgs& r) {
   const int64_t n = (r.tokens * r.slices + 3) / 4;
@@ -518,7 +522,7 @@ static void rot_run(const RotArgs& r, int64_t type, int mode, int w, hipStream_t
 // Sizes of a call into r; 0 or an error code.
 static int rot_check(RotArgs& r, int64_t B, int64_t N, int64_t H, int64_t Hk, int64_t Hv, int64_t D,
                      int64_t half, int64_t type, int64_t w_type, double eps, int norm,
-                     int inter, const char* fn) {
+                     int inter, bool backward, const char* fn) {
   const int64_t lim = (int64_t)1 << 30;
   if (B < 1 || N < 1 || B > lim || N > lim || H < 0 || Hk < 0 || H + Hk < 1 || H > 65535 || Hk > 65535 ||
       D < 1 || D > 256 || half < 0 || 2 * half > D)
@@ -538,7 +542,7 @@ static int rot_check(RotArgs& r, int64_t B, int64_t N, int64_t H, int64_t Hk, in
   r.norm = norm;
   r.eps = (float)eps;
   r.w_type = (int)w_type;
-  rot_plan(r, 64 / rot_lanes(r));
+  rot_plan(r, 64 / rot_lanes(r), backward);
   if ((double)B * (double)N * r.slices >= 4.0 * (double)((int64_t)1 << 24))
     return set_error(TPF_ERR_SHAPE, "%s: too many tokens", fn);
   return TPF_OK;
@@ -556,10 +560,10 @@ static int rot_width(const RotArgs& r, int64_t type, int w, const void* p, const
 
 static int rot_entry(tpf::RotArgs& r, const tpf_rotary_shape* s, const void* positions,
                      const double* frequencies, const void* qw, const void* kw, double eps,
-                     const char* fn) {
+                     bool backward, const char* fn) {
   if (!s) return tpf::set_error(TPF_ERR_ARG, "%s: null shape", fn);
   if (int rc = tpf::rot_check(r, s->B, s->N, s->H, s->Hk, 0, s->D, s->half, s->dtype, s->weight_dtype, eps,
-                              s->norm != 0, s->interleaved != 0, fn))
+                              s->norm != 0, s->interleaved != 0, backward, fn))
     return rc;
   if (s->half && !frequencies) return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
   if (s->position_bits != 32 && s->position_bits != 64)
@@ -586,7 +590,7 @@ extern "C" int tpf_rotary_forward(const void* q, const void* k, const void* posi
                                   const tpf_rotary_shape* shape, void* stream) {
   const char* fn = "tpf_rotary_forward";
   tpf::RotArgs r{};
-  if (int rc = rot_entry(r, shape, positions, frequencies, q_weight, k_weight, eps, fn)) return rc;
+  if (int rc = rot_entry(r, shape, positions, frequencies, q_weight, k_weight, eps, false, fn)) return rc;
   if ((shape->H && (!q || !q_out)) || (shape->Hk && (!k || !k_out)))
     return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
   r.x[0] = q; r.x[1] = k; r.y[0] = q_out; r.y[1] = k_out;
@@ -602,7 +606,7 @@ extern "C" int tpf_rotary_forward(const void* q, const void* k, const void* posi
 
 extern "C" int64_t tpf_rotary_backward_workspace_bytes(const tpf_rotary_shape* shape) {
   tpf::RotArgs r{};
-  if (rot_entry(r, shape, nullptr, (const double*)16, nullptr, nullptr, 0.0,
+  if (rot_entry(r, shape, nullptr, (const double*)16, nullptr, nullptr, 0.0, true,
                 "tpf_rotary_backward_workspace_bytes"))
     return -1;
   return tpf::rot_groups(r) * 2 * r.D * 4;
@@ -616,7 +620,7 @@ extern "C" int tpf_rotary_backward(const void* q, const void* k, const void* dq_
                                    const int64_t* grad_strides, void* stream) {
   const char* fn = "tpf_rotary_backward";
   tpf::RotArgs r{};
-  if (int rc = rot_entry(r, shape, positions, frequencies, q_weight, k_weight, eps, fn)) return rc;
+  if (int rc = rot_entry(r, shape, positions, frequencies, q_weight, k_weight, eps, true, fn)) return rc;
   if (!grad_strides || (shape->H && (!dq_out || !dq || (r.norm && !q))) ||
       (shape->Hk && (!dk_out || !dk || (r.norm && !k))))
     return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
@@ -690,7 +694,7 @@ extern "C" int tpf_paged_append(const void* q, const void* k, const void* v, con
     return tpf::set_error(TPF_ERR_ARG, "%s: dtype must be TPF_BF16 or TPF_F16", fn);
   if (s->Hk < 1) return tpf::set_error(TPF_ERR_SHAPE, "%s: no kv heads", fn);
   if (int rc = tpf::rot_check(r, 1, batch->T, s->H, s->Hk, s->Hk, s->D, s->half, s->dtype, s->weight_dtype,
-                              eps, s->norm != 0, s->interleaved != 0, fn))
+                              eps, s->norm != 0, s->interleaved != 0, false, fn))
     return rc;
   if (!k || !v || !k_cache || !v_cache || (s->H && (!q || !q_out)) || (s->half && !frequencies))
     return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);

@@ -19,9 +19,10 @@ import math
 import torch
 
 from . import _native
+from .activations import host_path
 from .attention import _device_supported
 from .rotary import _weight_type, check_rotation, rotation_operands
-from .window_attention import check_limits, limits
+from .window_attention import check_limits, host_limits, limits
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # TPF_BF16, TPF_F16
 _MAX_HEAD_DIM = 128
@@ -32,7 +33,7 @@ class PagedCache:
     """``pages`` pages of ``page`` states: ``k`` and ``v`` are [pages, kv_heads, page,
     head_dim], BF16 or FP16 (head_dim a multiple of 8 up to 128)."""
 
-    __slots__ = ("k", "v")
+    __slots__ = ("_k", "_v")
 
     def __init__(self, pages: int, kv_heads: int, page: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -62,7 +63,15 @@ class PagedCache:
                              "that is a multiple of 8 up to 128")
         if k.numel() // D > _MAX_STATES:
             raise ValueError("a cache holds 2^30 states of all kv heads at most")
-        self.k, self.v = k, v
+        self._k, self._v = k, v
+
+    @property
+    def k(self) -> torch.Tensor:
+        return self._k
+
+    @property
+    def v(self) -> torch.Tensor:
+        return self._v
 
     @property
     def pages(self) -> int:
@@ -172,6 +181,15 @@ def append_kv(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, tables: torch
     they hold.  No two sequences may append to one page.  Other cases raise
     ``ValueError`` before any launch.
     """
+    if (type(cache) is PagedCache
+            and host_path(k, v, tables, starts, lengths, *(
+                t for t in (q, frequencies, q_weight, k_weight) if t is not None))
+            and (eps is None or type(eps) is float)):
+        # The common form entirely in C++; None (nothing launched) for any other.
+        out = _native.host().append_kv(cache._k, cache._v, k, v, tables, starts, lengths, q, frequencies,
+                                       q_weight, k_weight, eps, bool(interleaved))
+        if out is not None:
+            return None if q is None else out
     tokens = [("k", k, None), ("v", v, None)] + ([] if q is None else [("q", q, None)])
     if isinstance(cache, PagedCache):
         tokens[0], tokens[1] = ("k", k, cache.kv_heads), ("v", v, cache.kv_heads)
@@ -241,6 +259,13 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, st
     [T, H, D], contiguous: a row that sees no state, or is of no sequence, is zeros.  Other
     cases raise ``ValueError`` before any launch.
     """
+    if (type(cache) is PagedCache and host_path(q, tables, starts, lengths)
+            and host_limits(window, sinks, scale)):
+        # The common form entirely in C++; None (nothing launched) for any other.
+        out = _native.host().paged_attention(q, cache._k, cache._v, tables, starts, lengths, window or 0,
+                                             sinks, scale)
+        if out is not None:
+            return out
     check_batch(_attention_unsupported, cache, tables, starts, lengths, [("q", q, None)])
     check_limits(_attention_unsupported, window, sinks, scale)
     if q.shape[1] < 1 or q.shape[1] % cache.kv_heads:

@@ -18,7 +18,7 @@ import numbers
 import torch
 
 from . import _native
-from .activations import _DTYPES, differentiable_once
+from .activations import _DTYPES, differentiable_once, host_path
 from .attention import _device_supported
 
 _MAX_HEAD_DIM = 256
@@ -202,6 +202,13 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | N
     and products are in 32 bits.  Gradients: q, k and the weights.  Other cases raise
     ``ValueError`` before any launch.
     """
+    if (host_path(q, k, *(t for t in (positions, frequencies, q_weight, k_weight) if t is not None))
+            and (eps is None or type(eps) is float)):
+        # The common form entirely in C++; None (nothing launched) for any other.
+        out = _native.host().qk_norm_rotary(q, k, positions, frequencies, q_weight, k_weight, eps,
+                                            bool(interleaved))
+        if out is not None:
+            return out
     _check(q, k, positions, frequencies, q_weight, k_weight, eps)
     if q.numel() + k.numel() == 0:
         edge = sum(w.reshape(-1)[:0].sum() for w in (q_weight, k_weight) if w is not None)

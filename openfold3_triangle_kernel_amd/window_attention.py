@@ -18,7 +18,7 @@ import numbers
 import torch
 
 from . import _native
-from .activations import differentiable_once
+from .activations import differentiable_once, host_path
 from .attention import _device_supported, shadow_enabled
 from .cross_attention import _grad_like, _operand, _strides
 
@@ -39,6 +39,12 @@ def check_limits(unsupported, window, sinks, scale) -> None:
         raise unsupported("sinks must be a whole number from 0 on")
     if scale is not None and not (isinstance(scale, numbers.Real) and 1e-30 < scale < 1e30):
         raise unsupported("scale must be a number between 1e-30 and 1e30")
+
+
+def host_limits(window, sinks, scale) -> bool:
+    """Whether these arguments are of the kinds that the C++ host path takes."""
+    return ((window is None or type(window) is int and 0 < window < 1 << 31) and type(sinks) is int
+            and 0 <= sinks < 1 << 31 and (scale is None or type(scale) is float))
 
 
 def limits(window, sinks) -> tuple[int, int]:
@@ -183,6 +189,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     to a multiple of 8 where it is none).  Other cases raise ``ValueError`` before any
     launch.
     """
+    if (host_path(q, k, v) and (key_mask is None or _native.host_eligible(key_mask))
+            and host_limits(window, sinks, scale)):
+        # The common form entirely in C++; None (nothing launched) for any other.
+        out = _native.host().window_attention(q, k, v, window or 0, sinks, key_mask, scale)
+        if out is not None:
+            return out
     _check(q, k, v, window, sinks, key_mask, scale)
     head_dim = q.shape[-1]
     if scale is None:
