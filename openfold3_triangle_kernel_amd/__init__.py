@@ -93,3 +93,7 @@ __all__ += ["window_attention"]
 from .paged import PagedCache, append_kv, paged_attention  # noqa: E402
 
 __all__ += ["PagedCache", "append_kv", "paged_attention"]
+
+from .self_block import SelfAttention  # noqa: E402
+
+__all__ += ["SelfAttention"]

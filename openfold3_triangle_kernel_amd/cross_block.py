@@ -26,35 +26,9 @@ from .cross_attention import additive_f32, cross_attention
 from .layernorm import layer_norm
 
 
-class CrossAttention(nn.Module):
-    """Cross attention with ``no_heads`` query heads of ``c_hidden`` channels on
-    ``no_kv_heads`` kv heads (default: as many).
-
-    ``activation_save`` is what the norms and projections keep for the backward:
-    ``"int8"`` (8 bits a value) or ``"full"``.  For single tokens, ``project_states``
-    forms the states' keys and values once and ``forward`` takes them as ``states``.
-    """
-
-    def __init__(self, c_q: int, c_kv: int, c_hidden: int, no_heads: int,
-                 no_kv_heads: int | None = None, gating: bool = True,
-                 activation_save: str = "int8", eps: float = 1e-5):
-        super().__init__()
-        no_kv_heads = no_heads if no_kv_heads is None else no_kv_heads
-        if min(c_q, c_kv, c_hidden, no_heads, no_kv_heads) < 1 or no_heads % no_kv_heads:
-            raise ValueError("sizes must be positive, the query heads a multiple of the kv heads")
-        if activation_save not in ("int8", "full"):
-            raise ValueError('activation_save must be "int8" or "full"')
-        self.c_q, self.c_kv, self.c_hidden = c_q, c_kv, c_hidden
-        self.no_heads, self.no_kv_heads = no_heads, no_kv_heads
-        self.activation_save, self.eps = activation_save, eps
-        self.layer_norm_q = nn.LayerNorm(c_q, eps=eps)
-        self.layer_norm_kv = nn.LayerNorm(c_kv, eps=eps)
-        hc, kc = no_heads * c_hidden, no_kv_heads * c_hidden
-        self.linear_q = nn.Linear(c_q, hc, bias=False)
-        self.linear_k = nn.Linear(c_kv, kc, bias=False)
-        self.linear_v = nn.Linear(c_kv, kc, bias=False)
-        self.linear_g = nn.Linear(c_q, hc, bias=False) if gating else None
-        self.linear_o = nn.Linear(hc, c_q, bias=False)
+class AttentionBlock(nn.Module):
+    """What the attention blocks share: the routing policy, the norms and the projections.
+    ``_widths`` are the channel counts of the streams."""
 
     def _supported(self, *tensors) -> tuple[bool, str]:
         for t in tensors:
@@ -63,7 +37,7 @@ class CrossAttention(nn.Module):
             ok, reason = _device_supported(t)
             if not ok:
                 return False, reason
-        if self.c_q % 8 or self.c_kv % 8 or self.c_hidden % 8 or self.c_hidden > 128:
+        if any(c % 8 for c in (*self._widths, self.c_hidden)) or self.c_hidden > 128:
             return False, "channel counts must be multiples of 8 and c_hidden at most 128"
         if any(p.dtype not in (torch.bfloat16, torch.float32) or p.device != tensors[0].device
                for p in self.parameters()):
@@ -91,6 +65,38 @@ class CrossAttention(nn.Module):
 
     def _heads(self, t: torch.Tensor) -> torch.Tensor:
         return t.unflatten(-1, (-1, self.c_hidden)).transpose(-2, -3)  # [*, heads, N, c_hidden]
+
+
+class CrossAttention(AttentionBlock):
+    """Cross attention with ``no_heads`` query heads of ``c_hidden`` channels on
+    ``no_kv_heads`` kv heads (default: as many).
+
+    ``activation_save`` is what the norms and projections keep for the backward:
+    ``"int8"`` (8 bits a value) or ``"full"``.  For single tokens, ``project_states``
+    forms the states' keys and values once and ``forward`` takes them as ``states``.
+    """
+
+    def __init__(self, c_q: int, c_kv: int, c_hidden: int, no_heads: int,
+                 no_kv_heads: int | None = None, gating: bool = True,
+                 activation_save: str = "int8", eps: float = 1e-5):
+        super().__init__()
+        no_kv_heads = no_heads if no_kv_heads is None else no_kv_heads
+        if min(c_q, c_kv, c_hidden, no_heads, no_kv_heads) < 1 or no_heads % no_kv_heads:
+            raise ValueError("sizes must be positive, the query heads a multiple of the kv heads")
+        if activation_save not in ("int8", "full"):
+            raise ValueError('activation_save must be "int8" or "full"')
+        self.c_q, self.c_kv, self.c_hidden = c_q, c_kv, c_hidden
+        self._widths = (c_q, c_kv)
+        self.no_heads, self.no_kv_heads = no_heads, no_kv_heads
+        self.activation_save, self.eps = activation_save, eps
+        self.layer_norm_q = nn.LayerNorm(c_q, eps=eps)
+        self.layer_norm_kv = nn.LayerNorm(c_kv, eps=eps)
+        hc, kc = no_heads * c_hidden, no_kv_heads * c_hidden
+        self.linear_q = nn.Linear(c_q, hc, bias=False)
+        self.linear_k = nn.Linear(c_kv, kc, bias=False)
+        self.linear_v = nn.Linear(c_kv, kc, bias=False)
+        self.linear_g = nn.Linear(c_q, hc, bias=False) if gating else None
+        self.linear_o = nn.Linear(hc, c_q, bias=False)
 
     def project_states(self, states: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values ``[*, no_kv_heads, Nk, c_hidden]`` of ``states`` ``[*, Nk, c_kv]``."""

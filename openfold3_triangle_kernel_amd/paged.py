@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _native
-from .activations import host_path
+from .activations import _DTYPES as _WEIGHT_DTYPES, host_path
 from .attention import _device_supported
 from .rotary import _weight_type, check_rotation, rotation_operands
 from .window_attention import check_limits, host_limits, limits
@@ -128,10 +128,10 @@ def check_batch(unsupported, cache, tables, starts, lengths, tokens) -> None:
         raise unsupported("too many tokens")
 
 
-def batch_struct(cache, tables, starts, lengths, T: int) -> _Batch:
+def batch_struct(k_cache, tables, starts, lengths, T: int) -> _Batch:
     S, width = tables.shape
     return _Batch(_native.ptr(tables), _native.ptr(starts), _native.ptr(lengths), S, T, width,
-                  tables.stride(0) if S > 1 else width, cache.page, cache.pages)
+                  tables.stride(0) if S > 1 else width, k_cache.shape[2], k_cache.shape[0])
 
 
 def _append_unsupported(reason: str):
@@ -143,20 +143,20 @@ class _AppendFn(torch.autograd.Function):
     would hide, are refused."""
 
     @staticmethod
-    def forward(ctx, q, k, v, cache, tables, starts, lengths, freq, qw, kw, eps, interleaved):
+    def forward(ctx, q, k, v, k_cache, v_cache, tables, starts, lengths, freq, qw, kw, eps, interleaved):
         T, Hk, D = k.shape
         H = 0 if q is None else q.shape[1]
-        out = k.new_empty((T, H, D))
+        out = torch.empty((T, H, D), device=k.device, dtype=k.dtype)
         strides = [s if n > 1 else 0 for t in (k if q is None else q, k, v)
                    for n, s in zip(t.shape[:2], t.stride())]
         shape = _AppendShape(H, Hk, D, 0 if freq is None else len(freq), _DTYPES[k.dtype],
-                             {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[_weight_type(qw, kw)],
+                             _WEIGHT_DTYPES[_weight_type(qw, kw)],
                              int(eps is not None), int(interleaved), *strides)
         ptr = _native.ptr
         with _native.device_ctx(k.device):
             _native.call("tpf_paged_append", ptr(q), ptr(k), ptr(v), ptr(freq), ptr(qw), ptr(kw),
-                         0.0 if eps is None else eps, ptr(out), ptr(cache.k), ptr(cache.v), shape,
-                         ctypes.byref(batch_struct(cache, tables, starts, lengths, T)),
+                         0.0 if eps is None else eps, ptr(out), ptr(k_cache), ptr(v_cache), shape,
+                         ctypes.byref(batch_struct(k_cache, tables, starts, lengths, T)),
                          _native.stream_of(k))
         ctx.mark_non_differentiable(out)
         return out
@@ -205,7 +205,7 @@ def append_kv(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, tables: torch
         return None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
     freq, qw, kw = rotation_operands(frequencies, q_weight, k_weight)
     q, k, v = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
-    out = _AppendFn.apply(q, k, v, cache, tables, starts, lengths, freq, qw, kw,
+    out = _AppendFn.apply(q, k, v, cache.k, cache.v, tables, starts, lengths, freq, qw, kw,
                           None if eps is None else float(eps), bool(interleaved))
     for t in (cache.k, cache.v):
         if not t.is_inference():
@@ -225,19 +225,19 @@ class _PagedFn(torch.autograd.Function):
     would hide, are refused."""
 
     @staticmethod
-    def forward(ctx, q, cache, tables, starts, lengths, window, sinks, scale):
+    def forward(ctx, q, k_cache, v_cache, tables, starts, lengths, window, sinks, scale):
         T, H, D = q.shape
-        out = q.new_empty((T, H, D))
+        out = torch.empty((T, H, D), device=q.device, dtype=q.dtype)
         strides = (s if n > 1 else 0 for n, s in zip(q.shape[:2], q.stride()))
-        shape = _PagedShape(H, cache.kv_heads, D, _DTYPES[q.dtype], window, sinks, *strides)
-        batch = ctypes.byref(batch_struct(cache, tables, starts, lengths, T))
+        shape = _PagedShape(H, k_cache.shape[1], D, _DTYPES[q.dtype], window, sinks, *strides)
+        batch = ctypes.byref(batch_struct(k_cache, tables, starts, lengths, T))
         ws_bytes = int(_native.query("tpf_paged_attention_workspace_bytes", shape, batch))
         if ws_bytes < 0:
             raise _attention_unsupported(_native.query("tpf_last_error").decode(errors="replace"))
         ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes > 0 else None
         ptr = _native.ptr
         with _native.device_ctx(q.device):
-            _native.call("tpf_paged_attention", ptr(q), ptr(cache.k), ptr(cache.v), ptr(out), ptr(ws),
+            _native.call("tpf_paged_attention", ptr(q), ptr(k_cache), ptr(v_cache), ptr(out), ptr(ws),
                          ws_bytes, shape, batch, scale, _native.stream_of(q))
         ctx.mark_non_differentiable(out)
         return out
@@ -279,7 +279,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, st
             or any(n > 1 and s % 8 for n, s in zip(q.shape[:2], q.stride()))):
         q = q.clone(memory_format=torch.contiguous_format)
     scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
-    return _PagedFn.apply(q, cache, tables, starts, lengths, *limits(window, sinks), scale)
+    return _PagedFn.apply(q, cache.k, cache.v, tables, starts, lengths, *limits(window, sinks), scale)
 
 
 __all__ = ["PagedCache", "append_kv", "paged_attention"]

@@ -60,7 +60,7 @@ def rotation_operands(frequencies, q_weight, k_weight):
     """(frequencies in 64 bits or None, the weights, contiguous and of one type)."""
     if frequencies is not None:
         frequencies = frequencies.to(torch.float64).contiguous() if len(frequencies) else None
-    q_weight, k_weight = (None if w is None else w.detach().contiguous() for w in (q_weight, k_weight))
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         q_weight, k_weight = q_weight.float(), k_weight.float()
     return frequencies, q_weight, k_weight
@@ -215,7 +215,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | N
         return tuple(t.clone() if isinstance(edge, int) else t + edge.to(t.dtype) for t in (q, k))
     prefix, N = q.shape[:-3], q.shape[-2]
     batch = math.prod(prefix)
-    if positions is not None and len(prefix) != 1 or positions is not None and positions.shape != (batch, N):
+    if positions is not None:
         positions = positions.expand(tuple(prefix) + (N,)).reshape(batch, N)
     freq, qw, kw = rotation_operands(frequencies, q_weight, k_weight)
     q4, k4 = (t if t.ndim == 4 else t.reshape((batch,) + t.shape[-3:]) for t in (q, k))
@@ -224,6 +224,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | N
     grad = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
     if grad:
+        qw, kw = (None if w is None else w.detach() for w in (qw, kw))
         out = _RotaryFn.apply(q4, k4, q_weight, k_weight, positions, freq, qw, kw, eps, bool(interleaved))
     else:
         out = _RotaryInference.apply(q4, k4, positions, freq, qw, kw, eps, bool(interleaved))

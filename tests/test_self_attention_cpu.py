@@ -96,7 +96,7 @@ def test_places_of_a_cache():
     """``tpf_paged_row`` on host arrays: the rule that the kernels share."""
     cache, _, tables, starts, lengths = _paged(S=3, width=3, page=4, pages=7)
     tables.copy_(torch.tensor([[6, 0, 3], [7, -1, 2], [1, 2 ** 31 - 1, 5]]))
-    batch = batch_struct(cache, tables, starts, lengths, 5)
+    batch = batch_struct(cache.k, tables, starts, lengths, 5)
     row = lambda s, j: _native.query("tpf_paged_row", ctypes.byref(batch), s, j)  # noqa: E731
     for s in range(3):
         for j in range(12):
@@ -126,7 +126,7 @@ def test_c_abi_answers_before_a_launch():
     shape[4] = 257
     assert _native.query("tpf_rotary_backward_workspace_bytes", shape) == -1
     cache, x, tables, starts, lengths = _paged()
-    batch = batch_struct(cache, tables, starts, lengths, 3)
+    batch = batch_struct(cache.k, tables, starts, lengths, 3)
     append = (ctypes.c_int64 * 14)(0, 2, 16, 0, 2, 2)
     with pytest.raises(RuntimeError, match="TPF_BF16 or TPF_F16"):
         _native.call("tpf_paged_append", None, 16, 16, None, None, None, 0.0, None, 16, 16, append,
@@ -206,7 +206,7 @@ def test_attention_c_abi_answers_before_a_launch():
     with pytest.raises(RuntimeError, match="workspace"):
         call(fn="tpf_window_backward_bf16")
     cache, x, tables, starts, lengths = _paged()
-    batch = batch_struct(cache, tables, starts, lengths, 3)
+    batch = batch_struct(cache.k, tables, starts, lengths, 3)
     paged = (ctypes.c_int64 * 8)(4, 2, 16, 0, 0, 0, 64, 16)
     size = lambda s=paged: q("tpf_paged_attention_workspace_bytes", s, ctypes.byref(batch))  # noqa: E731
     assert size() == 0
@@ -218,3 +218,95 @@ def test_attention_c_abi_answers_before_a_launch():
         assert size(bad) == -1
     batch.pages = 1 << 25
     assert size() == -1
+
+
+def test_block_on_the_cpu():
+    """The block's formulas in PyTorch: masks, windows, empty rows, the routing policy."""
+    from openfold3_triangle_kernel_amd import (SelfAttention, set_turbopairformer_strict,
+                                               stock_invocation_count)
+
+    torch.manual_seed(0)
+    block = SelfAttention(24, 8, 4, 2, window=3, sinks=1)
+    x = torch.randn(2, 6, 24, requires_grad=True)
+    before = stock_invocation_count()
+    out = block(x)
+    assert stock_invocation_count() == before + 1 and out.shape == x.shape
+    # A token that nothing later sees changes nothing later; all see the first one.
+    for at, seen_by in ((0, range(6)), (2, (2, 3, 4)), (5, (5,))):
+        other = x.detach().clone()
+        other[:, at, :12] += 1.0  # (the norm takes out what all channels share)
+        changed = (block(other) - out).abs().amax((0, 2)) > 1e-6
+        assert changed.tolist() == [i in seen_by for i in range(6)]
+    mask = torch.ones(2, 6, dtype=torch.bool)
+    mask[1, :4] = False
+    masked = block(x, mask)
+    assert torch.equal(masked[0], out[0]) and not masked[1, :4].any()
+    g, = torch.autograd.grad(masked.sum(), x)
+    assert torch.isfinite(g).all() and not g[1, :4].any()
+    assert block(x[:, :0]).shape == (2, 0, 24)
+    far = block(x, positions=torch.arange(6) + 1000)  # rotations are relative
+    assert (far - out).abs().max() <= 1e-4
+    wide = SelfAttention(24, 8, 4, 2, frequencies=block._frequencies["cpu"], window=3, sinks=1)
+    wide.load_state_dict(block.state_dict())
+    assert torch.equal(wide(x), out)
+    set_turbopairformer_strict(True)
+    try:
+        with pytest.raises(RuntimeError, match="strict"):
+            block(x)
+    finally:
+        set_turbopairformer_strict(False)
+    with pytest.raises(ValueError, match="BF16"):
+        block.step(x[0], None, None, None, None)
+    for bad in (dict(no_heads=3, no_kv_heads=2), dict(no_heads=2, activation_save="int4"),
+                dict(no_heads=2, window=0), dict(no_heads=2, sinks=-1), dict(no_heads=2, rotary_channels=3),
+                dict(no_heads=2, rotary_channels=10), dict(no_heads=2, frequencies=torch.ones(5))):
+        with pytest.raises(ValueError):
+            SelfAttention(8, 8, **bad)
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """The facades on host tensors, the native calls recorded instead of made."""
+    import sys
+
+    calls = []
+    monkeypatch.setattr(_native, "call", lambda name, *args: calls.append(name))
+    monkeypatch.setattr(_native, "query", lambda name, *args: 0)
+    for name in ("rotary", "window_attention", "paged"):
+        monkeypatch.setattr(sys.modules[f"openfold3_triangle_kernel_amd.{name}"], "_device_supported",
+                            lambda t: (True, ""))
+    return calls
+
+
+def _calls():
+    g = torch.Generator().manual_seed(0)
+    draw = lambda *shape: torch.randn(*shape, generator=g).bfloat16()  # noqa: E731
+    cache, x, tables, starts, lengths = _paged()
+    places = (tables, starts, lengths)
+    return {"rotary": (lambda q, k, w: qk_norm_rotary(q, k, None, _F, w, w, 1e-6),
+                       (draw(1, 2, 4, 16), draw(1, 2, 4, 16), draw(16))),
+            "window": (lambda q, k, v: window_attention(q, k, v, 3, 1),
+                       (draw(1, 2, 4, 16), draw(1, 2, 4, 16), draw(1, 2, 4, 16))),
+            "append": (lambda k, v, q: append_kv(cache, k, v, *places, q, _F), (x, x.clone(), draw(3, 4, 16))),
+            "paged": (lambda q: paged_attention(q, cache, *places), (draw(3, 4, 16),))}
+
+
+def test_forward_mode_and_transforms_are_refused(fake):
+    from torch.autograd import forward_ad
+
+    for call, operands in _calls().values():
+        for i in range(len(operands)):
+            for grad in (False, True):
+                with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                    ops = [t.clone() for t in operands]
+                    ops[i] = forward_ad.make_dual(ops[i], torch.ones_like(ops[i]))
+                    with pytest.raises((RuntimeError, NotImplementedError), match="forward|jvp"):
+                        call(*ops)
+        with pytest.raises(RuntimeError, match="functorch|vmap|data pointer"):
+            torch.vmap(lambda t: call(t, *operands[1:]))(operands[0][None].repeat(3, *[1] * operands[0].ndim))
+
+
+def test_traces_hold_the_operators(fake):
+    for name, (call, operands) in _calls().items():
+        graph = str(torch.jit.trace(call, operands, check_trace=False).graph)
+        assert "^_" in graph, f"{name}: no node for the operator in\n{graph}"
