@@ -16,21 +16,30 @@ constexpr int kSaMaxSplits = 256;
 
 __device__ const uint32_t kSaZeros[4] = {0, 0, 0, 0};
 
-// Loader of a [ROWS][DP] tile of a cache by NW waves from the states' rows.
+// Loader of the [ROWS][DP] tiles of a cache's K and V by NW waves from the states' rows.
 template <int DP, int ROWS, int NW>
 struct SPageLoader {
   static constexpr int CPR = DP / 8, NI = ROWS * CPR / 64 / NW;
-  static __device__ __forceinline__ void issue(const SAttnArgs& a, const u16* cache, uint64_t live, uint32_t row,
-                                               int w, u16* T) {
-    char* dst = reinterpret_cast<char*>(T);
+  static __device__ __forceinline__ void issue(const SAttnArgs& a, uint32_t row, int w, u16* K, u16* V) {
+    char *dk = reinterpret_cast<char*>(K), *dv = reinterpret_cast<char*>(V);
+    uint64_t ks[NI], vs[NI];
+    const uint64_t zeros = (uint64_t)(uintptr_t)kSaZeros;
+    const uint64_t apart = (uint64_t)(uintptr_t)a.v - (uint64_t)(uintptr_t)a.k;
 #pragma unroll
     for (int t = 0; t < NI; ++t) {
       const int p = 64 * (NI * w + t) + (int)(threadIdx.x & 63), r = p / CPR;
       const int chunk = (p - r * CPR) ^ xa_swz<DP>(r);
       const uint32_t at = __shfl(row, r);
-      const u16* src = cache + (uint64_t)at * (uint32_t)a.D + 8 * chunk;
-      if (!((live >> r) & 1) || 8 * chunk >= a.D) src = (const u16*)kSaZeros;
-      g2lds16(src, dst + (NI * w + t) * 1024);
+      uint64_t x = (uint64_t)(uintptr_t)a.k + (uint64_t)at * (uint32_t)(2 * a.D) + 16 * chunk;
+      const bool live = at != kSaDead && 8 * chunk < a.D;
+      asm volatile("" : "+v"(x));  // (formed by every lane: a branch around it would cost more)
+      ks[t] = live ? x : zeros;
+      vs[t] = live ? x + apart : zeros;
+    }
+#pragma unroll
+    for (int t = 0; t < NI; ++t) {
+      g2lds16((const void*)(uintptr_t)ks[t], dk + (NI * w + t) * 1024);
+      g2lds16((const void*)(uintptr_t)vs[t], dv + (NI * w + t) * 1024);
     }
   }
 };
@@ -207,6 +216,15 @@ __device__ __forceinline__ void sa_store4(const SAttnArgs& a, int64_t at, float 
 struct STile {
   int s, r0, R, pos;  // first row in the sequence, rows there, the first token's position
   int64_t token;      // the sequence's first token in the batch
+  // Sequence s_ of a paged batch (S: the rows behind the last one, without states).
+  __device__ __forceinline__ void sequence(const SAttnArgs& a, int s_) {
+    s = s_;
+    token = paged_start(a.t, s);
+    const int64_t next = s < a.t.S ? paged_start(a.t, s + 1) : a.t.T;
+    const int fresh = (int)(next > token ? next - token : 0);
+    R = sa_scalar(fresh * a.G);
+    pos = sa_scalar(s < a.t.S ? (int)paged_length(a.t, s) - fresh : -fresh);
+  }
   // Row tile `tile` of RT rows of a paged batch; false past a sequence's rows.  Sequence s
   // has the tiles from starts[s] G / RT + s on, which are enough for its rows whatever its
   // length; the rows behind the last one are those of a sequence S without states.
@@ -214,12 +232,8 @@ struct STile {
     // (T G is below 2^30, rt a power of two.)
     auto before = [&](int x) { return (int)((uint32_t)paged_start(a.t, x) * (uint32_t)a.G / (uint32_t)rt) + x; };
     s = __builtin_amdgcn_readfirstlane(paged_search(a.t.S, [&](int x) { return before(x) <= tile; }));
-    token = paged_start(a.t, s);
-    const int64_t next = s < a.t.S ? paged_start(a.t, s + 1) : a.t.T;
-    const int fresh = (int)(next > token ? next - token : 0);
-    R = sa_scalar(fresh * a.G);
+    sequence(a, s);
     r0 = sa_scalar((tile - before(s)) * rt);
-    pos = sa_scalar(s < a.t.S ? (int)paged_length(a.t, s) - fresh : -fresh);
     return r0 < R;
   }
   __device__ __forceinline__ int position(const SAttnArgs& a, int r) const {
@@ -227,34 +241,83 @@ struct STile {
   }
 };
 
-// Four waves of 32 QB rows share K and V tiles of 64 states, two stages deep.
-template <int DP, int QB, bool F16, bool STATS, bool PAGED>
-__global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
-  constexpr int KT = 64, TILE = KT * DP, RT = 128 * QB;
-  typedef SPoison<DP> Poison;
-  __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
-  __shared__ uint32_t poison[RT * Poison::WORDS], bad[2];
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  int64_t bh;
-  int unit;
-  if (!sa_unit(a.order, &bh, &unit)) return;
-  const int tile = (int)sa_div(unit, a.splits), split = unit - tile * a.splits;
-  const int b = PAGED ? 0 : (int)sa_div((uint32_t)bh, a.Hk), hk = (int)bh - b * a.Hk;
-  STile at;
-  if constexpr (PAGED) {
-    if (!at.find(a, tile, RT)) return;
-  } else {
-    at.s = b;
-    at.r0 = (a.tiles - 1 - tile) * RT;  // (later rows see more states)
-    at.R = a.R;
-    at.pos = 0;
-    at.token = (int64_t)b * a.N;
-  }
-  const int pmin = sa_scalar(at.position(a, at.r0)), pmax = sa_scalar(at.position(a, at.r0 + RT - 1));
-  const SSpan span(pmin, pmax, a.window, a.sinks);
-  const SParts parts(span.n, a.splits, kSaLeast);
-  if (a.splits > 1 && split >= parts.live) return;
+// Where a unit of rows leaves its results: as outputs, or unnormalised as parts `step` apart,
+// row by row from `base` on.
+struct SResult {
+  bool whole;
+  int64_t base;
+  int step;
+};
 
+// An even share of a paged batch's work.  Sequence s costs c_s = (row tiles) x (state tiles of
+// its span); the kv heads' sequences' row tiles' state tiles, in this order, are one axis of
+// Hk sum(c) tiles, of which workgroup w takes `share`, from w * share on: as many as every
+// other, whatever the lengths are (one workgroup a part of a sequence: 16 of 2047 to 8190
+// states left CUs idle a third of the time).  A unit (head, sequence, row tile) whose tiles
+// are all a workgroup's own is finished there; others leave a part in slot 2 w (one that began
+// before the workgroup's share) or 2 w + 1, and sattn_even_join_kernel finds the slots by the same sums.  Lane
+// l holds sequence l (64 at most).
+struct SEven {
+  int first, cost, tiles;  // before the sequence, its own, of its span
+  int total, share;        // of a head, of a workgroup
+  __device__ __forceinline__ void init(const SAttnArgs& a, int rt) {
+    const int l = threadIdx.x & 63;
+    const bool in = l < a.t.S;
+    const int64_t from = in ? paged_start(a.t, l) : 0, next = in ? paged_start(a.t, l + 1) : 0;
+    const int fresh = (int)(next > from ? next - from : 0);
+    const int len = in ? (int)paged_length(a.t, l) : 0;
+    // (Starts that do not ascend may ask for more rows than there are, and are not served.)
+    const bool fits = lanes_sum<64>((float)fresh) <= 1.01f * (float)a.t.T;
+    tiles = fresh && fits ? SSpan(len - fresh, len - 1, a.window, a.sinks).n : 0;
+    cost = (fresh * a.G + rt - 1) / rt * tiles;
+    int sum = cost;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(sum, o);
+      if (l >= o) sum += x;
+    }
+    first = sum - cost;
+    total = sa_scalar(__shfl(sum, 63));
+    const int even = (int)(((uint32_t)a.Hk * (uint32_t)total + a.even - 1) / (uint32_t)a.even);
+    share = sa_scalar(even > kSaLeast ? even : kSaLeast);
+  }
+};
+
+// The units that workgroup w of an even share takes: f(head, tile, span, first, end, result)
+// for the state tiles [first, end) of each.
+template <typename F>
+__device__ __forceinline__ void sa_even_units(const SAttnArgs& a, int rt, F f) {
+  SEven e;
+  e.init(a, rt);
+  if (e.total == 0) return;
+  const int w = blockIdx.x;
+  int64_t x = (int64_t)w * e.share;
+  const int64_t end = min(x + e.share, (int64_t)a.Hk * e.total);
+  while (x < end) {
+    const int hk = (int)sa_div((uint32_t)x, (uint32_t)e.total), y = (int)x - hk * e.total;
+    const int s = __builtin_ctzll(__ballot(e.first <= y && y < e.first + e.cost));
+    const int z = y - sa_scalar(__shfl(e.first, s)), n = sa_scalar(__shfl(e.tiles, s));
+    const int tile = (int)sa_div((uint32_t)z, (uint32_t)n), t0 = z - tile * n;
+    const int count = (int)min((int64_t)n - t0, end - x);
+    STile at;
+    at.sequence(a, s);
+    at.r0 = tile * rt;
+    const SSpan span(at.pos, at.pos + at.R / a.G - 1, a.window, a.sinks);
+    f(hk, at, span, t0, t0 + count, SResult{count == n, (int64_t)(2 * w + (t0 == 0 ? 1 : 0)) * rt, 1});
+    x += count;
+  }
+}
+
+// A unit of 128 QB rows: four waves of 32 QB rows share K and V tiles of 64 states, the tiles
+// [first, end) of the span, two stages deep.
+template <int DP, int QB, bool F16, bool STATS, bool PAGED>
+__device__ __forceinline__ void sattn_tile(const SAttnArgs& a, u16 (*smem)[2][64 * DP], uint32_t* poison,
+                                           uint32_t* bad, int b, int hk, const STile& at, const SSpan& span,
+                                           int first, int end, const SResult& result) {
+  constexpr int KT = 64, RT = 128 * QB;
+  typedef SPoison<DP> Poison;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int pmin = sa_scalar(at.position(a, at.r0)), pmax = sa_scalar(at.position(a, at.r0 + RT - 1));
   const int r0 = at.r0 + w * 32 * QB;
   const int p0 = sa_scalar(at.position(a, r0)), p1 = sa_scalar(at.position(a, r0 + 32 * QB - 1));
   STiles<PAGED, KT, 1> t;
@@ -269,14 +332,14 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
     lk.init(w, a.k_sn, a.D);
     lv.init(w, a.v_sn, a.D);
   }
-  t.init(span, split * parts.per, min(span.n, (split + 1) * parts.per), pmax + 1);
+  t.init(span, first, end, pmax + 1);
+  t.below = pmin - a.window + 1;
   SRows<DP, QB, F16, STATS> rows;
   rows.init(a, a.q + (PAGED ? at.token * a.q_sn : b * a.q_sb), hk, r0, at.R, at.pos);
 
   auto issue = [&](int st) {
     if constexpr (PAGED) {
-      SPageLoader<DP, KT, 4>::issue(a, kp, t.live, t.pages.row, w, smem[st][0]);
-      SPageLoader<DP, KT, 4>::issue(a, vp, t.live, t.pages.row, w, smem[st][1]);
+      SPageLoader<DP, KT, 4>::issue(a, t.pages.row, w, smem[st][0], smem[st][1]);
     } else {
       lk.issue(kp + (int64_t)t.k0 * a.k_sn, t.live, w, smem[st][0]);
       lv.issue(vp + (int64_t)t.k0 * a.v_sn, t.live, w, smem[st][1]);
@@ -333,7 +396,7 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
               Poison::apply(hurt, 32 * db + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), rows.o[qb][db][e]);
     }
     const int i = (int)fdiv((uint32_t)r, a.div_g), g = r - i * a.G;
-    if (a.splits == 1) {
+    if (result.whole) {
       const float inv = sa_inverse(n, rows.m[qb]);
       const int64_t o = ((at.token + i) * a.H + hk * a.G + g) * a.D;
 #pragma unroll
@@ -346,9 +409,9 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
             sa_store4<F16>(a, o + d, x[4 * g4] * inv, x[4 * g4 + 1] * inv, x[4 * g4 + 2] * inv,
                            x[4 * g4 + 3] * inv);
         }
-      if (STATS && lane < 32) a.lse[bh * a.R + r] = sa_lse(a, rows.m[qb], l);
+      if (STATS && lane < 32) a.lse[((int64_t)b * a.Hk + hk) * a.R + r] = sa_lse(a, rows.m[qb], l);
     } else {
-      const int64_t at_ = (hk * a.rows + at.token * a.G + r) * a.splits + split;
+      const int64_t at_ = result.base + (int64_t)(r - at.r0) * result.step;
       if (lane < 32) {
         a.part_ml[3 * at_] = rows.m[qb];
         a.part_ml[3 * at_ + 1] = l;
@@ -371,38 +434,68 @@ __global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
   }
 }
 
+// 32 heads, causal 4096 x 4096 x 128 on 8, twice, with the backward's statistics: 340 us.
+template <int DP, int QB, bool F16, bool STATS, bool PAGED>
+__global__ __launch_bounds__(256, 2) void sattn_fwd_kernel(SAttnArgs a) {
+  constexpr int RT = 128 * QB;
+  __shared__ __attribute__((aligned(1024))) u16 smem[2][2][64 * DP];
+  __shared__ uint32_t poison[RT * SPoison<DP>::WORDS], bad[2];
+  if constexpr (PAGED) {
+    if (a.even) {
+      sa_even_units(a, RT, [&](int hk, const STile& at, const SSpan& span, int first, int end,
+                               const SResult& result) {
+        __syncthreads();  // (the unit before is done with the tiles)
+        sattn_tile<DP, QB, F16, STATS, PAGED>(a, smem, poison, bad, 0, hk, at, span, first, end, result);
+      });
+      return;
+    }
+  }
+  int64_t bh;
+  int unit;
+  if (!sa_unit(a.order, &bh, &unit)) return;
+  const int tile = (int)sa_div(unit, a.splits), split = unit - tile * a.splits;
+  const int b = PAGED ? 0 : (int)sa_div((uint32_t)bh, a.Hk), hk = (int)bh - b * a.Hk;
+  STile at;
+  if constexpr (PAGED) {
+    if (!at.find(a, tile, RT)) return;
+  } else {
+    at.s = b;
+    at.r0 = (a.tiles - 1 - tile) * RT;  // (later rows see more states)
+    at.R = a.R;
+    at.pos = 0;
+    at.token = (int64_t)b * a.N;
+  }
+  const SSpan span(sa_scalar(at.position(a, at.r0)), sa_scalar(at.position(a, at.r0 + RT - 1)), a.window,
+                   a.sinks);
+  const SParts parts(span.n, a.splits, kSaLeast);
+  if (a.splits > 1 && split >= parts.live) return;
+  sattn_tile<DP, QB, F16, STATS, PAGED>(
+      a, smem, poison, bad, b, hk, at, span, split * parts.per, min(span.n, (split + 1) * parts.per),
+      SResult{a.splits == 1, (hk * a.rows + at.token * a.G + at.r0) * a.splits + split, a.splits});
+}
+
 // Few rows of a sequence (32 a workgroup; one decoded token above all): the states' bytes
 // are the bound.  Every wave streams tiles of 32 states of its own, two stages deep without
 // a barrier, and the four waves' results meet in LDS at the end.
 template <int DP, bool F16>
-__global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
-  constexpr int KT = 32, RT = 32, TILE = KT * DP, NI = KT * DP / 512;
+__device__ __forceinline__ void sattn_few(const SAttnArgs& a, u16 (*smem)[2][2][32 * DP], uint32_t* poison,
+                                          int hk, const STile& at, const SSpan& span, int first, int end,
+                                          const SResult& result) {
+  constexpr int KT = 32, RT = 32, NI = KT * DP / 512;
   constexpr int OP = DP + 4;  // pitch of the joined rows (f32)
   typedef SPoison<DP> Poison;
-  __shared__ __attribute__((aligned(1024))) u16 smem[4][2][2][TILE];
-  __shared__ uint32_t poison[RT * Poison::WORDS];
-  static_assert(sizeof(smem) >= 4 * 32 * (OP + 2) * 4, "the join fits");
+  static_assert(4 * sizeof(smem[0]) >= 4 * 32 * (OP + 2) * 4, "the join fits");
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  int64_t head;
-  int unit;
-  if (!sa_unit(a.order, &head, &unit)) return;
-  const int hk = (int)head, tile = (int)sa_div(unit, a.splits), split = unit - tile * a.splits;
-  STile at;
-  if (!at.find(a, tile, RT)) return;
   const int p0 = sa_scalar(at.position(a, at.r0)), p1 = sa_scalar(at.position(a, at.r0 + RT - 1));
-  const SSpan span(p0, p1, a.window, a.sinks);
-  const SParts parts(span.n, a.splits, kSaLeast);
-  if (a.splits > 1 && split >= parts.live) return;
-
   STiles<true, KT, 4> t;
   t.pages.init(a, at.s, hk);
-  t.init(span, 2 * split * parts.per + w, 2 * min(span.n, (split + 1) * parts.per), p1 + 1);
+  t.init(span, 2 * first + w, 2 * end, p1 + 1);
+  t.below = p0 - a.window + 1;
   SRows<DP, 1, F16, false> rows;
   rows.init(a, a.q + at.token * a.q_sn, hk, at.r0, at.R, at.pos);
 
   auto issue = [&](int st) {
-    SPageLoader<DP, KT, 1>::issue(a, a.k, t.live, t.pages.row, 0, smem[w][st][0]);
-    SPageLoader<DP, KT, 1>::issue(a, a.v, t.live, t.pages.row, 0, smem[w][st][1]);
+    SPageLoader<DP, KT, 1>::issue(a, t.pages.row, 0, smem[w][st][0], smem[w][st][1]);
   };
   for (int i = threadIdx.x; i < RT * Poison::WORDS; i += 256) poison[i] = 0;
   lds_barrier();
@@ -461,7 +554,7 @@ __global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
     f[x] = fast_exp2((MN[2 * (x * 32 + rl)] - m) * a.c);
     n += f[x] * MN[2 * (x * 32 + rl) + 1];
   }
-  const int64_t pr = (hk * a.rows + at.token * a.G + r) * a.splits + split;
+  const int64_t pr = result.base + (int64_t)rl * result.step;
   const float inv = sa_inverse(n, m);
   const int i = (int)fdiv((uint32_t)r, a.div_g), g = r - i * a.G;
   const int64_t out = ((at.token + i) * a.H + hk * a.G + g) * a.D;
@@ -475,14 +568,41 @@ __global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = Poison::apply(poison + rl * Poison::WORDS, d + e, o[e]);
-    if (a.splits == 1) sa_store4<F16>(a, out + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (result.whole) sa_store4<F16>(a, out + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     else *reinterpret_cast<f32x4*>(a.part_o + pr * a.D + d) = o;
   }
-  if (a.splits > 1 && (threadIdx.x & 7) == 0) {
+  if (!result.whole && (threadIdx.x & 7) == 0) {
     a.part_ml[3 * pr] = m;
     a.part_ml[3 * pr + 1] = n;
     a.part_ml[3 * pr + 2] = n;
   }
+}
+
+template <int DP, bool F16>
+__global__ __launch_bounds__(256, 1) void sattn_few_kernel(SAttnArgs a) {
+  constexpr int RT = 32;
+  __shared__ __attribute__((aligned(1024))) u16 smem[4][2][2][32 * DP];
+  __shared__ uint32_t poison[RT * SPoison<DP>::WORDS];
+  if (a.even) {
+    sa_even_units(a, RT, [&](int hk, const STile& at, const SSpan& span, int first, int end,
+                             const SResult& result) {
+      __syncthreads();  // (the unit before is done with the tiles)
+      sattn_few<DP, F16>(a, smem, poison, hk, at, span, first, end, result);
+    });
+    return;
+  }
+  int64_t head;
+  int unit;
+  if (!sa_unit(a.order, &head, &unit)) return;
+  const int hk = (int)head, tile = (int)sa_div(unit, a.splits), split = unit - tile * a.splits;
+  STile at;
+  if (!at.find(a, tile, RT)) return;
+  const SSpan span(sa_scalar(at.position(a, at.r0)), sa_scalar(at.position(a, at.r0 + RT - 1)), a.window,
+                   a.sinks);
+  const SParts parts(span.n, a.splits, kSaLeast);
+  if (a.splits > 1 && split >= parts.live) return;
+  sattn_few<DP, F16>(a, smem, poison, hk, at, span, split * parts.per, min(span.n, (split + 1) * parts.per),
+                     SResult{a.splits == 1, (hk * a.rows + at.token * a.G + at.r0) * a.splits + split, a.splits});
 }
 
 // Joins the parts of a row's states, a wave a row: o = sum_s 2^(c (m_s - m)) o_s / sum_s
@@ -497,13 +617,8 @@ __global__ __launch_bounds__(256) void sattn_join_kernel(SAttnArgs a, int rt) {
   STile at;
   int r;
   if constexpr (PAGED) {
-    at.s = __builtin_amdgcn_readfirstlane(
-        paged_search(a.t.S, [&](int x) { return paged_start(a.t, x) <= token; }));
-    at.token = paged_start(a.t, at.s);
-    const int64_t next = at.s < a.t.S ? paged_start(a.t, at.s + 1) : a.t.T;
-    const int fresh = (int)(next > at.token ? next - at.token : 0);
-    at.R = fresh * a.G;
-    at.pos = at.s < a.t.S ? (int)paged_length(a.t, at.s) - fresh : -fresh;
+    at.sequence(a, __builtin_amdgcn_readfirstlane(
+        paged_search(a.t.S, [&](int x) { return paged_start(a.t, x) <= token; })));
     r = (int)(row - at.token * a.G);
     if (r >= at.R) return;  // (starts that do not ascend)
   } else {
@@ -555,6 +670,61 @@ __global__ __launch_bounds__(256) void sattn_join_kernel(SAttnArgs a, int rt) {
   if (a.lse && lane == 0) a.lse[((int64_t)at.s * a.Hk + hk) * a.R + r] = sa_lse(a, m, l);
 }
 
+// The same for an even share.  Of every unit that workgroups share, the join's workgroup that
+// has the number of the second of them joins the rows, 32 rows each; the workgroups
+// behind them write the
+// zeros of tokens that see nothing (of no sequence, or of one without states), a wave a token.
+template <bool F16>
+__global__ __launch_bounds__(256) void sattn_even_join_kernel(SAttnArgs a, int rt) {
+  const int lane = threadIdx.x & 63, each = rt / 32, w = (int)sa_div(blockIdx.x, (uint32_t)each);
+  SEven e;
+  e.init(a, rt);
+  if (w >= a.even) {
+    const int64_t token = (int64_t)(blockIdx.x - a.even * each) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (token >= a.t.T) return;
+    const int s = __builtin_amdgcn_readfirstlane(
+        paged_search(a.t.S, [&](int x) { return paged_start(a.t, x) <= token; }));
+    if (s < a.t.S && __shfl(e.tiles, s) != 0) return;
+    uint2* out = reinterpret_cast<uint2*>(a.out + token * a.H * a.D);
+    for (int i = lane; i < a.H * a.D / 4; i += 64) out[i] = uint2{0, 0};
+    return;
+  }
+  const int64_t x = (int64_t)w * e.share;
+  if (w == 0 || x >= (int64_t)a.Hk * e.total) return;
+  const int hk = (int)sa_div((uint32_t)x, (uint32_t)e.total), y = (int)x - hk * e.total;
+  const int s = __builtin_ctzll(__ballot(e.first <= y && y < e.first + e.cost));
+  const int z = y - sa_scalar(__shfl(e.first, s)), n = sa_scalar(__shfl(e.tiles, s));
+  const int tile = (int)sa_div((uint32_t)z, (uint32_t)n), before = z - tile * n;
+  // Tiles of the unit before this workgroup's share: none, or more than the workgroup before has.
+  if (before == 0 || before > e.share) return;
+  const int parts = 2 + (n - before - 1) / e.share;
+  STile at;
+  at.sequence(a, s);
+  const int rows = min(rt, at.R - tile * rt), d = 4 * (threadIdx.x & 31);
+  if (d >= a.D) return;
+  const int first = 32 * ((int)blockIdx.x - w * each);
+  for (int r = first + (int)(threadIdx.x >> 5); r < min(rows, first + 32); r += 8) {
+    // Slot 2 (w - 1) + 1, then 2 w, 2 w + 2, ...
+    auto part = [&](int i) { return (int64_t)(i ? 2 * (w + i - 1) : 2 * w - 1) * rt + r; };
+    float m = kSaLow;
+    for (int i = 0; i < parts; ++i) m = xa_max(m, a.part_ml[3 * part(i)]);
+    float sum = 0.f;
+    f32x4 o = (f32x4)0.f;
+    for (int i = 0; i < parts; ++i) {
+      const int64_t p = part(i);
+      const float f = fast_exp2((a.part_ml[3 * p] - m) * a.c);
+      sum = fmaf(f, a.part_ml[3 * p + 2], sum);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + p * a.D + d);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = fmaf(f, v[c], o[c]);
+    }
+    const float inv = sa_inverse(sum, m);
+    const int all = tile * rt + r, i = (int)fdiv((uint32_t)all, a.div_g), g = all - i * a.G;
+    sa_store4<F16>(a, ((at.token + i) * a.H + hk * a.G + g) * a.D + d, o[0] * inv, o[1] * inv, o[2] * inv,
+                   o[3] * inv);
+  }
+}
+
 // Sizes that both forms share; 0 or an error code.
 static int sattn_check(SAttnArgs& a, int64_t H, int64_t Hk, int64_t D, int64_t window, int64_t sinks,
                        double scale, const char* fn) {
@@ -601,8 +771,9 @@ int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const ch
   return TPF_OK;
 }
 
-static int64_t sattn_part_floats(const SAttnArgs& a) {
-  return a.splits > 1 ? a.Hk * a.rows * a.splits * (a.D + 3) : 0;
+// Rows of the parts in memory.
+static int64_t sattn_part_rows(const SAttnArgs& a, int rt) {
+  return a.even ? (int64_t)2 * a.even * rt : a.splits > 1 ? a.Hk * a.rows * a.splits : 0;
 }
 
 // Parts of the states so that `units` workgroups become `target`, of 256 states at least.
@@ -645,6 +816,9 @@ static void window_pick(const SAttnArgs& a, int qb, hipStream_t s) {
 
 template <bool F16, bool PAGED>
 static void sattn_join(const SAttnArgs& a, int rt, hipStream_t s) {
+  if (a.even)
+    hipLaunchKernelGGL((sattn_even_join_kernel<F16>), dim3((unsigned)(a.even * (rt / 32) + (a.t.T + 3) / 4)),
+                       dim3(256), 0, s, a, rt);
   if (a.splits > 1)
     hipLaunchKernelGGL((sattn_join_kernel<F16, PAGED>), dim3((unsigned)((a.Hk * a.rows + 3) / 4)), dim3(256), 0,
                        s, a, rt);
@@ -671,14 +845,25 @@ static int paged_attn_check(SAttnArgs& a, const tpf_paged_shape* s, const tpf_pa
   return TPF_OK;
 }
 
-// Up to 32 rows a sequence on the mean run on the streaming kernel.  Either one's tiles are
-// counted for the most that the tokens can be; the parts for the tiles that are likely.
+// Up to 32 rows a sequence on the mean run on the streaming kernel.  Up to 64 sequences share
+// their work evenly over the workgroups that run at once, if a sequence can have 1024 states;
+// otherwise tiles are counted for the most that the tokens can be and the parts for those
+// that are likely.
 static int paged_plan(SAttnArgs& a) {
   const int rt = a.rows <= 32 * (int64_t)a.t.S ? 32 : 128;
+  const int64_t states = (int64_t)a.t.width * a.t.page;
   a.tiles = (int)(a.rows / rt) + a.t.S + 1;
+  a.splits = 1;
+  a.even = 0;
+  if (a.t.S <= 64 && states >= 1024 &&
+      ((double)a.rows / rt + a.t.S) * ((double)states / 64 + 1) * a.Hk < (double)((int64_t)1 << 30)) {
+    // Of the streaming kernel one runs on a CU above 64 channels, two from 33 on.
+    a.even = 256 * (rt == 128 ? 2 : a.D > 64 ? 1 : a.D > 32 ? 2 : 4);
+    return rt;
+  }
   int64_t units = a.rows / rt > a.t.S ? a.rows / rt : a.t.S;
   units *= a.Hk;
-  a.splits = sattn_splits(units < 1 ? 1 : units, 512, (int64_t)a.t.width * a.t.page);
+  a.splits = sattn_splits(units < 1 ? 1 : units, 512, states);
   while (a.splits > 1 && (double)a.tiles * a.Hk * a.splits > (double)kXaMaxGroups / 2) a.splits /= 2;
   a.order = sa_order(a.Hk, (int64_t)a.tiles * a.splits);
   return rt;
@@ -686,7 +871,7 @@ static int paged_plan(SAttnArgs& a) {
 
 template <int DP, bool F16>
 static void paged_launch(const SAttnArgs& a, int rt, hipStream_t s) {
-  const dim3 grid((unsigned)a.order.groups);
+  const dim3 grid((unsigned)(a.even ? a.even : a.order.groups));
   if (rt == 32) hipLaunchKernelGGL((sattn_few_kernel<DP, F16>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((sattn_fwd_kernel<DP, 1, F16, false, true>), grid, dim3(256), 0, s, a);
 }
@@ -705,8 +890,8 @@ static void paged_pick(const SAttnArgs& a, int rt, hipStream_t s) {
 extern "C" int64_t tpf_window_forward_workspace_bytes(const tpf_window_shape* shape) {
   tpf::SAttnArgs a{};
   if (tpf::window_check(a, shape, 1.0, "tpf_window_forward_workspace_bytes")) return -1;
-  tpf::window_plan(a);
-  return tpf::sattn_part_floats(a) * 4;
+  const int qb = tpf::window_plan(a);
+  return tpf::sattn_part_rows(a, 128 * qb) * (a.D + 3) * 4;
 }
 
 extern "C" int tpf_window_forward(const void* q, const void* k, const void* v, const void* mask, void* out,
@@ -723,14 +908,14 @@ extern "C" int tpf_window_forward(const void* q, const void* k, const void* v, c
        (uintptr_t)workspace) % 16)
     return tpf::set_error(TPF_ERR_ARG, "%s: tensors must start on 16 bytes", fn);
   const int qb = tpf::window_plan(a);
-  const int64_t floats = tpf::sattn_part_floats(a);
-  if (floats && (!workspace || workspace_bytes < floats * 4))
+  const int64_t parts = tpf::sattn_part_rows(a, 128 * qb);
+  if (parts && (!workspace || workspace_bytes < parts * (a.D + 3) * 4))
     return tpf::set_error(TPF_ERR_ARG, "%s: workspace too small", fn);
   a.q = (const tpf::u16*)q; a.k = (const tpf::u16*)k; a.v = (const tpf::u16*)v;
   a.mask = (const uint8_t*)mask;
   a.out = (tpf::u16*)out; a.res = (tpf::u16*)residual; a.lse = lse;
   a.part_o = (float*)workspace;
-  a.part_ml = floats ? a.part_o + a.Hk * a.rows * a.splits * a.D : nullptr;
+  a.part_ml = parts ? a.part_o + parts * a.D : nullptr;
   hipStream_t s = (hipStream_t)stream;
   if (shape->dtype == TPF_F16) {
     tpf::window_pick<true, false>(a, qb, s);
@@ -747,8 +932,8 @@ extern "C" int64_t tpf_paged_attention_workspace_bytes(const tpf_paged_shape* sh
                                                        const tpf_paged_batch* batch) {
   tpf::SAttnArgs a{};
   if (tpf::paged_attn_check(a, shape, batch, 1.0, "tpf_paged_attention_workspace_bytes")) return -1;
-  tpf::paged_plan(a);
-  return tpf::sattn_part_floats(a) * 4;
+  const int rt = tpf::paged_plan(a);
+  return tpf::sattn_part_rows(a, rt) * (a.D + 3) * 4;
 }
 
 extern "C" int tpf_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out,
@@ -762,13 +947,13 @@ extern "C" int tpf_paged_attention(const void* q, const void* k_cache, const voi
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)workspace) % 16)
     return tpf::set_error(TPF_ERR_ARG, "%s: tensors must start on 16 bytes", fn);
   const int rt = tpf::paged_plan(a);
-  const int64_t floats = tpf::sattn_part_floats(a);
-  if (floats && (!workspace || workspace_bytes < floats * 4))
+  const int64_t parts = tpf::sattn_part_rows(a, rt);
+  if (parts && (!workspace || workspace_bytes < parts * (a.D + 3) * 4))
     return tpf::set_error(TPF_ERR_ARG, "%s: workspace too small", fn);
   a.q = (const tpf::u16*)q; a.k = (const tpf::u16*)k_cache; a.v = (const tpf::u16*)v_cache;
   a.out = (tpf::u16*)out;
   a.part_o = (float*)workspace;
-  a.part_ml = floats ? a.part_o + a.Hk * a.rows * a.splits * a.D : nullptr;
+  a.part_ml = parts ? a.part_o + parts * a.D : nullptr;
   if (shape->dtype == TPF_F16) tpf::paged_pick<true>(a, rt, (hipStream_t)stream);
   else tpf::paged_pick<false>(a, rt, (hipStream_t)stream);
   return tpf::check_launch(fn);

@@ -46,9 +46,10 @@ struct SAttnArgs {
   float c;             // scale * log2(e)
   int window, sinks;   // window above every position where there is none, then no sinks
   int splits, tiles;   // most parts of a tile's states; row tiles of a batch entry
+  int even;            // workgroups that share a paged batch's state tiles evenly (SEven), or 0
   SOrder order;        // of the forward's or dQ's units
   int64_t rows;        // rows of a kv head in all
-  float* part_o;       // [Hk, rows, splits, D] unnormalised outputs of the parts
+  float* part_o;       // [Hk, rows, splits, D] (or SEven's) unnormalised outputs of the parts
   float* part_ml;      // the same by 3: their maxima and the two sums (SRows)
   PagedTables t;
 };
@@ -129,13 +130,15 @@ __device__ __forceinline__ bool sa_unit(const SOrder& o, int64_t* head, int* uni
   return *unit < o.units;
 }
 
+constexpr uint32_t kSaDead = 0xffffffffu;
+
 // Where states lie in the pages of sequence s under kv head hk: lane l holds the page of
 // table entry `first + l`, read once for 64 entries.
 template <int ROWS>
 struct SPages {
   const int32_t* table;
   int first, page, hk;
-  uint32_t row;  // of the lane's state: (page Hk + hk) P + place
+  uint32_t row;  // of the lane's state: (page Hk + hk) P + place, kSaDead where none lives
   __device__ __forceinline__ void init(const SAttnArgs& a, int s, int hk_) {
     table = a.t.tables + s * a.t.table_ld;
     first = -1 - 64;
@@ -150,12 +153,16 @@ struct SPages {
     if (e0 < first || e1 > first + 63) {
       first = e0;
       page = first + lane < a.t.width ? table[first + lane] : -1;
+      // (Waited for here: at its use the compiler would wait for every load under way.)
+      asm volatile("" : "+v"(page));
     }
     const int j = min(k0 + lane % ROWS, end - 1);
     const int e = (int)fdiv((uint32_t)j, a.t.div_page);
     const int p = __shfl(page, e - first);
+    const bool live = k0 + lane % ROWS < end && p >= 0 && p < a.t.pages;
     row = ((uint32_t)p * (uint32_t)a.Hk + (uint32_t)hk) * (uint32_t)a.t.page + (uint32_t)(j - e * a.t.page);
-    return __ballot(lane < ROWS && k0 + lane < end && p >= 0 && p < a.t.pages);
+    row = live ? row : kSaDead;
+    return __ballot(live && lane < ROWS);
   }
 };
 
@@ -166,6 +173,7 @@ struct STiles {
   SPages<ROWS> pages;
   const uint8_t* mask;
   int t, t1, end, k0;
+  int below = 0;  // states below this, but the sinks, are seen by no row (whose span is wider)
   uint32_t raw;
   uint64_t live;
   __device__ __forceinline__ int state(const SSpan& span, int i) const {
@@ -188,7 +196,7 @@ struct STiles {
       if (t >= t1) return false;
       k0 = state(span, t);
       if constexpr (PAGED) {
-        live = k0 < end ? pages.at(a, k0, end) : 0;
+        live = k0 < end && (k0 + ROWS > below || k0 < a.sinks) ? pages.at(a, k0, end) : 0;
       } else if (mask) {
         live = __ballot(raw != 0);
         raw = load(span, t + STEP);
