@@ -639,7 +639,7 @@ std::optional<std::tuple<Tensor, Tensor>> qk_norm_rotary(
       return std::nullopt;
   const int64_t B = q.size(0), N = q.size(2), D = q.size(3);
   if (type_code(q.scalar_type()) < 0 || k.size(0) != B || k.size(2) != N || k.size(3) != D || D > 256 ||
-      !rotation_plain(D, freq, qw, kw, eps, dev))
+      q.size(1) > 65535 || k.size(1) > 65535 || B * N >= (1 << 26) || !rotation_plain(D, freq, qw, kw, eps, dev))
     return std::nullopt;
   std::optional<Tensor> positions = positions_in;
   if (positions) {
@@ -769,7 +769,7 @@ std::optional<tpf_paged_batch> paged_batch(const Tensor& ck, const Tensor& table
       return std::nullopt;
   if (tables.dim() != 2 || starts.dim() != 1 || lengths.dim() != 1) return std::nullopt;
   const int64_t S = lengths.size(0), width = tables.size(1);
-  if (S < 1 || width < 1 || tables.size(0) != S || starts.size(0) != S + 1 || T < 1 || T >= (1 << 30) ||
+  if (S < 1 || width < 1 || tables.size(0) != S || starts.size(0) != S + 1 || T < 1 || T >= (1 << 26) ||
       width > (1 << 30) / ck.size(2))
     return std::nullopt;
   return tpf_paged_batch{(const int32_t*)cptr(tables), (const int32_t*)cptr(starts), (const int32_t*)cptr(lengths),
@@ -777,7 +777,7 @@ std::optional<tpf_paged_batch> paged_batch(const Tensor& ck, const Tensor& table
 }
 // New tokens [T, heads, D] of the cache's type that a call without gradients takes.
 bool tokens_plain(const Tensor& t, const Tensor& ck, int64_t T, c10::DeviceIndex dev) {
-  return plain(t, dev) && t.dim() == 3 && t.size(0) == T && t.size(1) > 0 && t.size(2) == ck.size(3) &&
+  return plain(t, dev) && t.dim() == 3 && t.size(0) == T && t.size(1) > 0 && t.size(1) <= 65535 && t.size(2) == ck.size(3) &&
          t.scalar_type() == ck.scalar_type() && t.stride(2) == 1 &&
          !(t.requires_grad() && at::GradMode::is_enabled());
 }

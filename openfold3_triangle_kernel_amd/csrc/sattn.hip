@@ -767,6 +767,10 @@ int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const ch
   a.v_sb = s->v_stride[0]; a.v_sh = s->v_stride[1]; a.v_sn = s->v_stride[2];
   a.mask_sb = s->mask_stride;
   a.B = (int)s->B; a.N = (int)s->N; a.R = (int)(a.G * s->N);
+  if (a.window >= a.N || a.sinks >= a.N) {  // every token sees all up to itself
+    a.window = 1 << 30;
+    a.sinks = 0;
+  }
   a.rows = (int64_t)a.B * a.R;
   return TPF_OK;
 }

@@ -24,9 +24,9 @@ struct SAttnGrad {
   int64_t dq_s[3], dk_s[3], dv_s[3];
   float scale;
   // The dK / dV launch: tiles of 128 states, the first `sunk` of them with sinks, whose rows
-  // are in `splits` parts of rchunk, those of the others in `parts`; without a window parts
-  // are the same runs of chunk_tiles tiles' rows for every tile (grad_unit).
-  int ktiles, sunk, splits, rchunk, parts, chunk_tiles;
+  // are in `splits` parts of schunk, those of the others in `parts` of rchunk; without a window
+  // parts are the same runs of chunk_tiles tiles' rows for every tile (grad_unit).
+  int ktiles, sunk, splits, schunk, rchunk, parts, chunk_tiles;
   SOrder order;
   float *part_k, *part_v;  // [parts, B*Hk, N, D], null without parts
   float *sunk_k, *sunk_v;  // [splits, B*Hk, 128 sunk, D]
@@ -225,8 +225,9 @@ __device__ __forceinline__ bool grad_unit(const SAttnGrad& ga, int unit, int* ti
     return true;
   }
   const int sinks = ga.sunk * ga.splits;
-  int t, p, n;
+  int t, p, n, chunk = ga.rchunk;
   if (unit < sinks) {
+    chunk = ga.schunk;
     t = (int)sa_div(unit, ga.splits);
     p = unit - t * ga.splits;
     n = a.R;
@@ -236,11 +237,11 @@ __device__ __forceinline__ bool grad_unit(const SAttnGrad& ga, int unit, int* ti
     t += ga.sunk;
     n = (int)min((int64_t)a.R, ((int64_t)min(t * 128 + 127, a.N - 1) + a.window) * a.G);
   }
-  const int64_t from = (int64_t)t * 128 * a.G + (int64_t)p * ga.rchunk;
+  const int64_t from = (int64_t)t * 128 * a.G + (int64_t)p * chunk;
   *tile = t;
   *part = p;
   *rbeg = (int)min(from, (int64_t)n);
-  *rend = (int)min(from + ga.rchunk, (int64_t)n);
+  *rend = (int)min(from + chunk, (int64_t)n);
   return true;
 }
 
@@ -485,7 +486,7 @@ static int window_grad_plan(SAttnGrad& g, const char* fn) {
   g.sunk = 0;
   g.splits = g.parts = 1;
   g.chunk_tiles = g.ktiles;
-  g.rchunk = a.R;
+  g.rchunk = g.schunk = a.R;
   int64_t units;
   if (a.window >= a.N) {
     int64_t parts = (1024 + BH * (g.ktiles + 1) - 1) / (BH * (g.ktiles + 1));
@@ -504,9 +505,18 @@ static int window_grad_plan(SAttnGrad& g, const char* fn) {
     if (parts < 1) parts = 1;
     rows = ((rows + parts - 1) / parts + 63) / 64 * 64;
     g.parts = (int)parts;
-    if (g.sunk && rows < 512) rows = 512;
     g.rchunk = (int)rows;
-    g.splits = (int)((a.R + rows - 1) / rows);
+    if (g.sunk) {
+      // The sinks' parts are as long as the others, unless more than 2048 would need memory.
+      int64_t most = 2048 / (BH * g.sunk);
+      if (most < 1) most = 1;
+      int64_t chunk = (a.R + most - 1) / most;
+      if (chunk < rows) chunk = rows;
+      if (chunk < 512) chunk = 512;
+      chunk = (chunk + 63) / 64 * 64;
+      g.schunk = (int)chunk;
+      g.splits = (int)((a.R + chunk - 1) / chunk);
+    }
     units = (int64_t)g.sunk * g.splits + (int64_t)(g.ktiles - g.sunk) * g.parts;
   }
   if (BH * (units + 8) > kXaMaxGroups || (double)BH * a.N * (a.D / 4) / 256 + 1 > (double)kXaMaxGroups / 2)

@@ -21,7 +21,7 @@ import torch
 from . import _native
 from .activations import _DTYPES as _WEIGHT_DTYPES, host_path
 from .attention import _device_supported
-from .rotary import _weight_type, check_rotation, rotation_operands
+from .rotary import _MAX_HEADS, _MAX_TOKENS, _weight_type, check_rotation, rotation_operands
 from .window_attention import check_limits, host_limits, limits
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # TPF_BF16, TPF_F16
@@ -124,8 +124,8 @@ def check_batch(unsupported, cache, tables, starts, lengths, tokens) -> None:
             raise unsupported("no gradients pass through a cache: call it under torch.no_grad()")
     if len({t.device for t in (cache.k, tables, starts, lengths, *(t for _, t, _ in tokens))}) != 1:
         raise unsupported("the cache, its tables and the tokens must share one device")
-    if T >= _MAX_STATES:
-        raise unsupported("too many tokens")
+    if T > _MAX_TOKENS or any(t.shape[1] > _MAX_HEADS for _, t, _ in tokens):
+        raise unsupported("at most 65535 heads and 2^26 - 1 tokens")
 
 
 def batch_struct(k_cache, tables, starts, lengths, T: int) -> _Batch:

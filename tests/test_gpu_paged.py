@@ -183,14 +183,14 @@ def test_attention(gpu, case):
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-@pytest.mark.parametrize("new", [1, 60])
-def test_attention_never_reads_what_is_not_there(gpu, bad, new):
+@pytest.mark.parametrize("new,lengths", [(1, [333, 200]), (60, [333, 200]), (1, [3333, 2000]), (60, [2333, 90])])
+def test_attention_never_reads_what_is_not_there(gpu, bad, new, lengths):
     """Places behind a sequence, other pages, pages that the cache does not have and states
     before the window never reach an output, whatever they hold; a later token of the
     chunk never reaches an earlier one."""
     from openfold3_triangle_kernel_amd import PagedCache, paged_attention
 
-    news, lengths = [new, new], [333, 200]
+    news = [new, new]
     cache, tables, starts, lens, T, g = _batch(gpu, news, lengths, 12, 2, 64, torch.bfloat16)
     q = torch.randn(T, 4, 64, generator=g).bfloat16().to(gpu)
     live = torch.zeros(cache.pages, 12, dtype=torch.bool)
@@ -211,7 +211,7 @@ def test_attention_never_reads_what_is_not_there(gpu, bad, new):
     assert torch.equal(paged_attention(q, dirty, freed, starts, lens, 40), want)
     # The chunk's last token.
     for t in (dirty.k, dirty.v):
-        t[tables[0, 332 // 12].item(), :, 332 % 12] = bad
+        t[tables[0, (lengths[0] - 1) // 12].item(), :, (lengths[0] - 1) % 12] = bad
     got = paged_attention(q, dirty, tables, starts, lens, None)
     want = paged_attention(q, clean, tables, starts, lens, None)
     rows = torch.ones(T, dtype=torch.bool, device=gpu)
@@ -247,15 +247,33 @@ def test_attention_without_pages_or_states(gpu):
     assert paged_attention(q[:0], cache, tables, starts, lens).shape == (0, 2, 32)
 
 
+def test_starts_that_do_not_ascend(gpu):
+    """They get no defined rows, but every access stays in bounds and what follows is right."""
+    from openfold3_triangle_kernel_amd import append_kv, paged_attention
+
+    for lengths in ([40, 50, 60], [2000, 50, 60]):
+        cache, tables, starts, lens, T, g = _batch(gpu, [2, 2, 2], lengths, 8, 1, 32, torch.bfloat16)
+        x = torch.randn(T, 1, 32, generator=g).bfloat16().to(gpu)
+        want = paged_attention(x, cache, tables, starts, lens)
+        kept = [t.clone() for t in (cache.k, cache.v)]
+        for bad in ([0, 5, 2, 6], [3, 2, 1, 0], [-7, 1 << 30, -5, 4], [6, 6, 0, 6]):
+            odd = torch.tensor(bad, dtype=torch.int32, device=gpu)
+            assert paged_attention(x, cache, tables, odd, lens).shape == x.shape
+            append_kv(cache, x, x, tables, odd, lens)
+        for t, k in zip((cache.k, cache.v), kept):
+            t.copy_(k)
+        assert torch.equal(paged_attention(x, cache, tables, starts, lens), want)
+
+
 def test_attention_far_pages(gpu):
     """Pages past 32-bit byte offsets."""
     from openfold3_triangle_kernel_amd import PagedCache, paged_attention
 
-    pages = 140000  # of 16 states of 2 kv heads of 128: 1.1 GB... times 2 bytes each
+    pages = 540000  # of 16 states of 2 kv heads of 128: 4.4 GB each
     k, v = (torch.zeros(pages, 2, 16, 128, device=gpu, dtype=torch.bfloat16) for _ in range(2))
     g = torch.Generator().manual_seed(4)
     small = [torch.randn(6, 2, 16, 128, generator=g).bfloat16().to(gpu) for _ in range(2)]
-    at = torch.tensor([3, pages - 1, 131072, 70001, 139990, 65535], device=gpu)
+    at = torch.tensor([3, pages - 1, 131072, 270001, 524288, 65535], device=gpu)
     k[at], v[at] = small
     starts, lens = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0, 5], [90]))
     q = torch.randn(5, 4, 128, generator=g).bfloat16().to(gpu)

@@ -134,6 +134,8 @@ FORWARD = [
     (2, 64, 64, 600, 64, 128, 4, "bf16", "head", "none"),  # 256 rows a workgroup
     (4, 64, 64, 513, 32, 0, 0, "fp16", "seq", "random"),
     (1, 40, 1, 70, 64, 9, 2, "bf16", "seq", "none"),
+    (1, 300, 1, 20, 32, 4, 1, "fp16", "head", "tail"),
+    (3, 1, 1, 1, 128, 1, 0, "bf16", "seq", "tail"),
 ]
 
 
@@ -170,6 +172,9 @@ BACKWARD = [
     (1, 5, 1, 400, 20, 3, 1, "head", "none"),
     (1, 40, 1, 40, 32, 9, 2, "seq", "none"),
     (1, 2, 2, 260, 72, 500, 9, "head", "tail"),
+    (1, 2, 1, 900, 64, 5, 600, "head", "none"),  # most tokens are sinks
+    (1, 2, 1, 300, 32, 5, 300, "seq", "tail"),  # all are
+    (2, 200, 1, 20, 64, 4, 1, "head", "none"),  # more heads to a kv head than a tile has rows
 ]
 
 

@@ -310,3 +310,25 @@ def test_traces_hold_the_operators(fake):
     for name, (call, operands) in _calls().items():
         graph = str(torch.jit.trace(call, operands, check_trace=False).graph)
         assert "^_" in graph, f"{name}: no node for the operator in\n{graph}"
+
+
+def test_sizes_that_a_launch_does_not_hold():
+    """Refused before any launch, the backward's before the forward."""
+    meta = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device="meta")  # noqa: E731
+    with pytest.raises(ValueError, match="2\\^26"):
+        qk_norm_rotary(meta(1, 1, 1 << 26, 8), meta(1, 1, 1 << 26, 8))
+    with pytest.raises(ValueError, match="65535 heads"):
+        qk_norm_rotary(meta(1, 65536, 1, 8), meta(1, 1, 1, 8))
+    most = (1 << 24) - 8
+    shape = lambda B, H, Hk, N, window=0, sinks=0: (ctypes.c_int64 * 18)(  # noqa: E731
+        B, H, Hk, N, 8, 0, window, sinks, 0)
+    forward = lambda *a: _native.query("tpf_window_forward_workspace_bytes", shape(*a)) >= 0  # noqa: E731
+    backward = lambda *a: _native.query("tpf_window_backward_workspace_bytes", shape(*a)) >= 0  # noqa: E731
+    assert forward(most // 16, 1, 1, 1) and backward(most // 16, 1, 1, 1)
+    assert not forward(most, 1, 1, 1) and not backward(most, 1, 1, 1)
+    assert not forward(1, 1, 1, (1 << 30) + 1) and not forward(1, 1 << 20, 1, 1 << 11)
+    assert forward(1, 1, 1, 1 << 28) and backward(1, 1, 1, 1 << 20)
+    # Sinks take memory for 2048 parts at most, whatever their number is.
+    for sinks in (1, 4, 1000, 16383, 16384, 1 << 30):
+        size = _native.query("tpf_window_backward_workspace_bytes", shape(1, 4, 1, 16384, 1, sinks))
+        assert 0 < size <= (2048 + 128) * 128 * 8 * 8 + 16 * 16384 + 2 * 16384 * 8 * 4 * 16
