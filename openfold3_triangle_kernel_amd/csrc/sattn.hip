@@ -788,10 +788,13 @@ static int sattn_splits(int64_t units, int64_t target, int64_t states) {
   return (int)(s < 1 ? 1 : s);
 }
 
-// 128 rows a workgroup, 256 up to 64 channels where those fill the chip twice.
+// 128 rows a workgroup, 256 up to 32 channels where those fill the chip twice: each K and V
+// fragment then feeds two products (16 heads on 4, 16384 tokens, window 1024: 76 us against 81
+// with 32 channels; with 64, whose registers leave no third wave to a SIMD, 203 us instead of 213
+// for 2 x 32 heads on 8, 4096 tokens, from 128 rows).
 static int window_plan(SAttnArgs& a) {
   const int64_t BH = (int64_t)a.B * a.Hk;
-  const int qb = a.D <= 64 && BH * ((a.R + 255) / 256) >= 512 ? 2 : 1;
+  const int qb = a.D <= 32 && BH * ((a.R + 255) / 256) >= 512 ? 2 : 1;
   a.tiles = (a.R + 128 * qb - 1) / (128 * qb);
   a.splits = sattn_splits(BH * a.tiles, 256, a.N);
   a.order = sa_order(BH, (int64_t)a.tiles * a.splits);
@@ -801,7 +804,7 @@ static int window_plan(SAttnArgs& a) {
 template <int DP, bool F16, bool STATS>
 static void window_launch(const SAttnArgs& a, int qb, hipStream_t s) {
   const dim3 grid((unsigned)a.order.groups);
-  if constexpr (DP <= 64) {
+  if constexpr (DP <= 32) {
     if (qb == 2) {
       hipLaunchKernelGGL((sattn_fwd_kernel<DP, 2, F16, STATS, false>), grid, dim3(256), 0, s, a);
       return;

@@ -131,7 +131,8 @@ FORWARD = [
     (1, 1, 1, 2049, 32, 0, 0, "fp16", "head", "none"),
     (1, 1, 1, 1100, 128, 1, 500, "bf16", "head", "none"),
     (1, 4, 1, 700, 48, 2000, 9, "bf16", "seq", "head"),  # a window past the tokens
-    (2, 64, 64, 600, 64, 128, 4, "bf16", "head", "none"),  # 256 rows a workgroup
+    (2, 64, 64, 600, 64, 128, 4, "bf16", "head", "none"),
+    (4, 64, 64, 600, 32, 128, 4, "bf16", "head", "none"),  # 256 rows a workgroup
     (4, 64, 64, 513, 32, 0, 0, "fp16", "seq", "random"),
     (1, 40, 1, 70, 64, 9, 2, "bf16", "seq", "none"),
     (1, 300, 1, 20, 32, 4, 1, "fp16", "head", "tail"),
@@ -172,6 +173,7 @@ BACKWARD = [
     (1, 5, 1, 400, 20, 3, 1, "head", "none"),
     (1, 40, 1, 40, 32, 9, 2, "seq", "none"),
     (1, 2, 2, 260, 72, 500, 9, "head", "tail"),
+    (8, 64, 64, 130, 24, 50, 2, "head", "tail"),  # 256 rows a workgroup
     (1, 2, 1, 900, 64, 5, 600, "head", "none"),  # most tokens are sinks
     (1, 2, 1, 300, 32, 5, 300, "seq", "tail"),  # all are
     (2, 200, 1, 20, 64, 4, 1, "head", "none"),  # more heads to a kv head than a tile has rows
@@ -233,13 +235,13 @@ def test_shared_heads_and_common_parts(gpu):
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("N,D,window,sinks", [(70, 64, None, 0), (200, 128, 50, 3), (150, 96, 20, 0),
-                                              (130, 32, 7, 100), (600, 64, 128, 4)])
+                                              (130, 32, 7, 100), (600, 64, 128, 4), (260, 32, 128, 4)])
 def test_what_a_row_does_not_see_never_reaches_it(gpu, bad, N, D, window, sinks):
     """Whatever a token holds, the rows that do not see it, and the gradients of the states
     that its row does not see, are those of zeros there; dropped tokens reach nothing."""
     from openfold3_triangle_kernel_amd import window_attention
 
-    heads = (64, 64) if N == 600 else (4, 2)  # (256 rows a workgroup)
+    heads = {600: (64, 64), 260: (256, 128)}.get(N, (4, 2))  # (260: 256 rows a workgroup)
     q, k, v = make(gpu, 2, *heads, N, D, seed=7)
     at = N // 2
     see = seen(torch.arange(N), N, window or 0, sinks).to(gpu)
