@@ -208,20 +208,29 @@ struct STiles {
   }
 };
 
-// Which of the 32 tile rows from rbase on hold a value that is not finite.
-template <int DP, bool F16>
-__device__ __forceinline__ uint32_t sa_bad_rows(const u16* T, int rbase) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  constexpr uint16_t top = F16 ? 0x7c00u : 0x7f80u;
+// The larger exponents of the pairs of x and `most`, whose two halves tell whether any of the
+// values that passed is not finite.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+template <bool F16>
+struct SExponents {
+  static constexpr uint16_t top = F16 ? 0x7c00u : 0x7f80u;
   u16x2 most = {0, 0};
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const u32x4 x = __builtin_bit_cast(u32x4, xa_frag<DP>(T, rbase, s));
+  __device__ __forceinline__ void add(bf16x8 f) {
+    const u32x4 x = __builtin_bit_cast(u32x4, f);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[e] & (top * 0x10001u)));
   }
-  const uint64_t rows = __ballot(most[0] == top || most[1] == top);
+  __device__ __forceinline__ bool bad() const { return most[0] == top || most[1] == top; }
+};
+
+// Which of the 32 tile rows from rbase on hold a value that is not finite.
+template <int DP, bool F16>
+__device__ __forceinline__ uint32_t sa_bad_rows(const u16* T, int rbase) {
+  SExponents<F16> x;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) x.add(xa_frag<DP>(T, rbase, s));
+  const uint64_t rows = __ballot(x.bad());
   return (uint32_t)(rows | rows >> 32);
 }
 // A fragment with zeros in the place of values that are not finite.
@@ -241,14 +250,18 @@ __device__ __forceinline__ bf16x8 sa_finite(bf16x8 f) {
 // there) that hold a value that is not finite; CLEAN: and puts zeros in the values' place.
 template <int DP, int NI, bool F16, bool CLEAN, typename F>
 __device__ __forceinline__ void sa_look(u16* T, int w, F mark) {
+  bf16x8* at = reinterpret_cast<bf16x8*>(T) + 64 * NI * w + (threadIdx.x & 63);
+  SExponents<F16> all;
 #pragma unroll
+  for (int t = 0; t < NI; ++t) all.add(at[64 * t]);
+  if (__ballot(all.bad()) == 0) return;
+#pragma unroll 1
   for (int t = 0; t < NI; ++t) {
-    const int p = 64 * (NI * w + t) + (int)(threadIdx.x & 63);
-    bf16x8* at = reinterpret_cast<bf16x8*>(T) + p;
-    const u32x4 x = __builtin_bit_cast(u32x4, *at), y = __builtin_bit_cast(u32x4, sa_finite<F16>(*at));
-    if (x[0] != y[0] || x[1] != y[1] || x[2] != y[2] || x[3] != y[3]) {
-      if constexpr (CLEAN) *at = __builtin_bit_cast(bf16x8, y);
-      mark(p / (DP / 8));
+    SExponents<F16> x;
+    x.add(at[64 * t]);
+    if (x.bad()) {
+      if constexpr (CLEAN) at[64 * t] = sa_finite<F16>(at[64 * t]);
+      mark((64 * (NI * w + t) + (int)(threadIdx.x & 63)) / (DP / 8));
     }
   }
 }

@@ -115,6 +115,16 @@ __global__ __launch_bounds__(256, 2) void sattn_dq_kernel(SAttnGrad ga) {
     }
   }
   delta = xor32_sum(delta);
+  {
+    // A row whose Q or dO is not finite has no delta: the other launch tells it by that.
+    SExponents<false> x;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      x.add(q[s]);
+      x.add(dO[s]);
+    }
+    if (xor32_sum(x.bad() ? 1.f : 0.f) != 0.f) delta = __builtin_nanf("");
+  }
   const float lse = ga.lse[bh * a.R + rc];
   if (lane < 32 && r < a.R) ga.delta[bh * a.R + r] = delta;
 
@@ -377,11 +387,15 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
       if (r0 + RT < rend) issue(r0 + RT, st ^ 1);
       u16 *Q = smem[st][0], *dO = smem[st][1];
       if (r0 < tfrom || r0 + RT > tto) {
-        // A row whose Q or dO is not finite: its statistic makes p and dS NaN.
-        auto mark = [&](int row) { stats[st][0][row] = __builtin_nanf(""); };
-        sa_look<DP, NI, false, true>(Q, w, mark);
-        sa_look<DP, NI, false, true>(dO, w, mark);
-        lds_barrier();
+        // Rows whose Q or dO is not finite (of those without a delta): the statistic makes p and
+        // dS NaN.  All waves see the same.
+        const float de = stats[st][1][lane & (RT - 1)];
+        if (__ballot(de != de)) {
+          auto mark = [&](int row) { stats[st][0][row] = __builtin_nanf(""); };
+          sa_look<DP, NI, false, true>(Q, w, mark);
+          sa_look<DP, NI, false, true>(dO, w, mark);
+          lds_barrier();
+        }
       }
 #pragma unroll
       for (int rb = 0; rb < RT / 32; ++rb) {
