@@ -258,9 +258,10 @@ __device__ __forceinline__ bool grad_unit(const SAttnGrad& ga, int unit, int* ti
 // dK and dV: four waves of 32 states each pass over tiles of RT of the rows that see them.
 // A state's column of the tiles depends on that state alone, so dead states are left to run
 // and their gradients written as 0.  Above 64 channels V stays in LDS (and at 128 the tiles
-// have 32 rows), so that a wave fits 256 registers and two run on a SIMD.
+// have 32 rows), so that a wave fits 256 registers and two run on a SIMD; with 64 channels three
+// do (16 heads on 4, 16384 tokens, window 1024: 225 us against 249 with two).
 template <int DP>
-__global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void sattn_dkdv_kernel(SAttnGrad ga) {
   constexpr bool VLDS = DP > 64;
   constexpr int RT = DP == 128 ? 32 : 64, TILE = RT * DP, DS = DP / 16, DB = DP / 32, CPR = DP / 8;
   constexpr int NI = RT * CPR / 256;
@@ -268,9 +269,10 @@ __global__ __launch_bounds__(256, 2) void sattn_dkdv_kernel(SAttnGrad ga) {
   __shared__ __attribute__((aligned(1024))) u16 smem[2][2][TILE];
   __shared__ __attribute__((aligned(1024))) float stats[2][2][64];
   __shared__ __attribute__((aligned(1024))) u16 vs[VLDS ? 128 * DP : 8];
-  // What each thread keeps here instead of in registers: above 64 channels none are left, and a
-  // spilled one's return from memory would wait for every load under way.
-  constexpr int KEPT = DP == 128 ? 2 + 2 * NI : DP > 64 ? 2 : 0;
+  // What each thread keeps here instead of in registers: from 64 channels on none are left, and
+  // a spilled one's return from memory would wait for every load under way (with 128 channels
+  // the launch took 1026 us instead of 639 so).
+  constexpr int KEPT = DP == 128 || DP == 64 ? 2 + 2 * NI : DP > 64 ? 2 : 0;
   __shared__ int kept[KEPT ? KEPT : 1][256];
   const SAttnArgs& a = ga.f;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
