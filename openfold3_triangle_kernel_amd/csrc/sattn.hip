@@ -252,8 +252,8 @@ struct SResult {
 // An even share of a paged batch's work.  Sequence s costs c_s = (row tiles) x (state tiles of
 // its span); the kv heads' sequences' row tiles' state tiles, in this order, are one axis of
 // Hk sum(c) tiles, of which workgroup w takes `share`, from w * share on: as many as every
-// other, whatever the lengths are (one workgroup a part of a sequence: 16 of 2047 to 8190
-// states left CUs idle a third of the time).  A unit (head, sequence, row tile) whose tiles
+// other, whatever the lengths are (16 tokens of sequences of 2047 to 8190 states: 89 us with the
+// join, 99 with a workgroup a part of a sequence and branches around the pages' addresses).  A unit (head, sequence, row tile) whose tiles
 // are all a workgroup's own is finished there; others leave a part in slot 2 w (one that began
 // before the workgroup's share) or 2 w + 1, and sattn_even_join_kernel finds the slots by the same sums.  Lane
 // l holds sequence l (64 at most).
@@ -436,7 +436,9 @@ __device__ __forceinline__ void sattn_tile(const SAttnArgs& a, u16 (*smem)[2][64
 
 // As many workgroups a CU as the registers hold without spilling (2 x 32 heads on 8, 4096 tokens
 // of 64 channels: 190 us with four, 203 with the three that the compiler would leave).  128
-// channels, with the backward's statistics: 340 us, 810 TFLOP/s of the two products.
+// channels, with the backward's statistics: 340 us, 810 TFLOP/s of the two products.  Paged, 8
+// chunks of up to 512 tokens, 16 heads on 4 of 96, window 2048: 66 us, with a part's first loads
+// and its way out and back through the join (16 us) in each of the two or three units a workgroup.
 template <int DP, int QB, bool F16, bool STATS, bool PAGED>
 __global__ __launch_bounds__(256, PAGED ? 2 : DP == 64 ? 4 : DP == 96 ? 3 : 2)
 void sattn_fwd_kernel(SAttnArgs a) {
@@ -479,7 +481,8 @@ void sattn_fwd_kernel(SAttnArgs a) {
 
 // Few rows of a sequence (32 a workgroup; one decoded token above all): the states' bytes
 // are the bound.  Every wave streams tiles of 32 states of its own, two stages deep without
-// a barrier, and the four waves' results meet in LDS at the end.
+// a barrier, and the four waves' results meet in LDS at the end.  16 tokens of 32 heads on 8 of
+// 128 over 403 MB of states: 81-85 us, 4.9 TB/s, the rate of a copy (the loads alone: 75-80).
 template <int DP, bool F16>
 __device__ __forceinline__ void sattn_few(const SAttnArgs& a, u16 (*smem)[2][2][32 * DP], uint32_t* poison,
                                           int hk, const STile& at, const SSpan& span, int first, int end,
@@ -793,8 +796,8 @@ static int sattn_splits(int64_t units, int64_t target, int64_t states) {
 
 // 128 rows a workgroup, 256 up to 32 channels where those fill the chip twice: each K and V
 // fragment then feeds two products (16 heads on 4, 16384 tokens, window 1024: 76 us against 81
-// with 32 channels; with 64, whose registers leave no third wave to a SIMD, 203 us instead of 213
-// for 2 x 32 heads on 8, 4096 tokens, from 128 rows).
+// with 32 channels).  With 64 channels 128 rows are faster, whose registers let more waves run on
+// a SIMD (2 x 32 heads on 8, 4096 tokens: 203 us with three against 213 with 256 rows).
 static int window_plan(SAttnArgs& a) {
   const int64_t BH = (int64_t)a.B * a.Hk;
   const int qb = a.D <= 32 && BH * ((a.R + 255) / 256) >= 512 ? 2 : 1;

@@ -8,9 +8,11 @@
 // attention's (xattn_bwd.hip): the first forms dQ and delta, a wave's lanes holding rows;
 // the second dK and dV, a wave's lanes holding states.  A state is seen by a run of rows:
 // from its own token's on, to the end of its window, or of the tokens for the sinks.  The
-// sinks' tiles of states therefore have far more rows than the others; their rows are split
-// over workgroups whose 32-bit sums are added in ascending order, so results do not change
-// from call to call.  7 products of 2 D operations a visible pair; bound by the matrix cores.
+// sinks' tiles of states therefore have far more rows than the others, and without a window the
+// first tiles twice the mean's; rows are split over workgroups whose 32-bit sums are added in
+// ascending order, so results do not change from call to call.  7 products of 2 D operations a
+// visible pair; bound by the matrix cores.  2 x 4096 tokens, 32 heads on 8 of 128: dQ 472 us (870
+// TFLOP/s), dK and dV 606 (900), the fold 20.
 #include "sattn.hpp"
 
 namespace tpf {
