@@ -82,7 +82,9 @@ class SelfAttention(AttentionBlock):
     def _rotation(self, device):
         f = self._frequencies.get(str(device))
         if f is None:
-            f = self._frequencies[str(device)] = self._frequencies["cpu"].to(device)
+            # (Outside inference mode, whose tensors a later backward could not keep.)
+            with torch.inference_mode(False):
+                f = self._frequencies[str(device)] = self._frequencies["cpu"].to(device)
         return f if len(f) else None
 
     def _streams(self, x: torch.Tensor, kernels: bool):
@@ -121,7 +123,7 @@ class SelfAttention(AttentionBlock):
         """New tokens ``x`` ``[T, c_in]`` of the sequences that ``tables``, ``starts`` and
         ``lengths`` describe (``append_kv``): their keys and values go into ``cache``, their
         rows are what ``forward`` gives for them among their sequences' tokens.  Inference,
-        on the kernels alone; can be captured and replayed."""
+        on the kernels alone; can be captured and replayed (after a first call on the device)."""
         ok, reason = self._supported(x)
         if not ok:
             raise ValueError(f"unsupported self-attention step: {reason}")

@@ -183,3 +183,13 @@ def test_stock_route_agrees(gpu):
     assert _rel(want, got) <= 12 * 2.0 ** -8
     with pytest.raises(ValueError, match="BF16"):
         block.step(x[0].float(), None, None, None, None)
+
+
+def test_trains_after_inference_mode(gpu):
+    block = _make(gpu)
+    x = torch.randn(1, 40, 128, device=gpu).bfloat16()
+    with torch.inference_mode():
+        want = block(x)
+    out = block(x)
+    out.float().sum().backward()
+    assert torch.equal(out, want) and all(p.grad is not None for p in block.parameters())

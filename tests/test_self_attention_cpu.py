@@ -332,3 +332,13 @@ def test_sizes_that_a_launch_does_not_hold():
     for sinks in (1, 4, 1000, 16383, 16384, 1 << 30):
         size = _native.query("tpf_window_backward_workspace_bytes", shape(1, 4, 1, 16384, 1, sinks))
         assert 0 < size <= (2048 + 128) * 128 * 8 * 8 + 16 * 16384 + 2 * 16384 * 8 * 4 * 16
+
+
+def test_frequencies_first_used_in_inference_mode_train():
+    """A backward keeps the device's copy: it is no inference tensor, whoever makes it."""
+    from openfold3_triangle_kernel_amd import SelfAttention
+
+    block = SelfAttention(16, 8, 2)
+    with torch.inference_mode():
+        copy = block._rotation(torch.device("meta"))
+    assert copy is block._rotation(torch.device("meta")) and not copy.is_inference()
