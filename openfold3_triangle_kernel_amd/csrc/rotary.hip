@@ -698,7 +698,7 @@ extern "C" int tpf_paged_append(const void* q, const void* k, const void* v, con
   if (int rc = tpf::rot_check(r, 1, batch->T, s->H, s->Hk, s->Hk, s->D, s->half, s->dtype, s->weight_dtype,
                               eps, s->norm != 0, s->interleaved != 0, false, fn))
     return rc;
-  if (!k || !v || !k_cache || !v_cache || (s->H && (!q || !q_out)) || (s->half && !frequencies))
+  if (!k || !v || (batch->pages && (!k_cache || !v_cache)) || (s->H && (!q || !q_out)) || (s->half && !frequencies))
     return tpf::set_error(TPF_ERR_ARG, "%s: null pointer", fn);
   r.x[0] = q; r.x[1] = k; r.x[2] = v;
   r.y[0] = q_out; r.y[1] = k_cache; r.y[2] = v_cache;

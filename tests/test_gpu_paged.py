@@ -341,3 +341,23 @@ def test_prompt_then_tokens(gpu):
         assert torch.equal(turned, heads(tq[0])[rows])
         out = paged_attention(turned, cache, table, starts, lens, window, sinks)
         check([heads(out)], [want[0][:, rows]], [err[0][:, rows]])
+
+
+def test_append_to_nothing(gpu):
+    """A cache without pages, tables without entries, no sequences: queries are turned all the
+    same where they have a sequence, and nothing is written."""
+    from openfold3_triangle_kernel_amd import PagedCache, append_kv
+
+    cache, tables, starts, lens, T, g = _batch(gpu, [3, 3], [40, 50], 8, 1, 32, torch.bfloat16)
+    q, k = (torch.randn(T, 1, 32, generator=g).bfloat16().to(gpu) for _ in range(2))
+    freq = torch.tensor([1.0, 0.1], dtype=torch.float64, device=gpu)
+    before = [t.clone() for t in (cache.k, cache.v)]
+    want = append_kv(PagedCache.of(*(t.clone() for t in before)), k, k, tables, starts, lens, q, freq)
+    empty = PagedCache.of(cache.k[:0], cache.v[:0])
+    assert torch.equal(append_kv(empty, k, k, tables, starts, lens, q, freq), want)
+    lens.clamp_(max=0)  # (what a table without entries holds)
+    short = append_kv(cache, k, k, tables[:, :0], starts, lens, q, freq)
+    assert torch.equal(short, append_kv(cache, k, k, tables, starts, lens, q, freq))
+    assert not append_kv(cache, k, k, tables[:0], starts[:1], lens[:0], q, freq).any()
+    assert append_kv(cache, k[:0], k[:0], tables, starts, lens, q[:0]).shape == (0, 1, 32)
+    assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1])

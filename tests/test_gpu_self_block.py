@@ -193,3 +193,17 @@ def test_trains_after_inference_mode(gpu):
     out = block(x)
     out.float().sum().backward()
     assert torch.equal(out, want) and all(p.grad is not None for p in block.parameters())
+
+
+def test_block_without_tokens(gpu):
+    block = _make(gpu)
+    x = torch.zeros(2, 0, 128, device=gpu, dtype=torch.bfloat16, requires_grad=True)
+    out = block(x)
+    out.sum().backward()
+    assert out.shape == x.shape and x.grad.shape == x.shape
+    cache = block.new_cache(2, 8, gpu)
+    none = torch.zeros(0, dtype=torch.int32, device=gpu)
+    out = block.step(x.detach()[0], cache, none.reshape(0, 1), none.new_zeros(1), none)
+    assert out.shape == (0, 128)
+    out = block.step(torch.randn(3, 128, device=gpu).bfloat16(), cache, none.reshape(0, 1), none.new_zeros(1), none)
+    assert not out.any() and not cache.k.any()  # tokens of no sequence
