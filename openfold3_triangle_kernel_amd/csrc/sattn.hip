@@ -256,7 +256,9 @@ struct SResult {
 // join, 99 with a workgroup a part of a sequence and branches around the pages' addresses).  A unit (head, sequence, row tile) whose tiles
 // are all a workgroup's own is finished there; others leave a part in slot 2 w (one that began
 // before the workgroup's share) or 2 w + 1, and sattn_even_join_kernel finds the slots by the same sums.  Lane
-// l holds sequence l (64 at most).
+// l holds sequence l (64 at most).  c_s counts a row tile's own span, and an XCD has
+// neighbouring workgroups, whose row tiles pass over the same states, also in the join (8 chunks
+// of up to 512 tokens, 16 heads on 4 of 96, window 2048, with the join: 67 us against 74).
 struct SEven {
   int first, cost, tiles;  // before the sequence, its own, of its span
   int total, share;        // of a head, of a workgroup
@@ -269,6 +271,8 @@ struct SEven {
     // (Starts that do not ascend may ask for more rows than there are, and are not served.)
     const bool fits = lanes_sum<64>((float)fresh) <= 1.01f * (float)a.t.T;
     tiles = fresh && fits ? SSpan(len - fresh, len - 1, a.window, a.sinks).n : 0;
+    // A row tile's own span, of (rt + G - 2) / G + 1 tokens at most, has at most this many.
+    tiles = min(tiles, (a.sinks + 63) / 64 + (a.window + (rt - 2) / a.G + 63) / 64 + 1);
     cost = (fresh * a.G + rt - 1) / rt * tiles;
     int sum = cost;
 #pragma unroll
@@ -290,7 +294,9 @@ __device__ __forceinline__ void sa_even_units(const SAttnArgs& a, int rt, F f) {
   SEven e;
   e.init(a, rt);
   if (e.total == 0) return;
-  const int w = blockIdx.x;
+  // (An XCD's workgroups, blockIdx % 8, take neighbouring runs: row tiles over the same states
+  // then find them in its L2.)
+  const int w = (int)(blockIdx.x & 7) * (a.even >> 3) + (int)(blockIdx.x >> 3);
   int64_t x = (int64_t)w * e.share;
   const int64_t end = min(x + e.share, (int64_t)a.Hk * e.total);
   while (x < end) {
@@ -302,8 +308,10 @@ __device__ __forceinline__ void sa_even_units(const SAttnArgs& a, int rt, F f) {
     STile at;
     at.sequence(a, s);
     at.r0 = tile * rt;
-    const SSpan span(at.pos, at.pos + at.R / a.G - 1, a.window, a.sinks);
-    f(hk, at, span, t0, t0 + count, SResult{count == n, (int64_t)(2 * w + (t0 == 0 ? 1 : 0)) * rt, 1});
+    const SSpan span(sa_scalar(at.position(a, at.r0)), sa_scalar(at.position(a, at.r0 + rt - 1)), a.window,
+                     a.sinks);  // (n tiles or fewer)
+    f(hk, at, span, min(t0, span.n), min(t0 + count, span.n),
+      SResult{count == n, (int64_t)(2 * w + (t0 == 0 ? 1 : 0)) * rt, 1});
     x += count;
   }
 }
@@ -437,8 +445,8 @@ __device__ __forceinline__ void sattn_tile(const SAttnArgs& a, u16 (*smem)[2][64
 // As many workgroups a CU as the registers hold without spilling (2 x 32 heads on 8, 4096 tokens
 // of 64 channels: 190 us with four, 203 with the three that the compiler would leave).  128
 // channels, with the backward's statistics: 340 us, 810 TFLOP/s of the two products.  Paged, 8
-// chunks of up to 512 tokens, 16 heads on 4 of 96, window 2048: 66 us, with a part's first loads
-// and its way out and back through the join (16 us) in each of the two or three units a workgroup.
+// chunks of up to 512 tokens, 16 heads on 4 of 96, window 2048: 62 us, with a part's first loads
+// and its way out and back through the join (12 us) in each of the two or three units a workgroup.
 template <int DP, int QB, bool F16, bool STATS, bool PAGED>
 __global__ __launch_bounds__(256, PAGED ? 2 : DP == 64 ? 4 : DP == 96 ? 3 : 2)
 void sattn_fwd_kernel(SAttnArgs a) {
@@ -682,11 +690,14 @@ __global__ __launch_bounds__(256) void sattn_join_kernel(SAttnArgs a, int rt) {
 // zeros of tokens that see nothing (of no sequence, or of one without states), a wave a token.
 template <bool F16>
 __global__ __launch_bounds__(256) void sattn_even_join_kernel(SAttnArgs a, int rt) {
-  const int lane = threadIdx.x & 63, each = rt / 32, w = (int)sa_div(blockIdx.x, (uint32_t)each);
+  // (Each XCD joins what its own workgroups left: a.even is a multiple of eight.)
+  const int lane = threadIdx.x & 63, each = rt / 32, joins = a.even * each, block = (int)blockIdx.x;
+  const int item = block < joins ? (block & 7) * (joins >> 3) + (block >> 3) : block;
+  const int w = (int)sa_div((uint32_t)item, (uint32_t)each);
   SEven e;
   e.init(a, rt);
   if (w >= a.even) {
-    const int64_t token = (int64_t)(blockIdx.x - a.even * each) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t token = (int64_t)(block - joins) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (token >= a.t.T) return;
     const int s = __builtin_amdgcn_readfirstlane(
         paged_search(a.t.S, [&](int x) { return paged_start(a.t, x) <= token; }));
@@ -708,26 +719,40 @@ __global__ __launch_bounds__(256) void sattn_even_join_kernel(SAttnArgs a, int r
   at.sequence(a, s);
   const int rows = min(rt, at.R - tile * rt), d = 4 * (threadIdx.x & 31);
   if (d >= a.D) return;
-  const int first = 32 * ((int)blockIdx.x - w * each);
-  for (int r = first + (int)(threadIdx.x >> 5); r < min(rows, first + 32); r += 8) {
-    // Slot 2 (w - 1) + 1, then 2 w, 2 w + 2, ...
-    auto part = [&](int i) { return (int64_t)(i ? 2 * (w + i - 1) : 2 * w - 1) * rt + r; };
-    float m = kSaLow;
-    for (int i = 0; i < parts; ++i) m = xa_max(m, a.part_ml[3 * part(i)]);
-    float sum = 0.f;
-    f32x4 o = (f32x4)0.f;
-    for (int i = 0; i < parts; ++i) {
-      const int64_t p = part(i);
-      const float f = fast_exp2((a.part_ml[3 * p] - m) * a.c);
-      sum = fmaf(f, a.part_ml[3 * p + 2], sum);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + p * a.D + d);
+  // Four rows a thread, whose loads go out together.
+  const int first = 32 * (item - w * each) + (int)(threadIdx.x >> 5);
+  int r[4];
+  float m[4], sum[4];
+  f32x4 o[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] = fmaf(f, v[c], o[c]);
+  for (int u = 0; u < 4; ++u) {
+    r[u] = min(first + 8 * u, rows - 1);
+    m[u] = kSaLow;
+    sum[u] = 0.f;
+    o[u] = (f32x4)0.f;
+  }
+#pragma unroll 2
+  for (int i = 0; i < parts; ++i) {
+    // Slot 2 (w - 1) + 1, then 2 w, 2 w + 2, ...
+    const int64_t slot = (int64_t)(i ? 2 * (w + i - 1) : 2 * w - 1) * rt;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float mi = a.part_ml[3 * (slot + r[u])], ni = a.part_ml[3 * (slot + r[u]) + 2];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + (slot + r[u]) * a.D + d);
+      const float to = xa_max(m[u], mi), f = fast_exp2((m[u] - to) * a.c), g = fast_exp2((mi - to) * a.c);
+      m[u] = to;
+      sum[u] = fmaf(g, ni, f * sum[u]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[u][c] = fmaf(g, v[c], f * o[u][c]);
     }
-    const float inv = sa_inverse(sum, m);
-    const int all = tile * rt + r, i = (int)fdiv((uint32_t)all, a.div_g), g = all - i * a.G;
-    sa_store4<F16>(a, ((at.token + i) * a.H + hk * a.G + g) * a.D + d, o[0] * inv, o[1] * inv, o[2] * inv,
-                   o[3] * inv);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (first + 8 * u >= rows) break;
+    const float inv = sa_inverse(sum[u], m[u]);
+    const int all = tile * rt + r[u], i = (int)fdiv((uint32_t)all, a.div_g), g = all - i * a.G;
+    sa_store4<F16>(a, ((at.token + i) * a.H + hk * a.G + g) * a.D + d, o[u][0] * inv, o[u][1] * inv,
+                   o[u][2] * inv, o[u][3] * inv);
   }
 }
 
