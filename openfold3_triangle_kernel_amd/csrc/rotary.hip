@@ -465,12 +465,16 @@ __global__ __launch_bounds__(256) void rot_fold_kernel(const float* part, int gr
 
 // A token's heads are shared by waves as long as there are fewer than 16384 (8192 backward,
 // whose workgroups take several tokens): 2 x 4096 tokens, 32 + 8 heads of 128 in 40 us forward
-// against 45 with 8192 and 43 with 40960; backward 71 against 79 with 16384.
+// against 45 with 8192 and 43 with 40960; backward 71 against 79 with 16384.  An append's waves
+// first find their token's place: 4096 (8 chunks of up to 1024 tokens, 16 heads of 80 and as many
+// keys and values: 22 us against 23 with 8192 and 24 with 16384; 8 of 256, 32 heads on 8 of 128: 14, 14, 16).
 static void rot_plan(RotArgs& r, int rows_per_wave, bool backward) {
   const int total = r.heads[0] + r.heads[1] + r.heads[2];
   const int most = (total + rows_per_wave - 1) / rows_per_wave;
-  int64_t s = ((backward ? 8192 : 16384) + r.tokens - 1) / r.tokens;
-  r.slices = (int)(s < 1 ? 1 : s > most ? most : s);
+  int64_t s = ((backward ? 8192 : r.heads[2] ? 4096 : 16384) + r.tokens - 1) / r.tokens;
+  s = s < 1 ? 1 : s > most ? most : s;
+  const int64_t turns = (most + s - 1) / s;  // (as few waves as take no more of them)
+  r.slices = (int)((most + turns - 1) / turns);
   r.div_slices = make_fastdiv((uint32_t)r.slices);
   r.div_n = make_fastdiv((uint32_t)r.N);
 }
