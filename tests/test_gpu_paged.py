@@ -182,6 +182,29 @@ def test_attention(gpu, case):
         check([again[rows]], [want], [err])
 
 
+@pytest.mark.parametrize("group", [1, 3, 5, 40])
+@pytest.mark.parametrize("sinks", [0, 1, 64, 129])
+def test_attention_spans(gpu, group, sinks):
+    """Row tiles whose spans begin and end anywhere in the tiles of states, shared evenly: of
+    whole chunks, and of tokens that begin before the first state."""
+    from test_gpu_window_attention import check
+
+    from openfold3_triangle_kernel_amd import paged_attention
+
+    news, lengths = [150, 3, 64, 61], [1337, 1200, 64, 1088]
+    cache, tables, starts, lens, T, g = _batch(gpu, news, lengths, 16, 1, 32, torch.bfloat16)
+    q = torch.randn(T, group, 32, generator=g).bfloat16().to(gpu)
+    for window in (1, 2, 63, 64, 65, 127, 1025):
+        out = paged_attention(q, cache, tables, starts, lens, window, sinks)
+        for rows, want, err in _attended(q, cache, tables, news, lengths, window, sinks):
+            check([out[rows]], [want], [err])
+    fewer = lens.clone()
+    fewer[2] = 20  # 64 new tokens, the last 20 of them states
+    out = paged_attention(q, cache, tables, starts, fewer, 65, sinks)
+    first = sum(news[:2])
+    assert not out[first:first + 44].any() and out[first + 44:first + 64].abs().amax(-1).min() > 0
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("new,lengths", [(1, [333, 200]), (60, [333, 200]), (1, [3333, 2000]), (60, [2333, 90])])
 def test_attention_never_reads_what_is_not_there(gpu, bad, new, lengths):
