@@ -200,6 +200,16 @@ def test_backward(gpu, case):
         assert not (grads[1] * dead).any() and not (grads[2] * dead).any()
 
 
+@pytest.mark.parametrize("case", [
+    # Parts of the states' rows that take turns: the last one shorter than the others.
+    (10, 16, 8, 640, 32, 400, 3, "seq", "none"),
+    (20, 9, 3, 600, 64, 400, 130, "head", "tail"),
+    (5, 16, 4, 2000, 128, 470, 1, "seq", "none"),
+], ids=str)
+def test_backward_in_uneven_parts(gpu, case):
+    test_backward(gpu, case)
+
+
 def test_gradients_against_differences(gpu):
     """Directional differences of the 64-bit formula at the BF16 operands: the gradient's own
     roundings (2^-9 relative, a few of them) bound the deviation."""
