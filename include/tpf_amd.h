@@ -654,8 +654,11 @@ int tpf_rotary_backward(const void* q, const void* k, const void* dq_out, const 
  * read there alone: starts are held to [0, T], lengths to the table's width, and a page
  * outside [0, pages) holds no state (it is neither written nor read).
  *
- * tpf_paged_row: page * page size + place of a state, -1 where there is none (host
- * arrays; the kernels' own rule).
+ * tpf_paged_row: page * page size + place of a state, -1 where there is none.
+ * tpf_paged_rows: with `group` rows a token (the query heads of a kv head), the sequence of
+ * the attention's tile `at` of tile_rows (32 or 128) rows, or (tile_rows 0) of row `at`; in
+ * rows[3] the tile's first row there, all its rows and its first token; -1 where no
+ * sequence has it.  Both on host arrays, by the functions that the kernels run.
  *
  * tpf_paged_append: norm and rotation (as above, by the states' numbers) of the new keys
  * k [T, Hk, D] on the way into the cache, their values v as they are, and the queries q
@@ -679,6 +682,8 @@ typedef struct tpf_append_shape {
   int64_t q_stride[2], k_stride[2], v_stride[2];
 } tpf_append_shape;
 int64_t tpf_paged_row(const tpf_paged_batch* batch, int64_t s, int64_t state);
+int64_t tpf_paged_rows(const tpf_paged_batch* batch, int64_t group, int64_t tile_rows, int64_t at,
+                       int64_t* rows);
 int tpf_paged_append(const void* q, const void* k, const void* v, const double* frequencies,
                      const void* q_weight, const void* k_weight, double eps, void* q_out,
                      void* k_cache, void* v_cache, const tpf_append_shape* shape,

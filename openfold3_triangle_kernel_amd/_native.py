@@ -166,6 +166,7 @@ SIGNATURES: dict[str, tuple] = {
     "tpf_rotary_backward_workspace_bytes": (_I64, [_P]),
     "tpf_rotary_backward": (_I32, [_P] * 8 + [_F64] + [_P] * 5 + [_I64] + [_P] * 3),
     "tpf_paged_row": (_I64, [_P, _I64, _I64]),
+    "tpf_paged_rows": (_I64, [_P, _I64, _I64, _I64, _P]),
     "tpf_paged_append": (_I32, [_P] * 6 + [_F64] + [_P] * 6),
     "tpf_paged_attention_workspace_bytes": (_I64, [_P, _P]),
     "tpf_paged_attention": (_I32, [_P] * 5 + [_I64, _P, _P, _F64, _P]),

@@ -247,7 +247,7 @@ __global__ __launch_bounds__(256) void rot_fwd_kernel(RotArgs r) {
   int64_t p = n, page = 0, place = 0;
   bool mine = true, placed = false;  // in a sequence; with a place in the cache
   if constexpr (PAGED) {
-    const int s = paged_search(r.t.S, [&](int x) { return paged_start(r.t, x) <= token; });
+    const int s = paged_search<PagedWave>(r.t.S, [&](int x) { return paged_start(r.t, x) <= token; });
     mine = s < r.t.S;
     if (mine) {
       p = paged_length(r.t, s) - paged_start(r.t, s + 1) + token;
@@ -686,6 +686,26 @@ extern "C" int64_t tpf_paged_row(const tpf_paged_batch* batch, int64_t s, int64_
   if (tpf::paged_check(t, batch, "tpf_paged_row") || s < 0 || s >= t.S) return -1;
   int64_t page, place;
   return tpf::paged_place(t, (int)s, state, &page, &place) ? page * t.page + place : -1;
+}
+
+extern "C" int64_t tpf_paged_rows(const tpf_paged_batch* batch, int64_t group, int64_t tile_rows, int64_t at,
+                                  int64_t* rows) {
+  tpf::PagedTables t{};
+  const int64_t lim = (int64_t)1 << 30;
+  if (tpf::paged_check(t, batch, "tpf_paged_rows") || !rows || group < 1 || group > lim / t.T ||
+      t.S > lim / 128 || at < 0)
+    return -1;
+  tpf::PagedRows r;
+  if (tile_rows == 0) {
+    if (at >= t.T * group || !r.row<tpf::PagedHost>(t, (int)group, at)) return -1;
+  } else if ((tile_rows != 32 && tile_rows != 128) || at > t.T * group / tile_rows + t.S ||
+             !r.tile<tpf::PagedHost>(t, (int)group, (int)tile_rows, (int)at)) {
+    return -1;
+  }
+  rows[0] = r.r0;
+  rows[1] = r.R;
+  rows[2] = r.token;
+  return r.s;
 }
 
 extern "C" int tpf_paged_append(const void* q, const void* k, const void* v, const double* frequencies,

@@ -213,28 +213,26 @@ __device__ __forceinline__ void sa_store4(const SAttnArgs& a, int64_t at, float 
 }
 
 // A tile of rows: of which sequence (or batch entry), and where its rows lie.
-struct STile {
-  int s, r0, R, pos;  // first row in the sequence, rows there, the first token's position
-  int64_t token;      // the sequence's first token in the batch
+struct STile : PagedRows {
+  int pos;  // the first token's position
   // Sequence s_ of a paged batch (S: the rows behind the last one, without states).
   __device__ __forceinline__ void sequence(const SAttnArgs& a, int s_) {
-    s = s_;
-    token = paged_start(a.t, s);
-    const int64_t next = s < a.t.S ? paged_start(a.t, s + 1) : a.t.T;
-    const int fresh = (int)(next > token ? next - token : 0);
-    R = sa_scalar(fresh * a.G);
-    pos = sa_scalar(s < a.t.S ? (int)paged_length(a.t, s) - fresh : -fresh);
+    PagedRows::sequence<PagedWave>(a.t, a.G, s_);
+    place(a);
   }
-  // Row tile `tile` of RT rows of a paged batch; false past a sequence's rows.  Sequence s
-  // has the tiles from starts[s] G / RT + s on, which are enough for its rows whatever its
-  // length; the rows behind the last one are those of a sequence S without states.
-  __device__ __forceinline__ bool find(const SAttnArgs& a, int tile, int rt) {
-    // (T G is below 2^30, rt a power of two.)
-    auto before = [&](int x) { return (int)((uint32_t)paged_start(a.t, x) * (uint32_t)a.G / (uint32_t)rt) + x; };
-    s = __builtin_amdgcn_readfirstlane(paged_search(a.t.S, [&](int x) { return before(x) <= tile; }));
-    sequence(a, s);
-    r0 = sa_scalar((tile - before(s)) * rt);
-    return r0 < R;
+  // Row tile `tile` of RT rows of a paged batch, or its row `at`; false where there is none.
+  __device__ __forceinline__ bool find(const SAttnArgs& a, int at, int rt) {
+    const bool in = tile<PagedWave>(a.t, a.G, rt, at);
+    place(a);
+    return in;
+  }
+  __device__ __forceinline__ bool find(const SAttnArgs& a, int64_t at) {
+    const bool in = row<PagedWave>(a.t, a.G, at);
+    place(a);
+    return in;
+  }
+  __device__ __forceinline__ void place(const SAttnArgs& a) {
+    pos = sa_scalar(s < a.t.S ? (int)paged_length(a.t, s) - fresh : -fresh);
   }
   __device__ __forceinline__ int position(const SAttnArgs& a, int r) const {
     return pos + (int)fdiv((uint32_t)(r < R ? r : R - 1), a.div_g);
@@ -627,16 +625,14 @@ __global__ __launch_bounds__(256) void sattn_join_kernel(SAttnArgs a, int rt) {
   const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= a.Hk * a.rows) return;
   const int hk = (int)(item / a.rows);
-  const int64_t row = item - hk * a.rows, token = row / a.G;
+  const int64_t row = item - hk * a.rows;
   STile at;
   int r;
   if constexpr (PAGED) {
-    at.sequence(a, __builtin_amdgcn_readfirstlane(
-        paged_search(a.t.S, [&](int x) { return paged_start(a.t, x) <= token; })));
-    r = (int)(row - at.token * a.G);
-    if (r >= at.R) return;  // (starts that do not ascend)
+    if (!at.find(a, row)) return;
+    r = at.r0;
   } else {
-    at.s = (int)(token / a.N);
+    at.s = (int)(row / a.R);
     at.token = (int64_t)at.s * a.N;
     at.R = a.R;
     at.pos = 0;
@@ -700,7 +696,7 @@ __global__ __launch_bounds__(256) void sattn_even_join_kernel(SAttnArgs a, int r
     const int64_t token = (int64_t)(block - joins) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (token >= a.t.T) return;
     const int s = __builtin_amdgcn_readfirstlane(
-        paged_search(a.t.S, [&](int x) { return paged_start(a.t, x) <= token; }));
+        paged_search<PagedWave>(a.t.S, [&](int x) { return paged_start(a.t, x) <= token; }));
     if (s < a.t.S && __shfl(e.tiles, s) != 0) return;
     uint2* out = reinterpret_cast<uint2*>(a.out + token * a.H * a.D);
     for (int i = lane; i < a.H * a.D / 4; i += 64) out[i] = uint2{0, 0};

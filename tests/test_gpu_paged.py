@@ -288,6 +288,28 @@ def test_starts_that_do_not_ascend(gpu):
         assert torch.equal(paged_attention(x, cache, tables, starts, lens), want)
 
 
+@pytest.mark.parametrize("news,length,heads", [
+    ([60, 50, 90], 600, 8),      # parts of the states and their join, tiles of many rows
+    ([100, 100, 100], 300, 4),   # whole tiles
+    ([2] * 70, 520, 8),          # few rows a sequence
+    ([7, 30, 1] * 25, 300, 12),  # more sequences than lanes
+], ids=str)
+def test_starts_that_do_not_ascend_in_tiles_of_many_rows(gpu, news, length, heads):
+    """As above outside the even share: tiles and rows that the search finds no sequence for."""
+    from openfold3_triangle_kernel_amd import paged_attention
+
+    cache, tables, starts, lens, T, g = _batch(gpu, news, [length] * len(news), 16, 2, 64, torch.bfloat16)
+    q = torch.randn(T, heads, 64, generator=g).bfloat16().to(gpu)
+    want = paged_attention(q, cache, tables, starts, lens)
+    S = len(news)
+    cut = starts.clone()
+    cut[S // 2 + 1:] = 0
+    for bad in (cut, starts.flip(0), starts[torch.randperm(S + 1, generator=g).to(gpu)],
+                torch.randint(-T, 2 * T, (S + 1,), generator=g, dtype=torch.int32).to(gpu)):
+        assert paged_attention(q, cache, tables, bad.contiguous(), lens).shape == q.shape
+    assert torch.equal(paged_attention(q, cache, tables, starts, lens), want)
+
+
 def test_attention_far_pages(gpu):
     """Pages past 32-bit byte offsets."""
     from openfold3_triangle_kernel_amd import PagedCache, paged_attention

@@ -106,6 +106,53 @@ def test_places_of_a_cache():
     assert row(3, 0) == row(-1, 0) == -1
 
 
+@pytest.mark.parametrize("S,T,G", [(3, 200, 4), (3, 1000, 4), (4, 300, 1), (70, 900, 3), (70, 5000, 8),
+                                   (200, 777, 40), (1, 65, 7)])
+def test_rows_of_a_batch(S, T, G):
+    """``tpf_paged_rows``, the rule by which the attention finds the rows of its tiles and of
+    its join: ascending starts give every row once, any others rows of the batch alone."""
+    cache, _, tables, starts, lengths = _paged(S=S)
+    batch = batch_struct(cache.k, tables, starts, lengths, T)
+    out = (ctypes.c_int64 * 3)()
+
+    def rows(tile_rows, at):
+        """(first row, all rows of its sequence, the sequence's first row in the batch)."""
+        if _native.query("tpf_paged_rows", ctypes.byref(batch), G, tile_rows, at, out) < 0:
+            return None
+        first, count, token = out
+        assert 0 <= first < count and 0 <= token and token * G + count <= T * G, (tile_rows, at, *out)
+        return first, count, token * G
+
+    def check(ascending):
+        for tile_rows in (32, 128):
+            met = torch.zeros(T * G, dtype=torch.int32)
+            for at in range(T * G // tile_rows + S + 1):
+                got = rows(tile_rows, at)
+                if got:
+                    first, count, base = got
+                    met[base + first:base + min(first + tile_rows, count)] += 1
+            assert not ascending or (met == 1).all()
+        for at in range(0, T * G, max(1, T * G // 500)):
+            got = rows(0, at)
+            assert got[0] + got[2] == at if got else not ascending
+
+    g = torch.Generator().manual_seed(S * T + G)
+    draw = lambda low, high: torch.randint(low, high, (S + 1,), generator=g, dtype=torch.int32)  # noqa: E731
+    for _ in range(4):
+        starts.copy_(draw(0, T + 1).sort()[0])
+        starts[0] = 0
+        check(True)
+        starts.copy_(draw(-T, 2 * T))
+        check(False)
+        starts.copy_(draw(0, T + 1).sort(descending=True)[0])
+        check(False)
+        starts.copy_(draw(0, T + 1).sort()[0])
+        starts[S // 2 + 1:] = 0  # (a batch's rows, then what a padded graph's array holds)
+        check(False)
+    for bad in ((0, 32, 0), (G, 64, 0), (G, 32, -1), (G, 32, T * G // 32 + S + 1), (G, 0, T * G), (1 << 30, 32, 0)):
+        assert _native.query("tpf_paged_rows", ctypes.byref(batch), *bad, out) == -1
+
+
 def test_c_abi_answers_before_a_launch():
     shape = (ctypes.c_int64 * 25)(1, 4, 2, 2, 16, 9, 0, 2, 1, 0, 64)
     with pytest.raises(RuntimeError, match="half=9"):
