@@ -188,9 +188,10 @@ struct SRows {
 __device__ __forceinline__ float sa_inverse(float n, float m) {
   return n == 0.f ? (m == kSaLow ? 0.f : __builtin_nanf("")) : 1.f / n;
 }
-// A row's log-sum-exp in powers of two; +inf for a row that sees no state: its p are 0.
+// A row's log-sum-exp in powers of two; +inf for a row that sees no state: its p are 0.  (A row
+// that has met scores of NaN alone, or beside others, keeps that maximum too: its sum is NaN.)
 __device__ __forceinline__ float sa_lse(const SAttnArgs& a, float m, float l) {
-  return m == kSaLow ? __builtin_inff() : fmaf(m, a.c, __log2f(l));
+  return l == 0.f && m == kSaLow ? __builtin_inff() : fmaf(m, a.c, __log2f(l));
 }
 
 // Writes four channels of a row's output at `at`, and what their rounding drops where

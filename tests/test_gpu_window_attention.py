@@ -307,6 +307,31 @@ def test_what_a_row_does_not_see_never_reaches_it(gpu, bad, N, D, window, sinks)
         assert torch.isfinite(b).all() and torch.equal(a, b)
 
 
+@pytest.mark.parametrize("N,window,at", [(40, None, 10), (40, 8, 10), (64, None, 0), (1500, 1, 700), (1500, 5, 1499),
+                                         (1500, None, 3)])
+def test_a_score_that_is_nan_reaches_every_value_gradient(gpu, N, window, at):
+    """Rows that see a NaN key have NaN probabilities: so have the value gradients of all
+    states that such a row sees, whether the row's states lie in one tile or in many."""
+    from openfold3_triangle_kernel_amd import window_attention
+
+    q, k, v = make(gpu, 1, 4, 2, N, 32, seed=9)
+    k[0, 0, at, 5] = float("nan")
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    dout = torch.randn(1, N, 4, 32, generator=torch.Generator().manual_seed(2)).bfloat16().to(gpu)
+    out = window_attention(*leaves, window)
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+    see = seen(torch.arange(N), N, window, 0).to(gpu)
+    rows = see[:, at]                   # that see the key
+    states = see[rows].any(0)           # that one of these sees
+    assert out[0, rows, :2].isnan().all() and torch.isfinite(out[0, ~rows]).all()
+    assert dq[0, :2, rows].isnan().all() and torch.isfinite(dq[0, :2, ~rows]).all()
+    for t in (dk, dv):
+        assert t[0, 0, states].isnan().all()
+        assert torch.isfinite(t[0, 0, ~states]).all()
+    for t in (out[0, :, 2:], dq[0, 2:], dk[0, 1], dv[0, 1]):
+        assert torch.isfinite(t).all()
+
+
 def test_rows_whose_scores_are_all_minus_infinity(gpu):
     """They are NaN, unlike rows that see no state."""
     from openfold3_triangle_kernel_amd import window_attention
