@@ -54,19 +54,20 @@ template <> struct RotType<TPF_F32> { typedef float E; };
 
 // Where a lane's sixteen channels are: entries 0 .. 7 are the pairs' first channels, 8 .. 15
 // the second ones.  With halves lane u < nr has the pairs 8 u .. 8 u + 7 and the others
-// sixteen channels that pass; interleaved, lane u has the channels 16 u .. 16 u + 15 and pairs
-// past the last are turned by 0.
+// sixteen channels that pass; interleaved, lane u has the channels 16 u .. 16 u + 15, and pairs
+// from `half` on pass as they are (turned by 0, an infinity would make its neighbour NaN).
 struct RotUnit {
-  int a0, b0, na, nb;
+  int a0, b0, na, nb, pairs;  // (pairs that turn)
   bool turns, inter;
   __device__ __forceinline__ RotUnit(const RotArgs& r, int u) {
     inter = r.inter;
+    pairs = r.half - 8 * u;
     if (inter) {
       a0 = 16 * u;
       b0 = 16 * u + 1;
       na = max(0, min(8, (r.D - 16 * u + 1) / 2));
       nb = max(0, min(8, (r.D - 16 * u) / 2));
-      turns = 8 * u < r.half;
+      turns = pairs > 0;
       return;
     }
     const int nr = (r.half + 7) / 8;
@@ -291,8 +292,8 @@ __global__ __launch_bounds__(256) void rot_fwd_kernel(RotArgs r) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float x = a[i], y = c[i];
-          a[i] = x * co[i] - y * si[i];
-          c[i] = y * co[i] + x * si[i];
+          a[i] = i < u.pairs ? x * co[i] - y * si[i] : x;
+          c[i] = i < u.pairs ? y * co[i] + x * si[i] : y;
         }
       }
     }
@@ -370,8 +371,8 @@ __global__ __launch_bounds__(256) void rot_bwd_kernel(RotArgs r) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float x = a[i], y = c[i];
-          a[i] = x * co[i] + y * si[i];
-          c[i] = y * co[i] - x * si[i];
+          a[i] = i < u.pairs ? x * co[i] + y * si[i] : x;
+          c[i] = i < u.pairs ? y * co[i] - x * si[i] : y;
         }
       }
       int head;

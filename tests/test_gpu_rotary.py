@@ -233,6 +233,50 @@ def test_values_that_are_not_finite_stay_in_their_row(gpu):
             assert not torch.isfinite(out[row]).all()
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("D,half,t", [(20, 5, "bf16"), (64, 3, "fp32"), (72, 18, "fp16"), (31, 13, "fp32")])
+def test_channels_that_pass_stay_apart(gpu, D, half, t, inter):
+    """A value that is not finite in a channel that only passes reaches no other channel, in
+    the forward, in the backward and on the way into a cache."""
+    from openfold3_triangle_kernel_amd import PagedCache, append_kv, qk_norm_rotary
+
+    q, k, g = _make(gpu, 1, 9, 4, 2, D, _T[t])
+    freq = _frequencies(half, gpu)
+    x = q.clone()
+    put = ((2 * half, float("inf")), (2 * half + 3, float("nan")), (D - 1, -float("inf")))
+    for c, v in put:
+        x[0, :, :, c] = v
+    clean, _ = qk_norm_rotary(q, k, None, freq, None, None, None, inter)
+    out, _ = qk_norm_rotary(x, k, None, freq, None, None, None, inter)
+    assert torch.equal(out[..., :2 * half], clean[..., :2 * half])
+    assert torch.equal(out[..., 2 * half:].nan_to_num(9.0), x[..., 2 * half:].nan_to_num(9.0))
+    leaf = q.clone().requires_grad_(True)
+    turned, _ = qk_norm_rotary(leaf, k, None, freq, None, None, None, inter)
+    dx, = torch.autograd.grad(turned, leaf, x, retain_graph=True)
+    want, = torch.autograd.grad(turned, leaf, q)
+    assert torch.equal(dx[..., :2 * half], want[..., :2 * half])
+    assert torch.equal(dx[..., 2 * half:].nan_to_num(9.0), x[..., 2 * half:].nan_to_num(9.0))
+    # With a norm an infinity makes its row's other channels 0 and itself NaN.
+    x = q.clone()
+    x[0, :, :, 2 * half] = float("inf")
+    out, _ = qk_norm_rotary(x, k, None, freq, None, None, 1e-6, inter)
+    assert out[..., 2 * half].isnan().all()
+    out[..., 2 * half] = 0.0
+    assert not out.any()
+    if D % 8 or t == "fp32":
+        return
+    cache = PagedCache(2, 2, 16, D, _T[t], gpu)
+    starts, lengths, tables = (torch.tensor(n, dtype=torch.int32, device=gpu) for n in ([0, 9], [9], [[1]]))
+    x = k[0].transpose(0, 1).clone()
+    x[..., 2 * half] = float("inf")
+    append_kv(cache, x, x, tables, starts, lengths, None, freq, None, None, None, inter)
+    _, want = qk_norm_rotary(q, k, None, freq, None, None, None, inter)
+    got = cache.k[1, :, :9]
+    assert torch.isposinf(got[..., 2 * half]).all()
+    keep = torch.arange(D, device=gpu) != 2 * half
+    assert torch.equal(got[..., keep], want[0][..., keep])
+
+
 def test_zero_heads_and_rows(gpu):
     from openfold3_triangle_kernel_amd import qk_norm_rotary
 
