@@ -275,6 +275,9 @@ __device__ __forceinline__ float buf_ldf(__amdgpu_buffer_rsrc_t r, uint32_t voff
   return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, voff, 0, 0));
 }
 
+// Workgroups of 256 threads a launch may have: below 2^32 threads, a multiple of 8.
+constexpr int64_t kMaxGroups = ((int64_t)1 << 24) - 8;
+
 // Division by a run-time invariant d (Granlund-Montgomery): for n < 2^31,
 // n / d = (umulhi(n, m) + n) >> s with s = ceil(log2 d),
 // m = floor(2^32 (2^s - d) / d) + 1.  Replaces 32/64-bit integer division

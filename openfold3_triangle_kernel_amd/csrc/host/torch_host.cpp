@@ -525,6 +525,8 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
 
 Tensor or_none(const std::optional<Tensor>& t) { return t.value_or(Tensor()); }
 
+constexpr int64_t kMaxTokens = (1 << 26) - 32;  // of a launch
+
 // Frequencies and weights as the kernels read them (D channels); nullopt-worthy ones are false.
 bool rotation_plain(int64_t D, const std::optional<Tensor>& freq, const std::optional<Tensor>& qw,
                     const std::optional<Tensor>& kw, const std::optional<double>& eps,
@@ -639,7 +641,7 @@ std::optional<std::tuple<Tensor, Tensor>> qk_norm_rotary(
       return std::nullopt;
   const int64_t B = q.size(0), N = q.size(2), D = q.size(3);
   if (type_code(q.scalar_type()) < 0 || k.size(0) != B || k.size(2) != N || k.size(3) != D || D > 256 ||
-      q.size(1) > 65535 || k.size(1) > 65535 || B * N >= (1 << 26) || !rotation_plain(D, freq, qw, kw, eps, dev))
+      q.size(1) > 65535 || k.size(1) > 65535 || B * N > kMaxTokens || !rotation_plain(D, freq, qw, kw, eps, dev))
     return std::nullopt;
   std::optional<Tensor> positions = positions_in;
   if (positions) {
@@ -769,7 +771,7 @@ std::optional<tpf_paged_batch> paged_batch(const Tensor& ck, const Tensor& table
       return std::nullopt;
   if (tables.dim() != 2 || starts.dim() != 1 || lengths.dim() != 1) return std::nullopt;
   const int64_t S = lengths.size(0), width = tables.size(1);
-  if (S < 1 || width < 1 || tables.size(0) != S || starts.size(0) != S + 1 || T < 1 || T >= (1 << 26) ||
+  if (S < 1 || width < 1 || tables.size(0) != S || starts.size(0) != S + 1 || T < 1 || T > kMaxTokens ||
       width > (1 << 30) / ck.size(2))
     return std::nullopt;
   return tpf_paged_batch{(const int32_t*)cptr(tables), (const int32_t*)cptr(starts), (const int32_t*)cptr(lengths),

@@ -550,7 +550,7 @@ static int rot_check(RotArgs& r, int64_t B, int64_t N, int64_t H, int64_t Hk, in
   r.eps = (float)eps;
   r.w_type = (int)w_type;
   rot_plan(r, 64 / rot_lanes(r), backward);
-  if ((double)B * (double)N * r.slices >= 4.0 * (double)((int64_t)1 << 24))
+  if ((double)B * (double)N * r.slices > 4.0 * (double)kMaxGroups)  // (four waves a workgroup)
     return set_error(TPF_ERR_SHAPE, "%s: too many tokens", fn);
   return TPF_OK;
 }

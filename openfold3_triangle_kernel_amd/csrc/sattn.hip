@@ -777,7 +777,7 @@ int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const ch
   const int64_t lim = (int64_t)1 << 30;
   if (s->B < 1 || s->N < 1 || s->B > lim || s->N > lim || a.G * s->N > lim ||
       (double)s->B * s->Hk * ((double)(a.G * s->N) / 64 + 1) * 64 > 2e9 ||
-      s->B * s->Hk * ((a.G * s->N + 127) / 128 + 8) > kXaMaxGroups)
+      s->B * s->Hk * ((a.G * s->N + 127) / 128 + 8) > kMaxGroups)
     return set_error(TPF_ERR_SHAPE, "%s: too many rows (B=%lld N=%lld)", fn, (long long)s->B, (long long)s->N);
   for (int i = 0; i < 3; ++i) {
     const int64_t* st = i == 0 ? s->q_stride : i == 1 ? s->k_stride : s->v_stride;
@@ -874,8 +874,8 @@ static int paged_attn_check(SAttnArgs& a, const tpf_paged_shape* s, const tpf_pa
   a.q_sn = s->q_stride[0]; a.q_sh = s->q_stride[1];
   a.B = a.t.S;
   a.rows = a.t.T * a.G;
-  if (a.rows > ((int64_t)1 << 30) || ((double)a.rows / 32 + a.t.S + 9) * a.Hk > (double)kXaMaxGroups / 2 ||
-      (double)a.rows * a.Hk / 4 + 1 > (double)kXaMaxGroups)
+  if (a.rows > ((int64_t)1 << 30) || ((double)a.rows / 32 + a.t.S + 9) * a.Hk > (double)kMaxGroups / 2 ||
+      (double)a.rows * a.Hk / 4 + 1 > (double)kMaxGroups)
     return set_error(TPF_ERR_SHAPE, "%s: too many rows", fn);
   return TPF_OK;
 }
@@ -900,7 +900,7 @@ static int paged_plan(SAttnArgs& a) {
   int64_t units = a.rows / rt > a.t.S ? a.rows / rt : a.t.S;
   units *= a.Hk;
   a.splits = sattn_splits(units < 1 ? 1 : units, 512, states);
-  while (a.splits > 1 && (double)a.tiles * a.Hk * a.splits > (double)kXaMaxGroups / 2) a.splits /= 2;
+  while (a.splits > 1 && (double)a.tiles * a.Hk * a.splits > (double)kMaxGroups / 2) a.splits /= 2;
   a.order = sa_order(a.Hk, (int64_t)a.tiles * a.splits);
   return rt;
 }

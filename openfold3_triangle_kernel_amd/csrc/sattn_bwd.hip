@@ -540,7 +540,7 @@ static int window_grad_plan(SAttnGrad& g, const char* fn) {
     }
     units = (int64_t)g.sunk * g.splits + (int64_t)(g.ktiles - g.sunk) * g.parts;
   }
-  if (BH * (units + 8) > kXaMaxGroups || (double)BH * a.N * (a.D / 4) / 256 + 1 > (double)kXaMaxGroups / 2)
+  if (BH * (units + 8) > kMaxGroups || (double)BH * a.N * (a.D / 4) / 256 + 1 > (double)kMaxGroups / 2)
     return set_error(TPF_ERR_SHAPE, "%s: too many states", fn);
   a.order = sa_order(BH, a.tiles);
   g.order = sa_order(BH, units);

@@ -594,7 +594,7 @@ int xattn_check(XAttnArgs& a, const tpf_xattn_shape* s, double scale, const char
   const int64_t G = s->H / s->Hk, lim = (int64_t)1 << 30;
   if (s->Nk > lim || s->Nq > lim || s->B > lim || s->H > lim || G * s->Nq > lim ||
       (double)s->B * s->Hk * ((double)(G * s->Nq) / 64 + 1) * 64 > 2e9 ||
-      s->B * s->Hk * ((G * s->Nq + 127) / 128) > kXaMaxGroups ||
+      s->B * s->Hk * ((G * s->Nq + 127) / 128) > kMaxGroups ||
       (double)s->B * s->Hk * ((double)s->Nk / 64 + 1) > 2e9)
     return set_error(TPF_ERR_SHAPE, "%s: too many rows or states", fn);
   for (int i = 0; i < 3; ++i) {

@@ -435,7 +435,7 @@ static void split_axis(int64_t groups, int64_t n, int64_t tile, int* splits, int
 static int grad_plan(XAttnGrad& g, const char* fn) {
   XAttnArgs& a = g.f;
   const int64_t BH = (int64_t)a.B * a.Hk;
-  if (BH * (((int64_t)a.Nk + 127) / 128) > kXaMaxGroups)
+  if (BH * (((int64_t)a.Nk + 127) / 128) > kMaxGroups)
     return set_error(TPF_ERR_SHAPE, "%s: too many states", fn);
   a.tiles = (a.R + 127) / 128;
   g.ktiles = (a.Nk + 127) / 128;

@@ -125,7 +125,7 @@ def check_batch(unsupported, cache, tables, starts, lengths, tokens) -> None:
     if len({t.device for t in (cache.k, tables, starts, lengths, *(t for _, t, _ in tokens))}) != 1:
         raise unsupported("the cache, its tables and the tokens must share one device")
     if T > _MAX_TOKENS or any(t.shape[1] > _MAX_HEADS for _, t, _ in tokens):
-        raise unsupported("at most 65535 heads and 2^26 - 1 tokens")
+        raise unsupported("at most 65535 heads and 2^26 - 32 tokens")
 
 
 def batch_struct(k_cache, tables, starts, lengths, T: int) -> _Batch:

@@ -22,7 +22,7 @@ from .activations import _DTYPES, differentiable_once, host_path
 from .attention import _device_supported
 
 _MAX_HEAD_DIM = 256
-_MAX_HEADS, _MAX_TOKENS = 65535, (1 << 26) - 1
+_MAX_HEADS, _MAX_TOKENS = 65535, (1 << 26) - 32  # (of a launch)
 _Shape = ctypes.c_int64 * 25  # tpf_rotary_shape
 
 
@@ -79,7 +79,7 @@ def _check(q, k, positions, frequencies, q_weight, k_weight, eps) -> None:
     if not 1 <= D <= _MAX_HEAD_DIM:
         raise _unsupported("requires 1<=D<=256")
     if max(q.shape[-3], k.shape[-3]) > _MAX_HEADS or math.prod(q.shape[:-3]) * q.shape[-2] > _MAX_TOKENS:
-        raise _unsupported("at most 65535 heads and 2^26 - 1 tokens")
+        raise _unsupported("at most 65535 heads and 2^26 - 32 tokens")
     if positions is not None:
         if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
             raise _unsupported("positions must be int32 or int64")

@@ -381,6 +381,25 @@ def test_sizes_that_a_launch_does_not_hold():
         assert 0 < size <= (2048 + 128) * 128 * 8 * 8 + 16 * 16384 + 2 * 16384 * 8 * 4 * 16
 
 
+def test_the_last_size_that_a_launch_holds():
+    """(2^24 - 8 workgroups of four waves, each with one token or more.)"""
+    meta = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device="meta")  # noqa: E731
+    most = (1 << 26) - 32
+    held = PagedCache.of(meta(5, 2, 4, 16), meta(5, 2, 4, 16))
+    places = [t.to("meta") for t in _paged()[2:]]
+    for T, match in ((most, "GPU"), (most + 1, "2\\^26"), ((1 << 26) - 1, "2\\^26")):
+        with pytest.raises(ValueError, match=match):
+            qk_norm_rotary(meta(1, 1, T, 8), meta(1, 1, T, 8))
+        x = meta(T, 2, 16)
+        with pytest.raises(ValueError, match=match):
+            append_kv(held, x, x, *places)
+        with pytest.raises(ValueError, match=match):
+            paged_attention(x, held, *places)
+        shape = (ctypes.c_int64 * 25)(1, T, 1, 1, 8, 0, 0, 2, 1, 0, 64)
+        size = _native.query("tpf_rotary_backward_workspace_bytes", shape)
+        assert size == (768 * 2 * 8 * 4 if T <= most else -1)
+
+
 def test_frequencies_first_used_in_inference_mode_train():
     """A backward keeps the device's copy: it is no inference tensor, whoever makes it."""
     from openfold3_triangle_kernel_amd import SelfAttention
