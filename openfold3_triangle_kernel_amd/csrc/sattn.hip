@@ -803,6 +803,9 @@ int window_check(SAttnArgs& a, const tpf_window_shape* s, double scale, const ch
   return TPF_OK;
 }
 
+// Workgroups of an even share's join: a unit's rows by 32, and a wave a token.
+static int64_t sattn_even_joins(const SAttnArgs& a, int rt) { return (int64_t)a.even * (rt / 32) + (a.t.T + 3) / 4; }
+
 // Rows of the parts in memory.
 static int64_t sattn_part_rows(const SAttnArgs& a, int rt) {
   return a.even ? (int64_t)2 * a.even * rt : a.splits > 1 ? a.Hk * a.rows * a.splits : 0;
@@ -852,8 +855,8 @@ static void window_pick(const SAttnArgs& a, int qb, hipStream_t s) {
 template <bool F16, bool PAGED>
 static void sattn_join(const SAttnArgs& a, int rt, hipStream_t s) {
   if (a.even)
-    hipLaunchKernelGGL((sattn_even_join_kernel<F16>), dim3((unsigned)(a.even * (rt / 32) + (a.t.T + 3) / 4)),
-                       dim3(256), 0, s, a, rt);
+    hipLaunchKernelGGL((sattn_even_join_kernel<F16>), dim3((unsigned)sattn_even_joins(a, rt)), dim3(256), 0, s, a,
+                       rt);
   if (a.splits > 1)
     hipLaunchKernelGGL((sattn_join_kernel<F16, PAGED>), dim3((unsigned)((a.Hk * a.rows + 3) / 4)), dim3(256), 0,
                        s, a, rt);
@@ -895,7 +898,8 @@ static int paged_plan(SAttnArgs& a) {
     // Workgroups that a CU runs at once: the streaming kernel's by their LDS, the tile kernel's by
     // their registers.
     a.even = 256 * (a.D > 64 ? (rt == 128 ? 2 : 1) : a.D > 32 ? (rt == 128 ? 3 : 2) : 4);
-    return rt;
+    if (sattn_even_joins(a, rt) <= kMaxGroups) return rt;
+    a.even = 0;
   }
   int64_t units = a.rows / rt > a.t.S ? a.rows / rt : a.t.S;
   units *= a.Hk;

@@ -400,6 +400,19 @@ def test_the_last_size_that_a_launch_holds():
         assert size == (768 * 2 * 8 * 4 if T <= most else -1)
 
 
+def test_the_even_share_of_many_tokens():
+    """The join of an even share has a wave a token beside its own workgroups: where a launch
+    does not hold them all, the grid is counted from the shapes (without parts here)."""
+    cache, _, tables, starts, lengths = _paged(S=2)
+    shape = (ctypes.c_int64 * 8)(1, 1, 8, 0, 0, 0, 8, 8)
+    for T, even in ((1 << 20, True), ((1 << 26) - 32 - 16384, True), ((1 << 26) - 31 - 16384, False),
+                    ((1 << 26) - 36, False)):
+        batch = batch_struct(cache.k, tables, starts, lengths, T)
+        batch.width, batch.page, batch.pages = 16, 64, 100
+        size = _native.query("tpf_paged_attention_workspace_bytes", shape, ctypes.byref(batch))
+        assert size == (2 * 1024 * 128 * (8 + 3) * 4 if even else 0)
+
+
 def test_frequencies_first_used_in_inference_mode_train():
     """A backward keeps the device's copy: it is no inference tensor, whoever makes it."""
     from openfold3_triangle_kernel_amd import SelfAttention
