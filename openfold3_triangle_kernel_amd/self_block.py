@@ -64,7 +64,7 @@ class SelfAttention(AttentionBlock):
         self.window, self.sinks, self.interleaved = window, sinks, interleaved
         self.activation_save, self.eps = activation_save, eps
         # In 64 bits whatever type the module is cast to; copies by device.
-        self._frequencies = {"cpu": frequencies.detach().to("cpu", torch.float64)}
+        self._frequencies = {"cpu": frequencies.detach().to("cpu", torch.float64, copy=True)}
         self.layer_norm = nn.LayerNorm(c_in, eps=eps)
         hc, kc = no_heads * c_hidden, no_kv_heads * c_hidden
         self.linear_q = nn.Linear(c_in, hc, bias=False)

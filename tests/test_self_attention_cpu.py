@@ -381,6 +381,16 @@ def test_sizes_that_a_launch_does_not_hold():
         assert 0 < size <= (2048 + 128) * 128 * 8 * 8 + 16 * 16384 + 2 * 16384 * 8 * 4 * 16
 
 
+def test_the_callers_frequencies_are_copied():
+    from openfold3_triangle_kernel_amd import SelfAttention
+
+    given = torch.tensor([0.7, 0.11, 0.03], dtype=torch.float64)
+    block, x = SelfAttention(16, 8, 2, frequencies=given), torch.randn(1, 9, 16)
+    want = block(x)
+    given.zero_()
+    assert torch.equal(block(x), want)
+
+
 def test_the_last_size_that_a_launch_holds():
     """(2^24 - 8 workgroups of four waves, each with one token or more.)"""
     meta = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device="meta")  # noqa: E731
