@@ -15,6 +15,7 @@ same formulas in PyTorch.
 from __future__ import annotations
 
 import math
+import warnings
 
 import torch
 from torch import nn
@@ -32,9 +33,10 @@ class SelfAttention(AttentionBlock):
     Tokens see the ``window`` tokens up to themselves (None: all before them) and the first
     ``sinks``.  The first ``rotary_channels`` channels of a head (default: all) are turned by
     ``position * rotary_base^(-2 c / rotary_channels)``, or by ``position * frequencies[c]``
-    where these are given; 0 leaves the rotation out.  ``qk_norm`` normalises the heads of q
-    and k.  ``activation_save`` as in ``CrossAttention``.  ``step`` takes new tokens of many
-    sequences through a paged cache.
+    where these are given; 0 leaves the rotation out.  A ``state_dict`` holds the frequencies;
+    loading one keeps the block's own and warns if they differ.  ``qk_norm`` normalises the
+    heads of q and k.  ``activation_save`` as in ``CrossAttention``.  ``step`` takes new tokens
+    of many sequences through a paged cache.
     """
 
     def __init__(self, c_in: int, c_hidden: int, no_heads: int, no_kv_heads: int | None = None,
@@ -78,6 +80,24 @@ class SelfAttention(AttentionBlock):
     def new_cache(self, pages: int, page: int, device="cuda") -> PagedCache:
         """A cache of ``pages`` pages of ``page`` states for ``step``."""
         return PagedCache(pages, self.no_kv_heads, page, self.c_hidden, torch.bfloat16, device)
+
+    def get_extra_state(self) -> torch.Tensor:
+        return self._frequencies["cpu"].clone()
+
+    def set_extra_state(self, state: torch.Tensor) -> None:
+        """The block's own frequencies stay (a context may be scaled by others); that a
+        checkpoint's differ, beyond roundings of a cast or a mean, is said."""
+        mine, given = self._frequencies["cpu"], state.detach().to("cpu", torch.float64)
+        if given.shape != mine.shape or not torch.allclose(
+                mine, given, rtol=max(1e-6, torch.finfo(state.dtype).eps), atol=0.0):
+            warnings.warn("SelfAttention: the checkpoint's block was made with other rotary frequencies; "
+                          "this block keeps its own", stacklevel=2)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, *rest):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, *rest)
+        key = prefix + "_extra_state"  # (earlier checkpoints have none)
+        if key in missing_keys:
+            missing_keys.remove(key)
 
     def _rotation(self, device):
         f = self._frequencies.get(str(device))

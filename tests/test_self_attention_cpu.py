@@ -381,6 +381,34 @@ def test_sizes_that_a_launch_does_not_hold():
         assert 0 < size <= (2048 + 128) * 128 * 8 * 8 + 16 * 16384 + 2 * 16384 * 8 * 4 * 16
 
 
+def test_a_checkpoint_of_other_frequencies_is_told():
+    """A block keeps the frequencies that it was made with, and says if they are not the
+    checkpoint's."""
+    import warnings
+
+    from openfold3_triangle_kernel_amd import SelfAttention
+
+    mine = torch.tensor([0.7, 0.11, 0.03], dtype=torch.float64)
+    block, x = SelfAttention(16, 8, 2, frequencies=mine), torch.randn(1, 9, 16)
+    want, state = block(x), block.state_dict()
+    alike = SelfAttention(16, 8, 2, frequencies=mine)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        alike.load_state_dict(state)
+        assert torch.equal(alike(x), want)
+        alike.load_state_dict({k: v.bfloat16() for k, v in state.items()})
+        alike.load_state_dict({k: v for k, v in state.items() if v.dtype != torch.float64})
+        none = [SelfAttention(16, 8, 2, rotary_channels=0) for _ in range(2)]
+        none[0].load_state_dict(none[1].state_dict())
+    for other in (dict(rotary_channels=6), dict(frequencies=2 * mine), dict(), dict(rotary_channels=0)):
+        other = torch.nn.Sequential(SelfAttention(16, 8, 2, **other))
+        own = other[0]._frequencies["cpu"].clone()
+        with pytest.warns(UserWarning, match="frequencies"):
+            other.load_state_dict({"0." + k: v for k, v in state.items()})
+        assert torch.equal(other[0]._frequencies["cpu"], own)
+        assert torch.equal(other[0].linear_q.weight, block.linear_q.weight)
+
+
 def test_the_callers_frequencies_are_copied():
     from openfold3_triangle_kernel_amd import SelfAttention
 
