@@ -57,7 +57,7 @@ class SelfAttention(AttentionBlock):
             if turned < 0 or turned % 2 or turned > c_hidden:
                 raise ValueError("rotary_channels must be even and at most c_hidden")
             frequencies = torch.tensor([rotary_base ** (-2.0 * c / turned) for c in range(turned // 2)],
-                                       dtype=torch.float64)
+                                       dtype=torch.float64, device="cpu")
         elif frequencies.ndim != 1 or 2 * len(frequencies) > c_hidden:
             raise ValueError("frequencies must have one axis, at most half the head's channels")
         self.c_in, self.c_hidden = c_in, c_hidden

@@ -419,6 +419,19 @@ def test_the_callers_frequencies_are_copied():
     assert torch.equal(block(x), want)
 
 
+def test_a_block_is_made_without_memory():
+    """Under the meta device, its parameters placed later."""
+    from openfold3_triangle_kernel_amd import SelfAttention
+
+    torch.manual_seed(0)
+    block, x = SelfAttention(16, 8, 2), torch.randn(1, 9, 16)
+    with torch.device("meta"):
+        empty = SelfAttention(16, 8, 2)
+    assert all(p.is_meta for p in empty.parameters())
+    empty.to_empty(device="cpu").load_state_dict(block.state_dict())
+    assert torch.equal(empty(x), block(x))
+
+
 def test_the_last_size_that_a_launch_holds():
     """(2^24 - 8 workgroups of four waves, each with one token or more.)"""
     meta = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device="meta")  # noqa: E731
