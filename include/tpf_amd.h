@@ -654,11 +654,12 @@ int tpf_rotary_backward(const void* q, const void* k, const void* dq_out, const 
  * read there alone: starts are held to [0, T], lengths to the table's width, and a page
  * outside [0, pages) holds no state (it is neither written nor read).
  *
- * tpf_paged_row: page * page size + place of a state, -1 where there is none.
+ * tpf_paged_row: page * page size + place of a state, -1 where there is none, by the append's
+ * own function (the attention finds 64 states' pages at a time by the same rule).
  * tpf_paged_rows: with `group` rows a token (the query heads of a kv head), the sequence of
  * the attention's tile `at` of tile_rows (32 or 128) rows, or (tile_rows 0) of row `at`; in
  * rows[3] the tile's first row there, all its rows and its first token; -1 where no
- * sequence has it.  Both on host arrays, by the functions that the kernels run.
+ * sequence has it, by the function that its kernels run.  Both on host arrays.
  *
  * tpf_paged_append: norm and rotation (as above, by the states' numbers) of the new keys
  * k [T, Hk, D] on the way into the cache, their values v as they are, and the queries q

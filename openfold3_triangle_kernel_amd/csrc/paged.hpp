@@ -107,7 +107,7 @@ struct PagedRows {
   // length.
   template <typename W>
   __host__ __device__ __forceinline__ bool tile(const PagedTables& t, int G, int rt, int tile) {
-    // (T G is 2^30 at most, and S rt below it.)
+    // (T G + S rt is below 2^31.)
     auto before = [&](int x) { return (int)((uint32_t)paged_start(t, x) * (uint32_t)G / (uint32_t)rt) + x; };
     sequence<W>(t, G, W::scalar(paged_search<W>(t.S, [&](int x) { return before(x) <= tile; })));
     r0 = W::scalar((tile - before(s)) * rt);

@@ -12,8 +12,8 @@
 // pairs (or sixteen channels that only pass), L lanes a row, and a wave takes the heads
 // of one token 64 / L at a time, so the angles of a token are formed once, a pair a
 // lane, and shared through LDS.  A turn's fraction is formed in 64 bits, position
-// times f / 2 pi less the nearest whole number: the angle is within 2^-25 of a turn at any
-// position below 2^28, where 32 bits would have lost it past a few thousand.  2 x 4096 tokens,
+// times f / 2 pi less the nearest whole number: the angle is within 2^-25 of a turn while position
+// times f is below 2^28 radians, where 32 bits would have lost it past a few thousand.  2 x 4096 tokens,
 // 32 + 8 heads of 128, BF16: 40 us forward (4.2 TB/s, what a copy reaches is 4.9), 69 backward
 // (3.6 TB/s: the weights' sums leave three waves a SIMD).
 #include "paged.hpp"
@@ -694,7 +694,7 @@ extern "C" int64_t tpf_paged_rows(const tpf_paged_batch* batch, int64_t group, i
   tpf::PagedTables t{};
   const int64_t lim = (int64_t)1 << 30;
   if (tpf::paged_check(t, batch, "tpf_paged_rows") || !rows || group < 1 || group > lim / t.T ||
-      t.S > lim / 128 || at < 0)
+      t.S > lim / 256 || at < 0)
     return -1;
   tpf::PagedRows r;
   if (tile_rows == 0) {

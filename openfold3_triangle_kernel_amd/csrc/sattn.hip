@@ -886,7 +886,9 @@ static int paged_attn_check(SAttnArgs& a, const tpf_paged_shape* s, const tpf_pa
 // Up to 32 rows a sequence on the mean run on the streaming kernel.  Up to 64 sequences share
 // their work evenly over the workgroups that run at once, if a sequence can have 1024 states;
 // otherwise tiles are counted for the most that the tokens can be and the parts for those
-// that are likely.
+// that are likely.  (One token of each of 64 sequences of 512 to 8191 states, 32 heads on 8 of
+// 128: 250 us, 5.1 TB/s; of 65: 280, 4.0 TB/s.  77 states in a table for 8192: 13 us, in a short
+// one 7: the host does not read the lengths.)
 static int paged_plan(SAttnArgs& a) {
   const int rt = a.rows <= 32 * (int64_t)a.t.S ? 32 : 128;
   const int64_t states = (int64_t)a.t.width * a.t.page;

@@ -201,8 +201,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | N
     ``eps`` None leaves the norm out; ``q_weight`` and ``k_weight`` [D] (BF16, FP16 or FP32)
     scale the normalised heads.  ``frequencies`` [half] are radians a position (kept in 64
     bits; None leaves the rotation out), ``positions`` whole numbers that broadcast to
-    [*B, N] (None: 0 .. N - 1); below 2^28 an angle is within 2^-22 radians.  Statistics
-    and products are in 32 bits.  Gradients: q, k and the weights.  Other cases raise
+    [*B, N] (None: 0 .. N - 1); while position times frequency is below 2^28 radians, an
+    angle is within 2^-22 of it.  Statistics and products are in 32 bits.  Gradients: q, k and the weights.  Other cases raise
     ``ValueError`` before any launch.
     """
     if (host_path(q, k, *(t for t in (positions, frequencies, q_weight, k_weight) if t is not None))
